@@ -8,7 +8,9 @@ and only token ids come back.  The C ABI is include/gsampler.h; this package is 
 Python host side.
 """
 from . import _lib  # noqa: F401
+from .kv_cache import GpuKvCache  # noqa: F401
 from .lm_head import GpuLmHead  # noqa: F401
+from .norm import GpuRmsNorm, RmsNormResult  # noqa: F401
 from .decoding import (  # noqa: F401
     DEFAULT_DECODING_CONFIG,
     DEFAULT_GENERATION_CONFIG,

@@ -25,6 +25,13 @@ GS_ENONFINITE = 9
 
 GS_DTYPE_F32 = 0
 GS_DTYPE_BF16 = 1
+GS_DTYPE_E4M3 = 2
+GS_DTYPE_INT8 = 3
+
+KV_ERR_SLOT = 1
+KV_ERR_PAGE = 2
+KV_ERR_LENGTH = 4
+KV_ERR_TIMEOUT = 8
 
 LM_ROUTE_AUTO = 0
 LM_ROUTE_FUSED = 1
@@ -58,6 +65,8 @@ EXPORTS = (
     "gs_lm_head_last_error", "gs_lm_head_logits", "gs_lm_head_sample", "gs_lm_head_check",
     "gs_lm_head_fused_calls", "gs_build_reasoning_mask_rows", "gs_nccl_unique_id", "gs_nccl_create",
     "gs_nccl_destroy", "gs_nccl_last_error", "gs_shard_sample", "gs_lm_head_set_route",
+    "gs_rms_norm", "gs_kv_cache_create", "gs_kv_cache_destroy", "gs_kv_cache_last_error", "gs_kv_cache_check",
+    "gs_kv_write", "gs_kv_read", "gs_attention",
 )
 
 NOALLOC_SCRATCH_BYTES = 8 << 20
@@ -142,6 +151,41 @@ class GsOutputs(ctypes.Structure):
     ]
 
 
+class GsRmsNormArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "residual", "weight", "residual_out", "out", "out_scale",
+                                               "row_sum")] + \
+               [(n, ctypes.c_int64) for n in ("rows", "hidden", "ld_x", "ld_residual", "ld_residual_out", "ld_out")] + \
+               [(n, ctypes.c_int32) for n in ("dtype", "weight_dtype", "out_dtype", "group")] + \
+               [(n, ctypes.c_float) for n in ("eps", "weight_offset", "srq_scale")]
+
+
+class GsKvCacheDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale")] + [("pages", ctypes.c_int64)] + \
+               [(n, ctypes.c_int32) for n in ("page_size", "kv_heads", "head_dim", "format")] + \
+               [(n, ctypes.c_int64) for n in ("k_page_stride", "k_head_stride", "k_token_stride", "v_page_stride",
+                                              "v_head_stride", "v_token_stride")]
+
+
+class GsKvRows(ctypes.Structure):
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int64) for n in ("k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride")] + \
+               [("slots", ctypes.c_void_p), ("tokens", ctypes.c_int64), ("dtype", ctypes.c_int32)]
+
+
+class GsAttentionArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "out", "lse", "q_start", "kv_len", "page_table")] + \
+               [(n, ctypes.c_int64) for n in ("tokens", "q_token_stride", "q_head_stride", "out_token_stride",
+                                              "out_head_stride", "page_table_stride", "page_table_cols")] + \
+               [(n, ctypes.c_int32) for n in ("seqs", "q_heads", "max_q", "max_kv", "window", "sinks")] + \
+               [("scale", ctypes.c_float)]
+
+
+def current_stream(device) -> int:
+    """The raw handle of torch's current stream on ``device``."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def build(force: bool = False) -> str:
     """Compiles libgsampler.so for sm_100a (make, nvcc)."""
     if force or not os.path.exists(LIB_PATH):
@@ -203,12 +247,21 @@ def lib() -> ctypes.CDLL:
     L.gs_nccl_last_error.argtypes = [P]
     L.gs_nccl_last_error.restype = ctypes.c_char_p
     L.gs_shard_sample.argtypes = [P, P, ctypes.POINTER(GsBatch), i64, i64, ctypes.POINTER(GsOutputs), i32, P]
+    L.gs_rms_norm.argtypes = [P, ctypes.POINTER(GsRmsNormArgs), P]
+    L.gs_kv_cache_create.argtypes = [P, ctypes.POINTER(GsKvCacheDesc), ctypes.POINTER(P)]
+    L.gs_kv_cache_destroy.argtypes = [P]
+    L.gs_kv_cache_last_error.argtypes = [P]
+    L.gs_kv_cache_last_error.restype = ctypes.c_char_p
+    L.gs_kv_cache_check.argtypes = [P, ctypes.POINTER(i32)]
+    L.gs_kv_write.argtypes = [P, ctypes.POINTER(GsKvRows), P]
+    L.gs_kv_read.argtypes = [P, ctypes.POINTER(GsKvRows), P]
+    L.gs_attention.argtypes = [P, ctypes.POINTER(GsAttentionArgs), P]
     L.gs_profile_enable.argtypes = [P, i32]
     L.gs_profile_read.argtypes = [P, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(i64),
                                   ctypes.POINTER(ctypes.c_double), ctypes.POINTER(i64)]
     for name in EXPORTS:
         if name not in ("gs_last_error", "gs_shard_record_bytes", "gs_constraint_last_error", "gs_lm_head_last_error",
-                        "gs_lm_head_fused_calls", "gs_nccl_last_error"):
+                        "gs_lm_head_fused_calls", "gs_nccl_last_error", "gs_kv_cache_last_error"):
             getattr(L, name).restype = ctypes.c_int
     L.gs_lm_head_fused_calls.restype = i64
     _lib = L

@@ -37,6 +37,8 @@ struct gs_ctx {
   int32_t* tok_dev = nullptr;
   double* lp_dev = nullptr;
   size_t tok_cap = 0;
+  // attention workspace (split-context partial results), allocated once by the first cache handle
+  unsigned char* attn_ws = nullptr;
   // kernel timing: events around the streaming pass and the merge of each gs_sample
   bool profile = false;
   std::vector<cudaEvent_t> ev_pool;
@@ -123,6 +125,13 @@ gs_status ensure_plans_slot(gs_ctx* c, int k, size_t n) {
 namespace gs {
 int ctx_device(const gs_ctx* c) { return c->device; }
 void ctx_set_error(gs_ctx* c, const char* msg) { c->err = msg; }
+cudaError_t ctx_attn_workspace(gs_ctx* c, size_t bytes, unsigned char** out) {
+  cudaError_t e = cudaSuccess;
+  if (!c->attn_ws) e = cudaMalloc(&c->attn_ws, bytes);
+  if (e != cudaSuccess) c->attn_ws = nullptr;
+  *out = c->attn_ws;
+  return e;
+}
 }  // namespace gs
 
 extern "C" {
@@ -157,6 +166,7 @@ gs_status gs_destroy(gs_ctx* c) {
   if (c->io) cudaFree(c->io);
   if (c->digest) cudaFree(c->digest);
   if (c->step_done) cudaFree(c->step_done);
+  if (c->attn_ws) cudaFree(c->attn_ws);
   if (c->tok_dev) cudaFree(c->tok_dev);
   if (c->lp_dev) cudaFree(c->lp_dev);
   for (int k = 0; k < gs_ctx::kPlanSlots; ++k) {

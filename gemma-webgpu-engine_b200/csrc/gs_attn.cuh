@@ -1,0 +1,128 @@
+// Shared types of the paged key/value cache and its attention kernels.
+#pragma once
+#include <string>
+
+#include "gs_device.cuh"
+#include "gs_internal.cuh"
+#include "gs_quant.cuh"
+#include "../../include/gsampler.h"
+
+struct gs_kv_cache {
+  gs_ctx* ctx = nullptr;
+  int device = 0;
+  int num_sms = 0;
+  gs_kv_cache_desc d{};
+  int page_shift = 0;
+  int32_t* flag = nullptr;       // device: GS_KV_ERR_* bits
+  unsigned char* ws = nullptr;   // the context's attention workspace (kAttnWsBytes)
+  std::string err;
+};
+
+namespace gs {
+
+// Workspace of split-context partial results: [partial][rows][head_dim] float32 outputs and
+// [partial][rows][2] maxima and sums.  The planner never asks for more.
+constexpr size_t kAttnWsBytes = 64u << 20;
+
+struct KvPool {
+  const unsigned char* k;
+  const unsigned char* v;
+  const float* k_scale;
+  const float* v_scale;
+  int64_t k_page, k_head, k_token;  // byte strides
+  int64_t v_page, v_head, v_token;
+  int32_t pages;
+  int32_t page_shift;
+  int32_t kv_heads;
+};
+
+struct AttnArgs {
+  KvPool kv;
+  const __nv_bfloat16* q;
+  __nv_bfloat16* out;
+  float* lse;
+  const int32_t* q_start;
+  const int32_t* kv_len;
+  const int32_t* table;
+  int64_t q_token, q_head, o_token, o_head;  // element strides
+  int64_t table_stride;
+  int64_t tokens;
+  int32_t table_cols;
+  int32_t seqs, q_heads, group;
+  int32_t max_q, max_kv;
+  int32_t window, sinks;
+  float scale_log2;     // scale · log2(e): scores in log2 units
+  int32_t chunk_tiles;  // context tiles per split
+  int32_t splits;       // partial slots per (sequence, head, row block)
+  float* part_o;        // [seq][row block][kv head][split][rows][head_dim]
+  float* part_ml;       // [..][rows][2]: running maximum (log2 units) and sum
+  int32_t* flag;
+};
+
+// What one block of query rows of a sequence sees: rows are (new token, head of the
+// group), row = token · group + head.
+struct RowRange {
+  int32_t q0;       // first new token of the sequence
+  int32_t nq;       // its new tokens
+  int32_t len;      // its cached tokens
+  int32_t rows;     // rows of this block
+  int32_t p0;       // position of new token 0
+  int32_t hi;       // tokens >= hi are hidden from every row
+  int32_t lo;       // tokens in [sink, lo) are hidden from every row (0 without a window)
+  int32_t sink;     // tokens below stay visible (0 without a window)
+  int32_t sink_tiles, first_tile, tiles;  // context tiles: [0, sink_tiles), then from first_tile
+  __device__ __forceinline__ int tile(int i) const { return i < sink_tiles ? i : first_tile + i - sink_tiles; }
+  __device__ __forceinline__ bool seen_by_any(int j) const { return j < hi && (j >= lo || j < sink); }
+};
+
+// Rows [r0, r0 + cap) of sequence b, context tiles of kTile tokens.
+template <int kTile>
+__device__ __forceinline__ RowRange row_range(const AttnArgs& A, int b, int r0, int cap) {
+  RowRange R;
+  R.q0 = A.q_start ? A.q_start[b] : b;
+  int q1 = A.q_start ? A.q_start[b + 1] : b + 1;
+  R.len = A.kv_len[b];
+  bool bad = R.len > A.max_kv || R.len < 0 || R.q0 < 0 || q1 > A.tokens || q1 - R.q0 > A.max_q;
+  R.len = min(max(R.len, 0), A.max_kv);
+  R.q0 = max(R.q0, 0);
+  q1 = static_cast<int>(min(static_cast<int64_t>(q1), A.tokens));
+  R.nq = max(q1 - R.q0, 0);
+  R.p0 = R.len - R.nq;
+  R.nq = min(R.nq, A.max_q);
+  R.rows = min(cap, R.nq * A.group - r0);
+  if (R.rows <= 0) {
+    R.rows = 0;
+    R.tiles = 0;
+    if (bad && r0 == 0 && threadIdx.x == 0) atomicOr(A.flag, GS_KV_ERR_LENGTH);
+    return R;
+  }
+  if (bad && threadIdx.x == 0) atomicOr(A.flag, GS_KV_ERR_LENGTH);
+  const int pf = R.p0 + r0 / A.group, pl = R.p0 + (r0 + R.rows - 1) / A.group;
+  R.hi = max(pl + 1, 0);
+  R.lo = A.window ? max(pf - A.window + 1, 0) : 0;
+  R.lo = min(R.lo, R.hi);
+  R.sink = A.window ? min(A.sinks, R.hi) : 0;
+  R.sink_tiles = (R.sink + kTile - 1) / kTile;
+  R.first_tile = max(R.lo / kTile, R.sink_tiles);
+  R.tiles = R.sink_tiles + max((R.hi + kTile - 1) / kTile - R.first_tile, 0);
+  return R;
+}
+
+// Context tiles of kTile tokens the widest row block of a call can see (host side).
+inline int64_t most_tiles(const AttnArgs& a, int tile, int rows_per_block) {
+  const int64_t all = (static_cast<int64_t>(a.max_kv) + tile - 1) / tile;
+  if (!a.window) return all;
+  const int64_t span = static_cast<int64_t>(a.window) + (rows_per_block + a.group - 1) / a.group + 1;
+  const int64_t w = (static_cast<int64_t>(a.sinks) + tile - 1) / tile + (span + tile - 1) / tile + 2;
+  return w < all ? w : all;
+}
+
+__device__ __forceinline__ float ex2(float x) { return ex2_approx(x); }
+
+// Few-row kernel (mma.sync, one 16-token tile per warp): any number of rows in blocks.
+cudaError_t launch_attn_rows(const gs_kv_cache* c, AttnArgs a, cudaStream_t st);
+// Joins the partial results of a split context.  rows_per_block and tile as in the kernel
+// that wrote them.
+cudaError_t launch_attn_join(const AttnArgs& a, int head_dim, int rows_per_block, int row_blocks, int tile, cudaStream_t st);
+
+}  // namespace gs

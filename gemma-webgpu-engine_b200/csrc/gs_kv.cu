@@ -1,0 +1,383 @@
+// Paged key/value cache: handle, quantising write, read back, and the attention entry.
+//
+// write  a = max(max|x|, 2^-64) over head_dim, code = round(x · (M / a)), scale = a / M
+// read   value = code · scale, rounded once
+// A row (one token and head) is head_dim / 8 neighbouring lanes of 8 elements each, so its
+// maximum is a shuffle reduction and every access is 16 bytes (8 for codes); one launch
+// covers keys and values.  Both directions move 3 bytes an element (bf16 beside codes) and
+// are bound by HBM for long chunks, by launch latency for one step.
+#include <cmath>
+#include <new>
+
+#include "gs_attn.cuh"
+
+namespace gs {
+namespace {
+
+struct KvRowsArgs {
+  KvPool kv;
+  unsigned char* k;  // the caller's rows
+  unsigned char* v;
+  int64_t k_token, k_head, v_token, v_head;  // elements
+  const int32_t* slots;
+  int64_t rows;      // tokens · kv_heads
+  int64_t slots_end; // pages · page_size
+  int32_t* flag;
+};
+
+struct SlotAt {
+  int64_t page;
+  int32_t off;
+  bool ok;
+};
+
+__device__ __forceinline__ SlotAt slot_at(const KvRowsArgs& A, int64_t token) {
+  const int32_t s = __ldg(A.slots + token);
+  SlotAt r;
+  r.ok = s >= 0 && s < A.slots_end;
+  if (s >= A.slots_end) atomicOr(A.flag, GS_KV_ERR_SLOT);
+  r.page = r.ok ? s >> A.kv.page_shift : 0;
+  r.off = r.ok ? s & ((1 << A.kv.page_shift) - 1) : 0;
+  return r;
+}
+
+template <bool BF16, bool VEC>
+__device__ __forceinline__ void load8(const void* p, float (&x)[8]) {
+  if constexpr (VEC) {
+    load_row<8, BF16>(p, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float y[1];
+      load_row<1, BF16>(static_cast<const unsigned char*>(p) + i * (BF16 ? 2 : 4), y);
+      x[i] = y[0];
+    }
+  }
+}
+template <bool BF16, bool VEC>
+__device__ __forceinline__ void store8(void* p, const float (&x)[8]) {
+  if constexpr (VEC) {
+    store_row<8, BF16>(p, x);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float y[1] = {x[i]};
+      store_row<1, BF16>(static_cast<unsigned char*>(p) + i * (BF16 ? 2 : 4), y);
+    }
+  }
+}
+
+template <int D, int FMT, bool BF16, bool VEC>
+__global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ KvRowsArgs A) {
+  constexpr int kLanes = D / 8;
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / kLanes;
+  const int at = (threadIdx.x % kLanes) * 8;
+  const bool value = blockIdx.y != 0;
+  const bool live = row < A.rows;
+  const int64_t token = live ? row / A.kv.kv_heads : 0;
+  const int head = live ? static_cast<int>(row % A.kv.kv_heads) : 0;
+  float x[8] = {};
+  SlotAt s{0, 0, false};
+  if (live) {
+    s = slot_at(A, token);
+    const int64_t e = value ? token * A.v_token + head * A.v_head : token * A.k_token + head * A.k_head;
+    if (s.ok) load8<BF16, VEC>((value ? A.v : A.k) + (e + at) * (BF16 ? 2 : 4), x);
+  }
+  unsigned char* pool = const_cast<unsigned char*>(value ? A.kv.v : A.kv.k);
+  pool += value ? s.page * A.kv.v_page + head * A.kv.v_head + s.off * A.kv.v_token
+                : s.page * A.kv.k_page + head * A.kv.k_head + s.off * A.kv.k_token;
+  if constexpr (FMT == GS_DTYPE_BF16) {
+    if (s.ok) store_row<8, true>(pool + at * 2, x);
+  } else {
+    constexpr float kMax = FMT == GS_DTYPE_E4M3 ? kE4m3Max : kInt8Max;
+    int m = 0;  // bits of max|x|: integer order is value order, NaN above all
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_int(x[i]) & 0x7fffffff);
+#pragma unroll
+    for (int o = kLanes >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(kFullMask, m, o));
+    const float inv = quant_inv(__int_as_float(m), kMax);
+    if (s.ok) {
+      uint2 c;
+      if constexpr (FMT == GS_DTYPE_E4M3) {
+        c.x = e4m3x4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+        c.y = e4m3x4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
+      } else {
+        c.x = int8x4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
+        c.y = int8x4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
+      }
+      *reinterpret_cast<uint2*>(pool + at) = c;
+      if (at == 0) {
+        float* sc = const_cast<float*>(value ? A.kv.v_scale : A.kv.k_scale);
+        sc[((s.page * A.kv.kv_heads + head) << A.kv.page_shift) + s.off] = quant_scale(__int_as_float(m), kMax);
+      }
+    }
+  }
+}
+
+template <int D, int FMT, bool BF16, bool VEC>
+__global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvRowsArgs A) {
+  constexpr int kLanes = D / 8;
+  const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / kLanes;
+  if (row >= A.rows) return;
+  const int at = (threadIdx.x % kLanes) * 8;
+  const bool value = blockIdx.y != 0;
+  const int64_t token = row / A.kv.kv_heads;
+  const int head = static_cast<int>(row % A.kv.kv_heads);
+  const SlotAt s = slot_at(A, token);
+  float x[8] = {};
+  if (s.ok) {
+    const unsigned char* pool = value ? A.kv.v + s.page * A.kv.v_page + head * A.kv.v_head + s.off * A.kv.v_token
+                                      : A.kv.k + s.page * A.kv.k_page + head * A.kv.k_head + s.off * A.kv.k_token;
+    if constexpr (FMT == GS_DTYPE_BF16) {
+      load_row<8, true>(pool + at * 2, x);
+    } else {
+      const uint2 c = *reinterpret_cast<const uint2*>(pool + at);
+      const float sc = (value ? A.kv.v_scale : A.kv.k_scale)[((s.page * A.kv.kv_heads + head) << A.kv.page_shift) + s.off];
+      const uint32_t w[2] = {c.x, c.y};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if constexpr (FMT == GS_DTYPE_E4M3) {
+          const float2 a = half2_float2(e4m3x2_half2(w[i] & 0xffffu)), b = half2_float2(e4m3x2_half2(w[i] >> 16));
+          x[4 * i] = a.x * sc, x[4 * i + 1] = a.y * sc, x[4 * i + 2] = b.x * sc, x[4 * i + 3] = b.y * sc;
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            x[4 * i + k] = static_cast<float>(static_cast<int8_t>((w[i] >> (8 * k)) & 0xffu)) * sc;
+        }
+      }
+    }
+  }
+  const int64_t e = value ? token * A.v_token + head * A.v_head : token * A.k_token + head * A.k_head;
+  store8<BF16, VEC>((value ? A.v : A.k) + (e + at) * (BF16 ? 2 : 4), x);
+}
+
+template <int D, int FMT, bool BF16>
+cudaError_t launch_rows2(const KvRowsArgs& a, bool write, bool vec, cudaStream_t st) {
+  const int64_t per = 256 / (D / 8);
+  const dim3 grid(static_cast<unsigned>((a.rows + per - 1) / per), 2);
+  if (write) {
+    if (vec) kv_write_kernel<D, FMT, BF16, true><<<grid, 256, 0, st>>>(a);
+    else kv_write_kernel<D, FMT, BF16, false><<<grid, 256, 0, st>>>(a);
+  } else {
+    if (vec) kv_read_kernel<D, FMT, BF16, true><<<grid, 256, 0, st>>>(a);
+    else kv_read_kernel<D, FMT, BF16, false><<<grid, 256, 0, st>>>(a);
+  }
+  return cudaGetLastError();
+}
+template <int D, int FMT>
+cudaError_t launch_rows1(const KvRowsArgs& a, bool write, bool bf16, bool vec, cudaStream_t st) {
+  return bf16 ? launch_rows2<D, FMT, true>(a, write, vec, st) : launch_rows2<D, FMT, false>(a, write, vec, st);
+}
+template <int D>
+cudaError_t launch_rows(const KvRowsArgs& a, int fmt, bool write, bool bf16, bool vec, cudaStream_t st) {
+  switch (fmt) {
+    case GS_DTYPE_BF16: return launch_rows1<D, GS_DTYPE_BF16>(a, write, bf16, vec, st);
+    case GS_DTYPE_E4M3: return launch_rows1<D, GS_DTYPE_E4M3>(a, write, bf16, vec, st);
+    default: return launch_rows1<D, GS_DTYPE_INT8>(a, write, bf16, vec, st);
+  }
+}
+
+gs_status kfail(gs_kv_cache* c, gs_status s, const char* m) {
+  c->err = m;
+  return s;
+}
+
+KvPool pool_of(const gs_kv_cache* c) {
+  const gs_kv_cache_desc& d = c->d;
+  const int64_t e = d.format == GS_DTYPE_BF16 ? 2 : 1;
+  KvPool p{};
+  p.k = static_cast<const unsigned char*>(d.k);
+  p.v = static_cast<const unsigned char*>(d.v);
+  p.k_scale = d.k_scale;
+  p.v_scale = d.v_scale;
+  p.k_page = d.k_page_stride * e, p.k_head = d.k_head_stride * e, p.k_token = d.k_token_stride * e;
+  p.v_page = d.v_page_stride * e, p.v_head = d.v_head_stride * e, p.v_token = d.v_token_stride * e;
+  p.pages = static_cast<int32_t>(d.pages);
+  p.page_shift = c->page_shift;
+  p.kv_heads = d.kv_heads;
+  return p;
+}
+
+gs_status move_rows(gs_kv_cache* c, const gs_kv_rows* r, void* stream, bool write) {
+  if (!c) return GS_EINVAL;
+  if (!r) return kfail(c, GS_EINVAL, "rows are required");
+  if (r->tokens < 0) return kfail(c, GS_EINVAL, "tokens must be >= 0");
+  if (r->tokens == 0) return GS_OK;
+  if (!r->k || !r->v || !r->slots) return kfail(c, GS_EINVAL, "k, v and slots are required");
+  if (r->dtype != GS_DTYPE_F32 && r->dtype != GS_DTYPE_BF16) return kfail(c, GS_EINVAL, "k and v must be float32 or bfloat16");
+  if (r->tokens > (1ll << 30)) return kfail(c, GS_EUNSUPPORTED, "at most 2^30 tokens per call");
+  const int64_t e = r->dtype == GS_DTYPE_F32 ? 4 : 2;
+  const int64_t st[4] = {r->k_token_stride, r->k_head_stride, r->v_token_stride, r->v_head_stride};
+  if (!write) {
+    const int64_t D = c->d.head_dim;
+    if ((c->d.kv_heads > 1 && (st[1] < D || st[3] < D)) || (r->tokens > 1 && (st[0] < D || st[2] < D)))
+      return kfail(c, GS_EINVAL, "output strides must not make rows overlap");
+  }
+  KvRowsArgs a{};
+  a.kv = pool_of(c);
+  a.k = static_cast<unsigned char*>(r->k);
+  a.v = static_cast<unsigned char*>(r->v);
+  a.k_token = st[0], a.k_head = st[1], a.v_token = st[2], a.v_head = st[3];
+  a.slots = r->slots;
+  a.rows = r->tokens * c->d.kv_heads;
+  a.slots_end = c->d.pages * c->d.page_size;
+  a.flag = c->flag;
+  if (a.rows > 0x7fffffffll * 8) return kfail(c, GS_EUNSUPPORTED, "tokens * kv_heads is at most 2^34");
+  bool vec = reinterpret_cast<uintptr_t>(r->k) % 16 == 0 && reinterpret_cast<uintptr_t>(r->v) % 16 == 0;
+  for (int64_t s : st) vec = vec && (s * e) % 16 == 0;
+  DeviceScope scope(c->device);
+  cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  const bool bf16 = r->dtype == GS_DTYPE_BF16;
+  const cudaError_t er = c->d.head_dim == 64    ? launch_rows<64>(a, c->d.format, write, bf16, vec, cs)
+                         : c->d.head_dim == 128 ? launch_rows<128>(a, c->d.format, write, bf16, vec, cs)
+                                                : launch_rows<256>(a, c->d.format, write, bf16, vec, cs);
+  if (er != cudaSuccess) return kfail(c, GS_ECUDA, cudaGetErrorString(er));
+  return GS_OK;
+}
+
+}  // namespace
+}  // namespace gs
+
+using namespace gs;
+
+extern "C" {
+
+gs_status gs_kv_cache_create(gs_ctx* ctx, const gs_kv_cache_desc* d, gs_kv_cache** out) {
+  if (!out) return GS_EINVAL;
+  *out = nullptr;
+  if (!ctx || !d) return GS_EINVAL;
+  auto bad = [&](gs_status s, const char* m) {
+    ctx_set_error(ctx, m);
+    return s;
+  };
+  if (d->format != GS_DTYPE_BF16 && d->format != GS_DTYPE_E4M3 && d->format != GS_DTYPE_INT8)
+    return bad(GS_EINVAL, "KV cache: format must be bfloat16, e4m3 or int8");
+  if (d->head_dim != 64 && d->head_dim != 128 && d->head_dim != 256)
+    return bad(GS_EUNSUPPORTED, "KV cache: head_dim must be 64, 128 or 256");
+  int shift = 0;
+  while (shift < 9 && (1 << shift) != d->page_size) ++shift;
+  if (shift < 4 || shift > 8) return bad(GS_EUNSUPPORTED, "KV cache: page_size must be 16, 32, 64, 128 or 256");
+  if (d->pages < 1 || d->pages > 0x7fffffffll / d->page_size)
+    return bad(GS_EINVAL, "KV cache: pages must be >= 1 and pages * page_size below 2^31");
+  if (d->kv_heads < 1 || d->kv_heads > 1024) return bad(GS_EINVAL, "KV cache: kv_heads must be in [1, 1024]");
+  if (!d->k || !d->v) return bad(GS_EINVAL, "KV cache: k and v are required");
+  if (d->format != GS_DTYPE_BF16 && (!d->k_scale || !d->v_scale))
+    return bad(GS_EINVAL, "KV cache: 8-bit formats need k_scale and v_scale");
+  const int64_t e = d->format == GS_DTYPE_BF16 ? 2 : 1;
+  const int64_t strides[6] = {d->k_page_stride, d->k_head_stride, d->k_token_stride,
+                              d->v_page_stride, d->v_head_stride, d->v_token_stride};
+  for (int64_t s : strides)
+    if (s < d->head_dim || (s * e) % 16 != 0 || s >= (1ll << 36))
+      return bad(GS_EINVAL, "KV cache: strides must be at least head_dim, whole 16-byte pieces and below 2^36");
+  if (reinterpret_cast<uintptr_t>(d->k) % 16 || reinterpret_cast<uintptr_t>(d->v) % 16)
+    return bad(GS_EINVAL, "KV cache: k and v must be 16-byte aligned");
+  auto* c = new (std::nothrow) gs_kv_cache();
+  if (!c) return bad(GS_ENOMEM, "KV cache: host allocation failed");
+  c->ctx = ctx;
+  c->device = ctx_device(ctx);
+  c->d = *d;
+  c->page_shift = shift;
+  DeviceScope scope(c->device);
+  cudaError_t er = cudaMalloc(&c->flag, 4);
+  if (er == cudaSuccess) er = cudaMemset(c->flag, 0, 4);
+  if (er == cudaSuccess) er = ctx_attn_workspace(ctx, kAttnWsBytes, &c->ws);
+  if (er == cudaSuccess) er = cudaDeviceGetAttribute(&c->num_sms, cudaDevAttrMultiProcessorCount, c->device);
+  if (er != cudaSuccess) {
+    ctx_set_error(ctx, cudaGetErrorString(er));
+    cudaFree(c->flag);
+    delete c;
+    return er == cudaErrorMemoryAllocation ? GS_ENOMEM : GS_ECUDA;
+  }
+  *out = c;
+  return GS_OK;
+}
+
+gs_status gs_kv_cache_destroy(gs_kv_cache* c) {
+  if (!c) return GS_OK;
+  DeviceScope scope(c->device);
+  cudaDeviceSynchronize();
+  cudaFree(c->flag);
+  delete c;
+  return GS_OK;
+}
+
+const char* gs_kv_cache_last_error(const gs_kv_cache* c) { return c ? c->err.c_str() : ""; }
+
+gs_status gs_kv_cache_check(gs_kv_cache* c, int32_t* bits) {
+  if (!c || !bits) return GS_EINVAL;
+  DeviceScope scope(c->device);
+  int32_t f = 0;
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpy(&f, c->flag, 4, cudaMemcpyDeviceToHost);
+  if (e == cudaSuccess && f) e = cudaMemset(c->flag, 0, 4);
+  if (e != cudaSuccess) return kfail(c, GS_ECUDA, cudaGetErrorString(e));
+  *bits = f;
+  if (f & GS_KV_ERR_TIMEOUT) return kfail(c, GS_ETIMEOUT, "a bounded wait inside the attention kernel ran out");
+  if (f & GS_KV_ERR_SLOT) return kfail(c, GS_EINVAL, "a slot lies past the cache");
+  if (f & GS_KV_ERR_PAGE) return kfail(c, GS_EINVAL, "a page-table entry is outside the cache");
+  if (f & GS_KV_ERR_LENGTH) return kfail(c, GS_EINVAL, "a sequence is longer than max_q or max_kv, or outside the tokens");
+  return GS_OK;
+}
+
+gs_status gs_kv_write(gs_kv_cache* c, const gs_kv_rows* rows, void* stream) { return move_rows(c, rows, stream, true); }
+gs_status gs_kv_read(gs_kv_cache* c, const gs_kv_rows* rows, void* stream) { return move_rows(c, rows, stream, false); }
+
+gs_status gs_attention(gs_kv_cache* c, const gs_attention_args* p, void* stream) {
+  if (!c) return GS_EINVAL;
+  if (!p) return kfail(c, GS_EINVAL, "arguments are required");
+  if (p->seqs < 0 || p->tokens < 0) return kfail(c, GS_EINVAL, "seqs and tokens must be >= 0");
+  if (p->seqs == 0 || p->tokens == 0) return GS_OK;
+  if (!p->q || !p->out || !p->kv_len || !p->page_table)
+    return kfail(c, GS_EINVAL, "q, out, kv_len and page_table are required");
+  if (!p->q_start && p->tokens != p->seqs) return kfail(c, GS_EINVAL, "without q_start every sequence has one token");
+  if (p->q_heads < 1 || p->q_heads % c->d.kv_heads != 0)
+    return kfail(c, GS_EINVAL, "q_heads must be a multiple of the cache's kv_heads");
+  if (p->max_q < 1 || p->max_kv < 0) return kfail(c, GS_EINVAL, "max_q >= 1 and max_kv >= 0 are required");
+  if (!p->q_start && p->max_q != 1) return kfail(c, GS_EINVAL, "without q_start max_q is 1");
+  if (p->window < 0 || p->sinks < 0 || (p->sinks > 0 && p->window == 0))
+    return kfail(c, GS_EINVAL, "window and sinks must be >= 0, sinks only beside a window");
+  if (!std::isfinite(p->scale)) return kfail(c, GS_EINVAL, "scale must be finite");
+  if (p->page_table_cols < 0 || p->page_table_stride < p->page_table_cols ||
+      p->page_table_cols * c->d.page_size < p->max_kv)
+    return kfail(c, GS_EINVAL, "the page table must have columns for max_kv tokens");
+  if (p->page_table_cols > 0x7fffffffll || p->tokens > 0x7fffffffll)
+    return kfail(c, GS_EUNSUPPORTED, "tokens and page table columns are at most 2^31 - 1");
+  const int64_t st[4] = {p->q_token_stride, p->q_head_stride, p->out_token_stride, p->out_head_stride};
+  for (int64_t s : st)
+    if (s < c->d.head_dim || s % 8 != 0) return kfail(c, GS_EINVAL, "q and out strides must be >= head_dim and multiples of 8");
+  if (reinterpret_cast<uintptr_t>(p->q) % 16 || reinterpret_cast<uintptr_t>(p->out) % 16)
+    return kfail(c, GS_EINVAL, "q and out must be 16-byte aligned");
+  const int64_t group = p->q_heads / c->d.kv_heads;
+  const int64_t most_rows = static_cast<int64_t>(p->max_q) * group;
+  if (most_rows > (1ll << 24) || most_rows / 8 * c->d.kv_heads > 0x7fffffffll)
+    return kfail(c, GS_EUNSUPPORTED, "max_q * (q_heads / kv_heads) is at most 2^24");
+  if (p->seqs > 65535) return kfail(c, GS_EUNSUPPORTED, "at most 65535 sequences per call");
+  AttnArgs a{};
+  a.kv = pool_of(c);
+  a.q = static_cast<const __nv_bfloat16*>(p->q);
+  a.out = static_cast<__nv_bfloat16*>(p->out);
+  a.lse = p->lse;
+  a.q_start = p->q_start;
+  a.kv_len = p->kv_len;
+  a.table = p->page_table;
+  a.q_token = st[0], a.q_head = st[1], a.o_token = st[2], a.o_head = st[3];
+  a.table_stride = p->page_table_stride;
+  a.table_cols = static_cast<int32_t>(p->page_table_cols);
+  a.tokens = p->tokens;
+  a.seqs = p->seqs;
+  a.q_heads = p->q_heads;
+  a.group = static_cast<int32_t>(group);
+  a.max_q = p->max_q;
+  a.max_kv = p->max_kv;
+  // (a window that covers max_kv tokens hides nothing)
+  a.window = p->window >= p->max_kv ? 0 : p->window;
+  a.sinks = a.window ? (p->sinks < p->max_kv ? p->sinks : p->max_kv) : 0;
+  a.scale_log2 = static_cast<float>(static_cast<double>(p->scale) * 1.4426950408889634);
+  a.flag = c->flag;
+  DeviceScope scope(c->device);
+  const cudaError_t e = launch_attn_rows(c, a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return kfail(c, GS_ECUDA, cudaGetErrorString(e));
+  return GS_OK;
+}
+
+}  // extern "C"

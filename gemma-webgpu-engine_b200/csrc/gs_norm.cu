@@ -1,0 +1,330 @@
+// Residual + RMS norm with an 8-bit output (gs_rms_norm).
+//
+//   h = x + residual,  y = h · (Σh²/n + eps)^-1/2 · (offset + w),
+//   e4m3: a = max(max|y|, 2^-64) per group, code = round(y · (448 / a)), scale = a / 448.
+//
+// One pass over the data: a row's threads keep its float32 h in registers between the sum
+// of squares, the group maxima and the store, so each input is read once and each output
+// written once (bf16 -> e4m3 with residual: 7 bytes an element; HBM-bound for many rows,
+// launch latency for few).  Sums and maxima are float32; h is rounded only where it is
+// stored to residual_out.
+#include <cmath>
+
+#include "gs_device.cuh"
+#include "gs_internal.cuh"
+#include "gs_quant.cuh"
+#include "../../include/gsampler.h"
+
+namespace gs {
+namespace {
+
+struct NormArgs {
+  const void* x;
+  const void* residual;
+  const void* weight;
+  void* residual_out;
+  void* out;
+  float* out_scale;
+  float* row_sum;
+  int64_t rows;
+  int64_t ld_x, ld_residual, ld_residual_out, ld_out;
+  int32_t hidden;
+  int32_t group;   // columns per scale (hidden when one scale a row)
+  int32_t groups;  // scales per row
+  int32_t weight_bf16;
+  float eps, offset, srq_scale;
+};
+
+enum { kOutF32 = 0, kOutBf16 = 1, kOutE4m3 = 2, kOutSrq = 3 };
+
+template <int V>
+__device__ __forceinline__ void load_weight(const NormArgs& A, int col, float (&w)[V]) {
+  if (!A.weight) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) w[i] = 1.0f;
+    return;
+  }
+  if (A.weight_bf16) load_row<V, true>(static_cast<const unsigned short*>(A.weight) + col, w);
+  else load_row<V, false>(static_cast<const float*>(A.weight) + col, w);
+#pragma unroll
+  for (int i = 0; i < V; ++i) w[i] += A.offset;
+}
+
+// TPR = blockDim.x threads per row (a multiple of 32), blockDim.y rows per block; thread t
+// holds the row's V-element pieces t, t + TPR, ...  V = 8: 16-byte (bf16) or two 16-byte
+// (f32) accesses, all pointers and strides 16-byte aligned and hidden % 8 == 0; V = 1:
+// any alignment and width.
+template <bool BF16, int OUT, int V, int PIECES>
+__global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ NormArgs A) {
+  __shared__ float red[32];
+  __shared__ int redi[32];
+  extern __shared__ int gmax[];  // V = 1, several groups: [blockDim.y][groups] bits of max|y|
+  const int t = threadIdx.x, tpr = blockDim.x, warps = tpr >> 5;
+  const int wid = threadIdx.y * warps + (t >> 5), lane = t & 31;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
+  const bool live = row < A.rows;
+  using T = typename std::conditional<BF16, unsigned short, float>::type;
+  float h[PIECES][V];
+  float sq = 0.0f;
+  if (live) {
+    const T* x = static_cast<const T*>(A.x) + row * A.ld_x;
+    const T* r = A.residual ? static_cast<const T*>(A.residual) + row * A.ld_residual : nullptr;
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+      const int col = (t + p * tpr) * V;
+      if (col < A.hidden) load_row<V, BF16>(x + col, h[p]);
+    }
+    if (r) {
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) {
+        const int col = (t + p * tpr) * V;
+        if (col < A.hidden) {
+          float b[V];
+          load_row<V, BF16>(r + col, b);
+#pragma unroll
+          for (int i = 0; i < V; ++i) h[p][i] += b[i];
+        }
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+      const int col = (t + p * tpr) * V;
+      if (col < A.hidden) {
+        if (A.residual_out) store_row<V, BF16>(static_cast<T*>(A.residual_out) + row * A.ld_residual_out + col, h[p]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) sq = fmaf(h[p][i], h[p][i], sq);
+      }
+    }
+  }
+  sq = warp_sum_f(sq);
+  if (warps > 1) {
+    if (lane == 0) red[wid] = sq;
+    __syncthreads();
+    sq = 0.0f;
+    for (int w = 0; w < warps; ++w) sq += red[threadIdx.y * warps + w];
+  }
+  const float rstd = 1.0f / sqrtf(sq / static_cast<float>(A.hidden) + A.eps);
+#pragma unroll
+  for (int p = 0; p < PIECES; ++p) {
+    const int col = (t + p * tpr) * V;
+    if (col < A.hidden && live) {
+      float w[V];
+      load_weight<V>(A, col, w);
+#pragma unroll
+      for (int i = 0; i < V; ++i) h[p][i] = h[p][i] * rstd * w[i];
+    }
+  }
+  if constexpr (OUT == kOutF32 || OUT == kOutBf16) {
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+      const int col = (t + p * tpr) * V;
+      if (col < A.hidden && live) {
+        using O = typename std::conditional<OUT == kOutBf16, unsigned short, float>::type;
+        store_row<V, OUT == kOutBf16>(static_cast<O*>(A.out) + row * A.ld_out + col, h[p]);
+      }
+    }
+  } else if constexpr (OUT == kOutSrq) {
+    int qs = 0;
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+      const int col = (t + p * tpr) * V;
+      if (col < A.hidden && live) {
+        float o[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float q = fminf(fmaxf(rintf(__fdiv_rn(h[p][i], A.srq_scale)), -128.0f), 127.0f);
+          qs += static_cast<int>(q);
+          o[i] = __fmul_rn(q, A.srq_scale);
+        }
+        store_row<V, false>(static_cast<float*>(A.out) + row * A.ld_out + col, o);
+      }
+    }
+    qs = warp_sum_i(qs);
+    if (warps > 1) {
+      if (lane == 0) redi[wid] = qs;
+      __syncthreads();
+      qs = 0;
+      for (int w = 0; w < warps; ++w) qs += redi[threadIdx.y * warps + w];
+    }
+    if (t == 0 && live && A.row_sum) A.row_sum[row] = __fmul_rn(static_cast<float>(qs), A.srq_scale);
+  } else {
+    // max|y| as the bits of a non-negative float: integer order is value order, NaN above all
+    unsigned char* out = static_cast<unsigned char*>(A.out) + row * A.ld_out;
+    float* scales = A.out_scale + row * A.groups;
+    int gm[PIECES];
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+      gm[p] = 0;
+      const int col = (t + p * tpr) * V;
+      if (col < A.hidden && live)
+#pragma unroll
+        for (int i = 0; i < V; ++i) gm[p] = max(gm[p], __float_as_int(h[p][i]) & 0x7fffffff);
+    }
+    if (A.groups == 1) {
+      int m = 0;
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) m = max(m, gm[p]);
+      m = __reduce_max_sync(kFullMask, m);
+      if (warps > 1) {
+        if (lane == 0) redi[wid] = m;
+        __syncthreads();
+        m = 0;
+        for (int w = 0; w < warps; ++w) m = max(m, redi[threadIdx.y * warps + w]);
+      }
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) gm[p] = m;
+      if (t == 0 && live) scales[0] = quant_scale(__int_as_float(m), kE4m3Max);
+    } else if (V == 8) {
+      // a group is group / 8 consecutive pieces, so as many neighbouring lanes (4, 8 or 16)
+      const int span = A.group >> 3;
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) {
+        for (int o = span >> 1; o > 0; o >>= 1) gm[p] = max(gm[p], __shfl_xor_sync(kFullMask, gm[p], o));
+        const int col = (t + p * tpr) * V;
+        if (col < A.hidden && live && (lane & (span - 1)) == 0)
+          scales[col / A.group] = quant_scale(__int_as_float(gm[p]), kE4m3Max);
+      }
+    } else {
+      int* gr = gmax + threadIdx.y * A.groups;
+      for (int g = t; g < A.groups; g += tpr) gr[g] = 0;
+      __syncthreads();
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) {
+        const int col = (t + p * tpr) * V;
+        if (col < A.hidden && live) atomicMax(gr + col / A.group, gm[p]);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p) {
+        const int col = (t + p * tpr) * V;
+        if (col < A.hidden && live) gm[p] = gr[col / A.group];
+      }
+      if (live)
+        for (int g = t; g < A.groups; g += tpr) scales[g] = quant_scale(__int_as_float(gr[g]), kE4m3Max);
+    }
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p) {
+      const int col = (t + p * tpr) * V;
+      if (col < A.hidden && live) {
+        const float inv = quant_inv(__int_as_float(gm[p]), kE4m3Max);
+        if constexpr (V == 8) {
+          uint2 c;
+          c.x = e4m3x4(h[p][0] * inv, h[p][1] * inv, h[p][2] * inv, h[p][3] * inv);
+          c.y = e4m3x4(h[p][4] * inv, h[p][5] * inv, h[p][6] * inv, h[p][7] * inv);
+          *reinterpret_cast<uint2*>(out + col) = c;
+        } else {
+          out[col] = static_cast<unsigned char>(e4m3x2(h[p][0] * inv, 0.0f) & 0xffu);
+        }
+      }
+    }
+  }
+}
+
+template <bool BF16, int OUT, int V>
+cudaError_t launch_norm_v(const NormArgs& a, cudaStream_t st) {
+  // One warp per row while its pieces fit 4 a lane; wider rows take more threads at 2 or 4
+  // pieces each.  256-thread blocks then hold several rows.
+  const int pieces = (a.hidden + V - 1) / V;
+  constexpr int kMost = V == 8 ? 4 : 32;
+  int tpr = 32;
+  const int want = V == 8 ? (a.rows <= 296 ? 1 : 2) : 4;
+  while (tpr < 1024 && tpr * want < pieces) tpr <<= 1;
+  const int rpb = tpr >= 256 ? 1 : 256 / tpr;
+  const int per = (pieces + tpr - 1) / tpr;
+  const dim3 block(tpr, rpb);
+  const unsigned grid = static_cast<unsigned>((a.rows + rpb - 1) / rpb);
+  const size_t smem = (OUT == kOutE4m3 && V == 1 && a.groups > 1) ? sizeof(int) * rpb * a.groups : 0;
+  if (per <= 1) norm_kernel<BF16, OUT, V, 1><<<grid, block, smem, st>>>(a);
+  else if (per <= 2) norm_kernel<BF16, OUT, V, 2><<<grid, block, smem, st>>>(a);
+  else if (per <= 4) norm_kernel<BF16, OUT, V, 4><<<grid, block, smem, st>>>(a);
+  else norm_kernel<BF16, OUT, V, kMost><<<grid, block, smem, st>>>(a);
+  return cudaGetLastError();
+}
+
+template <bool BF16, int OUT>
+cudaError_t launch_norm_o(const NormArgs& a, bool vec, cudaStream_t st) {
+  return vec ? launch_norm_v<BF16, OUT, 8>(a, st) : launch_norm_v<BF16, OUT, 1>(a, st);
+}
+
+template <bool BF16>
+cudaError_t launch_norm(const NormArgs& a, int out, bool vec, cudaStream_t st) {
+  switch (out) {
+    case kOutF32: return launch_norm_o<BF16, kOutF32>(a, vec, st);
+    case kOutBf16: return launch_norm_o<BF16, kOutBf16>(a, vec, st);
+    case kOutE4m3: return launch_norm_o<BF16, kOutE4m3>(a, vec, st);
+    default: return launch_norm_o<BF16, kOutSrq>(a, vec, st);
+  }
+}
+
+gs_status nfail(gs_ctx* c, gs_status s, const char* m) {
+  ctx_set_error(c, m);
+  return s;
+}
+
+}  // namespace
+}  // namespace gs
+
+using namespace gs;
+
+extern "C" gs_status gs_rms_norm(gs_ctx* ctx, const gs_rms_norm_args* p, void* stream) {
+  if (!ctx || !p) return GS_EINVAL;
+  if (p->rows < 0 || p->hidden <= 0) return nfail(ctx, GS_EINVAL, "RMS norm: rows >= 0 and hidden >= 1 are required");
+  if (p->hidden > GS_MAX_NORM_HIDDEN) return nfail(ctx, GS_EUNSUPPORTED, "RMS norm: hidden is at most 32768");
+  if (p->rows == 0) return GS_OK;
+  if (p->rows > 0x7fffffffll) return nfail(ctx, GS_EUNSUPPORTED, "RMS norm: at most 2^31 - 1 rows");
+  const bool in_ok = (p->dtype == GS_DTYPE_F32 || p->dtype == GS_DTYPE_BF16) &&
+                     (!p->weight || p->weight_dtype == GS_DTYPE_F32 || p->weight_dtype == GS_DTYPE_BF16);
+  if (!in_ok || (p->out_dtype != GS_DTYPE_F32 && p->out_dtype != GS_DTYPE_BF16 && p->out_dtype != GS_DTYPE_E4M3))
+    return nfail(ctx, GS_EINVAL, "RMS norm: float32 or bfloat16 inputs and float32, bfloat16 or e4m3 output");
+  if (!p->x || !p->out) return nfail(ctx, GS_EINVAL, "RMS norm: x and out are required");
+  if (p->ld_x < p->hidden || p->ld_out < p->hidden || (p->residual && p->ld_residual < p->hidden) ||
+      (p->residual_out && p->ld_residual_out < p->hidden))
+    return nfail(ctx, GS_EINVAL, "RMS norm: row strides must be at least hidden");
+  if (!(p->eps >= 0.0f) || !std::isfinite(p->eps) || !std::isfinite(p->weight_offset) || !(p->srq_scale >= 0.0f) ||
+      !std::isfinite(p->srq_scale))
+    return nfail(ctx, GS_EINVAL, "RMS norm: eps and srq_scale must be finite and >= 0, weight_offset finite");
+  if (p->srq_scale != 0.0f && p->out_dtype != GS_DTYPE_F32)
+    return nfail(ctx, GS_EINVAL, "RMS norm: srq_scale goes with a float32 output");
+  if (p->group != 0 && p->group != 32 && p->group != 64 && p->group != 128)
+    return nfail(ctx, GS_EINVAL, "RMS norm: group must be 0, 32, 64 or 128");
+  if (p->out_dtype == GS_DTYPE_E4M3 && !p->out_scale) return nfail(ctx, GS_EINVAL, "RMS norm: out_scale is required");
+  if (p->out_dtype != GS_DTYPE_E4M3 && p->group != 0)
+    return nfail(ctx, GS_EINVAL, "RMS norm: groups go with an e4m3 output");
+  NormArgs a{};
+  a.x = p->x;
+  a.residual = p->residual;
+  a.weight = p->weight;
+  a.residual_out = p->residual_out;
+  a.out = p->out;
+  a.out_scale = p->out_scale;
+  a.row_sum = p->row_sum;
+  a.rows = p->rows;
+  a.ld_x = p->ld_x;
+  a.ld_residual = p->ld_residual;
+  a.ld_residual_out = p->ld_residual_out;
+  a.ld_out = p->ld_out;
+  a.hidden = static_cast<int32_t>(p->hidden);
+  a.group = p->group ? p->group : a.hidden;
+  a.groups = (a.hidden + a.group - 1) / a.group;
+  a.weight_bf16 = p->weight_dtype == GS_DTYPE_BF16;
+  a.eps = p->eps;
+  a.offset = p->weight_offset;
+  a.srq_scale = p->srq_scale;
+  // 16-byte accesses need every row to start on 16 bytes (8 for codes) and whole pieces
+  auto fits = [&](const void* ptr, int64_t ld, int dtype) {
+    if (!ptr) return true;
+    const int64_t e = dtype == GS_DTYPE_F32 ? 4 : dtype == GS_DTYPE_BF16 ? 2 : 1;
+    const uintptr_t al = dtype == GS_DTYPE_E4M3 ? 8 : 16;
+    return reinterpret_cast<uintptr_t>(ptr) % al == 0 && (p->rows == 1 || (ld * e) % static_cast<int64_t>(al) == 0);
+  };
+  const bool vec = p->hidden % 8 == 0 && fits(p->x, p->ld_x, p->dtype) && fits(p->residual, p->ld_residual, p->dtype) &&
+                   fits(p->residual_out, p->ld_residual_out, p->dtype) && fits(p->out, p->ld_out, p->out_dtype) &&
+                   fits(p->weight, p->hidden, p->weight_dtype);
+  const int out = p->srq_scale != 0.0f ? kOutSrq : p->out_dtype == GS_DTYPE_E4M3 ? kOutE4m3
+                  : p->out_dtype == GS_DTYPE_BF16 ? kOutBf16 : kOutF32;
+  DeviceScope scope(ctx_device(ctx));
+  const cudaError_t e = p->dtype == GS_DTYPE_BF16 ? launch_norm<true>(a, out, vec, static_cast<cudaStream_t>(stream))
+                                                  : launch_norm<false>(a, out, vec, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return nfail(ctx, GS_ECUDA, cudaGetErrorString(e));
+  return GS_OK;
+}

@@ -37,6 +37,9 @@ typedef enum gs_status {
 } gs_status;
 
 enum { GS_DTYPE_F32 = 0, GS_DTYPE_BF16 = 1 };
+/* 8-bit types, with float32 scales beside the codes: e4m3 (largest code 448) and int8
+ * (largest code 127).  Outputs of gs_rms_norm (e4m3) and formats of a key/value cache. */
+enum { GS_DTYPE_E4M3 = 2, GS_DTYPE_INT8 = 3 };
 
 /* Per-row flags written to gs_outputs.flags. */
 enum {
@@ -299,6 +302,125 @@ int64_t gs_lm_head_fused_calls(const gs_lm_head* h);
 #define GS_LM_ROUTE_FUSED 1
 #define GS_LM_ROUTE_TWO_STEP 2
 gs_status gs_lm_head_set_route(gs_lm_head* h, int32_t route);
+
+/* ---- Residual + RMS norm with an 8-bit output: the pass before a product ----
+ * Per row, in float32:  h = x + residual;  y = h · (mean(h²) + eps)^-1/2 · (weight_offset + weight)
+ * h goes to residual_out rounded to `dtype` (y is formed from the unrounded h).  out is
+ *   GS_DTYPE_F32 / GS_DTYPE_BF16   y, rounded once; with srq_scale != 0 (GS_DTYPE_F32 only)
+ *                 y on the grid of srq(y, srq_scale) = clamp(rint(y / srq_scale), -128, 127) ·
+ *                 srq_scale, and row_sum[row] = srq_scale · Σ codes: the activation and
+ *                 activation_sum that gs_lm_head_logits / gs_lm_head_sample read
+ *                 (src/webgpu/decode-ple-proj-norm-codes.ts:251-258 is the reference's
+ *                 producing pass);
+ *   GS_DTYPE_E4M3 codes round(y · (448 / a)) and out_scale = a / 448, a = max(max|y|, 2^-64)
+ *                 over each group of `group` columns (0: the whole row; the last group of
+ *                 a row may be short).  out_scale is [rows][ceil(hidden / group)].
+ * A NaN or infinity in a row makes that row's mean, and so its y, NaN (or 0 where h is
+ * finite and the mean infinite), as the formula does; its scales follow. */
+typedef struct gs_rms_norm_args {
+  const void* x;            /* device [rows][ld_x] of `dtype` */
+  const void* residual;     /* device [rows][ld_residual] of `dtype`, or NULL (h = x) */
+  const void* weight;       /* device [hidden] of weight_dtype, or NULL (y = h · rstd) */
+  void* residual_out;       /* device [rows][ld_residual_out] of `dtype`, or NULL; may be x or residual itself */
+  void* out;                /* device [rows][ld_out] of out_dtype */
+  float* out_scale;         /* device, GS_DTYPE_E4M3 only */
+  float* row_sum;           /* device [rows], srq_scale != 0 only */
+  int64_t rows, hidden;     /* hidden <= GS_MAX_NORM_HIDDEN */
+  int64_t ld_x, ld_residual, ld_residual_out, ld_out; /* elements between rows, >= hidden */
+  int32_t dtype;            /* GS_DTYPE_F32 / GS_DTYPE_BF16 */
+  int32_t weight_dtype;     /* GS_DTYPE_F32 / GS_DTYPE_BF16 */
+  int32_t out_dtype;        /* GS_DTYPE_F32 / GS_DTYPE_BF16 / GS_DTYPE_E4M3 */
+  int32_t group;            /* 0, 32, 64 or 128 */
+  float eps, weight_offset, srq_scale;
+} gs_rms_norm_args;
+#define GS_MAX_NORM_HIDDEN 32768
+/* Asynchronous on `stream`; allocates nothing. */
+gs_status gs_rms_norm(gs_ctx* ctx, const gs_rms_norm_args* args, void* stream);
+
+/* ---- Paged key/value cache, quantised as it is written, and attention over it ----
+ * (No entry of its own in the reference's sampling path: this is the state of the decode
+ * step whose logits are sampled.)  The caller owns the memory: `pages` pages of page_size
+ * tokens, each [kv_heads][page_size][head_dim] by default (any strides whose rows of
+ * head_dim are contiguous and 16-byte aligned), and for 8-bit formats one float32 scale
+ * per page, head and token, contiguous [pages][kv_heads][page_size].  A slot is
+ * page · page_size + offset. */
+typedef struct gs_kv_cache_desc {
+  void* k;                  /* device */
+  void* v;
+  float* k_scale;           /* device, 8-bit formats only */
+  float* v_scale;
+  int64_t pages;            /* pages * page_size < 2^31 */
+  int32_t page_size;        /* 16, 32, 64, 128 or 256 */
+  int32_t kv_heads;         /* 1 .. 1024 */
+  int32_t head_dim;         /* 64, 128 or 256 */
+  int32_t format;           /* GS_DTYPE_BF16, GS_DTYPE_E4M3 or GS_DTYPE_INT8 */
+  int64_t k_page_stride, k_head_stride, k_token_stride; /* elements */
+  int64_t v_page_stride, v_head_stride, v_token_stride;
+} gs_kv_cache_desc;
+typedef struct gs_kv_cache gs_kv_cache;
+
+/* Binds a handle to the memory (which it neither reads nor clears here).  The first handle
+ * of a context allocates the workspace of its attention calls; no later call allocates. */
+gs_status gs_kv_cache_create(gs_ctx* ctx, const gs_kv_cache_desc* desc, gs_kv_cache** out);
+gs_status gs_kv_cache_destroy(gs_kv_cache* c);
+const char* gs_kv_cache_last_error(const gs_kv_cache* c);
+/* Errors that the kernels found in device data since the last check (synchronising):
+ * a slot past the cache (skipped), a page-table entry outside [0, pages) or past the
+ * table's columns (its tokens read as zeros), a sequence longer than max_q / max_kv (cut
+ * off).  GS_EINVAL when any bit is set; GS_ETIMEOUT when a bounded wait ran out. */
+#define GS_KV_ERR_SLOT 1
+#define GS_KV_ERR_PAGE 2
+#define GS_KV_ERR_LENGTH 4
+#define GS_KV_ERR_TIMEOUT 8
+gs_status gs_kv_cache_check(gs_kv_cache* c, int32_t* bits);
+
+/* New keys and values into the cache: for token t, head h, the row x of head_dim values
+ * (float32 or bfloat16, contiguous) is stored at slots[t] as bf16, or as codes
+ * round(x · (M / a)) with the scale a / M, a = max(max|x|, 2^-64), M = 448 (e4m3) or 127
+ * (int8).  A negative slot is skipped (padding); slots must not repeat within a call. */
+typedef struct gs_kv_rows {
+  void* k;                  /* device [tokens][kv_heads][head_dim] by the strides below */
+  void* v;
+  int64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride; /* elements */
+  const int32_t* slots;     /* device [tokens] */
+  int64_t tokens;
+  int32_t dtype;            /* GS_DTYPE_F32 / GS_DTYPE_BF16 */
+} gs_kv_rows;
+gs_status gs_kv_write(gs_kv_cache* c, const gs_kv_rows* rows, void* stream);
+/* The rows at slots[t] read back (code · scale, rounded once); zeros for a negative slot. */
+gs_status gs_kv_read(gs_kv_cache* c, const gs_kv_rows* rows, void* stream);
+
+/* Attention of new tokens over the cache.  Sequence b has the new tokens
+ * [q_start[b], q_start[b + 1]) of q (q_start NULL: one token each, token b) and kv_len[b]
+ * tokens in the cache, the new ones included and last: new token i stands at position
+ * p = kv_len - n + i and sees cached token j when j <= p and (window == 0, or
+ * j > p - window, or j < sinks).  Cached token j of sequence b is at page
+ * page_table[b · page_table_stride + j / page_size].  Query head g reads key/value head
+ * g / (q_heads / kv_heads).  Per row, with s_j = scale · q·k_j over the tokens it sees:
+ *   lse = log Σ e^(s_j),  out = Σ e^(s_j - lse) v_j
+ * rounded once to bf16.  A row that sees nothing gives out 0 and lse -inf.  What no row of
+ * a call sees (tokens past kv_len, before every window) is not read.
+ * Scores, maxima, sums and the accumulated output are float32; a row's weights
+ * e^(s_j - running max), times the value's scale, are rounded to bf16 (float16 beside an
+ * 8-bit cache in the few-row kernel) for the second product.
+ * The calls of one context use its workspace: order them on the GPU (one stream, or
+ * events between streams), as for gs_sample. */
+typedef struct gs_attention_args {
+  const void* q;            /* device bf16 [tokens][q_heads][head_dim] by the strides below */
+  void* out;                /* device bf16, same shape */
+  float* lse;               /* device [tokens][q_heads], or NULL */
+  const int32_t* q_start;   /* device [seqs + 1], or NULL (tokens == seqs, one each) */
+  const int32_t* kv_len;    /* device [seqs] */
+  const int32_t* page_table;/* device [seqs][page_table_stride] */
+  int64_t tokens, q_token_stride, q_head_stride, out_token_stride, out_head_stride; /* elements */
+  int64_t page_table_stride, page_table_cols;
+  int32_t seqs, q_heads;
+  int32_t max_q;            /* bound on a sequence's new tokens (host knowledge: it sizes the launch) */
+  int32_t max_kv;           /* bound on kv_len */
+  int32_t window, sinks;    /* 0: no window.  sinks only beside a window */
+  float scale;
+} gs_attention_args;
+gs_status gs_attention(gs_kv_cache* c, const gs_attention_args* args, void* stream);
 
 /* Elementwise soft cap, the same routine the sampling pass applies (no reference
  * counterpart: the reference never applies its declared cap). */

@@ -1,0 +1,230 @@
+"""GpuKvCache.attend against the formula in float64, over masks, layouts and lengths."""
+import pytest
+import torch
+
+import operator_refs as R
+
+pytestmark = pytest.mark.gpu
+
+
+class Case:
+    def __init__(self, sampler, pkg, lens, heads, group, dim, page, form, seed=0, poison=None, layout="hnd", window=0,
+                 sinks=0):
+        """lens: (new tokens, cached tokens) per sequence.  poison: every cached value and scale
+        that no row of its sequence may read."""
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        need = [-(-n // page) for _, n in lens]
+        pages = max(1, sum(need)) + 1
+        k, v, ks, vs = R.make_pool(gen, pages, heads, page, dim, form, "cuda")
+        order = torch.randperm(pages, generator=gen, device="cuda").to(torch.int32)
+        cols = max(1, max(need)) + 1
+        self.table = torch.full((len(lens), cols), -1, dtype=torch.int32, device="cuda")
+        at = 0
+        for i, n in enumerate(need):
+            self.table[i, :n] = order[at:at + n]
+            at += n
+        self.max_kv = max(1, max(n for _, n in lens))
+        if poison is not None:
+            seen = torch.zeros((pages, page), dtype=torch.bool, device="cuda")
+            for b, (nq, n) in enumerate(lens):
+                lo = max(0, n - nq - window + 1) if window else 0
+                for j in range(n):
+                    if (j >= lo or j < sinks) and nq > 0:
+                        seen[self.table[b, j // page].long(), j % page] = True
+            hide = ~seen[:, None, :, None].expand_as(k)
+            if form == "bf16":
+                k.masked_fill_(hide, poison)
+                v.masked_fill_(hide, poison)
+            else:
+                code = 0x7f if form == "e4m3" else 0x80
+                k.view(torch.uint8).masked_fill_(hide, code)
+                v.view(torch.uint8).masked_fill_(hide, code)
+                ks.masked_fill_(hide[..., 0], poison)
+                vs.masked_fill_(hide[..., 0], poison)
+        if layout == "nhd":  # token-major pages
+            k, v = (t.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3) for t in (k, v))
+        self.kd, self.vd = R.pool_values(k, ks), R.pool_values(v, vs)
+        self.cache = pkg.GpuKvCache(sampler, k, v, ks, vs)
+        starts = [0]
+        for nq, _ in lens:
+            starts.append(starts[-1] + nq)
+        self.starts, self.lens, self.page = starts, lens, page
+        self.q_start = torch.tensor(starts, dtype=torch.int32, device="cuda")
+        self.kv_len = torch.tensor([n for _, n in lens], dtype=torch.int32, device="cuda")
+        self.q = (1.5 * torch.randn((starts[-1], heads * group, dim), generator=gen, device="cuda")).to(torch.bfloat16)
+        self.scale = dim ** -0.5
+        self.window, self.sinks = window, sinks
+        self.max_q = max(1, max(nq for nq, _ in lens))
+
+    def run(self, **kw):
+        a = dict(max_q=self.max_q, max_kv=self.max_kv, scale=self.scale, window=self.window, sinks=self.sinks, lse=True)
+        a.update(kw)
+        out, lse = self.cache.attend(self.q, self.q_start, self.kv_len, self.table, **a)
+        torch.cuda.synchronize()
+        self.cache.check()
+        return out, lse
+
+    def reference(self):
+        return R.attend(self.q, self.starts, [n for _, n in self.lens], self.table, self.kd, self.vd, self.page,
+                        self.scale, self.window, self.sinks)
+
+    def check(self, what="", **kw):
+        out, lse = self.run(**kw)
+        R.check_attend(out, lse, self.reference(), what)
+        return out, lse
+
+
+FORMS = ["bf16", "e4m3", "int8"]
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("group", [1, 3, 8, 16])
+def test_single_tokens(pkg, sampler, form, dim, group):
+    lens = [(1, 1), (1, 2), (1, 15), (1, 16), (1, 17), (1, 63), (1, 65), (1, 200)]
+    Case(sampler, pkg, lens, 2, group, dim, 16, form, seed=dim + group, poison=float("nan")).check()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lens", [[(5, 5), (2, 70), (1, 33), (7, 129)], [(40, 40), (33, 300)], [(130, 131), (1, 400)],
+                                  [(257, 600)]])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (20, 3), (1, 0)])
+def test_chunks(pkg, sampler, form, dim, lens, window, sinks):
+    Case(sampler, pkg, lens, 2, 3, dim, 32, form, seed=dim, poison=float("nan"), window=window, sinks=sinks).check()
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("layout", ["hnd", "nhd"])
+@pytest.mark.parametrize("lens", [[(1, 300), (1, 257)], [(100, 300), (30, 257)]])
+def test_pages_and_layouts(pkg, sampler, page, layout, lens):
+    for form in ("bf16", "int8"):
+        Case(sampler, pkg, lens, 3, 2, 128, page, form, layout=layout, poison=float("inf"), window=90, sinks=5).check()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("many", [False, True])
+def test_rows_that_see_nothing(pkg, sampler, form, many):
+    """No cached tokens; more new tokens than cached ones (the first rows stand before position 0);
+    no new tokens."""
+    n = 60 if many else 4
+    lens = [(1, 0), (n, 0), (n, 2), (0, 20), (n, n + 1)]
+    c = Case(sampler, pkg, lens, 2, 4, 64, 16, form, poison=float("nan"))
+    out, lse = c.check()
+    assert (out[:1 + n] == 0).all() and torch.isinf(lse[:1 + n]).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("lens,window,sinks", [([(1, 5000)], 0, 0), ([(1, 4100), (1, 3)], 0, 0), ([(3, 5000)], 3000, 4),
+                                               ([(20, 2500)], 0, 0)])
+def test_split_context(pkg, sampler, form, lens, window, sinks):
+    """Few rows and a long context: the context is split over blocks and joined."""
+    Case(sampler, pkg, lens, 1, 2, 128, 64, form, poison=float("nan"), window=window, sinks=sinks).check()
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_large_scores_and_spread_scales(pkg, sampler, form):
+    """Scores far apart (one token takes nearly all the weight, late in the context), and cached
+    rows whose scales differ by orders of magnitude."""
+    c = Case(sampler, pkg, [(1, 500), (3, 300)], 2, 4, 128, 16, form, seed=3)
+    c.scale = 1.0
+    if form != "bf16":
+        f = torch.exp2(torch.randint(-12, 5, c.cache.v_scale.shape, device="cuda").float())
+        c.cache.v_scale.mul_(f)
+        c.vd = R.pool_values(c.cache.v, c.cache.v_scale)
+    c.check()
+
+
+@pytest.mark.parametrize("lens", [[(1, 40), (1, 7)], [(70, 140), (9, 9)]])
+def test_strided_query_and_output(pkg, sampler, lens):
+    c = Case(sampler, pkg, lens, 2, 2, 64, 16, "bf16")
+    want, _ = c.check()
+    tokens = c.q.shape[0]
+    wide = torch.zeros((tokens, 9, 64), dtype=torch.bfloat16, device="cuda")
+    wide[:, 1:8:2][:, :4] = c.q
+    c.q = wide[:, 1:8:2]
+    buf = torch.full((tokens, 4, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+    out, _ = c.run(out=buf[:, :, 64:])
+    assert torch.equal(out, want) and (buf[:, :, :64] == 7).all()
+
+
+def test_decode_form_without_starts(pkg, sampler):
+    c = Case(sampler, pkg, [(1, 90), (1, 20), (1, 0)], 2, 4, 128, 16, "e4m3")
+    want, want_lse = c.check()
+    out, lse = c.cache.attend(c.q, None, c.kv_len, c.table, max_kv=c.max_kv, scale=c.scale, lse=True)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("lens", [[(1, 700), (1, 33)], [(90, 700), (33, 33)]])
+def test_same_bits_every_time_on_another_stream_and_in_a_graph(pkg, sampler, lens):
+    c = Case(sampler, pkg, lens, 2, 4, 128, 16, "bf16")
+    want, want_lse = c.run()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        out, lse = c.cache.attend(c.q, c.q_start, c.kv_len, c.table, max_q=c.max_q, max_kv=c.max_kv, scale=c.scale, lse=True)
+    s.synchronize()
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    graph = torch.cuda.CUDAGraph()
+    out.zero_()
+    with torch.cuda.graph(graph):
+        c.cache.attend(c.q, c.q_start, c.kv_len, c.table, max_q=c.max_q, max_kv=c.max_kv, scale=c.scale, out=out, lse_out=lse)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+def test_gradient_of_lse_is_the_attention_output(pkg, sampler):
+    """d lse / d q = scale · Σ p k: with values equal to the keys the output is that gradient
+    over scale; checked against central differences of the kernel's own lse."""
+    c = Case(sampler, pkg, [(1, 50)], 1, 1, 64, 16, "bf16", seed=9)
+    c.cache.v.copy_(c.cache.k)
+    out, _ = c.run()
+    base = c.q.clone()
+    step = 0.25  # exact in bf16 next to the rounded q below
+    base = (base * 4).round() / 4
+    c.q = base
+    out, _ = c.run()
+    grad = []
+    for i in range(0, 64, 7):
+        f = []
+        for sgn in (1, -1):
+            c.q = base.clone()
+            c.q[0, 0, i] += sgn * step
+            f.append(c.run()[1].double().item())
+        grad.append((f[0] - f[1]) / (2 * step))
+    got = out.double()[0, 0, ::7] * c.scale
+    # third derivative of lse along one axis <= scale^3 · max|k|^3 · 2, times step^2 / 6
+    kmax = c.kd.abs().max().item()
+    tol = 2 * (c.scale * kmax) ** 3 * step ** 2 / 6 + 1e-4 / step + 2.0 ** -8 * c.scale * kmax
+    assert (got - torch.tensor(grad, device="cuda", dtype=torch.float64)).abs().max().item() <= tol
+
+
+def test_bad_table_and_lengths_are_reported(pkg, sampler):
+    c = Case(sampler, pkg, [(1, 100), (1, 40)], 1, 2, 64, 16, "bf16")
+    good, _ = c.run()
+    kept = c.table.clone()
+    c.table[1, 1] = 10 ** 6
+    out, _ = c.cache.attend(c.q, c.q_start, c.kv_len, c.table, max_kv=c.max_kv, scale=c.scale)
+    with pytest.raises(ValueError, match="page"):
+        c.cache.check()
+    assert torch.equal(out[0], good[0])
+    c.cache.check()
+    c.table.copy_(kept)
+    c.kv_len[0] = 5000
+    c.cache.attend(c.q, c.q_start, c.kv_len, c.table, max_kv=c.max_kv, scale=c.scale)
+    with pytest.raises(ValueError, match="longer"):
+        c.cache.check()
+
+
+def test_refusals(pkg, sampler):
+    c = Case(sampler, pkg, [(1, 30), (1, 30)], 2, 2, 64, 16, "bf16")
+    ok = dict(q=c.q, q_start=c.q_start, kv_len=c.kv_len, page_table=c.table, max_kv=30, scale=0.1)
+    bad = [dict(q=c.q.float()), dict(q=c.q[..., :32]), dict(q=c.q[:, :3]), dict(q_start=c.q_start[:2]),
+           dict(kv_len=c.kv_len.long()), dict(page_table=c.table[:1]), dict(max_kv=10 ** 6), dict(max_kv=-1),
+           dict(window=-1), dict(sinks=3), dict(scale=float("nan")), dict(max_q=0), dict(q=c.q[:1], q_start=None),
+           dict(out=c.q.float()), dict(lse_out=torch.zeros((2, 3), device="cuda")),
+           dict(q=c.q.cpu()), dict(kv_len=c.kv_len.cpu())]
+    for change in bad:
+        with pytest.raises(ValueError):
+            c.cache.attend(**{**ok, **change})
+    c.cache.attend(**ok)
