@@ -15,6 +15,7 @@ struct gs_kv_cache {
   int page_shift = 0;
   int32_t* flag = nullptr;       // device: GS_KV_ERR_* bits
   unsigned char* ws = nullptr;   // the context's attention workspace (kAttnWsBytes)
+  alignas(64) unsigned char maps[256] = {};  // tensor maps of a bf16 cache's pools
   std::string err;
 };
 
@@ -121,6 +122,10 @@ __device__ __forceinline__ float ex2(float x) { return ex2_approx(x); }
 
 // Few-row kernel (mma.sync, one 16-token tile per warp): any number of rows in blocks.
 cudaError_t launch_attn_rows(const gs_kv_cache* c, AttnArgs a, cudaStream_t st);
+// Many-row kernel (tcgen05), and the tensor maps it reads a bf16 cache by (an error text, or
+// nullptr).
+cudaError_t launch_attn_tile(const gs_kv_cache* c, AttnArgs a, cudaStream_t st);
+const char* make_attn_maps(gs_kv_cache* c);
 // Joins the partial results of a split context.  rows_per_block and tile as in the kernel
 // that wrote them.
 cudaError_t launch_attn_join(const AttnArgs& a, int head_dim, int rows_per_block, int row_blocks, int tile, cudaStream_t st);

@@ -1,0 +1,728 @@
+// Attention of many query rows over the paged cache (prompt chunks) on the tcgen05 tensor cores.
+//
+// A block owns kTileRows query rows of one key/value head (new tokens × heads of the group,
+// so the group shares every cached byte) and walks its context in tiles of 128 tokens:
+//   S = Q K^T (128 x 128, float32 in tensor memory), weights P = 2^(c S - c m) in bf16 written
+//   over S, O += P V (A operand from tensor memory), one row per softmax thread, so that the
+//   row's maximum and sum need no shuffles.
+// The reference point m is moved only when a tile's maximum passes it by 2^8: float32 sums and
+// bf16 weights hold 2^8 as well as 1, and rescaling O (128 x D in tensor memory) then happens a
+// few times a row instead of once a tile.
+//
+// Bound: 4 D multiply-adds a score at 4096 a clock and SM, against one 2^x a score at 16 a
+// clock: at D = 128 both take 1024 clocks per 128 x 128 tile, so two query tiles take turns
+// (D <= 128): one tile's products run under the other's softmax.  At D = 256 the products take twice
+// as long as the softmax and the output alone fills half of tensor memory: one query tile, two
+// score buffers.
+//
+// Tensor memory (512 columns): S0 at 0, S1 at 128, O0 at 256, O1 at 256 + D.
+// Warps: softmax warpgroup(s) first (warp % 4 = its tensor-memory lanes), then the MMA issuer,
+// then the loaders: one warp issuing TMA boxes (bf16 pages go straight to the swizzled operand
+// layout) or four warps widening 8-bit codes to bf16 (exact) into the same layout, scales beside
+// them (K's multiplies the score, V's the weight before it is rounded).
+// Order of products and of shared-memory stages: K(0) .. K(SB-1), then V(j), K(j + SB) for each j:
+// P(j) overlays S(j), and the tensor core takes one thread's products in order, so S(j + SB) is
+// issued right behind the product that reads P(j).
+// Every wait is bounded (1 s); a wait that runs out sets GS_KV_ERR_TIMEOUT, ends the block's loops,
+// waits (bounded) for copies and products in flight and frees tensor memory.
+#include <cuda.h>
+
+#include "gs_attn.cuh"
+
+namespace gs {
+namespace {
+
+constexpr int kTT = 128;  // context tokens per tile
+
+template <int D, int FMT>
+struct TilePlan {
+  static constexpr bool kBf = FMT == GS_DTYPE_BF16;
+  static constexpr int NQ = D == 256 ? 1 : 2;   // query tiles of 128 rows
+  static constexpr int SB = D == 256 ? 2 : 1;   // score buffers per query tile
+  static constexpr int kRows = 128 * NQ;
+  static constexpr int kPer = D == 256 ? 2 : 1;               // stages per K or V tile
+  static constexpr int kKTok = kTT, kKCols = D == 256 ? 128 : D;   // one K stage: tokens x columns
+  static constexpr int kVTok = D == 256 ? 64 : kTT, kVCols = D;    // one V stage
+  static constexpr int kStage = kKTok * kKCols * 2;
+  static constexpr int kStages = D == 64 ? 8 : kBf ? 5 : 4;
+  static constexpr int kScaleSlots = 8;  // tiles whose scales are held: more than the stages reach ahead
+  static constexpr int kQ = NQ * 128 * D * 2;
+  static constexpr int kOffStage = kQ;
+  static constexpr int kOffScale = kOffStage + kStages * kStage;
+  static constexpr int kOffBar = kOffScale + (kBf ? 0 : kScaleSlots * 2 * kTT * 4);
+  static constexpr int kSmem = kOffBar + 512 + 1024;  // barriers, alignment slack
+  // Warpgroups: softmax (NQ), then the MMA issuer with the TMA loader beside it, then the widening
+  // loaders.  Registers a thread: a row of 128 scores lives in its softmax thread; the shares add
+  // up to what the block is launched with.
+  static constexpr int kSoftWarps = 4 * NQ, kMmaWarp = kSoftWarps, kLoadWarp = kSoftWarps + (kBf ? 1 : 4);
+  static constexpr int kLoadWarps = kBf ? 1 : 4;
+  static constexpr int kGroups = NQ + (kBf ? 1 : 2);
+  static constexpr int kThreads = 128 * kGroups;
+  static constexpr int kRegs = kGroups == 2 ? 248 : kGroups == 3 ? 168 : 128;
+  static constexpr int kSoftRegs = kGroups == 2 ? 248 : kBf ? 200 : NQ == 1 ? 224 : 176;
+  static constexpr int kMmaRegs = kGroups == 2 ? 248 : kBf ? 104 : NQ == 1 ? 96 : 64;
+  static constexpr int kLoadRegs = kBf ? 0 : NQ == 1 ? 184 : 96;
+  static_assert(NQ * kSoftRegs + kMmaRegs + kLoadRegs == kGroups * kRegs, "register shares");
+  static_assert(kVTok * kVCols * 2 == kStage, "K and V stages are one size");
+  static_assert(kSmem <= 227 * 1024, "shared memory");
+};
+
+constexpr uint32_t kIdescQK = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+template <int D>
+constexpr uint32_t kIdescPV = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((static_cast<uint32_t>(D) >> 3) << 17) |
+                              ((128u >> 4) << 24);  // bit 16: B is MN-major (V as it lies: token rows)
+
+// 128-byte swizzled operands.  K-major: 8-row groups 1024 bytes apart (stride offset).  MN-major:
+// blocks of 64 columns `lead` bytes apart (leading offset), 8-token groups 1024 bytes apart.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lead) {
+  return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(lead >> 4) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void commit_to(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void arrive_on(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ bool elected() {
+  uint32_t p = 0;
+  asm volatile("{\n\t.reg .pred P;\n\telect.sync _|P, 0xffffffff;\n\tselp.b32 %0, 1, 0, P;\n\t}" : "=r"(p));
+  return p != 0;
+}
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, int x, int tok, int head, int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(tok), "r"(head), "r"(page), "r"(smem_addr(bar))
+      : "memory");
+}
+// 32 consecutive columns of this thread's lane.
+__device__ __forceinline__ void tm_ld32(uint32_t a, float* v) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(a));
+}
+__device__ __forceinline__ void tm_st32(uint32_t a, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(a),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tm_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// This warpgroup's registers a thread, from `From` at launch.
+template <int From, int To>
+__device__ __forceinline__ void set_regs() {
+  if constexpr (To > From) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(To));
+  if constexpr (To < From) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(To));
+}
+
+// Four 8-bit codes as two bf16 pairs, exact (at most 8 significand bits).
+template <int FMT>
+__device__ __forceinline__ uint2 widen_bf16(uint32_t codes) {
+  if constexpr (FMT == GS_DTYPE_E4M3) {
+    const float2 a = half2_float2(e4m3x2_half2(codes & 0xffffu)), b = half2_float2(e4m3x2_half2(codes >> 16));
+    return make_uint2(bf16x2(a.x, a.y), bf16x2(b.x, b.y));
+  } else {
+    // byte + 128 as the low mantissa of 2^23, minus 2^23 + 128
+    const uint32_t u = codes ^ 0x80808080u;
+    float f[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540 + i)) - 8388736.0f;
+    return make_uint2(bf16x2(f[0], f[1]), bf16x2(f[2], f[3]));
+  }
+}
+
+struct TileMaps {
+  CUtensorMap k, v;
+};
+
+template <int D, int FMT>
+__global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
+    attn_tile_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ TileMaps maps) {
+  using P = TilePlan<D, FMT>;
+  constexpr int NQ = P::NQ, SB = P::SB;
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t raw = smem_addr(smem_raw);
+  unsigned char* sm = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + P::kOffBar);
+  uint64_t* full = bars;                   // [kStages]
+  uint64_t* freeb = full + P::kStages;     // [kStages]
+  uint64_t* s_full = freeb + P::kStages;   // [2]: score buffer (query tile, or tile parity)
+  uint64_t* p_full = s_full + 2;           // [2]
+  uint64_t* o_done = p_full + 2;           // [NQ]
+  uint64_t* m_done = o_done + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(m_done + 1);
+  volatile int* stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int b = blockIdx.z;
+  const int blocks = gridDim.y / A.kv.kv_heads;
+  const int head = blockIdx.y / blocks;
+  const int rb = blocks - 1 - static_cast<int>(blockIdx.y % blocks);  // longest contexts first
+  const int r0 = rb * P::kRows;
+  const RowRange R = row_range<kTT>(A, b, r0, P::kRows);
+  if (R.rows == 0) return;
+  int nsplit = (R.tiles + A.chunk_tiles - 1) / A.chunk_tiles;
+  nsplit = nsplit < 1 ? 1 : nsplit > A.splits ? A.splits : nsplit;
+  const int split = blockIdx.x;
+  if (split >= nsplit) return;
+  const int t_begin = split * A.chunk_tiles;
+  const int t_end = split == nsplit - 1 ? R.tiles : t_begin + A.chunk_tiles;
+  const int n = t_end - t_begin;
+
+  if (tid == 0) {
+    for (int s = 0; s < P::kStages; ++s) {
+      mbar_init(full + s, P::kBf ? 1 : 128);
+      mbar_init(freeb + s, 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(s_full + s, 1);
+      mbar_init(p_full + s, 128);
+      mbar_init(o_done + s, 1);
+    }
+    mbar_init(m_done, 1);
+    *stop = 0;
+  }
+  if (warp == P::kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(tmem_slot)) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  // ---- Q: [query tile][64-column block][128 rows][128 bytes], swizzled; rows past the block zero
+  {
+    constexpr int kCh = D / 8;
+    const uint32_t flip = A.scale_log2 < 0.0f ? 0x80008000u : 0u;  // (a negative scale: -q and |scale|)
+    for (int id = tid; id < P::kRows * kCh; id += P::kThreads) {
+      const int r = id / kCh, ch = id % kCh;
+      uint4 x = make_uint4(0u, 0u, 0u, 0u);
+      if (r < R.rows) {
+        const int row = r0 + r;
+        x = *reinterpret_cast<const uint4*>(A.q + (R.q0 + row / A.group) * A.q_token + (head * A.group + row % A.group) * A.q_head + ch * 8);
+        x.x ^= flip, x.y ^= flip, x.z ^= flip, x.w ^= flip;
+      }
+      const int rr = r & 127, blk = (r >> 7) * (D / 64) + (ch >> 3), c = ch & 7;
+      *reinterpret_cast<uint4*>(sm + blk * 16384 + rr * 128 + ((c ^ (rr & 7)) << 4)) = x;
+    }
+    fence_async();
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto give_up = [&]() {
+    *stop = 1;
+    atomicOr(A.flag, GS_KV_ERR_TIMEOUT);
+  };
+
+  // ---------------- loaders ----------------
+  auto load = [&]() {
+    const int32_t* table = A.table + b * A.table_stride;
+    const int shift = A.kv.page_shift, page_mask = (1 << shift) - 1;
+    auto page_of = [&](int tok) {  // the page of a context token, checked
+      const int col = tok >> shift;
+      int pg = col < A.table_cols ? __ldg(table + col) : -1;
+      if (pg < 0 || pg >= A.kv.pages) {
+        atomicOr(A.flag, GS_KV_ERR_PAGE);
+        pg = 0;
+      }
+      return pg;
+    };
+    // item i of the stage order: K(0) .. K(SB - 1), then V(j), K(j + SB) in turn
+    const int items = 2 * n;
+    auto item = [&](int i, bool& value, int& j) {
+      if (i < (SB < n ? SB : n)) {
+        value = false, j = i;
+        return;
+      }
+      const int k = i - (SB < n ? SB : n);
+      if (k < 2 * (n - SB)) value = (k & 1) == 0, j = value ? k >> 1 : (k >> 1) + SB;
+      else value = true, j = k - (n - SB > 0 ? n - SB : 0);
+    };
+    if constexpr (P::kBf) {
+      int issued = 0;
+      bool ok = true;
+      for (int i = 0; i < items && ok && !*stop; ++i) {
+        bool value;
+        int j;
+        item(i, value, j);
+        for (int h = 0; h < P::kPer; ++h) {
+          const int at = issued % P::kStages, round = issued / P::kStages;
+          if (round > 0) ok = __all_sync(kFullMask, mbar_wait(freeb + at, static_cast<uint32_t>((round - 1) & 1), kWaitNs));
+          if (!ok) break;
+          const int toks = value ? P::kVTok : P::kKTok;
+          const int box = min(1 << shift, toks);  // tokens per box
+          const int groups = toks / box;
+          const int cols = (value ? P::kVCols : P::kKCols) / 64;
+          const int j0 = R.tile(t_begin + j) * kTT + (value ? h * P::kVTok : 0);
+          // lane g: token group g (at most 8); a group past every row's last token stays as it is
+          const int tok = j0 + lane * box;
+          const bool real = lane < groups && tok < R.hi;
+          const int pg = real ? page_of(tok) : 0;
+          const unsigned live = __ballot_sync(kFullMask, real);
+          const uint32_t bytes = static_cast<uint32_t>(__popc(live) * box * cols * 128);
+          if (lane == 0) {
+            if (bytes) mbar_expect_tx(full + at, bytes);
+            else arrive_on(full + at);
+          }
+          __syncwarp();
+          if (real) {
+            const uint32_t dst = smem_addr(sm + P::kOffStage + at * P::kStage) + lane * box * 128;
+            for (int cb = 0; cb < cols; ++cb)
+              tma_box(dst + cb * toks * 128, value ? &maps.v : &maps.k, cb * 64 + (value ? 0 : h * P::kKCols), tok & page_mask,
+                      head, pg, full + at);
+          }
+          __syncwarp();
+          ++issued;
+        }
+      }
+      if (!ok) give_up();
+      if (*stop)  // copies in flight land before the block ends
+        for (int k = max(0, issued - P::kStages); k < issued; ++k)
+          mbar_wait(full + k % P::kStages, static_cast<uint32_t>((k / P::kStages) & 1), kWaitNs);
+    } else {
+      const int lt = tid - 32 * P::kLoadWarp;
+      constexpr int kCh = P::kStage / 2 / 16 / 128;  // 16-byte pieces of codes per thread and stage
+      uint4 x[kCh];
+      float sk = 0.0f, sv = 0.0f;
+      // the codes of stage k of the order (kPer per item) into registers
+      auto fetch = [&](int k) {
+        bool value;
+        int j;
+        item(k / P::kPer, value, j);
+        const int h = k % P::kPer;
+        const int per_row = (value ? P::kVCols : P::kKCols) / 16;
+        const int j0 = R.tile(t_begin + j) * kTT + (value ? h * P::kVTok : 0);
+        const int64_t sp = value ? A.kv.v_page : A.kv.k_page, sh = value ? A.kv.v_head : A.kv.k_head,
+                      stt = value ? A.kv.v_token : A.kv.k_token;
+        const unsigned char* base = (value ? A.kv.v : A.kv.k) + head * sh + (value ? 0 : h * P::kKCols);
+#pragma unroll
+        for (int u = 0; u < kCh; ++u) {
+          const int id = lt + 128 * u, tr = id / per_row, ch = id % per_row;
+          const int tok = j0 + tr;
+          x[u] = make_uint4(0u, 0u, 0u, 0u);
+          if (R.seen_by_any(tok)) x[u] = __ldg(reinterpret_cast<const uint4*>(base + page_of(tok) * sp + (tok & page_mask) * stt + ch * 16));
+        }
+        // K items bring both scales of the tile, token lt per thread: the softmax reads V's too before
+        // V itself has to be there
+        if (!value && h == 0) {
+          const int tk = R.tile(t_begin + j) * kTT + lt;
+          sk = sv = 0.0f;
+          if (R.seen_by_any(tk)) {
+            const int64_t e = ((static_cast<int64_t>(page_of(tk)) * A.kv.kv_heads + head) << shift) + (tk & page_mask);
+            sk = __ldg(A.kv.k_scale + e);
+            sv = __ldg(A.kv.v_scale + e);
+          }
+        }
+      };
+      const int total = items * P::kPer;
+      bool ok = true;
+      if (total > 0) fetch(0);
+      for (int k = 0; k < total && !*stop; ++k) {
+        bool value;
+        int j;
+        item(k / P::kPer, value, j);
+        const int h = k % P::kPer;
+        const int at = k % P::kStages, round = k / P::kStages;
+        if (round > 0) ok = __all_sync(kFullMask, mbar_wait(freeb + at, static_cast<uint32_t>((round - 1) & 1), kWaitNs));
+        if (!ok) {
+          give_up();
+          break;
+        }
+        const int per_row = (value ? P::kVCols : P::kKCols) / 16;
+        const int toks = value ? P::kVTok : P::kKTok;
+        unsigned char* st = sm + P::kOffStage + at * P::kStage;
+#pragma unroll
+        for (int u = 0; u < kCh; ++u) {
+          const int id = lt + 128 * u, tr = id / per_row, ch = id % per_row;
+          const uint2 a = widen_bf16<FMT>(x[u].x), b2 = widen_bf16<FMT>(x[u].y), c2 = widen_bf16<FMT>(x[u].z), d2 = widen_bf16<FMT>(x[u].w);
+          unsigned char* dst = st + (ch >> 2) * (toks * 128) + tr * 128;
+          const int c0 = (ch & 3) * 2;
+          *reinterpret_cast<uint4*>(dst + ((c0 ^ (tr & 7)) << 4)) = make_uint4(a.x, a.y, b2.x, b2.y);
+          *reinterpret_cast<uint4*>(dst + (((c0 + 1) ^ (tr & 7)) << 4)) = make_uint4(c2.x, c2.y, d2.x, d2.y);
+        }
+        if (!value && h == 0) {
+          float* sc = reinterpret_cast<float*>(sm + P::kOffScale) + (j % P::kScaleSlots) * (2 * kTT) + lt;
+          sc[0] = sk;
+          sc[kTT] = sv;
+        }
+        fence_async();
+        arrive_on(full + at);
+        if (k + 1 < total) fetch(k + 1);
+      }
+    }
+    __syncwarp();
+  };
+
+  if (warp < P::kSoftWarps) {
+    // ---------------- softmax: one query row per thread ----------------
+    set_regs<P::kRegs, P::kSoftRegs>();
+    const int s = NQ == 2 ? warp >> 2 : 0;  // query tile
+    const int quad = warp & 3;
+    const int r = s * 128 + quad * 32 + lane;
+    const int row = r0 + min(r, R.rows - 1);
+    const int p = R.p0 + row / A.group;
+    const int lo = A.window ? max(p - A.window + 1, 0) : 0;
+    const float c = fmaxf(fabsf(A.scale_log2), 1e-30f);  // (0 would turn a hidden score's -inf into NaN)
+    const float slack = 8.0f / c;
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const uint32_t o_at = lane_base + 256u + static_cast<uint32_t>(s * D);
+    float m = -INFINITY;
+    float2 l2 = make_float2(0.0f, 0.0f);
+    for (int j = 0; j < n && !*stop; ++j) {
+      const int buf = NQ == 2 ? s : (j & 1);
+      const uint32_t ph = static_cast<uint32_t>((j / SB) & 1);
+      const uint32_t s_at = lane_base + static_cast<uint32_t>(buf * 128);
+      const int j0 = R.tile(t_begin + j) * kTT;
+      if (!__all_sync(kFullMask, mbar_wait(s_full + buf, ph, kWaitNs))) {
+        give_up();
+        break;
+      }
+      fence_after();
+      float x[128];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) tm_ld32(s_at + 32 * q, x + 32 * q);
+      tm_wait_ld();
+      const float* sc = reinterpret_cast<const float*>(sm + P::kOffScale) + (j % P::kScaleSlots) * (2 * kTT);
+      if constexpr (!P::kBf) {
+#pragma unroll
+        for (int i = 0; i < 128; i += 4) {
+          const float4 k4 = *reinterpret_cast<const float4*>(sc + i);
+          x[i] *= k4.x, x[i + 1] *= k4.y, x[i + 2] *= k4.z, x[i + 3] *= k4.w;
+        }
+      }
+      const bool whole = j0 + kTT - 1 <= p && (j0 >= lo || j0 + kTT <= R.sink);
+      if (!__all_sync(kFullMask, whole)) {
+        const int hi_c = p + 1 - j0, lo_c = lo - j0, sk_c = R.sink - j0;
+#pragma unroll
+        for (int i = 0; i < 128; ++i) x[i] = (i < hi_c && (i >= lo_c || i < sk_c)) ? x[i] : -INFINITY;
+      }
+      float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+      for (int i = 4; i < 128; i += 8) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) mx[u] = i + 4 + u < 128 ? fmaxf(fmaxf(mx[u], x[i + u]), x[i + 4 + u]) : fmaxf(mx[u], x[i + u]);
+      }
+      const float tm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      const bool move = tm > m + slack || (m == -INFINITY && tm > m);
+      if (__any_sync(kFullMask, move)) {
+        const float mn = move ? tm : m;
+        const float al = m == -INFINITY ? 0.0f : ex2((m - mn) * c);
+        m = mn;
+        l2.x *= al, l2.y *= al;
+        if (j > 0) {
+          bool ok = true;
+          if constexpr (SB == 2) ok = mbar_wait(o_done, static_cast<uint32_t>((j - 1) & 1), kWaitNs);
+          if (!__all_sync(kFullMask, ok)) {
+            give_up();
+            break;
+          }
+          fence_after();
+#pragma unroll
+          for (int q = 0; q < D / 32; ++q) {
+            float o[32];
+            tm_ld32(o_at + 32 * q, o);
+            tm_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] *= al;
+            tm_st32(o_at + 32 * q, reinterpret_cast<uint32_t*>(o));
+          }
+        }
+      }
+      const float mc = m == -INFINITY ? 0.0f : -m * c;
+      uint32_t* w = reinterpret_cast<uint32_t*>(x);
+#pragma unroll
+      for (int i = 0; i < 128; i += 2) {
+        float2 t = __ffma2_rn(make_float2(x[i], x[i + 1]), make_float2(c, c), make_float2(mc, mc));
+        t.x = ex2(t.x), t.y = ex2(t.y);
+        l2 = __fadd2_rn(l2, t);
+        if constexpr (!P::kBf) {
+          const float2 v2 = *reinterpret_cast<const float2*>(sc + kTT + i);
+          t = __fmul2_rn(t, v2);
+        }
+        w[i >> 1] = bf16x2(t.x, t.y);
+      }
+      tm_st32(s_at, w);
+      tm_st32(s_at + 32, w + 32);
+      tm_wait_st();
+      fence_before();
+      arrive_on(p_full + buf);
+    }
+    // ---- epilogue
+    const float l = l2.x + l2.y;
+    bool ok = *stop == 0;
+    if (n > 0 && ok) {
+      // (two score buffers: the product before the last may still run, and a wait by parity must not
+      // be a phase ahead)
+      if (SB == 2 && n > 1) ok = mbar_wait(o_done, static_cast<uint32_t>((n - 2) & 1), kWaitNs);
+      ok = ok && mbar_wait(o_done + s, static_cast<uint32_t>((n - 1) & 1), kWaitNs);
+      if (!ok) give_up();
+    }
+    ok = __all_sync(kFullMask, ok);
+    if (ok) {
+      fence_after();
+      const bool live = r < R.rows;
+      const int64_t t = R.q0 + row / A.group;
+      const int hq = head * A.group + row % A.group;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const int64_t part = ((static_cast<int64_t>(b) * gridDim.y + rb * A.kv.kv_heads + head) * A.splits + split) * P::kRows + r;
+#pragma unroll
+      for (int q = 0; q < D / 32; ++q) {
+        float o[32];
+        if (n > 0) {
+          tm_ld32(o_at + 32 * q, o);
+          tm_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+        }
+        if (live && nsplit == 1) {
+          uint4* dst = reinterpret_cast<uint4*>(A.out + t * A.o_token + hq * A.o_head + 32 * q);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            dst[i] = make_uint4(bf16x2(o[8 * i] * inv, o[8 * i + 1] * inv), bf16x2(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
+                                bf16x2(o[8 * i + 4] * inv, o[8 * i + 5] * inv), bf16x2(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
+        } else if (live) {
+          float4* dst = reinterpret_cast<float4*>(A.part_o + part * D + 32 * q);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        }
+      }
+      if (live) {
+        const float mc = m * c;  // (log2 units)
+        if (nsplit == 1) {
+          if (A.lse) A.lse[t * A.q_heads + hq] = l == 0.0f ? -INFINITY : (mc + log2f(l)) * 0.6931471805599453f;
+        } else {
+          *reinterpret_cast<float2*>(A.part_ml + part * 2) = make_float2(m == -INFINITY ? m : mc, l);
+        }
+      }
+    }
+    fence_before();
+  } else if (warp < P::kMmaWarp + 4) {
+   set_regs<P::kRegs, P::kMmaRegs>();
+   if (warp == P::kMmaWarp) {
+    // ---------------- MMA issuer ----------------
+    const bool leader = elected();
+    int cnt = 0;  // stages consumed
+    auto stage_ready = [&](int at) {
+      return __all_sync(kFullMask, mbar_wait(full + at % P::kStages, static_cast<uint32_t>((at / P::kStages) & 1), kWaitNs));
+    };
+    // S(query tile s, buffer buf) = Q K^T over stages at .. at + kPer - 1
+    auto scores = [&](int s, int buf, int at) {
+      if (leader) {
+#pragma unroll
+        for (int h = 0; h < P::kPer; ++h) {
+          const uint32_t ka = smem_addr(sm + P::kOffStage + ((at + h) % P::kStages) * P::kStage);
+          const uint32_t qa = smem_addr(sm + s * (D / 64) * 16384 + h * (P::kKCols / 64) * 16384);
+#pragma unroll
+          for (int k = 0; k < P::kKCols / 16; ++k) {
+            const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
+            mma_ss(tmem + buf * 128, desc_sw128(qa + off, 16), desc_sw128(ka + off, 16), kIdescQK, (h | k) != 0 ? 1u : 0u);
+          }
+        }
+      }
+      __syncwarp();
+    };
+    // zeros in the rows of a V stage that no query row of the block sees: their weights are 0,
+    // and what the pages hold there may be a NaN
+    auto clean = [&](int at, int j, int h) {
+      const int j0 = R.tile(t_begin + j) * kTT + h * P::kVTok;
+      const bool hidden = j0 + P::kVTok > R.hi || (j0 < R.lo && j0 + P::kVTok > R.sink);
+      if (!P::kBf || !hidden) return;
+      unsigned char* st = sm + P::kOffStage + (at % P::kStages) * P::kStage;
+      for (int id = lane; id < P::kVTok * (D / 8); id += 32) {
+        const int tr = id / (D / 8), ch = id % (D / 8);
+        if (!R.seen_by_any(j0 + tr))
+          *reinterpret_cast<uint4*>(st + (ch >> 3) * (P::kVTok * 128) + tr * 128 + ((ch & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+      }
+      fence_async();
+      __syncwarp();
+    };
+    bool ok = true;
+    for (int i = 0; ok && i < SB && i < n; ++i) {
+      for (int h = 0; ok && h < P::kPer; ++h) ok = stage_ready(cnt + h);
+      if (!ok) break;
+      fence_after();
+      for (int s = 0; s < NQ; ++s) {
+        scores(s, NQ == 2 ? s : i, cnt);
+        if (leader) {
+          commit_to(s_full + (NQ == 2 ? s : i));
+          if (s == NQ - 1)
+            for (int h = 0; h < P::kPer; ++h) commit_to(freeb + (cnt + h) % P::kStages);
+        }
+        __syncwarp();
+      }
+      cnt += P::kPer;
+    }
+    for (int j = 0; ok && j < n && !*stop; ++j) {
+      const int v_at = cnt, k_at = cnt + P::kPer;
+      const bool more = j + SB < n;
+      for (int s = 0; ok && s < NQ; ++s) {
+        const int buf = NQ == 2 ? s : (j & 1);
+        if (s == 0)
+          for (int h = 0; ok && h < P::kPer; ++h) {
+            ok = stage_ready(v_at + h);
+            if (ok) clean(v_at + h, j, h);
+          }
+        ok = ok && __all_sync(kFullMask, mbar_wait(p_full + buf, static_cast<uint32_t>((j / SB) & 1), kWaitNs));
+        if (!ok) break;
+        fence_after();
+        if (leader) {
+#pragma unroll
+          for (int h = 0; h < P::kPer; ++h) {
+            const uint32_t va = smem_addr(sm + P::kOffStage + ((v_at + h) % P::kStages) * P::kStage);
+#pragma unroll
+            for (int k = 0; k < P::kVTok / 16; ++k)
+              mma_ts(tmem + 256 + s * D, tmem + buf * 128 + (h * P::kVTok + k * 16) / 2, desc_sw128(va + k * 2048, P::kVTok * 128),
+                     kIdescPV<D>, (j | h | k) != 0 ? 1u : 0u);
+          }
+          commit_to(o_done + s);
+          if (s == NQ - 1)
+            for (int h = 0; h < P::kPer; ++h) commit_to(freeb + (v_at + h) % P::kStages);
+        }
+        __syncwarp();
+        if (more) {
+          if (s == 0)
+            for (int h = 0; ok && h < P::kPer; ++h) ok = stage_ready(k_at + h);
+          if (!ok) break;
+          fence_after();
+          scores(s, buf, k_at);
+          if (leader) {
+            commit_to(s_full + buf);
+            if (s == NQ - 1)
+              for (int h = 0; h < P::kPer; ++h) commit_to(freeb + (k_at + h) % P::kStages);
+          }
+          __syncwarp();
+        }
+      }
+      cnt += more ? 2 * P::kPer : P::kPer;
+    }
+    if (!ok) give_up();
+    // every product has completed before tensor memory is freed
+    if (leader) commit_to(m_done);
+    __syncwarp();
+    if (!__all_sync(kFullMask, mbar_wait(m_done, 0, kWaitNs))) give_up();
+   } else if constexpr (P::kBf) {
+    if (warp == P::kLoadWarp) load();
+   }
+  } else {
+   if constexpr (!P::kBf) set_regs<P::kRegs, P::kLoadRegs>();
+   load();
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == P::kMmaWarp) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+template <int D, int FMT>
+cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
+  using P = TilePlan<D, FMT>;
+  const int blocks = static_cast<int>((static_cast<int64_t>(a.max_q) * a.group + P::kRows - 1) / P::kRows);
+  const int64_t items = static_cast<int64_t>(a.seqs) * a.kv.kv_heads * blocks;
+  const int64_t tiles = most_tiles(a, kTT, P::kRows);
+  // Splits: only while the blocks do not fill the SMs, each of at least 8 tiles, within the workspace.
+  int64_t splits = c->num_sms / items;
+  const int64_t by_len = tiles / 8;
+  splits = splits > by_len ? by_len : splits;
+  const int64_t slot = static_cast<int64_t>(P::kRows) * (D + 2) * 4;
+  const int64_t by_ws = static_cast<int64_t>(kAttnWsBytes) / (items * slot);
+  splits = splits > by_ws ? by_ws : splits;
+  if (splits < 1) splits = 1;
+  const int64_t chunk = tiles > 0 ? (tiles + splits - 1) / splits : 1;
+  a.chunk_tiles = static_cast<int32_t>(chunk);
+  a.splits = static_cast<int32_t>(tiles > 0 ? (tiles + chunk - 1) / chunk : 1);
+  a.part_o = reinterpret_cast<float*>(c->ws);
+  a.part_ml = a.part_o + items * a.splits * P::kRows * D;
+  static std::atomic<uint64_t> done{0};
+  if (device_todo(done)) {
+    cudaFuncAttributes at;
+    cudaError_t e = cudaFuncGetAttributes(&at, attn_tile_kernel<D, FMT>);
+    // (the warpgroups' shares must not exceed what the block is launched with)
+    if (e == cudaSuccess && P::kSoftRegs != P::kRegs && at.numRegs != P::kRegs) e = cudaErrorInvalidKernelImage;
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(attn_tile_kernel<D, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, P::kSmem);
+    if (e != cudaSuccess) return e;
+    mark_device_done(done);
+  }
+  const dim3 grid(static_cast<unsigned>(a.splits), static_cast<unsigned>(a.kv.kv_heads * blocks), static_cast<unsigned>(a.seqs));
+  if (grid.y > 65535) return cudaErrorInvalidConfiguration;
+  attn_tile_kernel<D, FMT><<<grid, P::kThreads, P::kSmem, st>>>(a, *reinterpret_cast<const TileMaps*>(c->maps));
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || a.splits == 1) return e;
+  return launch_attn_join(a, D, P::kRows, blocks, kTT, st);
+}
+
+template <int D>
+cudaError_t go_fmt(const gs_kv_cache* c, const AttnArgs& a, cudaStream_t st) {
+  switch (c->d.format) {
+    case GS_DTYPE_BF16: return go<D, GS_DTYPE_BF16>(c, a, st);
+    case GS_DTYPE_E4M3: return go<D, GS_DTYPE_E4M3>(c, a, st);
+    default: return go<D, GS_DTYPE_INT8>(c, a, st);
+  }
+}
+
+}  // namespace
+
+cudaError_t launch_attn_tile(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
+  return c->d.head_dim == 64 ? go_fmt<64>(c, a, st) : c->d.head_dim == 128 ? go_fmt<128>(c, a, st) : go_fmt<256>(c, a, st);
+}
+
+// The bf16 pools as (head_dim, page token, head, page) tensors, boxes of 64 columns (one
+// 128-byte swizzle row) by as many tokens as a page and a stage share.
+const char* make_attn_maps(gs_kv_cache* c) {
+  static_assert(sizeof(TileMaps) <= sizeof(c->maps), "room for two tensor maps");
+  const gs_kv_cache_desc& d = c->d;
+  if (d.format != GS_DTYPE_BF16) return nullptr;
+  void* fn = nullptr;
+  cudaDriverEntryPointQueryResult res;
+  if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &res) != cudaSuccess ||
+      res != cudaDriverEntryPointSuccess || !fn)
+    return "cuTensorMapEncodeTiled is not available";
+  auto encode = reinterpret_cast<CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                              const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill)>(fn);
+  TileMaps* m = reinterpret_cast<TileMaps*>(c->maps);
+  for (int v = 0; v < 2; ++v) {
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d.head_dim), static_cast<cuuint64_t>(d.page_size),
+                                static_cast<cuuint64_t>(d.kv_heads), static_cast<cuuint64_t>(d.pages)};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(v ? d.v_token_stride : d.k_token_stride) * 2,
+                                   static_cast<cuuint64_t>(v ? d.v_head_stride : d.k_head_stride) * 2,
+                                   static_cast<cuuint64_t>(v ? d.v_page_stride : d.k_page_stride) * 2};
+    const int most = v && d.head_dim == 256 ? 64 : kTT;
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(d.page_size < most ? d.page_size : most), 1, 1};
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    const CUresult r = encode(v ? &m->v : &m->k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, v ? d.v : d.k, dims, strides, box, ones,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return "KV cache: these strides do not make a tensor map";
+  }
+  return nullptr;
+}
+
+}  // namespace gs

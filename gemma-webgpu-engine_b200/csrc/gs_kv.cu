@@ -177,6 +177,9 @@ cudaError_t launch_rows(const KvRowsArgs& a, int fmt, bool write, bool bf16, boo
   }
 }
 
+// Rows (new tokens × heads of a group) up to which the few-row kernel is taken.
+constexpr int64_t kFewRows = 32;
+
 gs_status kfail(gs_kv_cache* c, gs_status s, const char* m) {
   c->err = m;
   return s;
@@ -288,6 +291,12 @@ gs_status gs_kv_cache_create(gs_ctx* ctx, const gs_kv_cache_desc* d, gs_kv_cache
     delete c;
     return er == cudaErrorMemoryAllocation ? GS_ENOMEM : GS_ECUDA;
   }
+  if (const char* m = make_attn_maps(c)) {
+    ctx_set_error(ctx, m);
+    cudaFree(c->flag);
+    delete c;
+    return GS_EUNSUPPORTED;
+  }
   *out = c;
   return GS_OK;
 }
@@ -375,7 +384,8 @@ gs_status gs_attention(gs_kv_cache* c, const gs_attention_args* p, void* stream)
   a.scale_log2 = static_cast<float>(static_cast<double>(p->scale) * 1.4426950408889634);
   a.flag = c->flag;
   DeviceScope scope(c->device);
-  const cudaError_t e = launch_attn_rows(c, a, static_cast<cudaStream_t>(stream));
+  cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = most_rows > kFewRows ? launch_attn_tile(c, a, cs) : launch_attn_rows(c, a, cs);
   if (e != cudaSuccess) return kfail(c, GS_ECUDA, cudaGetErrorString(e));
   return GS_OK;
 }
