@@ -180,10 +180,16 @@ class GsAttentionArgs(ctypes.Structure):
                [("scale", ctypes.c_float)]
 
 
+_raw_stream = None
+
+
 def current_stream(device) -> int:
     """The raw handle of torch's current stream on ``device``."""
-    import torch
-    return torch._C._cuda_getCurrentRawStream(device.index)
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+        _raw_stream = torch._C._cuda_getCurrentRawStream
+    return _raw_stream(device.index)
 
 
 def build(force: bool = False) -> str:
@@ -247,15 +253,15 @@ def lib() -> ctypes.CDLL:
     L.gs_nccl_last_error.argtypes = [P]
     L.gs_nccl_last_error.restype = ctypes.c_char_p
     L.gs_shard_sample.argtypes = [P, P, ctypes.POINTER(GsBatch), i64, i64, ctypes.POINTER(GsOutputs), i32, P]
-    L.gs_rms_norm.argtypes = [P, ctypes.POINTER(GsRmsNormArgs), P]
+    L.gs_rms_norm.argtypes = [P, P, P]  # (GsRmsNormArgs, or its packed bytes)
     L.gs_kv_cache_create.argtypes = [P, ctypes.POINTER(GsKvCacheDesc), ctypes.POINTER(P)]
     L.gs_kv_cache_destroy.argtypes = [P]
     L.gs_kv_cache_last_error.argtypes = [P]
     L.gs_kv_cache_last_error.restype = ctypes.c_char_p
     L.gs_kv_cache_check.argtypes = [P, ctypes.POINTER(i32)]
-    L.gs_kv_write.argtypes = [P, ctypes.POINTER(GsKvRows), P]
-    L.gs_kv_read.argtypes = [P, ctypes.POINTER(GsKvRows), P]
-    L.gs_attention.argtypes = [P, ctypes.POINTER(GsAttentionArgs), P]
+    L.gs_kv_write.argtypes = [P, P, P]  # (GsKvRows, or its packed bytes)
+    L.gs_kv_read.argtypes = [P, P, P]  # (GsKvRows, or its packed bytes)
+    L.gs_attention.argtypes = [P, P, P]  # (GsAttentionArgs, or its packed bytes)
     L.gs_profile_enable.argtypes = [P, i32]
     L.gs_profile_read.argtypes = [P, ctypes.POINTER(ctypes.c_double), ctypes.POINTER(i64),
                                   ctypes.POINTER(ctypes.c_double), ctypes.POINTER(i64)]

@@ -16,10 +16,11 @@
 // score buffers.
 //
 // Tensor memory (512 columns): S0 at 0, S1 at 128, O0 at 256, O1 at 256 + D.
-// Warps: softmax warpgroup(s) first (warp % 4 = its tensor-memory lanes), then the MMA issuer,
-// then the loaders: one warp issuing TMA boxes (bf16 pages go straight to the swizzled operand
-// layout) or four warps widening 8-bit codes to bf16 (exact) into the same layout, scales beside
-// them (K's multiplies the score, V's the weight before it is rounded).
+// Warps: softmax warpgroup(s) first (warp % 4 = its tensor-memory lanes), then the MMA issuer and the
+// loader (TMA boxes; bf16 pages go straight to the swizzled operand layout), then, beside an 8-bit
+// cache, four warps that widen the loaded codes to float16 operands: K's exact, V's times its scale;
+// K's scale multiplies the float32 score.  Q is brought into float16 by a power of two per row and the
+// weights, at most 2^8, are float16 as well.
 // Order of products and of shared-memory stages: K(0) .. K(SB-1), then V(j), K(j + SB) for each j:
 // P(j) overlays S(j), and the tensor core takes one thread's products in order, so S(j + SB) is
 // issued right behind the product that reads P(j).
@@ -44,33 +45,43 @@ struct TilePlan {
   static constexpr int kKTok = kTT, kKCols = D == 256 ? 128 : D;   // one K stage: tokens x columns
   static constexpr int kVTok = D == 256 ? 64 : kTT, kVCols = D;    // one V stage
   static constexpr int kStage = kKTok * kKCols * 2;
-  static constexpr int kStages = D == 64 ? 8 : kBf ? 5 : 4;
-  static constexpr int kScaleSlots = 8;  // tiles whose scales are held: more than the stages reach ahead
+  static constexpr int kStages = kBf ? (D == 64 ? 8 : 5) : (D == 64 ? 6 : 3);
+  static constexpr int kEl = kBf ? 2 : 1;
+  static constexpr int kInner = D * kEl < 128 ? D * kEl : 128;  // bytes of a row in one TMA box
+  static constexpr int kRawStage = kBf ? 0 : kStage / 2;        // codes of one stage
+  static constexpr int kRawStages = kBf ? 0 : D == 64 ? 6 : 3;
+  // Tiles whose scales are held: K(j + 8) is loaded only after the codes of an earlier V were taken
+  // (raw and operand stages reach at most 6 tiles ahead of the products).
+  static constexpr int kScaleSlots = 8;
   static constexpr int kQ = NQ * 128 * D * 2;
   static constexpr int kOffStage = kQ;
-  static constexpr int kOffScale = kOffStage + kStages * kStage;
-  static constexpr int kOffBar = kOffScale + (kBf ? 0 : kScaleSlots * 2 * kTT * 4);
+  static constexpr int kOffRaw = kOffStage + kStages * kStage;
+  static constexpr int kOffScale = kOffRaw + kRawStages * kRawStage;       // [slot][K, V][kTT] float
+  static constexpr int kOffQf = kOffScale + (kBf ? 0 : kScaleSlots * 2 * kTT * 4);  // [kRows] float
+  static constexpr int kOffRef = kOffQf + (kBf ? 0 : kRows * 4);           // [slot] float
+  static constexpr int kOffBar = kOffRef + (kBf ? 0 : 128);
   static constexpr int kSmem = kOffBar + 512 + 1024;  // barriers, alignment slack
   // Warpgroups: softmax (NQ), then the MMA issuer with the TMA loader beside it, then the widening
   // loaders.  Registers a thread: a row of 128 scores lives in its softmax thread; the shares add
   // up to what the block is launched with.
-  static constexpr int kSoftWarps = 4 * NQ, kMmaWarp = kSoftWarps, kLoadWarp = kSoftWarps + (kBf ? 1 : 4);
-  static constexpr int kLoadWarps = kBf ? 1 : 4;
+  static constexpr int kSoftWarps = 4 * NQ, kMmaWarp = kSoftWarps, kLoadWarp = kSoftWarps + 1, kWidenWarp = kSoftWarps + 4;
   static constexpr int kGroups = NQ + (kBf ? 1 : 2);
   static constexpr int kThreads = 128 * kGroups;
   static constexpr int kRegs = kGroups == 2 ? 248 : kGroups == 3 ? 168 : 128;
   static constexpr int kSoftRegs = kGroups == 2 ? 248 : kBf ? 200 : NQ == 1 ? 224 : 176;
   static constexpr int kMmaRegs = kGroups == 2 ? 248 : kBf ? 104 : NQ == 1 ? 96 : 64;
-  static constexpr int kLoadRegs = kBf ? 0 : NQ == 1 ? 184 : 96;
+  static constexpr int kLoadRegs = kBf ? 0 : NQ == 1 ? 184 : 96;  // (widening warps)
   static_assert(NQ * kSoftRegs + kMmaRegs + kLoadRegs == kGroups * kRegs, "register shares");
   static_assert(kVTok * kVCols * 2 == kStage, "K and V stages are one size");
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
-constexpr uint32_t kIdescQK = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
-template <int D>
-constexpr uint32_t kIdescPV = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((static_cast<uint32_t>(D) >> 3) << 17) |
-                              ((128u >> 4) << 24);  // bit 16: B is MN-major (V as it lies: token rows)
+// tcgen05.mma kind::f16: f32 accumulators, bf16 or f16 operands (both the same), M = 128.
+template <bool BF16>
+constexpr uint32_t kIdescQK = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+template <int D, bool BF16>
+constexpr uint32_t kIdescPV = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 16) |
+                              ((static_cast<uint32_t>(D) >> 3) << 17) | ((128u >> 4) << 24);  // bit 16: B MN-major (V's token rows)
 
 // 128-byte swizzled operands.  K-major: 8-row groups 1024 bytes apart (stride offset).  MN-major:
 // blocks of 64 columns `lead` bytes apart (leading offset), 8-token groups 1024 bytes apart.
@@ -142,21 +153,39 @@ __device__ __forceinline__ void set_regs() {
   if constexpr (To < From) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(To));
 }
 
-// Four 8-bit codes as two bf16 pairs, exact (at most 8 significand bits).
+// Four 8-bit codes as two float16 pairs, exact.  int8: byte + 128 becomes the low mantissa of
+// 1024, minus 1152.
 template <int FMT>
-__device__ __forceinline__ uint2 widen_bf16(uint32_t codes) {
+__device__ __forceinline__ uint2 widen_half(uint32_t codes) {
+  uint2 r;
   if constexpr (FMT == GS_DTYPE_E4M3) {
-    const float2 a = half2_float2(e4m3x2_half2(codes & 0xffffu)), b = half2_float2(e4m3x2_half2(codes >> 16));
-    return make_uint2(bf16x2(a.x, a.y), bf16x2(b.x, b.y));
+    r.x = e4m3x2_half2(codes & 0xffffu);
+    r.y = e4m3x2_half2(codes >> 16);
   } else {
-    // byte + 128 as the low mantissa of 2^23, minus 2^23 + 128
     const uint32_t u = codes ^ 0x80808080u;
-    float f[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540 + i)) - 8388736.0f;
-    return make_uint2(bf16x2(f[0], f[1]), bf16x2(f[2], f[3]));
+    const uint32_t l = __byte_perm(u, 0x64646464u, 0x4140), h = __byte_perm(u, 0x64646464u, 0x4342);
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r.x) : "r"(l), "r"(0x64806480u));
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r.y) : "r"(h), "r"(0x64806480u));
   }
+  return r;
 }
+__device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t half2_mul(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ void bulk_in(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+               "r"(bytes), "r"(smem_addr(bar))
+               : "memory");
+}
+
+constexpr float kVUp = 128.0f;  // V operands: code · scale / vref · kVUp
 
 struct TileMaps {
   CUtensorMap k, v;
@@ -177,6 +206,8 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
   uint64_t* p_full = s_full + 2;           // [2]
   uint64_t* o_done = p_full + 2;           // [NQ]
   uint64_t* m_done = o_done + 2;
+  uint64_t* raw_full = m_done + 2;                  // [kRawStages]
+  uint64_t* raw_free = raw_full + P::kRawStages;    // [kRawStages]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(m_done + 1);
   volatile int* stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -207,6 +238,10 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
       mbar_init(o_done + s, 1);
     }
     mbar_init(m_done, 1);
+    for (int s = 0; s < P::kRawStages; ++s) {
+      mbar_init(raw_full + s, 1);
+      mbar_init(raw_free + s, 128);
+    }
     *stop = 0;
   }
   if (warp == P::kMmaWarp) {
@@ -225,6 +260,23 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
         x = *reinterpret_cast<const uint4*>(A.q + (R.q0 + row / A.group) * A.q_token + (head * A.group + row % A.group) * A.q_head + ch * 8);
         x.x ^= flip, x.y ^= flip, x.z ^= flip, x.w ^= flip;
       }
+      if constexpr (!P::kBf) {
+        // float16 by a power of two per row (bf16 has fewer mantissa bits: exact except for components
+        // below 2^-17 of the row's largest); the lanes of a row are neighbours
+        uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        float mx = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(fabsf(bf16_lo(w[i])), fabsf(bf16_hi(w[i]))));
+#pragma unroll
+        for (int o = kCh >> 1; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, o));
+        int e = static_cast<int>((__float_as_uint(mx) >> 23) & 0xffu) - 127;
+        e = mx == 0.0f || e > 127 ? 0 : min(max(e, -120), 120);
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = half2_of(bf16_lo(w[i]) * down, bf16_hi(w[i]) * down);
+        x = make_uint4(w[0], w[1], w[2], w[3]);
+        if (ch == 0) reinterpret_cast<float*>(sm + P::kOffQf)[r] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+      }
       const int rr = r & 127, blk = (r >> 7) * (D / 64) + (ch >> 3), c = ch & 7;
       *reinterpret_cast<uint4*>(sm + blk * 16384 + rr * 128 + ((c ^ (rr & 7)) << 4)) = x;
     }
@@ -237,6 +289,18 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
   auto give_up = [&]() {
     *stop = 1;
     atomicOr(A.flag, GS_KV_ERR_TIMEOUT);
+  };
+
+  // item i of the stage order: K(0) .. K(SB - 1), then V(j), K(j + SB) in turn
+  const int items = 2 * n;
+  auto item = [&](int i, bool& value, int& j) {
+    if (i < (SB < n ? SB : n)) {
+      value = false, j = i;
+      return;
+    }
+    const int k = i - (SB < n ? SB : n);
+    if (k < 2 * (n - SB)) value = (k & 1) == 0, j = value ? k >> 1 : (k >> 1) + SB;
+    else value = true, j = k - (n - SB > 0 ? n - SB : 0);
   };
 
   // ---------------- loaders ----------------
@@ -252,128 +316,133 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
       }
       return pg;
     };
-    // item i of the stage order: K(0) .. K(SB - 1), then V(j), K(j + SB) in turn
-    const int items = 2 * n;
-    auto item = [&](int i, bool& value, int& j) {
-      if (i < (SB < n ? SB : n)) {
-        value = false, j = i;
-        return;
-      }
-      const int k = i - (SB < n ? SB : n);
-      if (k < 2 * (n - SB)) value = (k & 1) == 0, j = value ? k >> 1 : (k >> 1) + SB;
-      else value = true, j = k - (n - SB > 0 ? n - SB : 0);
-    };
-    if constexpr (P::kBf) {
-      int issued = 0;
-      bool ok = true;
-      for (int i = 0; i < items && ok && !*stop; ++i) {
-        bool value;
-        int j;
-        item(i, value, j);
-        for (int h = 0; h < P::kPer; ++h) {
-          const int at = issued % P::kStages, round = issued / P::kStages;
-          if (round > 0) ok = __all_sync(kFullMask, mbar_wait(freeb + at, static_cast<uint32_t>((round - 1) & 1), kWaitNs));
-          if (!ok) break;
-          const int toks = value ? P::kVTok : P::kKTok;
-          const int box = min(1 << shift, toks);  // tokens per box
-          const int groups = toks / box;
-          const int cols = (value ? P::kVCols : P::kKCols) / 64;
-          const int j0 = R.tile(t_begin + j) * kTT + (value ? h * P::kVTok : 0);
-          // lane g: token group g (at most 8); a group past every row's last token stays as it is
-          const int tok = j0 + lane * box;
-          const bool real = lane < groups && tok < R.hi;
-          const int pg = real ? page_of(tok) : 0;
-          const unsigned live = __ballot_sync(kFullMask, real);
-          const uint32_t bytes = static_cast<uint32_t>(__popc(live) * box * cols * 128);
-          if (lane == 0) {
-            if (bytes) mbar_expect_tx(full + at, bytes);
-            else arrive_on(full + at);
-          }
-          __syncwarp();
-          if (real) {
-            const uint32_t dst = smem_addr(sm + P::kOffStage + at * P::kStage) + lane * box * 128;
-            for (int cb = 0; cb < cols; ++cb)
-              tma_box(dst + cb * toks * 128, value ? &maps.v : &maps.k, cb * 64 + (value ? 0 : h * P::kKCols), tok & page_mask,
-                      head, pg, full + at);
-          }
-          __syncwarp();
-          ++issued;
-        }
-      }
-      if (!ok) give_up();
-      if (*stop)  // copies in flight land before the block ends
-        for (int k = max(0, issued - P::kStages); k < issued; ++k)
-          mbar_wait(full + k % P::kStages, static_cast<uint32_t>((k / P::kStages) & 1), kWaitNs);
-    } else {
-      const int lt = tid - 32 * P::kLoadWarp;
-      constexpr int kCh = P::kStage / 2 / 16 / 128;  // 16-byte pieces of codes per thread and stage
-      uint4 x[kCh];
-      float sk = 0.0f, sv = 0.0f;
-      // the codes of stage k of the order (kPer per item) into registers
-      auto fetch = [&](int k) {
-        bool value;
-        int j;
-        item(k / P::kPer, value, j);
-        const int h = k % P::kPer;
-        const int per_row = (value ? P::kVCols : P::kKCols) / 16;
-        const int j0 = R.tile(t_begin + j) * kTT + (value ? h * P::kVTok : 0);
-        const int64_t sp = value ? A.kv.v_page : A.kv.k_page, sh = value ? A.kv.v_head : A.kv.k_head,
-                      stt = value ? A.kv.v_token : A.kv.k_token;
-        const unsigned char* base = (value ? A.kv.v : A.kv.k) + head * sh + (value ? 0 : h * P::kKCols);
-#pragma unroll
-        for (int u = 0; u < kCh; ++u) {
-          const int id = lt + 128 * u, tr = id / per_row, ch = id % per_row;
-          const int tok = j0 + tr;
-          x[u] = make_uint4(0u, 0u, 0u, 0u);
-          if (R.seen_by_any(tok)) x[u] = __ldg(reinterpret_cast<const uint4*>(base + page_of(tok) * sp + (tok & page_mask) * stt + ch * 16));
-        }
-        // K items bring both scales of the tile, token lt per thread: the softmax reads V's too before
-        // V itself has to be there
-        if (!value && h == 0) {
-          const int tk = R.tile(t_begin + j) * kTT + lt;
-          sk = sv = 0.0f;
-          if (R.seen_by_any(tk)) {
-            const int64_t e = ((static_cast<int64_t>(page_of(tk)) * A.kv.kv_heads + head) << shift) + (tk & page_mask);
-            sk = __ldg(A.kv.k_scale + e);
-            sv = __ldg(A.kv.v_scale + e);
-          }
-        }
-      };
-      const int total = items * P::kPer;
-      bool ok = true;
-      if (total > 0) fetch(0);
-      for (int k = 0; k < total && !*stop; ++k) {
-        bool value;
-        int j;
-        item(k / P::kPer, value, j);
-        const int h = k % P::kPer;
-        const int at = k % P::kStages, round = k / P::kStages;
-        if (round > 0) ok = __all_sync(kFullMask, mbar_wait(freeb + at, static_cast<uint32_t>((round - 1) & 1), kWaitNs));
-        if (!ok) {
-          give_up();
-          break;
-        }
-        const int per_row = (value ? P::kVCols : P::kKCols) / 16;
+    // The stages of a bf16 cache are the operands themselves; of an 8-bit one the codes, which the
+    // widening warps turn into operands.
+    constexpr int kRing = P::kBf ? P::kStages : P::kRawStages;
+    constexpr int kRingStage = P::kBf ? P::kStage : P::kRawStage;
+    uint64_t* ring_full = P::kBf ? full : raw_full;
+    uint64_t* ring_free = P::kBf ? freeb : raw_free;
+    unsigned char* ring = sm + (P::kBf ? P::kOffStage : P::kOffRaw);
+    int issued = 0;
+    bool ok = true;
+    for (int i = 0; i < items && ok && !*stop; ++i) {
+      bool value;
+      int j;
+      item(i, value, j);
+      for (int h = 0; h < P::kPer; ++h) {
+        const int at = issued % kRing, round = issued / kRing;
+        if (round > 0) ok = __all_sync(kFullMask, mbar_wait(ring_free + at, static_cast<uint32_t>((round - 1) & 1), kWaitNs));
+        if (!ok) break;
         const int toks = value ? P::kVTok : P::kKTok;
-        unsigned char* st = sm + P::kOffStage + at * P::kStage;
-#pragma unroll
-        for (int u = 0; u < kCh; ++u) {
-          const int id = lt + 128 * u, tr = id / per_row, ch = id % per_row;
-          const uint2 a = widen_bf16<FMT>(x[u].x), b2 = widen_bf16<FMT>(x[u].y), c2 = widen_bf16<FMT>(x[u].z), d2 = widen_bf16<FMT>(x[u].w);
-          unsigned char* dst = st + (ch >> 2) * (toks * 128) + tr * 128;
-          const int c0 = (ch & 3) * 2;
-          *reinterpret_cast<uint4*>(dst + ((c0 ^ (tr & 7)) << 4)) = make_uint4(a.x, a.y, b2.x, b2.y);
-          *reinterpret_cast<uint4*>(dst + (((c0 + 1) ^ (tr & 7)) << 4)) = make_uint4(c2.x, c2.y, d2.x, d2.y);
+        const int box = min(1 << shift, toks);  // tokens per box
+        const int groups = toks / box;
+        const int cols = (value ? P::kVCols : P::kKCols) * P::kEl / P::kInner;
+        const int j0 = R.tile(t_begin + j) * kTT + (value ? h * P::kVTok : 0);
+        // lane g: token group g (at most 8); a group past every row's last token stays as it is
+        const int tok = j0 + lane * box;
+        const bool real = lane < groups && tok < R.hi;
+        const int pg = real ? page_of(tok) : 0;
+        const bool scales = !P::kBf && !value && h == 0;  // both scales of a tile come with its K codes
+        const unsigned live = __ballot_sync(kFullMask, real);
+        const uint32_t bytes = static_cast<uint32_t>(__popc(live) * box * (cols * P::kInner + (scales ? 8 : 0)));
+        if (lane == 0) {
+          if (bytes) mbar_expect_tx(ring_full + at, bytes);
+          else arrive_on(ring_full + at);
         }
-        if (!value && h == 0) {
-          float* sc = reinterpret_cast<float*>(sm + P::kOffScale) + (j % P::kScaleSlots) * (2 * kTT) + lt;
-          sc[0] = sk;
-          sc[kTT] = sv;
+        __syncwarp();
+        if (real) {
+          const uint32_t dst = smem_addr(ring + at * kRingStage) + lane * box * P::kInner;
+          for (int cb = 0; cb < cols; ++cb)
+            tma_box(dst + cb * toks * P::kInner, value ? &maps.v : &maps.k, cb * (P::kInner / P::kEl) + (value ? 0 : h * P::kKCols),
+                    tok & page_mask, head, pg, ring_full + at);
+          if (scales) {
+            const uint32_t sd = smem_addr(sm + P::kOffScale) + ((j % P::kScaleSlots) * 2 * kTT + lane * box) * 4;
+            const int64_t e = ((static_cast<int64_t>(pg) * A.kv.kv_heads + head) << shift) + (tok & page_mask);
+            bulk_in(sd, A.kv.k_scale + e, box * 4, ring_full + at);
+            bulk_in(sd + kTT * 4, A.kv.v_scale + e, box * 4, ring_full + at);
+          }
         }
-        fence_async();
-        arrive_on(full + at);
-        if (k + 1 < total) fetch(k + 1);
+        __syncwarp();
+        ++issued;
       }
+    }
+    if (!ok) give_up();
+    if (*stop)  // copies in flight land before the block ends
+      for (int k = max(0, issued - kRing); k < issued; ++k)
+        mbar_wait(ring_full + k % kRing, static_cast<uint32_t>((k / kRing) & 1), kWaitNs);
+    __syncwarp();
+  };
+
+  // ---------------- widening warps (8-bit): codes -> float16 operands ----------------
+  // V's scale goes into V here, relative to a power of two at or above every V scale so far (vref, from
+  // 2^-100 up, kept beside the tile's scales for the softmax) and times 2^7, which leaves the largest
+  // code within float16: rows whose scale is 2^-21 of the largest are still held to 2^-11.
+  auto widen = [&]() {
+    const int lt = tid - 32 * P::kWidenWarp;
+    constexpr int kPieces = P::kRawStage / 16 / 128;  // 16-byte pieces of codes per thread and stage
+    constexpr int kRowPieces = P::kInner / 16;
+    float vref = 7.888609052210118e-31f, vprev = vref;  // after K(j_last) and before it
+    int j_last = -1;
+    const int total = items * P::kPer;
+    for (int k = 0; k < total && !*stop; ++k) {
+      bool value;
+      int j;
+      item(k / P::kPer, value, j);
+      const int h = k % P::kPer;
+      const int rs = k % P::kRawStages, at = k % P::kStages;
+      bool ok = mbar_wait(raw_full + rs, static_cast<uint32_t>((k / P::kRawStages) & 1), kWaitNs);
+      if (k >= P::kStages) ok = ok && mbar_wait(freeb + at, static_cast<uint32_t>((k / P::kStages - 1) & 1), kWaitNs);
+      if (!__all_sync(kFullMask, ok)) {
+        give_up();
+        break;
+      }
+      const int j0 = R.tile(t_begin + j) * kTT;
+      float* sc = reinterpret_cast<float*>(sm + P::kOffScale) + (j % P::kScaleSlots) * (2 * kTT);
+      if (!value && h == 0) {
+        // every warp takes the tile's largest V scale of visible tokens (bits of positive floats in order)
+        uint32_t mx = 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const float v = sc[kTT + lane + 32 * u];
+          if (R.seen_by_any(j0 + lane + 32 * u) && v < INFINITY) mx = max(mx, __float_as_uint(fmaxf(v, 0.0f)));
+        }
+        mx = __reduce_max_sync(kFullMask, mx);
+        const float top = __uint_as_float(mx > 0x7e800000u ? 0x7f000000u : (mx + 0x7fffffu) & 0x7f800000u);  // up to a power of two
+        vprev = vref;
+        vref = fmaxf(vref, top);
+        j_last = j;
+        if (lt == 0) reinterpret_cast<float*>(sm + P::kOffRef)[j % P::kScaleSlots] = vref;
+      }
+      const float vinv = kVUp / (j == j_last ? vref : vprev);  // (K runs at most one tile ahead of V)
+      const int toks = value ? P::kVTok : P::kKTok;
+      const int jt = j0 + (value ? h * P::kVTok : 0);
+      const bool edge = jt + toks > R.hi || (jt < R.lo && jt + toks > R.sink);  // some token no row sees
+      const unsigned char* src = sm + P::kOffRaw + rs * P::kRawStage;
+      unsigned char* dst = sm + P::kOffStage + at * P::kStage;
+#pragma unroll
+      for (int u = 0; u < kPieces; ++u) {
+        const int id = lt + 128 * u, ch = id % kRowPieces, rowid = id / kRowPieces;
+        const int cb = rowid / toks, tr = rowid % toks;  // column block of kInner codes, token
+        const uint4 x = *reinterpret_cast<const uint4*>(src + id * 16);
+        uint2 q[4] = {widen_half<FMT>(x.x), widen_half<FMT>(x.y), widen_half<FMT>(x.z), widen_half<FMT>(x.w)};
+        if (value) {
+          const float f = sc[kTT + h * P::kVTok + tr] * vinv;
+          const uint32_t f2 = half2_of(f, f);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) q[i].x = half2_mul(q[i].x, f2), q[i].y = half2_mul(q[i].y, f2);
+          if (edge && !R.seen_by_any(jt + tr)) q[0] = q[1] = q[2] = q[3] = make_uint2(0u, 0u);
+        }
+        const int hc = cb * (P::kInner / 64) + (ch >> 2);  // 64-column operand block
+        const int c0 = (ch & 3) * 2, odd = hc & 1;
+        unsigned char* rowp = dst + hc * (toks * 128) + tr * 128;
+        // (lanes of the two blocks store their halves in opposite order: no two in one bank)
+        const uint4 lo = make_uint4(q[0].x, q[0].y, q[1].x, q[1].y), hi = make_uint4(q[2].x, q[2].y, q[3].x, q[3].y);
+        *reinterpret_cast<uint4*>(rowp + (((c0 + odd) ^ (tr & 7)) << 4)) = odd ? hi : lo;
+        *reinterpret_cast<uint4*>(rowp + (((c0 + 1 - odd) ^ (tr & 7)) << 4)) = odd ? lo : hi;
+      }
+      fence_async();
+      arrive_on(raw_free + rs);
+      arrive_on(full + at);
     }
     __syncwarp();
   };
@@ -387,12 +456,15 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
     const int row = r0 + min(r, R.rows - 1);
     const int p = R.p0 + row / A.group;
     const int lo = A.window ? max(p - A.window + 1, 0) : 0;
-    const float c = fmaxf(fabsf(A.scale_log2), 1e-30f);  // (0 would turn a hidden score's -inf into NaN)
+    float c = fabsf(A.scale_log2);
+    if constexpr (!P::kBf) c *= reinterpret_cast<const float*>(sm + P::kOffQf)[r];
+    c = fmaxf(c, 1e-30f);  // (0 would turn a hidden score's -inf into NaN)
     const float slack = 8.0f / c;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const uint32_t o_at = lane_base + 256u + static_cast<uint32_t>(s * D);
     float m = -INFINITY;
     float2 l2 = make_float2(0.0f, 0.0f);
+    float vref = 1.0f;  // (8-bit) what O is relative to
     for (int j = 0; j < n && !*stop; ++j) {
       const int buf = NQ == 2 ? s : (j & 1);
       const uint32_t ph = static_cast<uint32_t>((j / SB) & 1);
@@ -429,11 +501,15 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
       }
       const float tm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       const bool move = tm > m + slack || (m == -INFINITY && tm > m);
-      if (__any_sync(kFullMask, move)) {
+      float vnew = vref;
+      if constexpr (!P::kBf) vnew = reinterpret_cast<const float*>(sm + P::kOffRef)[j % P::kScaleSlots];
+      if (__any_sync(kFullMask, move || vnew != vref)) {
         const float mn = move ? tm : m;
-        const float al = m == -INFINITY ? 0.0f : ex2((m - mn) * c);
+        float al = m == -INFINITY ? 0.0f : ex2((m - mn) * c);
         m = mn;
         l2.x *= al, l2.y *= al;
+        al *= vref / vnew;
+        vref = vnew;
         if (j > 0) {
           bool ok = true;
           if constexpr (SB == 2) ok = mbar_wait(o_done, static_cast<uint32_t>((j - 1) & 1), kWaitNs);
@@ -460,11 +536,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
         float2 t = __ffma2_rn(make_float2(x[i], x[i + 1]), make_float2(c, c), make_float2(mc, mc));
         t.x = ex2(t.x), t.y = ex2(t.y);
         l2 = __fadd2_rn(l2, t);
-        if constexpr (!P::kBf) {
-          const float2 v2 = *reinterpret_cast<const float2*>(sc + kTT + i);
-          t = __fmul2_rn(t, v2);
-        }
-        w[i >> 1] = bf16x2(t.x, t.y);
+        w[i >> 1] = P::kBf ? bf16x2(t.x, t.y) : half2_of(t.x, t.y);
       }
       tm_st32(s_at, w);
       tm_st32(s_at + 32, w + 32);
@@ -488,7 +560,8 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
       const bool live = r < R.rows;
       const int64_t t = R.q0 + row / A.group;
       const int hq = head * A.group + row % A.group;
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const float ounit = P::kBf ? 1.0f : vref / kVUp;  // what O is in units of
+      const float inv = l == 0.0f ? 0.0f : ounit / l;
       const int64_t part = ((static_cast<int64_t>(b) * gridDim.y + rb * A.kv.kv_heads + head) * A.splits + split) * P::kRows + r;
 #pragma unroll
       for (int q = 0; q < D / 32; ++q) {
@@ -509,7 +582,8 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
         } else if (live) {
           float4* dst = reinterpret_cast<float4*>(A.part_o + part * D + 32 * q);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          for (int i = 0; i < 8; ++i)
+            dst[i] = make_float4(o[4 * i] * ounit, o[4 * i + 1] * ounit, o[4 * i + 2] * ounit, o[4 * i + 3] * ounit);
         }
       }
       if (live) {
@@ -541,7 +615,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
 #pragma unroll
           for (int k = 0; k < P::kKCols / 16; ++k) {
             const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-            mma_ss(tmem + buf * 128, desc_sw128(qa + off, 16), desc_sw128(ka + off, 16), kIdescQK, (h | k) != 0 ? 1u : 0u);
+            mma_ss(tmem + buf * 128, desc_sw128(qa + off, 16), desc_sw128(ka + off, 16), kIdescQK<P::kBf>, (h | k) != 0 ? 1u : 0u);
           }
         }
       }
@@ -598,7 +672,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
 #pragma unroll
             for (int k = 0; k < P::kVTok / 16; ++k)
               mma_ts(tmem + 256 + s * D, tmem + buf * 128 + (h * P::kVTok + k * 16) / 2, desc_sw128(va + k * 2048, P::kVTok * 128),
-                     kIdescPV<D>, (j | h | k) != 0 ? 1u : 0u);
+                     kIdescPV<D, P::kBf>, (j | h | k) != 0 ? 1u : 0u);
           }
           commit_to(o_done + s);
           if (s == NQ - 1)
@@ -626,12 +700,12 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
     if (leader) commit_to(m_done);
     __syncwarp();
     if (!__all_sync(kFullMask, mbar_wait(m_done, 0, kWaitNs))) give_up();
-   } else if constexpr (P::kBf) {
-    if (warp == P::kLoadWarp) load();
+   } else if (warp == P::kLoadWarp) {
+    load();
    }
-  } else {
-   if constexpr (!P::kBf) set_regs<P::kRegs, P::kLoadRegs>();
-   load();
+  } else if constexpr (!P::kBf) {
+   set_regs<P::kRegs, P::kLoadRegs>();
+   widen();
   }
   fence_before();
   __syncthreads();
@@ -693,12 +767,13 @@ cudaError_t launch_attn_tile(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) 
   return c->d.head_dim == 64 ? go_fmt<64>(c, a, st) : c->d.head_dim == 128 ? go_fmt<128>(c, a, st) : go_fmt<256>(c, a, st);
 }
 
-// The bf16 pools as (head_dim, page token, head, page) tensors, boxes of 64 columns (one
-// 128-byte swizzle row) by as many tokens as a page and a stage share.
+// The pools as (head_dim, page token, head, page) tensors, boxes of at most 128 bytes of a row (bf16:
+// one swizzle row) by as many tokens as a page and a stage share.
 const char* make_attn_maps(gs_kv_cache* c) {
   static_assert(sizeof(TileMaps) <= sizeof(c->maps), "room for two tensor maps");
   const gs_kv_cache_desc& d = c->d;
-  if (d.format != GS_DTYPE_BF16) return nullptr;
+  const bool bf16 = d.format == GS_DTYPE_BF16;
+  const cuuint64_t el = bf16 ? 2 : 1;
   void* fn = nullptr;
   cudaDriverEntryPointQueryResult res;
   if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &res) != cudaSuccess ||
@@ -711,14 +786,14 @@ const char* make_attn_maps(gs_kv_cache* c) {
   for (int v = 0; v < 2; ++v) {
     const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d.head_dim), static_cast<cuuint64_t>(d.page_size),
                                 static_cast<cuuint64_t>(d.kv_heads), static_cast<cuuint64_t>(d.pages)};
-    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(v ? d.v_token_stride : d.k_token_stride) * 2,
-                                   static_cast<cuuint64_t>(v ? d.v_head_stride : d.k_head_stride) * 2,
-                                   static_cast<cuuint64_t>(v ? d.v_page_stride : d.k_page_stride) * 2};
+    const cuuint64_t strides[3] = {static_cast<cuuint64_t>(v ? d.v_token_stride : d.k_token_stride) * el,
+                                   static_cast<cuuint64_t>(v ? d.v_head_stride : d.k_head_stride) * el,
+                                   static_cast<cuuint64_t>(v ? d.v_page_stride : d.k_page_stride) * el};
     const int most = v && d.head_dim == 256 ? 64 : kTT;
-    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(d.page_size < most ? d.page_size : most), 1, 1};
+    const cuuint32_t box[4] = {static_cast<cuuint32_t>(bf16 ? 64 : d.head_dim < 128 ? 64 : 128), static_cast<cuuint32_t>(d.page_size < most ? d.page_size : most), 1, 1};
     const cuuint32_t ones[4] = {1, 1, 1, 1};
-    const CUresult r = encode(v ? &m->v : &m->k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, v ? d.v : d.k, dims, strides, box, ones,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+    const CUresult r = encode(v ? &m->v : &m->k, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, v ? d.v : d.k, dims, strides, box, ones,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, bf16 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return "KV cache: these strides do not make a tensor map";
   }

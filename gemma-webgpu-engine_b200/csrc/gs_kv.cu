@@ -266,6 +266,8 @@ gs_status gs_kv_cache_create(gs_ctx* ctx, const gs_kv_cache_desc* d, gs_kv_cache
   if (!d->k || !d->v) return bad(GS_EINVAL, "KV cache: k and v are required");
   if (d->format != GS_DTYPE_BF16 && (!d->k_scale || !d->v_scale))
     return bad(GS_EINVAL, "KV cache: 8-bit formats need k_scale and v_scale");
+  if (reinterpret_cast<uintptr_t>(d->k_scale) % 16 || reinterpret_cast<uintptr_t>(d->v_scale) % 16)
+    return bad(GS_EINVAL, "KV cache: scales must be 16-byte aligned");
   const int64_t e = d->format == GS_DTYPE_BF16 ? 2 : 1;
   const int64_t strides[6] = {d->k_page_stride, d->k_head_stride, d->k_token_stride,
                               d->v_page_stride, d->v_head_stride, d->v_token_stride};

@@ -8,9 +8,15 @@ page · page_size + offset; a sequence's cached token j lies in page page_table[
 from __future__ import annotations
 
 import ctypes
+import struct
 
 from . import _lib
 from .sampling import SamplerError
+
+# gs_kv_rows and gs_attention_args, packed in one go (a field-wise fill of the ctypes structures costs
+# the host more than the launch)
+_KV_ROWS = struct.Struct("=2Q4qQqi4x")
+_ATTENTION_ARGS = struct.Struct("=6Q7q6if4x")
 
 
 class GpuKvCache:
@@ -51,6 +57,8 @@ class GpuKvCache:
         d.pages, d.page_size, d.kv_heads, d.head_dim, d.format = pages, page_size, heads, dim, formats[k.dtype]
         d.k_page_stride, d.k_head_stride, d.k_token_stride = k.stride()[:3]
         d.v_page_stride, d.v_head_stride, d.v_token_stride = v.stride()[:3]
+        self._int32, self._bf16 = torch.int32, torch.bfloat16
+        self._types = {torch.bfloat16: _lib.GS_DTYPE_BF16, torch.float32: _lib.GS_DTYPE_F32}
         self._h = ctypes.c_void_p()
         st = self._L.gs_kv_cache_create(sampler.handle, ctypes.byref(d), ctypes.byref(self._h))
         if st != _lib.GS_OK:
@@ -86,24 +94,24 @@ class GpuKvCache:
         raise ValueError(msg) if st == _lib.GS_EINVAL else SamplerError(st, msg)
 
     def _index(self, t, what, dims):
-        if t.dtype != self._torch.int32 or t.dim() != dims or t.device != self._device:
+        if t.dtype is not self._int32 or t.dim() != dims or t.get_device() != self._sampler.device:
             raise ValueError(f"{what} must be an int32 tensor of {dims} dimension(s) on the sampler's device")
-        if t.shape[-1] > 1 and t.stride(-1) != 1:
+        if not t.is_contiguous() and t.shape[-1] > 1 and t.stride(-1) != 1:
             raise ValueError(f"{what} must be contiguous")
 
     def _move(self, call, k, v, slots, stream):
-        torch = self._torch
         self._index(slots, "slots", 1)
-        n = slots.shape[0]
-        if k.dtype != v.dtype or k.dtype not in (torch.bfloat16, torch.float32):
+        dtype = self._types.get(k.dtype)
+        if dtype is None or v.dtype is not k.dtype:
             raise ValueError("k and v must both be float32 or bfloat16")
-        for t in (k, v):
-            if tuple(t.shape) != (n, self.kv_heads, self.head_dim) or t.stride(2) != 1 or t.device != self._device:
-                raise ValueError(f"k and v must be [{n}, {self.kv_heads}, {self.head_dim}] with contiguous rows on the device")
-        r = _lib.GsKvRows(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                          slots.data_ptr(), n,
-                          _lib.GS_DTYPE_BF16 if k.dtype == torch.bfloat16 else _lib.GS_DTYPE_F32)
-        st = call(self._h, ctypes.byref(r), _lib.current_stream(self._device) if stream is None else stream)
+        n = slots.shape[0]
+        shape, dev = (n, self.kv_heads, self.head_dim), self._sampler.device
+        k0, k1, k2 = k.stride() if k.dim() == 3 else (0, 0, 0)
+        v0, v1, v2 = v.stride() if v.dim() == 3 else (0, 0, 0)
+        if k.shape != shape or v.shape != shape or k2 != 1 or v2 != 1 or k.get_device() != dev or v.get_device() != dev:
+            raise ValueError(f"k and v must be {list(shape)} with contiguous rows on the sampler's device")
+        st = call(self._h, _KV_ROWS.pack(k.data_ptr(), v.data_ptr(), k0, k1, v0, v1, slots.data_ptr(), n, dtype),
+                  _lib.current_stream(self._device) if stream is None else stream)
         if st != _lib.GS_OK:
             self._fail(st)
 
@@ -115,10 +123,10 @@ class GpuKvCache:
     def read(self, slots, out=None, dtype=None, stream=None):
         """(k, v) [tokens, kv_heads, head_dim] at ``slots`` as ``dtype`` (bfloat16, or float32)."""
         if out is None:
-            shape = (slots.shape[0], self.kv_heads, self.head_dim)
+            heads, dim = self.kv_heads, self.head_dim
             t = self._torch.bfloat16 if dtype is None else dtype
-            out = (self._torch.empty(shape, dtype=t, device=self._device),
-                   self._torch.empty(shape, dtype=t, device=self._device))
+            k = self._torch.empty_strided((slots.shape[0], heads, dim), (heads * dim, dim, 1), dtype=t, device=self._device)
+            out = (k, self._torch.empty_like(k))
         self._move(self._L.gs_kv_read, out[0], out[1], slots, stream)
         return out
 
@@ -128,46 +136,47 @@ class GpuKvCache:
         sequence b has tokens [q_start[b], q_start[b + 1]) (None: one each) and kv_len[b] cached
         tokens, its new ones last.  ``window`` > 0: a token sees the last ``window`` positions and
         the first ``sinks``.  Returns (out like q, log-sum-exp [tokens, q_heads] or None)."""
-        torch = self._torch
-        if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[2] != self.head_dim or q.device != self._device:
-            raise ValueError(f"q must be bfloat16 [tokens, q_heads, {self.head_dim}] on the sampler's device")
-        if q.stride(2) != 1:
+        torch, dim, dev = self._torch, self.head_dim, self._sampler.device
+        if q.dtype is not self._bf16 or q.dim() != 3 or q.shape[2] != dim or q.get_device() != dev:
+            raise ValueError(f"q must be bfloat16 [tokens, q_heads, {dim}] on the sampler's device")
+        tokens, heads, _ = q.shape
+        # (a stride over a single token or head is never used: it is set to one that passes the checks)
+        qt, qh, qd = q.stride()
+        qt, qh = qt if tokens > 1 else heads * dim, qh if heads > 1 else dim
+        if qd != 1:
             raise ValueError("q rows must be contiguous")
-        tokens, heads, dim = q.shape
         self._index(kv_len, "kv_len", 1)
         self._index(page_table, "page_table", 2)
         seqs = kv_len.shape[0]
-        if page_table.shape[0] != seqs:
+        rows, cols = page_table.shape
+        if rows != seqs:
             raise ValueError("page_table must have one row per sequence")
-        a = _lib.GsAttentionArgs()
+        starts = 0
         if q_start is not None:
             self._index(q_start, "q_start", 1)
             if q_start.shape[0] != seqs + 1:
                 raise ValueError("q_start must hold one entry more than kv_len")
-            a.q_start = q_start.data_ptr()
+            starts = q_start.data_ptr()
         if out is None:
-            out = torch.empty((tokens, heads, dim), dtype=torch.bfloat16, device=self._device)
-        elif out.dtype != torch.bfloat16 or out.shape != q.shape or out.stride(2) != 1 or out.device != self._device:
-            raise ValueError("out must be bfloat16 of q's shape with contiguous rows")
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            ot, oh = heads * dim, dim
+        else:
+            if out.dtype is not self._bf16 or out.shape != q.shape or out.stride(2) != 1 or out.get_device() != dev:
+                raise ValueError("out must be bfloat16 of q's shape with contiguous rows on the sampler's device")
+            ot = out.stride(0) if tokens > 1 else heads * dim
+            oh = out.stride(1) if heads > 1 else dim
         if lse_out is not None:
-            if lse_out.dtype != torch.float32 or tuple(lse_out.shape) != (tokens, heads) or not lse_out.is_contiguous():
-                raise ValueError("lse_out must be contiguous float32 [tokens, q_heads]")
+            if lse_out.dtype != torch.float32 or lse_out.shape != (tokens, heads) or not lse_out.is_contiguous() or \
+                    lse_out.get_device() != dev:
+                raise ValueError("lse_out must be contiguous float32 [tokens, q_heads] on the sampler's device")
         elif lse:
-            lse_out = torch.empty((tokens, heads), dtype=torch.float32, device=self._device)
-        a.q, a.out, a.kv_len, a.page_table = q.data_ptr(), out.data_ptr(), kv_len.data_ptr(), page_table.data_ptr()
-        if lse_out is not None:
-            a.lse = lse_out.data_ptr()
-        # (a stride over a single token or head is never used: it is set to one that passes the checks)
-        a.q_token_stride = q.stride(0) if tokens > 1 else heads * dim
-        a.q_head_stride = q.stride(1) if heads > 1 else dim
-        a.out_token_stride = out.stride(0) if tokens > 1 else heads * dim
-        a.out_head_stride = out.stride(1) if heads > 1 else dim
-        a.tokens, a.seqs, a.q_heads = tokens, seqs, heads
-        a.page_table_cols = page_table.shape[1]
-        a.page_table_stride = page_table.stride(0) if seqs > 1 else page_table.shape[1]
-        a.max_q, a.max_kv, a.window, a.sinks, a.scale = max_q, max_kv, window, sinks, scale
-        st = self._L.gs_attention(self._h, ctypes.byref(a),
-                                  _lib.current_stream(self._device) if stream is None else stream)
+            lse_out = torch.empty_strided((tokens, heads), (heads, 1), dtype=torch.float32, device=self._device)
+        st = self._L.gs_attention(
+            self._h, _ATTENTION_ARGS.pack(
+                q.data_ptr(), out.data_ptr(), lse_out.data_ptr() if lse_out is not None else 0, starts, kv_len.data_ptr(),
+                page_table.data_ptr(), tokens, qt, qh, ot, oh, page_table.stride(0) if seqs > 1 else cols, cols, seqs, heads,
+                max_q, max_kv, window, sinks, scale),
+            _lib.current_stream(self._device) if stream is None else stream)
         if st != _lib.GS_OK:
             self._fail(st)
         return out, lse_out

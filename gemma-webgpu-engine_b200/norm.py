@@ -7,14 +7,16 @@ scale per row or per group of columns, or (``srq_scale``) on the int8 grid that
 """
 from __future__ import annotations
 
-import ctypes
+import struct
 from dataclasses import dataclass
 
 from . import _lib
 from .sampling import SamplerError
 
+_RMS_NORM_ARGS = struct.Struct("=7Q6q4i3f4x")  # gs_rms_norm_args
 
-@dataclass
+
+@dataclass(slots=True)
 class RmsNormResult:
     out: object              # [rows, hidden] of the output type
     scale: object = None     # [rows, groups] float32 (e4m3)
@@ -52,72 +54,55 @@ class GpuRmsNorm:
         self._device = torch.device("cuda", sampler.device)
         self._out_type = {"bf16": torch.bfloat16, "f32": torch.float32, "e4m3": torch.float8_e4m3fn,
                           "srq": torch.float32}[out]
-        a = _lib.GsRmsNormArgs()
-        if weight is not None:
-            a.weight = weight.data_ptr()
-            a.weight_dtype = _lib.GS_DTYPE_BF16 if weight.dtype == torch.bfloat16 else _lib.GS_DTYPE_F32
-        a.hidden = self.hidden
-        a.out_dtype = {"bf16": _lib.GS_DTYPE_BF16, "f32": _lib.GS_DTYPE_F32, "e4m3": _lib.GS_DTYPE_E4M3,
-                       "srq": _lib.GS_DTYPE_F32}[out]
-        a.group = self.group
-        a.eps, a.weight_offset, a.srq_scale = float(eps), float(weight_offset), float(srq_scale)
-        self._fixed = bytes(a)
+        # gs_rms_norm_args is filled by one struct.pack a call: (pointers, sizes, types) around what is fixed
+        self._weight_ptr = weight.data_ptr() if weight is not None else 0
+        self._tail = (_lib.GS_DTYPE_BF16 if weight is not None and weight.dtype == torch.bfloat16 else _lib.GS_DTYPE_F32,
+                      {"bf16": _lib.GS_DTYPE_BF16, "f32": _lib.GS_DTYPE_F32, "e4m3": _lib.GS_DTYPE_E4M3,
+                       "srq": _lib.GS_DTYPE_F32}[out], self.group, float(eps), float(weight_offset), float(srq_scale))
+        self._types = {torch.bfloat16: _lib.GS_DTYPE_BF16, torch.float32: _lib.GS_DTYPE_F32}
 
-    def _rows(self, t, what, like=None):
-        if t.dim() != 2 or t.shape[1] != self.hidden:
-            raise ValueError(f"{what} must be [rows, {self.hidden}]")
-        if t.stride(1) != 1 and self.hidden > 1:
+    def _stride(self, t, what, rows, dtype):
+        if t.dtype is not dtype or t.get_device() != self._sampler.device or t.shape != (rows, self.hidden):
+            raise ValueError(f"{what} must be {dtype} [{rows}, {self.hidden}] on the sampler's device")
+        s0, s1 = t.stride()
+        if s1 != 1 and self.hidden > 1:
             raise ValueError(f"{what} rows must be contiguous")
-        if t.device != self._device:
-            raise ValueError(f"{what} must be on the sampler's device")
-        if like is not None and (t.dtype != like.dtype or t.shape[0] != like.shape[0]):
-            raise ValueError(f"{what} must have x's type and rows")
-        return t.stride(0) if t.shape[0] > 1 else self.hidden
+        return s0 if rows > 1 else self.hidden
 
     def __call__(self, x, residual=None, *, out: RmsNormResult | None = None, stream=None) -> RmsNormResult:
         """The norm of x (+ residual), both [rows, hidden] float32 or bfloat16.  ``out``: a result
         to write into (its ``residual`` may be the residual itself)."""
-        torch = self._torch
-        if x.dtype == torch.bfloat16:
-            dtype = _lib.GS_DTYPE_BF16
-        elif x.dtype == torch.float32:
-            dtype = _lib.GS_DTYPE_F32
-        else:
+        torch, hidden, xt = self._torch, self.hidden, x.dtype
+        dtype = self._types.get(xt)
+        if dtype is None:
             raise ValueError("x must be float32 or bfloat16")
-        a = _lib.GsRmsNormArgs.from_buffer_copy(self._fixed)
-        a.ld_x = self._rows(x, "x")
+        if x.dim() != 2:
+            raise ValueError(f"x must be [rows, {hidden}]")
         rows = x.shape[0]
-        a.dtype, a.rows, a.x = dtype, rows, x.data_ptr()
-        if residual is not None:
-            a.ld_residual = self._rows(residual, "residual", x)
-            a.residual = residual.data_ptr()
+        ld_x = self._stride(x, "x", rows, xt)
+        ld_r = self._stride(residual, "residual", rows, xt) if residual is not None else 0
         if out is None:
             dev = self._device
             out = RmsNormResult(
-                torch.empty((rows, self.hidden), dtype=self._out_type, device=dev),
-                torch.empty((rows, self.groups), dtype=torch.float32, device=dev) if self.out == "e4m3" else None,
-                torch.empty((rows, self.hidden), dtype=x.dtype, device=dev) if residual is not None else None,
+                torch.empty_like(x, dtype=self._out_type, memory_format=torch.contiguous_format),
+                torch.empty_strided((rows, self.groups), (self.groups, 1), dtype=torch.float32, device=dev)
+                if self.out == "e4m3" else None,
+                torch.empty_like(x, memory_format=torch.contiguous_format) if residual is not None else None,
                 torch.empty(rows, dtype=torch.float32, device=dev) if self.out == "srq" else None)
-            a.ld_out = a.ld_residual_out = self.hidden
+            ld_out = ld_ro = hidden
         else:
-            a.ld_out = self._rows(out.out, "out.out")
-            if out.out.dtype != self._out_type or out.out.shape[0] != rows:
-                raise ValueError("out.out must have the output type and x's rows")
-            if out.residual is not None:
-                a.ld_residual_out = self._rows(out.residual, "out.residual", x)
+            ld_out = self._stride(out.out, "out.out", rows, self._out_type)
+            ld_ro = self._stride(out.residual, "out.residual", rows, xt) if out.residual is not None else 0
             for t, shape in ((out.scale, (rows, self.groups)), (out.row_sum, (rows,))):
-                if t is not None and (t.dtype != torch.float32 or tuple(t.shape) != shape or not t.is_contiguous()):
-                    raise ValueError(f"out's scale and row_sum must be contiguous float32 {shape}")
-        a.out = out.out.data_ptr()
-        if out.residual is not None:
-            a.residual_out = out.residual.data_ptr()
-        if out.scale is not None:
-            a.out_scale = out.scale.data_ptr()
-        if out.row_sum is not None:
-            a.row_sum = out.row_sum.data_ptr()
-        if stream is None:
-            stream = _lib.current_stream(self._device)
-        st = self._L.gs_rms_norm(self._sampler.handle, ctypes.byref(a), stream)
+                if t is not None and (t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous() or
+                                      t.get_device() != self._sampler.device):
+                    raise ValueError(f"out's scale and row_sum must be contiguous float32 {shape} on the sampler's device")
+        a = _RMS_NORM_ARGS.pack(
+            x.data_ptr(), residual.data_ptr() if residual is not None else 0, self._weight_ptr,
+            out.residual.data_ptr() if out.residual is not None else 0, out.out.data_ptr(),
+            out.scale.data_ptr() if out.scale is not None else 0, out.row_sum.data_ptr() if out.row_sum is not None else 0,
+            rows, hidden, ld_x, ld_r, ld_ro, ld_out, dtype, *self._tail)
+        st = self._L.gs_rms_norm(self._sampler.handle, a, _lib.current_stream(self._device) if stream is None else stream)
         if st != _lib.GS_OK:
             msg = self._sampler.last_error()
             raise ValueError(msg) if st == _lib.GS_EINVAL else SamplerError(st, msg)

@@ -123,10 +123,11 @@ def test_split_context(pkg, sampler, form, lens, window, sinks):
 
 
 @pytest.mark.parametrize("form", FORMS)
-def test_large_scores_and_spread_scales(pkg, sampler, form):
+@pytest.mark.parametrize("lens,dim", [([(1, 500), (3, 300)], 128), ([(40, 700)], 64), ([(40, 700)], 128), ([(40, 700)], 256)])
+def test_large_scores_and_spread_scales(pkg, sampler, form, lens, dim):
     """Scores far apart (one token takes nearly all the weight, late in the context), and cached
     rows whose scales differ by orders of magnitude."""
-    c = Case(sampler, pkg, [(1, 500), (3, 300)], 2, 4, 128, 16, form, seed=3)
+    c = Case(sampler, pkg, lens, 2, 4, dim, 16, form, seed=3)
     c.scale = 1.0
     if form != "bf16":
         f = torch.exp2(torch.randint(-12, 5, c.cache.v_scale.shape, device="cuda").float())

@@ -47,3 +47,16 @@ def test_null_handles_and_arguments_are_refused(pkg):
     assert lib.gs_kv_cache_check(None, None) == L.GS_EINVAL
     assert lib.gs_kv_cache_destroy(None) == L.GS_OK
     assert lib.gs_kv_cache_last_error(None) == b""
+
+
+def test_packed_arguments_have_the_structs_layout(pkg):
+    """norm.py and kv_cache.py pack the argument structures with struct formats."""
+    import importlib
+    norm = importlib.import_module("gemma-webgpu-engine_b200.norm")
+    kv = importlib.import_module("gemma-webgpu-engine_b200.kv_cache")
+    L = pkg._lib
+    for packer, cls in ((norm._RMS_NORM_ARGS, L.GsRmsNormArgs), (kv._KV_ROWS, L.GsKvRows), (kv._ATTENTION_ARGS, L.GsAttentionArgs)):
+        assert packer.size == ctypes.sizeof(cls), cls
+        values = [i + 1 for i in range(len(cls._fields_))]
+        got = cls.from_buffer_copy(packer.pack(*values))
+        assert [int(getattr(got, f)) for f, _ in cls._fields_] == values
