@@ -30,11 +30,22 @@ struct KvPool {
   const unsigned char* v;
   const float* k_scale;
   const float* v_scale;
-  int64_t k_page, k_head, k_token;  // byte strides
-  int64_t v_page, v_head, v_token;
+  // strides in 16-byte pieces: each product below is one 32 x 32 -> 64-bit multiply-add
+  uint32_t k_page, k_head, k_token;
+  uint32_t v_page, v_head, v_token;
   int32_t pages;
   int32_t page_shift;
   int32_t kv_heads;
+  __device__ __forceinline__ const unsigned char* at(bool value, int page, int head, int off) const {
+    const uint64_t e = static_cast<uint64_t>(static_cast<uint32_t>(page)) * (value ? v_page : k_page) +
+                       static_cast<uint64_t>(static_cast<uint32_t>(head)) * (value ? v_head : k_head) +
+                       static_cast<uint64_t>(static_cast<uint32_t>(off)) * (value ? v_token : k_token);
+    return (value ? v : k) + (e << 4);
+  }
+  __device__ __forceinline__ const float* scale_at(bool value, int page, int head, int off) const {
+    const uint64_t e = static_cast<uint64_t>(static_cast<uint32_t>(page)) * static_cast<uint32_t>(kv_heads) + static_cast<uint32_t>(head);
+    return (value ? v_scale : k_scale) + (e << page_shift) + off;
+  }
 };
 
 struct AttnArgs {

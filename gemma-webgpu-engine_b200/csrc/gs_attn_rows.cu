@@ -225,21 +225,21 @@ __global__ void __launch_bounds__(kRowsThreads) attn_rows_kernel(const __grid_co
     if (i < i_end) {
       const int j0 = R.tile(i) * kRT;
       const int off = j0 & ((1 << A.kv.page_shift) - 1);
-      const int64_t pg = page < 0 ? 0 : page;
-      const unsigned char* kp = A.kv.k + pg * A.kv.k_page + head * A.kv.k_head + off * A.kv.k_token;
-      const unsigned char* vp = A.kv.v + pg * A.kv.v_page + head * A.kv.v_head + off * A.kv.v_token;
+      const int pg = page < 0 ? 0 : page;
+      const unsigned char* kp = A.kv.at(false, pg, head, off);
+      const unsigned char* vp = A.kv.at(true, pg, head, off);
       const uint32_t ks = ring_s + stage * P::kStage, vs = ks + P::kTileBytes;
 #pragma unroll
       for (int u = 0; u < P::kChunks / 2; ++u) {
         const int id = lane + 32 * u, r = id / P::kChunks, ch = id % P::kChunks;
         const bool real = page >= 0 && R.seen_by_any(j0 + r);
         const uint32_t at = piece<P::kChunks>(r, ch);
-        cp_async16(ks + at, kp + r * A.kv.k_token + ch * 16, real);
-        cp_async16(vs + at, vp + r * A.kv.v_token + ch * 16, real);
+        cp_async16(ks + at, kp + (static_cast<uint64_t>(static_cast<uint32_t>(r)) * A.kv.k_token + ch) * 16, real);
+        cp_async16(vs + at, vp + (static_cast<uint64_t>(static_cast<uint32_t>(r)) * A.kv.v_token + ch) * 16, real);
       }
       if constexpr (!kBf) {
         const int r = lane & 15;
-        const float* sc = (lane < 16 ? A.kv.k_scale : A.kv.v_scale) + ((pg * A.kv.kv_heads + head) << A.kv.page_shift) + off + r;
+        const float* sc = A.kv.scale_at(lane >= 16, pg, head, off + r);
         cp_async4(ks + 2 * P::kTileBytes + lane * 4, sc, page >= 0 && R.seen_by_any(j0 + r));
       }
     }

@@ -357,9 +357,8 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
                     tok & page_mask, head, pg, ring_full + at);
           if (scales) {
             const uint32_t sd = smem_addr(sm + P::kOffScale) + ((j % P::kScaleSlots) * 2 * kTT + lane * box) * 4;
-            const int64_t e = ((static_cast<int64_t>(pg) * A.kv.kv_heads + head) << shift) + (tok & page_mask);
-            bulk_in(sd, A.kv.k_scale + e, box * 4, ring_full + at);
-            bulk_in(sd + kTT * 4, A.kv.v_scale + e, box * 4, ring_full + at);
+            bulk_in(sd, A.kv.scale_at(false, pg, head, tok & page_mask), box * 4, ring_full + at);
+            bulk_in(sd + kTT * 4, A.kv.scale_at(true, pg, head, tok & page_mask), box * 4, ring_full + at);
           }
         }
         __syncwarp();

@@ -18,20 +18,20 @@ struct KvRowsArgs {
   KvPool kv;
   unsigned char* k;  // the caller's rows
   unsigned char* v;
-  int64_t k_token, k_head, v_token, v_head;  // elements
+  uint32_t k_token, k_head, v_token, v_head;  // elements
   const int32_t* slots;
-  int64_t rows;      // tokens · kv_heads
+  int64_t tokens;
   int64_t slots_end; // pages · page_size
   int32_t* flag;
 };
 
 struct SlotAt {
-  int64_t page;
+  int32_t page;
   int32_t off;
   bool ok;
 };
 
-__device__ __forceinline__ SlotAt slot_at(const KvRowsArgs& A, int64_t token) {
+__device__ __forceinline__ SlotAt slot_at(const KvRowsArgs& A, uint32_t token) {
   const int32_t s = __ldg(A.slots + token);
   SlotAt r;
   r.ok = s >= 0 && s < A.slots_end;
@@ -41,19 +41,11 @@ __device__ __forceinline__ SlotAt slot_at(const KvRowsArgs& A, int64_t token) {
   return r;
 }
 
-template <bool BF16, bool VEC>
-__device__ __forceinline__ void load8(const void* p, float (&x)[8]) {
-  if constexpr (VEC) {
-    load_row<8, BF16>(p, x);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float y[1];
-      load_row<1, BF16>(static_cast<const unsigned char*>(p) + i * (BF16 ? 2 : 4), y);
-      x[i] = y[0];
-    }
-  }
+// Element offset of (token, head) in the caller's rows.
+__device__ __forceinline__ uint64_t row_at(const KvRowsArgs& A, bool value, uint32_t token, uint32_t head) {
+  return static_cast<uint64_t>(token) * (value ? A.v_token : A.k_token) + static_cast<uint64_t>(head) * (value ? A.v_head : A.k_head);
 }
+
 template <bool BF16, bool VEC>
 __device__ __forceinline__ void store8(void* p, const float (&x)[8]) {
   if constexpr (VEC) {
@@ -67,102 +59,149 @@ __device__ __forceinline__ void store8(void* p, const float (&x)[8]) {
   }
 }
 
-template <int D, int FMT, bool BF16, bool VEC>
-__global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ KvRowsArgs A) {
+// U tokens per group of lanes, `step` apart, their loads issued together: one row (16 bytes a thread)
+// keeps too few bytes in flight for a long chunk, and a step's few rows are better spread.
+template <int D, int FMT, bool BF16, bool VEC, int U>
+__global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ KvRowsArgs A, uint32_t step) {
   constexpr int kLanes = D / 8;
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / kLanes;
+  const uint32_t row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  const uint32_t token0 = row / static_cast<uint32_t>(A.kv.kv_heads);
+  const int head = static_cast<int>(row - token0 * A.kv.kv_heads);
   const int at = (threadIdx.x % kLanes) * 8;
   const bool value = blockIdx.y != 0;
-  const bool live = row < A.rows;
-  const int64_t token = live ? row / A.kv.kv_heads : 0;
-  const int head = live ? static_cast<int>(row % A.kv.kv_heads) : 0;
-  float x[8] = {};
-  SlotAt s{0, 0, false};
-  if (live) {
-    s = slot_at(A, token);
-    const int64_t e = value ? token * A.v_token + head * A.v_head : token * A.k_token + head * A.k_head;
-    if (s.ok) load8<BF16, VEC>((value ? A.v : A.k) + (e + at) * (BF16 ? 2 : 4), x);
+  constexpr int kWords = BF16 ? 1 : 2;
+  uint4 raw[U][kWords];
+  SlotAt s[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t token = token0 + u * step;
+    s[u] = SlotAt{0, 0, false};
+    if (token0 < step && token < A.tokens) s[u] = slot_at(A, token);
   }
-  unsigned char* pool = const_cast<unsigned char*>(value ? A.kv.v : A.kv.k);
-  pool += value ? s.page * A.kv.v_page + head * A.kv.v_head + s.off * A.kv.v_token
-                : s.page * A.kv.k_page + head * A.kv.k_head + s.off * A.kv.k_token;
-  if constexpr (FMT == GS_DTYPE_BF16) {
-    if (s.ok) store_row<8, true>(pool + at * 2, x);
-  } else {
-    constexpr float kMax = FMT == GS_DTYPE_E4M3 ? kE4m3Max : kInt8Max;
-    int m = 0;  // bits of max|x|: integer order is value order, NaN above all
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_int(x[i]) & 0x7fffffff);
+  for (int u = 0; u < U; ++u) {
 #pragma unroll
-    for (int o = kLanes >> 1; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(kFullMask, m, o));
-    const float inv = quant_inv(__int_as_float(m), kMax);
-    if (s.ok) {
-      uint2 c;
-      if constexpr (FMT == GS_DTYPE_E4M3) {
-        c.x = e4m3x4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-        c.y = e4m3x4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
-      } else {
-        c.x = int8x4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv);
-        c.y = int8x4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv);
-      }
-      *reinterpret_cast<uint2*>(pool + at) = c;
-      if (at == 0) {
-        float* sc = const_cast<float*>(value ? A.kv.v_scale : A.kv.k_scale);
-        sc[((s.page * A.kv.kv_heads + head) << A.kv.page_shift) + s.off] = quant_scale(__int_as_float(m), kMax);
+    for (int i = 0; i < kWords; ++i) raw[u][i] = make_uint4(0u, 0u, 0u, 0u);
+    if (!s[u].ok) continue;
+    const unsigned char* src = (value ? A.v : A.k) + (row_at(A, value, token0 + u * step, head) + at) * (BF16 ? 2 : 4);
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) raw[u][i] = reinterpret_cast<const uint4*>(src)[i];
+    } else if constexpr (BF16) {
+      const unsigned short* h = reinterpret_cast<const unsigned short*>(src);
+      raw[u][0] = make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
+    } else {
+      const uint32_t* h = reinterpret_cast<const uint32_t*>(src);
+      raw[u][0] = make_uint4(h[0], h[1], h[2], h[3]);
+      raw[u][kWords - 1] = make_uint4(h[4], h[5], h[6], h[7]);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    float v[8];
+    load_row<8, BF16>(raw[u], v);
+    unsigned char* pool = const_cast<unsigned char*>(A.kv.at(value, s[u].page, head, s[u].off));
+    if constexpr (FMT == GS_DTYPE_BF16) {
+      if (s[u].ok) store_row<8, true>(pool + at * 2, v);
+    } else {
+      constexpr float kMax = FMT == GS_DTYPE_E4M3 ? kE4m3Max : kInt8Max;
+      float m = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(v[i]));
+#pragma unroll
+      for (int o = kLanes >> 1; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(kFullMask, m, o));
+      const float inv = quant_inv(m, kMax);
+      if (s[u].ok) {
+        uint2 c;
+        if constexpr (FMT == GS_DTYPE_E4M3) {
+          c.x = e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+          c.y = e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+        } else {
+          c.x = int8x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+          c.y = int8x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+        }
+        *reinterpret_cast<uint2*>(pool + at) = c;
+        if (at == 0) *const_cast<float*>(A.kv.scale_at(value, s[u].page, head, s[u].off)) = quant_scale(m, kMax);
       }
     }
   }
 }
 
-template <int D, int FMT, bool BF16, bool VEC>
-__global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvRowsArgs A) {
+template <int D, int FMT, bool BF16, bool VEC, int U>
+__global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvRowsArgs A, uint32_t step) {
   constexpr int kLanes = D / 8;
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / kLanes;
-  if (row >= A.rows) return;
+  const uint32_t row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+  const uint32_t token0 = row / static_cast<uint32_t>(A.kv.kv_heads);
+  const int head = static_cast<int>(row - token0 * A.kv.kv_heads);
+  if (token0 >= step) return;
   const int at = (threadIdx.x % kLanes) * 8;
   const bool value = blockIdx.y != 0;
-  const int64_t token = row / A.kv.kv_heads;
-  const int head = static_cast<int>(row % A.kv.kv_heads);
-  const SlotAt s = slot_at(A, token);
-  float x[8] = {};
-  if (s.ok) {
-    const unsigned char* pool = value ? A.kv.v + s.page * A.kv.v_page + head * A.kv.v_head + s.off * A.kv.v_token
-                                      : A.kv.k + s.page * A.kv.k_page + head * A.kv.k_head + s.off * A.kv.k_token;
+  uint4 raw[U];  // 8 elements: bf16, or codes in .x and .y
+  float sc[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t token = token0 + u * step;
+    raw[u] = make_uint4(0u, 0u, 0u, 0u);
+    sc[u] = 0.0f;
+    if (token >= A.tokens) continue;
+    const SlotAt s = slot_at(A, token);
+    if (!s.ok) continue;
+    const unsigned char* pool = A.kv.at(value, s.page, head, s.off);
     if constexpr (FMT == GS_DTYPE_BF16) {
-      load_row<8, true>(pool + at * 2, x);
+      raw[u] = *reinterpret_cast<const uint4*>(pool + at * 2);
     } else {
       const uint2 c = *reinterpret_cast<const uint2*>(pool + at);
-      const float sc = (value ? A.kv.v_scale : A.kv.k_scale)[((s.page * A.kv.kv_heads + head) << A.kv.page_shift) + s.off];
-      const uint32_t w[2] = {c.x, c.y};
+      raw[u].x = c.x, raw[u].y = c.y;
+      sc[u] = *A.kv.scale_at(value, s.page, head, s.off);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t token = token0 + u * step;
+    if (token >= A.tokens) continue;
+    float x[8];
+    if constexpr (FMT == GS_DTYPE_BF16) {
+      const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[2 * i] = bf16_lo(w[i]), x[2 * i + 1] = bf16_hi(w[i]);
+    } else {
+      const uint32_t w[2] = {raw[u].x, raw[u].y};
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if constexpr (FMT == GS_DTYPE_E4M3) {
           const float2 a = half2_float2(e4m3x2_half2(w[i] & 0xffffu)), b = half2_float2(e4m3x2_half2(w[i] >> 16));
-          x[4 * i] = a.x * sc, x[4 * i + 1] = a.y * sc, x[4 * i + 2] = b.x * sc, x[4 * i + 3] = b.y * sc;
+          x[4 * i] = a.x * sc[u], x[4 * i + 1] = a.y * sc[u], x[4 * i + 2] = b.x * sc[u], x[4 * i + 3] = b.y * sc[u];
         } else {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            x[4 * i + k] = static_cast<float>(static_cast<int8_t>((w[i] >> (8 * k)) & 0xffu)) * sc;
+            x[4 * i + k] = static_cast<float>(static_cast<int8_t>((w[i] >> (8 * k)) & 0xffu)) * sc[u];
         }
       }
     }
+    store8<BF16, VEC>((value ? A.v : A.k) + (row_at(A, value, token, head) + at) * (BF16 ? 2 : 4), x);
   }
-  const int64_t e = value ? token * A.v_token + head * A.v_head : token * A.k_token + head * A.k_head;
-  store8<BF16, VEC>((value ? A.v : A.k) + (e + at) * (BF16 ? 2 : 4), x);
 }
 
-template <int D, int FMT, bool BF16>
-cudaError_t launch_rows2(const KvRowsArgs& a, bool write, bool vec, cudaStream_t st) {
-  const int64_t per = 256 / (D / 8);
-  const dim3 grid(static_cast<unsigned>((a.rows + per - 1) / per), 2);
+template <int D, int FMT, bool BF16, bool VEC>
+cudaError_t launch_rows3(const KvRowsArgs& a, bool write, cudaStream_t st) {
+  constexpr int64_t per = 256 / (D / 8);
+  constexpr int U = 4;
+  // (four rows a thread from about two blocks an SM on)
+  const bool many = VEC && a.tokens * a.kv.kv_heads >= 148 * 2 * per * U;
+  const uint32_t step = static_cast<uint32_t>(many ? (a.tokens + U - 1) / U : a.tokens);
+  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(step) * a.kv.kv_heads + per - 1) / per), 2);
   if (write) {
-    if (vec) kv_write_kernel<D, FMT, BF16, true><<<grid, 256, 0, st>>>(a);
-    else kv_write_kernel<D, FMT, BF16, false><<<grid, 256, 0, st>>>(a);
+    if (VEC && many) kv_write_kernel<D, FMT, BF16, VEC, VEC ? U : 1><<<grid, 256, 0, st>>>(a, step);
+    else kv_write_kernel<D, FMT, BF16, VEC, 1><<<grid, 256, 0, st>>>(a, step);
   } else {
-    if (vec) kv_read_kernel<D, FMT, BF16, true><<<grid, 256, 0, st>>>(a);
-    else kv_read_kernel<D, FMT, BF16, false><<<grid, 256, 0, st>>>(a);
+    if (VEC && many) kv_read_kernel<D, FMT, BF16, VEC, VEC ? U : 1><<<grid, 256, 0, st>>>(a, step);
+    else kv_read_kernel<D, FMT, BF16, VEC, 1><<<grid, 256, 0, st>>>(a, step);
   }
   return cudaGetLastError();
+}
+template <int D, int FMT, bool BF16>
+cudaError_t launch_rows2(const KvRowsArgs& a, bool write, bool vec, cudaStream_t st) {
+  return vec ? launch_rows3<D, FMT, BF16, true>(a, write, st) : launch_rows3<D, FMT, BF16, false>(a, write, st);
 }
 template <int D, int FMT>
 cudaError_t launch_rows1(const KvRowsArgs& a, bool write, bool bf16, bool vec, cudaStream_t st) {
@@ -193,8 +232,9 @@ KvPool pool_of(const gs_kv_cache* c) {
   p.v = static_cast<const unsigned char*>(d.v);
   p.k_scale = d.k_scale;
   p.v_scale = d.v_scale;
-  p.k_page = d.k_page_stride * e, p.k_head = d.k_head_stride * e, p.k_token = d.k_token_stride * e;
-  p.v_page = d.v_page_stride * e, p.v_head = d.v_head_stride * e, p.v_token = d.v_token_stride * e;
+  auto pieces = [&](int64_t stride) { return static_cast<uint32_t>(stride * e / 16); };
+  p.k_page = pieces(d.k_page_stride), p.k_head = pieces(d.k_head_stride), p.k_token = pieces(d.k_token_stride);
+  p.v_page = pieces(d.v_page_stride), p.v_head = pieces(d.v_head_stride), p.v_token = pieces(d.v_token_stride);
   p.pages = static_cast<int32_t>(d.pages);
   p.page_shift = c->page_shift;
   p.kv_heads = d.kv_heads;
@@ -220,12 +260,15 @@ gs_status move_rows(gs_kv_cache* c, const gs_kv_rows* r, void* stream, bool writ
   a.kv = pool_of(c);
   a.k = static_cast<unsigned char*>(r->k);
   a.v = static_cast<unsigned char*>(r->v);
-  a.k_token = st[0], a.k_head = st[1], a.v_token = st[2], a.v_head = st[3];
+  for (int64_t s : st)
+    if (s < 0 || s >= (1ll << 32)) return kfail(c, GS_EUNSUPPORTED, "strides of k and v must be in [0, 2^32)");
+  a.k_token = static_cast<uint32_t>(st[0]), a.k_head = static_cast<uint32_t>(st[1]);
+  a.v_token = static_cast<uint32_t>(st[2]), a.v_head = static_cast<uint32_t>(st[3]);
   a.slots = r->slots;
-  a.rows = r->tokens * c->d.kv_heads;
+  a.tokens = r->tokens;
   a.slots_end = c->d.pages * c->d.page_size;
   a.flag = c->flag;
-  if (a.rows > 0x7fffffffll * 8) return kfail(c, GS_EUNSUPPORTED, "tokens * kv_heads is at most 2^34");
+  if (r->tokens * c->d.kv_heads > 0x7fffffffll) return kfail(c, GS_EUNSUPPORTED, "tokens * kv_heads is at most 2^31 - 1");
   bool vec = reinterpret_cast<uintptr_t>(r->k) % 16 == 0 && reinterpret_cast<uintptr_t>(r->v) % 16 == 0;
   for (int64_t s : st) vec = vec && (s * e) % 16 == 0;
   DeviceScope scope(c->device);
@@ -272,8 +315,8 @@ gs_status gs_kv_cache_create(gs_ctx* ctx, const gs_kv_cache_desc* d, gs_kv_cache
   const int64_t strides[6] = {d->k_page_stride, d->k_head_stride, d->k_token_stride,
                               d->v_page_stride, d->v_head_stride, d->v_token_stride};
   for (int64_t s : strides)
-    if (s < d->head_dim || (s * e) % 16 != 0 || s >= (1ll << 36))
-      return bad(GS_EINVAL, "KV cache: strides must be at least head_dim, whole 16-byte pieces and below 2^36");
+    if (s < d->head_dim || (s * e) % 16 != 0 || s >= (1ll << 35))
+      return bad(GS_EINVAL, "KV cache: strides must be at least head_dim, whole 16-byte pieces and below 2^35");
   if (reinterpret_cast<uintptr_t>(d->k) % 16 || reinterpret_cast<uintptr_t>(d->v) % 16)
     return bad(GS_EINVAL, "KV cache: k and v must be 16-byte aligned");
   auto* c = new (std::nothrow) gs_kv_cache();

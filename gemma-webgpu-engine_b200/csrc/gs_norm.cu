@@ -37,6 +37,52 @@ struct NormArgs {
 
 enum { kOutF32 = 0, kOutBf16 = 1, kOutE4m3 = 2, kOutSrq = 3 };
 
+// Rows of V values by packed float32 pairs (the kernel is bound by issue slots, not by HBM, when its
+// inputs are bf16).
+template <int V>
+__device__ __forceinline__ void add_row(float (&a)[V], const float (&b)[V]) {
+  if constexpr (V == 1) a[0] += b[0];
+  else
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 r = __fadd2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]));
+      a[i] = r.x, a[i + 1] = r.y;
+    }
+}
+template <int V>
+__device__ __forceinline__ void mul_row(float (&a)[V], const float (&b)[V]) {
+  if constexpr (V == 1) a[0] *= b[0];
+  else
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 r = __fmul2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]));
+      a[i] = r.x, a[i + 1] = r.y;
+    }
+}
+template <int V>
+__device__ __forceinline__ void scale_row(float (&a)[V], float f) {
+  float b[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) b[i] = f;
+  mul_row(a, b);
+}
+template <int V>
+__device__ __forceinline__ void square_row(const float (&a)[V], float2& s) {
+  if constexpr (V == 1) s.x = fmaf(a[0], a[0], s.x);
+  else
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 x = make_float2(a[i], a[i + 1]);
+      s = __ffma2_rn(x, x, s);
+    }
+}
+// 448 / a for a >= 2^-64 by the approximate reciprocal (1 ulp; a code differs from the quotient's only
+// where the product lies that near a rounding boundary), which is 0 from 2^126 on: there the quotient.
+__device__ __forceinline__ float norm_inv(float a) {
+  const float f = quant_floor(a);
+  return f < 8.0e37f ? kE4m3Max * __fdividef(1.0f, f) : __fdiv_rn(kE4m3Max, f);
+}
+
 template <int V>
 __device__ __forceinline__ void load_weight(const NormArgs& A, int col, float (&w)[V]) {
   if (!A.weight) {
@@ -46,18 +92,26 @@ __device__ __forceinline__ void load_weight(const NormArgs& A, int col, float (&
   }
   if (A.weight_bf16) load_row<V, true>(static_cast<const unsigned short*>(A.weight) + col, w);
   else load_row<V, false>(static_cast<const float*>(A.weight) + col, w);
+  float o[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) w[i] += A.offset;
+  for (int i = 0; i < V; ++i) o[i] = A.offset;
+  add_row(w, o);
+}
+
+// max of non-negative values over the warp: their bits in integer order are in value order, NaN above all.
+__device__ __forceinline__ float warp_max_bits(float v) {
+  return __int_as_float(__reduce_max_sync(kFullMask, __float_as_int(v) & 0x7fffffff));
 }
 
 // TPR = blockDim.x threads per row (a multiple of 32), blockDim.y rows per block; thread t
 // holds the row's V-element pieces t, t + TPR, ...  V = 8: 16-byte (bf16) or two 16-byte
 // (f32) accesses, all pointers and strides 16-byte aligned and hidden % 8 == 0; V = 1:
 // any alignment and width.
-template <bool BF16, int OUT, int V, int PIECES>
-__global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ NormArgs A) {
+template <bool BF16, int OUT, int V, int PIECES, int MAXT>
+__global__ void __launch_bounds__(MAXT) norm_kernel(const __grid_constant__ NormArgs A) {
   __shared__ float red[32];
   __shared__ int redi[32];
+  __shared__ float red2[32];
   extern __shared__ int gmax[];  // V = 1, several groups: [blockDim.y][groups] bits of max|y|
   const int t = threadIdx.x, tpr = blockDim.x, warps = tpr >> 5;
   const int wid = threadIdx.y * warps + (t >> 5), lane = t & 31;
@@ -65,7 +119,7 @@ __global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ Norm
   const bool live = row < A.rows;
   using T = typename std::conditional<BF16, unsigned short, float>::type;
   float h[PIECES][V];
-  float sq = 0.0f;
+  float2 sq2 = make_float2(0.0f, 0.0f);
   if (live) {
     const T* x = static_cast<const T*>(A.x) + row * A.ld_x;
     const T* r = A.residual ? static_cast<const T*>(A.residual) + row * A.ld_residual : nullptr;
@@ -81,8 +135,7 @@ __global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ Norm
         if (col < A.hidden) {
           float b[V];
           load_row<V, BF16>(r + col, b);
-#pragma unroll
-          for (int i = 0; i < V; ++i) h[p][i] += b[i];
+          add_row(h[p], b);
         }
       }
     }
@@ -91,12 +144,11 @@ __global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ Norm
       const int col = (t + p * tpr) * V;
       if (col < A.hidden) {
         if (A.residual_out) store_row<V, BF16>(static_cast<T*>(A.residual_out) + row * A.ld_residual_out + col, h[p]);
-#pragma unroll
-        for (int i = 0; i < V; ++i) sq = fmaf(h[p][i], h[p][i], sq);
+        square_row(h[p], sq2);
       }
     }
   }
-  sq = warp_sum_f(sq);
+  float sq = warp_sum_f(sq2.x + sq2.y);
   if (warps > 1) {
     if (lane == 0) red[wid] = sq;
     __syncthreads();
@@ -110,8 +162,8 @@ __global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ Norm
     if (col < A.hidden && live) {
       float w[V];
       load_weight<V>(A, col, w);
-#pragma unroll
-      for (int i = 0; i < V; ++i) h[p][i] = h[p][i] * rstd * w[i];
+      scale_row(h[p], rstd);
+      mul_row(h[p], w);
     }
   }
   if constexpr (OUT == kOutF32 || OUT == kOutBf16) {
@@ -148,41 +200,40 @@ __global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ Norm
     }
     if (t == 0 && live && A.row_sum) A.row_sum[row] = __fmul_rn(static_cast<float>(qs), A.srq_scale);
   } else {
-    // max|y| as the bits of a non-negative float: integer order is value order, NaN above all
     unsigned char* out = static_cast<unsigned char*>(A.out) + row * A.ld_out;
     float* scales = A.out_scale + row * A.groups;
-    int gm[PIECES];
+    float gm[PIECES];
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-      gm[p] = 0;
+      gm[p] = 0.0f;
       const int col = (t + p * tpr) * V;
       if (col < A.hidden && live)
 #pragma unroll
-        for (int i = 0; i < V; ++i) gm[p] = max(gm[p], __float_as_int(h[p][i]) & 0x7fffffff);
+        for (int i = 0; i < V; ++i) gm[p] = max_nan(gm[p], fabsf(h[p][i]));
     }
     if (A.groups == 1) {
-      int m = 0;
+      float m = 0.0f;
 #pragma unroll
-      for (int p = 0; p < PIECES; ++p) m = max(m, gm[p]);
-      m = __reduce_max_sync(kFullMask, m);
+      for (int p = 0; p < PIECES; ++p) m = max_nan(m, gm[p]);
+      m = warp_max_bits(m);
       if (warps > 1) {
-        if (lane == 0) redi[wid] = m;
+        if (lane == 0) red2[wid] = m;
         __syncthreads();
-        m = 0;
-        for (int w = 0; w < warps; ++w) m = max(m, redi[threadIdx.y * warps + w]);
+        m = 0.0f;
+        for (int w = 0; w < warps; ++w) m = max_nan(m, red2[threadIdx.y * warps + w]);
       }
 #pragma unroll
       for (int p = 0; p < PIECES; ++p) gm[p] = m;
-      if (t == 0 && live) scales[0] = quant_scale(__int_as_float(m), kE4m3Max);
+      if (t == 0 && live) scales[0] = quant_scale(m, kE4m3Max);
     } else if (V == 8) {
       // a group is group / 8 consecutive pieces, so as many neighbouring lanes (4, 8 or 16)
       const int span = A.group >> 3;
 #pragma unroll
       for (int p = 0; p < PIECES; ++p) {
-        for (int o = span >> 1; o > 0; o >>= 1) gm[p] = max(gm[p], __shfl_xor_sync(kFullMask, gm[p], o));
+        for (int o = span >> 1; o > 0; o >>= 1) gm[p] = max_nan(gm[p], __shfl_xor_sync(kFullMask, gm[p], o));
         const int col = (t + p * tpr) * V;
         if (col < A.hidden && live && (lane & (span - 1)) == 0)
-          scales[col / A.group] = quant_scale(__int_as_float(gm[p]), kE4m3Max);
+          scales[col / A.group] = quant_floor(gm[p]) * (1.0f / kE4m3Max);
       }
     } else {
       int* gr = gmax + threadIdx.y * A.groups;
@@ -190,14 +241,16 @@ __global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ Norm
       __syncthreads();
 #pragma unroll
       for (int p = 0; p < PIECES; ++p) {
-        const int col = (t + p * tpr) * V;
-        if (col < A.hidden && live) atomicMax(gr + col / A.group, gm[p]);
+        // a warp's 32 columns lie in one group (groups are multiples of 32 columns)
+        const int col = t + p * tpr;
+        const int m = __float_as_int(warp_max_bits(gm[p]));
+        if (lane == 0 && col < A.hidden) atomicMax(gr + col / A.group, m);
       }
       __syncthreads();
 #pragma unroll
       for (int p = 0; p < PIECES; ++p) {
         const int col = (t + p * tpr) * V;
-        if (col < A.hidden && live) gm[p] = gr[col / A.group];
+        if (col < A.hidden && live) gm[p] = __int_as_float(gr[col / A.group]);
       }
       if (live)
         for (int g = t; g < A.groups; g += tpr) scales[g] = quant_scale(__int_as_float(gr[g]), kE4m3Max);
@@ -206,11 +259,12 @@ __global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ Norm
     for (int p = 0; p < PIECES; ++p) {
       const int col = (t + p * tpr) * V;
       if (col < A.hidden && live) {
-        const float inv = quant_inv(__int_as_float(gm[p]), kE4m3Max);
+        const float inv = norm_inv(gm[p]);
         if constexpr (V == 8) {
           uint2 c;
-          c.x = e4m3x4(h[p][0] * inv, h[p][1] * inv, h[p][2] * inv, h[p][3] * inv);
-          c.y = e4m3x4(h[p][4] * inv, h[p][5] * inv, h[p][6] * inv, h[p][7] * inv);
+          scale_row(h[p], inv);
+          c.x = e4m3x4(h[p][0], h[p][1], h[p][2], h[p][3]);
+          c.y = e4m3x4(h[p][4], h[p][5], h[p][6], h[p][7]);
           *reinterpret_cast<uint2*>(out + col) = c;
         } else {
           out[col] = static_cast<unsigned char>(e4m3x2(h[p][0] * inv, 0.0f) & 0xffu);
@@ -222,22 +276,25 @@ __global__ void __launch_bounds__(1024) norm_kernel(const __grid_constant__ Norm
 
 template <bool BF16, int OUT, int V>
 cudaError_t launch_norm_v(const NormArgs& a, cudaStream_t st) {
-  // One warp per row while its pieces fit 4 a lane; wider rows take more threads at 2 or 4
-  // pieces each.  256-thread blocks then hold several rows.
   const int pieces = (a.hidden + V - 1) / V;
-  constexpr int kMost = V == 8 ? 4 : 32;
   int tpr = 32;
-  const int want = V == 8 ? (a.rows <= 296 ? 1 : 2) : 4;
+  const int want = a.rows <= 296 ? 1 : V == 8 ? 2 : 4;
   while (tpr < 1024 && tpr * want < pieces) tpr <<= 1;
   const int rpb = tpr >= 256 ? 1 : 256 / tpr;
   const int per = (pieces + tpr - 1) / tpr;
   const dim3 block(tpr, rpb);
   const unsigned grid = static_cast<unsigned>((a.rows + rpb - 1) / rpb);
   const size_t smem = (OUT == kOutE4m3 && V == 1 && a.groups > 1) ? sizeof(int) * rpb * a.groups : 0;
-  if (per <= 1) norm_kernel<BF16, OUT, V, 1><<<grid, block, smem, st>>>(a);
-  else if (per <= 2) norm_kernel<BF16, OUT, V, 2><<<grid, block, smem, st>>>(a);
-  else if (per <= 4) norm_kernel<BF16, OUT, V, 4><<<grid, block, smem, st>>>(a);
-  else norm_kernel<BF16, OUT, V, kMost><<<grid, block, smem, st>>>(a);
+  const bool wide = tpr > 256;
+  if (per <= 1 && !wide) norm_kernel<BF16, OUT, V, 1, 256><<<grid, block, smem, st>>>(a);
+  else if (per <= 1) norm_kernel<BF16, OUT, V, 1, 1024><<<grid, block, smem, st>>>(a);
+  else if (per <= 2 && !wide) norm_kernel<BF16, OUT, V, 2, 256><<<grid, block, smem, st>>>(a);
+  else if (per <= 2) norm_kernel<BF16, OUT, V, 2, 1024><<<grid, block, smem, st>>>(a);
+  else if (per <= 4 && !wide) norm_kernel<BF16, OUT, V, 4, 256><<<grid, block, smem, st>>>(a);
+  else if (per <= 4) norm_kernel<BF16, OUT, V, 4, 1024><<<grid, block, smem, st>>>(a);
+  else if (per <= 8) norm_kernel<BF16, OUT, V, V == 1 ? 8 : 4, 1024><<<grid, block, smem, st>>>(a);
+  else if (per <= 16) norm_kernel<BF16, OUT, V, V == 1 ? 16 : 4, 1024><<<grid, block, smem, st>>>(a);
+  else norm_kernel<BF16, OUT, V, V == 1 ? 32 : 4, 1024><<<grid, block, smem, st>>>(a);
   return cudaGetLastError();
 }
 
