@@ -15,7 +15,7 @@ struct gs_kv_cache {
   int page_shift = 0;
   int32_t* flag = nullptr;       // device: GS_KV_ERR_* bits
   unsigned char* ws = nullptr;   // the context's attention workspace (kAttnWsBytes)
-  alignas(64) unsigned char maps[256] = {};  // tensor maps of a bf16 cache's pools
+  alignas(64) unsigned char maps[512] = {};  // tensor maps of the pools: many-row kernel's, few-row kernel's
   std::string err;
 };
 
@@ -64,8 +64,9 @@ struct AttnArgs {
   int32_t max_q, max_kv;
   int32_t window, sinks;
   float scale_log2;     // scale · log2(e): scores in log2 units
-  int32_t chunk_tiles;  // context tiles per split
-  int32_t splits;       // partial slots per (sequence, head, row block)
+  int32_t chunk_tiles;  // context tiles per split (0: every context in `splits` even parts)
+  int32_t splits;       // partial results per (sequence, head, row block)
+  int32_t cluster;      // blocks per partial result (few-row kernel)
   float* part_o;        // [seq][row block][kv head][split][rows][head_dim]
   float* part_ml;       // [..][rows][2]: running maximum (log2 units) and sum
   int32_t* flag;
@@ -133,8 +134,7 @@ __device__ __forceinline__ float ex2(float x) { return ex2_approx(x); }
 
 // Few-row kernel (mma.sync, one 16-token tile per warp): any number of rows in blocks.
 cudaError_t launch_attn_rows(const gs_kv_cache* c, AttnArgs a, cudaStream_t st);
-// Many-row kernel (tcgen05), and the tensor maps it reads a bf16 cache by (an error text, or
-// nullptr).
+// Many-row kernel (tcgen05), and the tensor maps both read a cache by (an error text, or nullptr).
 cudaError_t launch_attn_tile(const gs_kv_cache* c, AttnArgs a, cudaStream_t st);
 const char* make_attn_maps(gs_kv_cache* c);
 // Joins the partial results of a split context.  rows_per_block and tile as in the kernel

@@ -13,17 +13,25 @@
 // heads wastes no registers on padding; O^T takes head_dim / 4 registers a lane per 8 rows.
 // S^T's accumulators become the B operand of the second product by one 8x8 transpose each.
 //
-// Every warp walks its own tiles (every fourth of the block's split) through a private ring of
-// shared-memory stages filled by 16-byte cp.async, so the loop has no block barrier and
-// 96 to 128 KB are in flight per SM; warps meet once, at the end, to join their (m, l, O).
-// Tokens hidden from every row of the block are filled with zeros instead of read.
+// Every warp walks its own tiles (every fourth of the block's share) through a private ring of
+// shared-memory stages that one lane fills by TMA boxes of 16 tokens in the swizzled layout ldmatrix
+// reads without bank conflicts: the loop has no block barrier, and 64 to 128 KB are in flight per SM.
+// A row's reference point m moves only when a score passes it by 2^8 (as V's reference scale does
+// when a larger one comes), so the usual tile needs one vote instead of reductions and rescaling.
+// Values of tokens hidden from every row of the block are set to zero before they are used.
+//
+// A context is shared evenly by the blocks of a cluster (up to 8), which join their (m, l, O) through
+// distributed shared memory; several clusters per context write partial results, joined by a second
+// launch.
 //
 // 8-bit codes are widened to float16 (exact for e4m3 and int8) in registers, K's scale
 // multiplies the finished score, V's scale the weight: 2^(s - m) · (scale / largest scale so
-// far) · 1024, which float16 holds to 11 bits down to 2^-24 of the largest; the factor is
+// far) · 2^7, at most 2^15, which float16 holds to 11 bits down to 2^-21 of the largest; the factor is
 // taken out of O at the end.  q is brought into float16's range by a power of two per row
 // (bfloat16 has fewer mantissa bits: exact except for components below 2^-17 of the row's
 // largest).  Beside a bf16 cache the weights are bf16, as q and v are.
+#include <cuda.h>
+
 #include "gs_attn.cuh"
 
 namespace gs {
@@ -32,37 +40,40 @@ namespace {
 constexpr int kRowsWarps = 4;
 constexpr int kRowsThreads = kRowsWarps * 32;
 constexpr int kRT = 16;  // tokens per warp tile
-constexpr float kPScale = 1024.0f;
+constexpr float kPScale = 128.0f;
+constexpr float kSlack = 8.0f;  // log2 units a score may pass the reference by
 
 template <int D, int FMT>
 struct RowsPlan {
-  static constexpr int kEl = FMT == GS_DTYPE_BF16 ? 2 : 1;
-  static constexpr int kRow = D * kEl;                         // bytes of one token's K (or V) row
-  static constexpr int kChunks = kRow / 16;                    // 16-byte pieces per row: 4 .. 32
-  static constexpr int kTileBytes = kRT * kRow;                // K or V of one tile
-  static constexpr int kStage = 2 * kTileBytes + (FMT == GS_DTYPE_BF16 ? 0 : 2 * kRT * 4);
-  static constexpr int kWant = 96 * 1024 / (kRowsWarps * kStage);
-  static constexpr int kStages = kWant < 3 ? 3 : kWant > 6 ? 6 : kWant;
+  static constexpr bool kBf = FMT == GS_DTYPE_BF16;
+  static constexpr int kEl = kBf ? 2 : 1;
+  static constexpr int kRow = D * kEl;                       // bytes of one token's K (or V) row
+  static constexpr int kInner = kRow < 128 ? kRow : 128;     // bytes of a row in one TMA box
+  static constexpr int kCols = kRow / kInner;                // boxes across a row
+  static constexpr int kTileBytes = kRT * kRow;              // K or V of one tile
+  static constexpr int kSub = kTileBytes <= 2048 ? 2 : 1;    // tiles per stage
+  static constexpr int kStage = kSub * 2 * kTileBytes;
+  static constexpr int kStages = 3;
   static constexpr int kRing = kRowsWarps * kStages * kStage;
+  static constexpr int kScale = kBf ? 0 : kSub * 2 * kRT * 4;  // scales of a stage
 };
 
 template <int D, int FMT, int NB>
-constexpr int rows_smem() {
-  constexpr int ring = RowsPlan<D, FMT>::kRing;
-  constexpr int join = kRowsWarps * 8 * NB * (D + 4) * 4;
-  return (ring > join ? ring : join) + NB * (D / 16) * 32 * 8;  // + Q fragments
-}
+struct RowsSmem {
+  using P = RowsPlan<D, FMT>;
+  static constexpr int kRows = 8 * NB;
+  static constexpr int kJoin = kRowsWarps * kRows * (D + 4) * 4;
+  static constexpr int kMain = P::kRing > kJoin ? P::kRing : kJoin;
+  static constexpr int kOffScale = kMain;
+  static constexpr int kOffQ = kOffScale + kRowsWarps * P::kStages * P::kScale;
+  static constexpr int kTotal = kOffQ + NB * (D / 16) * 32 * 8 + 1024;  // Q fragments, alignment slack
+};
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool real) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(real ? 4 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ void box_in(uint32_t dst, const CUtensorMap* map, int x, int tok, int head, int page, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(tok), "r"(head), "r"(page), "r"(smem_addr(bar))
+      : "memory");
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -114,25 +125,67 @@ __device__ __forceinline__ void widen4(uint32_t codes, uint32_t& lo, uint32_t& h
   }
 }
 
-// Byte offset of 16-byte piece c of row r in a tile, pieces permuted so that 8 rows'
-// equal pieces lie in different banks (rows of 64 bytes: two rows share 128 bytes).
-template <int CH>
+// Byte offset of 16-byte piece c of row r in a tile as the TMA boxes lay it: blocks of kInner bytes of
+// all 16 rows, pieces permuted by the row (128-byte swizzle; 64-byte for the narrowest rows).
+template <int INNER>
 __device__ __forceinline__ uint32_t piece(int r, int c) {
-  if constexpr (CH == 4) return static_cast<uint32_t>(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
-  else return static_cast<uint32_t>(r * CH * 16 + ((c ^ (r & 7)) << 4));
+  if constexpr (INNER == 64) return static_cast<uint32_t>(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+  else return static_cast<uint32_t>((c >> 3) * (kRT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+struct RowsMaps {
+  CUtensorMap k, v;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 ld_rank4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float2 ld_rank2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a));
+  return v;
+}
+
+// Blocks per SM the register budget leaves room for (the rings' sizes allow as many).
+template <int D, int FMT, int NB>
+constexpr int rows_occupancy() {
+  const int by_smem = 227 * 1024 / (RowsSmem<D, FMT, NB>::kTotal + 1024);
+  const int by_regs = D * NB <= 128 ? 4 : D * NB <= 256 ? 3 : 2;
+  return by_smem < by_regs ? (by_smem < 1 ? 1 : by_smem) : by_regs;
 }
 
 template <int D, int FMT, int NB>
-__global__ void __launch_bounds__(kRowsThreads) attn_rows_kernel(const __grid_constant__ AttnArgs A) {
+__global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
+    attn_rows_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ RowsMaps maps) {
   using P = RowsPlan<D, FMT>;
-  constexpr bool kBf = FMT == GS_DTYPE_BF16;
+  using S = RowsSmem<D, FMT, NB>;
+  constexpr bool kBf = P::kBf;
   constexpr int kRows = 8 * NB;
   constexpr int KS = D / 16;  // k-steps of the first product, 16-wide value blocks of the second
-  extern __shared__ __align__(128) unsigned char smem[];
-  constexpr int kQOff = rows_smem<D, FMT, NB>() - NB * KS * 32 * 8;
-  uint2* qfrag = reinterpret_cast<uint2*>(smem + kQOff);  // [NB][KS][32]
+  constexpr bool kQRegs = D * NB <= 128;
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t raw = smem_addr(smem_raw);
+  unsigned char* smem = smem_raw + (((raw + 1023u) & ~1023u) - raw);
+  uint2* qfrag = reinterpret_cast<uint2*>(smem + S::kOffQ);  // [NB][KS][32]
   __shared__ float s_m[kRowsWarps][kRows], s_l[kRowsWarps][kRows], s_f[kRowsWarps];
   __shared__ float s_qf[kRows];
+  __shared__ __align__(8) float s_ml[kRows][2];  // the block's joined maximum and sum
+  __shared__ __align__(8) uint64_t s_bar[kRowsWarps][P::kStages];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, c = lane & 3;
@@ -140,12 +193,71 @@ __global__ void __launch_bounds__(kRowsThreads) attn_rows_kernel(const __grid_co
   const int head = blockIdx.y % A.kv.kv_heads, rb = blockIdx.y / A.kv.kv_heads;
   const int r0 = rb * kRows;
   const RowRange R = row_range<kRT>(A, b, r0, kRows);
-  if (R.rows == 0) return;
-  int nsplit = (R.tiles + A.chunk_tiles - 1) / A.chunk_tiles;
-  nsplit = nsplit < 1 ? 1 : nsplit > A.splits ? A.splits : nsplit;
-  const int split = blockIdx.x;
-  if (split >= nsplit) return;
-  const int i_end = split == nsplit - 1 ? R.tiles : (split + 1) * A.chunk_tiles;
+  if (R.rows == 0) return;  // (the whole cluster)
+  // this block's tiles: an even share of the context's
+  const int share = (R.tiles + A.splits * A.cluster - 1) / (A.splits * A.cluster);
+  const int i_begin = min(static_cast<int>(blockIdx.x) * share, R.tiles);
+  const int i_end = min(i_begin + share, R.tiles);
+  if (lane < P::kStages) mbar_init(&s_bar[warp][lane], 1);
+  __syncwarp();
+
+  // ---- the warp's ring: stage n holds tiles i_begin + (n · 4 + warp) · kSub ..
+  const uint32_t ring = smem_addr(smem) + warp * (P::kStages * P::kStage);
+  const uint32_t scales = smem_addr(smem + S::kOffScale) + warp * (P::kStages * P::kScale);
+  const int32_t* table = A.table + b * A.table_stride;
+  const int per_page = A.kv.page_shift - 4;  // log2 of tiles per page
+  const int page_mask = (1 << A.kv.page_shift) - 1;
+  const int first = i_begin + warp * P::kSub;
+  constexpr int kStep = kRowsWarps * P::kSub;
+  const int n_stages = i_end > first ? (i_end - first + kStep - 1) / kStep : 0;
+  int pages = 0;       // table entries of the warp's next 32 tiles
+  int pages_at = -1;   // which 32
+  auto fetch = [&](int n) {
+    const int t = n * P::kSub;  // the warp's tile number
+    if ((t >> 5) != pages_at) {
+      pages_at = t >> 5;
+      const int tl = (pages_at << 5) + lane;
+      const int il = first + tl / P::kSub * kStep + tl % P::kSub;
+      pages = -1;
+      if (il < i_end) {
+        const int col = R.tile(il) >> per_page;
+        if (col < A.table_cols) pages = __ldg(table + col);
+        if (pages < 0 || pages >= A.kv.pages) {
+          pages = 0;
+          atomicOr(A.flag, GS_KV_ERR_PAGE);
+        }
+      }
+    }
+    int pg[P::kSub];
+#pragma unroll
+    for (int u = 0; u < P::kSub; ++u) pg[u] = __shfl_sync(kFullMask, pages, (t + u) & 31);
+    if (lane == 0 && n < n_stages) {
+      const int st = n % P::kStages;
+      uint64_t* bar = &s_bar[warp][st];
+      const int i0 = first + n * kStep;
+      const int live = P::kSub == 1 || i0 + 1 < i_end ? P::kSub : 1;
+      mbar_expect_tx(bar, live * (2 * P::kTileBytes + (kBf ? 0 : 2 * kRT * 4)));
+#pragma unroll
+      for (int u = 0; u < P::kSub; ++u) {
+        if (u >= live) break;
+        const int off = (R.tile(i0 + u) * kRT) & page_mask;
+        const uint32_t ks = ring + st * P::kStage + u * 2 * P::kTileBytes;
+#pragma unroll
+        for (int cb = 0; cb < P::kCols; ++cb) {
+          box_in(ks + cb * (kRT * P::kInner), &maps.k, cb * (P::kInner / P::kEl), off, head, pg[u], bar);
+          box_in(ks + P::kTileBytes + cb * (kRT * P::kInner), &maps.v, cb * (P::kInner / P::kEl), off, head, pg[u], bar);
+        }
+        if constexpr (!kBf) {
+          const uint32_t sd = scales + st * P::kScale + u * (2 * kRT * 4);
+          bulk_g2s_addr(sd, A.kv.scale_at(false, pg[u], head, off), kRT * 4, bar);
+          bulk_g2s_addr(sd + kRT * 4, A.kv.scale_at(true, pg[u], head, off), kRT * 4, bar);
+        }
+      }
+    }
+    __syncwarp();
+  };
+#pragma unroll
+  for (int s = 0; s < P::kStages - 1; ++s) fetch(s);
 
   // ---- Q fragments (B operand: k = 2c.. of row n = g), once
   for (int nb = warp; nb < NB; nb += kRowsWarps) {
@@ -186,6 +298,15 @@ __global__ void __launch_bounds__(kRowsThreads) attn_rows_kernel(const __grid_co
     if (c == 0) s_qf[r] = f * A.scale_log2;
   }
   __syncthreads();
+  uint2 qreg[kQRegs ? NB * KS : 1];
+  if constexpr (kQRegs) {
+#pragma unroll
+    for (int k = 0; k < NB * KS; ++k) qreg[k] = qfrag[k * 32 + lane];
+  }
+  auto qf_at = [&](int nb, int k) {
+    if constexpr (kQRegs) return qreg[nb * KS + k];
+    else return qfrag[(nb * KS + k) * 32 + lane];
+  };
 
   float qf[NB][2];
   int pos[NB][2];  // position of the lane's two rows
@@ -199,53 +320,6 @@ __global__ void __launch_bounds__(kRowsThreads) attn_rows_kernel(const __grid_co
     }
   const int p_min = R.p0 + r0 / A.group, p_max = R.hi - 1;
 
-  // ---- the warp's ring
-  unsigned char* ring = smem + warp * (P::kStages * P::kStage);
-  const uint32_t ring_s = smem_addr(ring);
-  const int32_t* table = A.table + b * A.table_stride;
-  const int per_page = A.kv.page_shift - 4;  // log2 of tiles per page
-  int pages = 0;       // table entries of 32 consecutive tiles of this warp
-  int pages_at = -1;   // which 32
-  auto fetch = [&](int n, int stage) {  // the warp's n-th tile
-    const int i = split * A.chunk_tiles + warp + n * kRowsWarps;
-    if ((n >> 5) != pages_at) {
-      pages_at = n >> 5;
-      const int il = split * A.chunk_tiles + warp + ((pages_at << 5) + lane) * kRowsWarps;
-      pages = -1;
-      if (il < i_end) {
-        const int col = R.tile(il) >> per_page;
-        if (col < A.table_cols) pages = __ldg(table + col);
-        if (pages < 0 || pages >= A.kv.pages) {
-          pages = -1;
-          atomicOr(A.flag, GS_KV_ERR_PAGE);
-        }
-      }
-    }
-    const int page = __shfl_sync(kFullMask, pages, n & 31);
-    if (i < i_end) {
-      const int j0 = R.tile(i) * kRT;
-      const int off = j0 & ((1 << A.kv.page_shift) - 1);
-      const int pg = page < 0 ? 0 : page;
-      const unsigned char* kp = A.kv.at(false, pg, head, off);
-      const unsigned char* vp = A.kv.at(true, pg, head, off);
-      const uint32_t ks = ring_s + stage * P::kStage, vs = ks + P::kTileBytes;
-#pragma unroll
-      for (int u = 0; u < P::kChunks / 2; ++u) {
-        const int id = lane + 32 * u, r = id / P::kChunks, ch = id % P::kChunks;
-        const bool real = page >= 0 && R.seen_by_any(j0 + r);
-        const uint32_t at = piece<P::kChunks>(r, ch);
-        cp_async16(ks + at, kp + (static_cast<uint64_t>(static_cast<uint32_t>(r)) * A.kv.k_token + ch) * 16, real);
-        cp_async16(vs + at, vp + (static_cast<uint64_t>(static_cast<uint32_t>(r)) * A.kv.v_token + ch) * 16, real);
-      }
-      if constexpr (!kBf) {
-        const int r = lane & 15;
-        const float* sc = A.kv.scale_at(lane >= 16, pg, head, off + r);
-        cp_async4(ks + 2 * P::kTileBytes + lane * 4, sc, page >= 0 && R.seen_by_any(j0 + r));
-      }
-    }
-    cp_commit();
-  };
-
   float o[NB][KS][4];
   float m[NB][2], l[NB][2];
 #pragma unroll
@@ -257,179 +331,192 @@ __global__ void __launch_bounds__(kRowsThreads) attn_rows_kernel(const __grid_co
 #pragma unroll
       for (int u = 0; u < 4; ++u) o[nb][k][u] = 0.0f;
   }
-  float vref = 0.0f;  // largest V scale so far (8-bit)
+  float vref = 0.0f, vinv = 0.0f;  // (8-bit) largest V scale so far, kPScale over it
 
-  const int first = split * A.chunk_tiles + warp;
-  const int n_tiles = i_end > first ? (i_end - first + kRowsWarps - 1) / kRowsWarps : 0;
-#pragma unroll
-  for (int s = 0; s < P::kStages - 1; ++s) fetch(s, s);
   int stage = 0;
-  for (int n = 0; n < n_tiles; ++n) {
-    cp_wait<P::kStages - 2>();
-    __syncwarp();
-    {
-      int ns = stage + P::kStages - 1;
-      ns = ns >= P::kStages ? ns - P::kStages : ns;
-      fetch(n + P::kStages - 1, ns);
+  uint32_t phase = 0;
+  for (int n = 0; n < n_stages; ++n) {
+    if (!mbar_wait(&s_bar[warp][stage], phase, kWaitNs)) {
+      // (bounded: the other copies in flight get the same limit once more before the block ends)
+      atomicOr(A.flag, GS_KV_ERR_TIMEOUT);
+      for (int k = n + 1; k < n + P::kStages - 1 && k < n_stages; ++k)
+        mbar_wait(&s_bar[warp][k % P::kStages], static_cast<uint32_t>((k / P::kStages) & 1), kWaitNs);
+      break;
     }
-    const uint32_t ks = ring_s + stage * P::kStage, vs = ks + P::kTileBytes;
-    const int j0 = R.tile(first + n * kRowsWarps) * kRT;
-    // ---- S^T = K Q^T
-    float s[NB][4];
+    __syncwarp();  // every lane is done with the stage before this one: it is the next fetch's
+    fetch(n + P::kStages - 1);
+    const int i0 = first + n * kStep;
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int u = 0; u < 4; ++u) s[nb][u] = 0.0f;
-    {
-      float s2[NB][4];  // a second chain halves the dependent products
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) s2[nb][u] = 0.0f;
-      const int mr = lane & 15, mh = lane >> 4;  // matrix row and half of this lane's address
-#pragma unroll
-      for (int k = 0; k < KS; k += 2) {
-        if constexpr (kBf) {
-          uint32_t a[4], a2[4];
-          ldsm4(ks + piece<P::kChunks>(mr, 2 * k + mh), a);
-          ldsm4(ks + piece<P::kChunks>(mr, 2 * k + 2 + mh), a2);
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            const uint2 q0 = qfrag[(nb * KS + k) * 32 + lane], q1 = qfrag[(nb * KS + k + 1) * 32 + lane];
-            mma16<true>(s[nb], a[0], a[1], a[2], a[3], q0.x, q0.y);
-            mma16<true>(s2[nb], a2[0], a2[1], a2[2], a2[3], q1.x, q1.y);
-          }
-        } else {
-          uint32_t x[4];  // rows g / g + 8 of pieces k, k + 1: bytes 4c .. 4c + 3
-          ldsm4(ks + piece<P::kChunks>(mr, k + mh), x);
-          uint32_t a0, a1, a2, a3, e0, e1, e2, e3;
-          widen4<FMT>(x[0], a0, a2);
-          widen4<FMT>(x[1], a1, a3);
-          widen4<FMT>(x[2], e0, e2);
-          widen4<FMT>(x[3], e1, e3);
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            const uint2 q0 = qfrag[(nb * KS + k) * 32 + lane], q1 = qfrag[(nb * KS + k + 1) * 32 + lane];
-            mma16<false>(s[nb], a0, a1, a2, a3, q0.x, q0.y);
-            mma16<false>(s2[nb], e0, e1, e2, e3, q1.x, q1.y);
-          }
-        }
-      }
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-        for (int u = 0; u < 4; ++u) s[nb][u] += s2[nb][u];
-    }
-    // ---- scores in log2 units; lane: tokens j0 + g, j0 + g + 8, rows 2c, 2c + 1
-    float ksc[2] = {1.0f, 1.0f}, vsc[2] = {1.0f, 1.0f};
-    if constexpr (!kBf) {
-      const float* sc = reinterpret_cast<const float*>(ring + stage * P::kStage + 2 * P::kTileBytes);
-      ksc[0] = sc[g], ksc[1] = sc[g + 8], vsc[0] = sc[16 + g], vsc[1] = sc[24 + g];
-    }
-    const bool whole = j0 + kRT - 1 <= p_min && (!A.window || j0 > p_max - A.window || j0 + kRT <= A.sinks);
-    float mx[NB][2];
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) s[nb][u] *= qf[nb][u & 1] * ksc[u >> 1];
+    for (int sub = 0; sub < P::kSub; ++sub) {
+      if (P::kSub > 1 && sub > 0 && i0 + sub >= i_end) break;
+      const uint32_t ks = ring + stage * P::kStage + sub * 2 * P::kTileBytes, vs = ks + P::kTileBytes;
+      const int j0 = R.tile(i0 + sub) * kRT;
+      const bool whole = j0 + kRT - 1 <= p_min && (!A.window || j0 > p_max - A.window || j0 + kRT <= A.sinks);
       if (!whole) {
+        // tokens no row sees (past the context, before every window): their pages may hold anything
+        constexpr int kPc = P::kRow / 16;
+        bool wrote = false;
+        for (int id = lane; id < kRT * kPc; id += 32) {
+          const int r = id / kPc, ch = id % kPc;
+          if (!R.seen_by_any(j0 + r)) {
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vs + piece<P::kInner>(r, ch)), "r"(0u) : "memory");
+            wrote = true;
+          }
+        }
+        if (wrote) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (before the stage's next copy)
+        __syncwarp();
+      }
+      // ---- S^T = K Q^T
+      float s[NB][4];
+      {
+        float s2[NB][4];  // a second chain halves the dependent products
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int j = j0 + g + 8 * (u >> 1), p = pos[nb][u & 1];
-          const bool seen = j <= p && (!A.window || j > p - A.window || j < A.sinks);
-          s[nb][u] = seen ? s[nb][u] : -INFINITY;
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) s[nb][u] = s2[nb][u] = 0.0f;
+        const int mr = lane & 15, mh = lane >> 4;  // matrix row and half of this lane's address
+#pragma unroll
+        for (int k = 0; k < KS; k += 2) {
+          if constexpr (kBf) {
+            uint32_t a[4], a2[4];
+            ldsm4(ks + piece<P::kInner>(mr, 2 * k + mh), a);
+            ldsm4(ks + piece<P::kInner>(mr, 2 * k + 2 + mh), a2);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+              const uint2 q0 = qf_at(nb, k), q1 = qf_at(nb, k + 1);
+              mma16<true>(s[nb], a[0], a[1], a[2], a[3], q0.x, q0.y);
+              mma16<true>(s2[nb], a2[0], a2[1], a2[2], a2[3], q1.x, q1.y);
+            }
+          } else {
+            uint32_t x[4];  // rows g / g + 8 of pieces k, k + 1: bytes 4c .. 4c + 3
+            ldsm4(ks + piece<P::kInner>(mr, k + mh), x);
+            uint32_t a0, a1, a2, a3, e0, e1, e2, e3;
+            widen4<FMT>(x[0], a0, a2);
+            widen4<FMT>(x[1], a1, a3);
+            widen4<FMT>(x[2], e0, e2);
+            widen4<FMT>(x[3], e1, e3);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+              const uint2 q0 = qf_at(nb, k), q1 = qf_at(nb, k + 1);
+              mma16<false>(s[nb], a0, a1, a2, a3, q0.x, q0.y);
+              mma16<false>(s2[nb], e0, e1, e2, e3, q1.x, q1.y);
+            }
+          }
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) s[nb][u] += s2[nb][u];
+      }
+      // ---- scores in log2 units; lane: tokens j0 + g, j0 + g + 8, rows 2c, 2c + 1
+      float ksc[2] = {1.0f, 1.0f}, vsc[2] = {1.0f, 1.0f};
+      if constexpr (!kBf) {
+        const float* sc = reinterpret_cast<const float*>(smem + S::kOffScale) + ((warp * P::kStages + stage) * P::kSub + sub) * 2 * kRT;
+        ksc[0] = sc[g], ksc[1] = sc[g + 8], vsc[0] = sc[16 + g], vsc[1] = sc[24 + g];
+        if (!whole) {
+          if (!R.seen_by_any(j0 + g)) vsc[0] = 0.0f;
+          if (!R.seen_by_any(j0 + g + 8)) vsc[1] = 0.0f;
         }
       }
-      mx[nb][0] = max_nan(s[nb][0], s[nb][2]);
-      mx[nb][1] = max_nan(s[nb][1], s[nb][3]);
-    }
-    float vmx = vsc[0];
-    if constexpr (!kBf) vmx = fmaxf(vsc[0], vsc[1]);
+      bool move = !kBf && fmaxf(vsc[0], vsc[1]) > vref;
 #pragma unroll
-    for (int d = 4; d < 32; d <<= 1) {
+      for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
+        for (int u = 0; u < 4; ++u) s[nb][u] *= kBf ? qf[nb][u & 1] : qf[nb][u & 1] * ksc[u >> 1];
+        if (!whole) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) mx[nb][h] = max_nan(mx[nb][h], __shfl_xor_sync(kFullMask, mx[nb][h], d));
-      if constexpr (!kBf) vmx = fmaxf(vmx, __shfl_xor_sync(kFullMask, vmx, d));
-    }
-    float vfac = 1.0f, vmul0 = 1.0f, vmul1 = 1.0f;
-    if constexpr (!kBf) {
-      const float vnew = fmaxf(vref, vmx);
-      if (vnew > vref) {
-        vfac = vref / vnew;
-        vref = vnew;
+          for (int u = 0; u < 4; ++u) {
+            const int j = j0 + g + 8 * (u >> 1), p = pos[nb][u & 1];
+            const bool seen = j <= p && (!A.window || j > p - A.window || j < A.sinks);
+            s[nb][u] = seen ? s[nb][u] : -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) move = move || fmaxf(s[nb][h], s[nb][2 + h]) > m[nb][h] + kSlack;
       }
-      const float inv = vref > 0.0f ? kPScale / vref : 0.0f;
-      vmul0 = vsc[0] * inv;
-      vmul1 = vsc[1] * inv;
-    }
-    uint32_t pb[NB][2];
-    float al[NB][2];
-    bool same = vfac == 1.0f;
+      if (__any_sync(kFullMask, move)) {
+        // new references: every row's largest score so far, the largest V scale so far
+        float vfac = 1.0f;
+        if constexpr (!kBf) {
+          float vm = fmaxf(vref, fmaxf(vsc[0], vsc[1]));
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
+          for (int d = 4; d < 32; d <<= 1) vm = fmaxf(vm, __shfl_xor_sync(kFullMask, vm, d));
+          vfac = vm > vref ? vref / vm : 1.0f;
+          vref = vm;
+          vinv = vref > 0.0f ? kPScale / vref : 0.0f;
+        }
+        float al[NB][2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float mn = max_nan(m[nb][h], mx[nb][h]);
-        const float ref = mn == -INFINITY ? 0.0f : mn;
-        al[nb][h] = ex2(m[nb][h] - ref);
-        m[nb][h] = mn;
-        s[nb][h] = ex2(s[nb][h] - ref);
-        s[nb][2 + h] = ex2(s[nb][2 + h] - ref);
-        l[nb][h] = l[nb][h] * al[nb][h] + (s[nb][h] + s[nb][2 + h]);
-        same = same && al[nb][h] == 1.0f;
-        al[nb][h] *= vfac;
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float mx = fmaxf(s[nb][h], s[nb][2 + h]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, d));
+            mx = fmaxf(m[nb][h], mx);
+            const float f = m[nb][h] == mx ? 1.0f : ex2(m[nb][h] - mx);
+            m[nb][h] = mx;
+            l[nb][h] *= f;
+            al[nb][h] = f * vfac;
+          }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int k = 0; k < KS; ++k)
+#pragma unroll
+            for (int u = 0; u < 4; ++u) o[nb][k][u] *= al[nb][u & 1];
       }
+      uint32_t pb[NB][2];
+      const float vmul0 = vsc[0] * vinv, vmul1 = vsc[1] * vinv;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float ref = m[nb][h] == -INFINITY ? 0.0f : m[nb][h];
+          s[nb][h] = ex2(s[nb][h] - ref);
+          s[nb][2 + h] = ex2(s[nb][2 + h] - ref);
+          l[nb][h] += s[nb][h] + s[nb][2 + h];
+        }
+        if constexpr (kBf) {
+          pb[nb][0] = transpose8(bf16x2(s[nb][0], s[nb][1]));
+          pb[nb][1] = transpose8(bf16x2(s[nb][2], s[nb][3]));
+        } else {
+          pb[nb][0] = transpose8(half2_of(s[nb][0] * vmul0, s[nb][1] * vmul0));
+          pb[nb][1] = transpose8(half2_of(s[nb][2] * vmul1, s[nb][3] * vmul1));
+        }
+      }
+      // ---- O^T += V^T P^T
       if constexpr (kBf) {
-        pb[nb][0] = transpose8(bf16x2(s[nb][0], s[nb][1]));
-        pb[nb][1] = transpose8(bf16x2(s[nb][2], s[nb][3]));
+        // address lane: token (lane & 7) + 8 · (lane >> 4), 8-value block (lane >> 3) & 1
+        const int vt = (lane & 7) + ((lane >> 4) << 3), vh = (lane >> 3) & 1;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          uint32_t a[4];
+          ldsm4t(vs + piece<P::kInner>(vt, 2 * k + vh), a);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) mma16<true>(o[nb][k], a[0], a[1], a[2], a[3], pb[nb][0], pb[nb][1]);
+        }
       } else {
-        pb[nb][0] = transpose8(half2_of(s[nb][0] * vmul0, s[nb][1] * vmul0));
-        pb[nb][1] = transpose8(half2_of(s[nb][2] * vmul1, s[nb][3] * vmul1));
-      }
-    }
-    if (!__all_sync(kFullMask, same)) {
+        // pairs of codes as 16-bit units: values 2g, 2g + 1 of a 16-value block for tokens 2c, 2c + 1
+        const int vt = (lane & 7) + (((lane >> 3) & 1) << 3), vh = lane >> 4;
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb)
+        for (int k = 0; k < KS; k += 2) {
+          uint32_t x[4];
+          ldsm4t(vs + piece<P::kInner>(vt, k + vh), x);
 #pragma unroll
-        for (int k = 0; k < KS; ++k)
+          for (int w = 0; w < 2; ++w) {
+            uint32_t a0, a1, a2, a3;
+            widen4<FMT>(__byte_perm(x[2 * w], 0u, 0x3120), a0, a1);
+            widen4<FMT>(__byte_perm(x[2 * w + 1], 0u, 0x3120), a2, a3);
 #pragma unroll
-          for (int u = 0; u < 4; ++u) o[nb][k][u] *= al[nb][u & 1];
-    }
-    // ---- O^T += V^T P^T
-    if constexpr (kBf) {
-      // address lane: token (lane & 7) + 8 · (lane >> 4), 8-value block (lane >> 3) & 1
-      const int vt = (lane & 7) + ((lane >> 4) << 3), vh = (lane >> 3) & 1;
-#pragma unroll
-      for (int k = 0; k < KS; ++k) {
-        uint32_t a[4];
-        ldsm4t(vs + piece<P::kChunks>(vt, 2 * k + vh), a);
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) mma16<true>(o[nb][k], a[0], a[1], a[2], a[3], pb[nb][0], pb[nb][1]);
-      }
-    } else {
-      // pairs of codes as 16-bit units: values 2g, 2g + 1 of a 16-value block for tokens 2c, 2c + 1
-      const int vt = (lane & 7) + (((lane >> 3) & 1) << 3), vh = lane >> 4;
-#pragma unroll
-      for (int k = 0; k < KS; k += 2) {
-        uint32_t x[4];
-        ldsm4t(vs + piece<P::kChunks>(vt, k + vh), x);
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          uint32_t a0, a1, a2, a3;
-          widen4<FMT>(__byte_perm(x[2 * w], 0u, 0x3120), a0, a1);
-          widen4<FMT>(__byte_perm(x[2 * w + 1], 0u, 0x3120), a2, a3);
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) mma16<false>(o[nb][k + w], a0, a1, a2, a3, pb[nb][0], pb[nb][1]);
+            for (int nb = 0; nb < NB; ++nb) mma16<false>(o[nb][k + w], a0, a1, a2, a3, pb[nb][0], pb[nb][1]);
+          }
         }
       }
     }
-    stage = stage + 1 == P::kStages ? 0 : stage + 1;
-    __syncwarp();  // the stage just read is the next fetch's
+    if (++stage == P::kStages) stage = 0, phase ^= 1;
   }
-  cp_wait<0>();
-  __syncthreads();
+  __syncthreads();  // (the rings are done with)
 
   // ---- join the warps
 #pragma unroll
@@ -455,9 +542,24 @@ __global__ void __launch_bounds__(kRowsThreads) attn_rows_kernel(const __grid_co
         os[(8 * nb + 2 * c + (u & 1)) * (D + 4) + d] = o[nb][k][u];
       }
   __syncthreads();
-  const float* oj = reinterpret_cast<const float*>(smem);
-  const bool whole_context = nsplit == 1;
-  const int64_t part = (static_cast<int64_t>(b) * gridDim.y + blockIdx.y) * A.splits + split;
+  float* oj = reinterpret_cast<float*>(smem);
+  const bool alone = A.cluster == 1;
+  const int64_t part = (static_cast<int64_t>(b) * gridDim.y + blockIdx.y) * A.splits + blockIdx.x / A.cluster;
+  // the (m, l, O) of one row piece to where it goes: the result, or this cluster's partial one
+  auto put = [&](int r, int d, float M, float L, float4 acc) {
+    if (A.splits == 1) {
+      const int row = r0 + r;
+      const int64_t t = R.q0 + row / A.group;
+      const int hq = head * A.group + row % A.group;
+      const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+      const uint2 w = make_uint2(bf16x2(acc.x * inv, acc.y * inv), bf16x2(acc.z * inv, acc.w * inv));
+      *reinterpret_cast<uint2*>(A.out + t * A.o_token + hq * A.o_head + d) = w;
+      if (A.lse && d == 0) A.lse[t * A.q_heads + hq] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+    } else {
+      *reinterpret_cast<float4*>(A.part_o + (part * kRows + r) * D + d) = acc;
+      if (d == 0) *reinterpret_cast<float2*>(A.part_ml + (part * kRows + r) * 2) = make_float2(M, L);
+    }
+  };
   for (int e = tid; e < R.rows * (D / 4); e += kRowsThreads) {
     const int r = e / (D / 4), d = (e % (D / 4)) * 4;
     float M = -INFINITY;
@@ -474,23 +576,50 @@ __global__ void __launch_bounds__(kRowsThreads) attn_rows_kernel(const __grid_co
       const float4 x = *reinterpret_cast<const float4*>(oj + (w * kRows + r) * (D + 4) + d);
       acc.x += fo * x.x, acc.y += fo * x.y, acc.z += fo * x.z, acc.w += fo * x.w;
     }
-    if (whole_context) {
-      const int row = r0 + r;
-      const int64_t t = R.q0 + row / A.group;
-      const int hq = head * A.group + row % A.group;
-      const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-      const uint2 w = make_uint2(bf16x2(acc.x * inv, acc.y * inv), bf16x2(acc.z * inv, acc.w * inv));
-      *reinterpret_cast<uint2*>(A.out + t * A.o_token + hq * A.o_head + d) = w;
-      if (A.lse && d == 0) A.lse[t * A.q_heads + hq] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+    if (alone) {
+      put(r, d, M, L, acc);
     } else {
-      *reinterpret_cast<float4*>(A.part_o + (part * kRows + r) * D + d) = acc;
-      if (d == 0) *reinterpret_cast<float2*>(A.part_ml + (part * kRows + r) * 2) = make_float2(M, L);
+      // (into warp 0's part, whose same four values this thread has just read)
+      *reinterpret_cast<float4*>(oj + r * (D + 4) + d) = acc;
+      if (d == 0) s_ml[r][0] = M, s_ml[r][1] = L;
     }
   }
+  if (alone) return;
+  // ---- join the cluster: its blocks take the row pieces in turn
+  cluster_sync();
+  const uint32_t rank = cluster_rank();
+  const uint32_t o_at = smem_addr(oj), ml_at = smem_addr(&s_ml[0][0]);
+  for (int e = static_cast<int>(rank) * kRowsThreads + tid; e < R.rows * (D / 4); e += A.cluster * kRowsThreads) {
+    const int r = e / (D / 4), d = (e % (D / 4)) * 4;
+    float2 ml[8];
+    float4 x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < A.cluster) {
+        ml[k] = ld_rank2(in_rank(ml_at + r * 8, k));
+        x[k] = ld_rank4(in_rank(o_at + (r * (D + 4) + d) * 4, k));
+      }
+    float M = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < A.cluster) M = max_nan(M, ml[k].x);
+    const float ref = M == -INFINITY ? 0.0f : M;
+    float L = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < A.cluster) {
+        const float f = ex2(ml[k].x - ref);
+        L += f * ml[k].y;
+        acc.x += f * x[k].x, acc.y += f * x[k].y, acc.z += f * x[k].z, acc.w += f * x[k].w;
+      }
+    put(r, d, M, L, acc);
+  }
+  cluster_sync();  // (no block leaves while its shared memory is read)
 }
 
-// One block per query row: its splits' (m, l, O) joined as the warps' are above.  kTile and
-// rows per block as in the kernel that wrote them, so that the number of splits agrees.
+// One block per query row: its splits' (m, l, O) joined as the warps' are above.  kTile, rows per block
+// and chunk_tiles as in the kernel that wrote them, so that the number of splits agrees.
 template <int D, int kTile>
 __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ AttnArgs A, int rows_per_block) {
   constexpr int kVec = D / 4, kParts = 128 / kVec;  // threads across head_dim, splits in parallel
@@ -500,8 +629,11 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
   const int r = blockIdx.x, r0 = rb * rows_per_block, tid = threadIdx.x;
   const RowRange R = row_range<kTile>(A, b, r0, rows_per_block);
   if (r >= R.rows) return;
-  int nsplit = (R.tiles + A.chunk_tiles - 1) / A.chunk_tiles;
-  nsplit = nsplit < 1 ? 1 : nsplit > A.splits ? A.splits : nsplit;
+  int nsplit = A.splits;  // (the few-row kernel writes every partial result)
+  if (A.chunk_tiles > 0) {
+    nsplit = (R.tiles + A.chunk_tiles - 1) / A.chunk_tiles;
+    nsplit = nsplit < 1 ? 1 : nsplit > A.splits ? A.splits : nsplit;
+  }
   if (nsplit == 1) return;
   const int64_t part0 = (static_cast<int64_t>(b) * gridDim.y + blockIdx.y) * A.splits;
   const float* ml = A.part_ml + (part0 * rows_per_block + r) * 2;
@@ -549,43 +681,59 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
 template <int D, int FMT, int NB>
 cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
   constexpr int kRows = 8 * NB;
+  using P = RowsPlan<D, FMT>;
+  constexpr int smem = RowsSmem<D, FMT, NB>::kTotal;
   const int blocks = static_cast<int>((static_cast<int64_t>(a.max_q) * a.group + kRows - 1) / kRows);
   const int64_t items = static_cast<int64_t>(a.seqs) * a.kv.kv_heads * blocks;
-  // Splits: enough blocks to fill the SMs about four times over (contexts are ragged), each
-  // at least 16 tiles (256 tokens, four a warp), within the workspace.
+  // Blocks per context: enough for two rounds of the SMs (contexts are ragged), each of at least two
+  // stages a warp.  Up to 8 are one cluster; more are clusters of 8 whose partial results are joined.
   const int64_t tiles = most_tiles(a, kRT, kRows);
-  int64_t splits = (4ll * c->num_sms + items - 1) / items;
-  const int64_t by_len = (tiles + 15) / 16;
-  splits = splits > by_len ? by_len : splits;
+  const int64_t slots = static_cast<int64_t>(c->num_sms) * rows_occupancy<D, FMT, NB>();
+  int64_t want = 2 * slots / items;
+  const int64_t by_len = (tiles + 2 * kRowsWarps * P::kSub - 1) / (2 * kRowsWarps * P::kSub);
+  want = want > by_len ? by_len : want;
+  int cluster = 1;
+  while (cluster < 8 && cluster * 2 <= want) cluster *= 2;
+  int64_t splits = want / cluster;
   const int64_t slot = static_cast<int64_t>(kRows) * (D + 2) * 4;
   const int64_t by_ws = static_cast<int64_t>(kAttnWsBytes) / (items * slot);
   splits = splits > by_ws ? by_ws : splits;
-  if (splits < 1) splits = 1;
-  int64_t chunk = tiles > 0 ? (tiles + splits - 1) / splits : 1;
-  chunk = (chunk + kRowsWarps - 1) / kRowsWarps * kRowsWarps;
-  a.chunk_tiles = static_cast<int32_t>(chunk);
-  a.splits = static_cast<int32_t>(tiles > 0 ? (tiles + chunk - 1) / chunk : 1);
+  if (splits < 1 || cluster < 8) splits = 1;
+  a.cluster = cluster;
+  a.chunk_tiles = 0;
+  a.splits = static_cast<int32_t>(splits);
   a.part_o = reinterpret_cast<float*>(c->ws);
-  a.part_ml = a.part_o + items * a.splits * kRows * D;
-  constexpr int smem = rows_smem<D, FMT, NB>();
+  a.part_ml = a.part_o + items * splits * kRows * D;
   static std::atomic<uint64_t> done{0};
   if (device_todo(done)) {
     const cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<D, FMT, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     mark_device_done(done);
   }
-  const dim3 grid(static_cast<unsigned>(a.splits), static_cast<unsigned>(a.kv.kv_heads * blocks), static_cast<unsigned>(a.seqs));
-  if (grid.y > 65535) return cudaErrorInvalidConfiguration;
-  attn_rows_kernel<D, FMT, NB><<<grid, kRowsThreads, smem, st>>>(a);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || a.splits == 1) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(splits * cluster), static_cast<unsigned>(a.kv.kv_heads * blocks), static_cast<unsigned>(a.seqs));
+  if (cfg.gridDim.y > 65535) return cudaErrorInvalidConfiguration;
+  cfg.blockDim = dim3(kRowsThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = static_cast<unsigned>(cluster);
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_rows_kernel<D, FMT, NB>, a, *reinterpret_cast<const RowsMaps*>(c->maps + 256));
+  if (e != cudaSuccess || splits == 1) return e;
   return launch_attn_join(a, D, kRows, blocks, kRT, st);
 }
 
 template <int D, int FMT>
 cudaError_t go_nb(const gs_kv_cache* c, const AttnArgs& a, cudaStream_t st) {
   const int64_t rows = static_cast<int64_t>(a.max_q) * a.group;
-  return rows <= 8 ? go<D, FMT, 1>(c, a, st) : go<D, FMT, 2>(c, a, st);
+  if (rows <= 8) return go<D, FMT, 1>(c, a, st);
+  // (32 rows of head_dim 256 would need 256 registers a thread for O alone: two passes of 16)
+  if (rows <= 16 || D == 256) return go<D, FMT, 2>(c, a, st);
+  return go<D, FMT, D == 256 ? 2 : 4>(c, a, st);
 }
 template <int D>
 cudaError_t go_fmt(const gs_kv_cache* c, const AttnArgs& a, cudaStream_t st) {

@@ -18,9 +18,8 @@
 // Tensor memory (512 columns): S0 at 0, S1 at 128, O0 at 256, O1 at 256 + D.
 // Warps: softmax warpgroup(s) first (warp % 4 = its tensor-memory lanes), then the MMA issuer and the
 // loader (TMA boxes; bf16 pages go straight to the swizzled operand layout), then, beside an 8-bit
-// cache, four warps that widen the loaded codes to float16 operands: K's exact, V's times its scale;
-// K's scale multiplies the float32 score.  Q is brought into float16 by a power of two per row and the
-// weights, at most 2^8, are float16 as well.
+// cache, four warps that widen the loaded codes to float16 operands (exact).  K's scale multiplies the
+// float32 score, V's the float16 weight.  Q is brought into float16 by a power of two per row.
 // Order of products and of shared-memory stages: K(0) .. K(SB-1), then V(j), K(j + SB) for each j:
 // P(j) overlays S(j), and the tensor core takes one thread's products in order, so S(j + SB) is
 // issued right behind the product that reads P(j).
@@ -174,19 +173,6 @@ __device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ uint32_t half2_mul(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-__device__ __forceinline__ void bulk_in(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
-               "r"(bytes), "r"(smem_addr(bar))
-               : "memory");
-}
-
-constexpr float kVUp = 128.0f;  // V operands: code · scale / vref · kVUp
-
 struct TileMaps {
   CUtensorMap k, v;
 };
@@ -357,8 +343,8 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
                     tok & page_mask, head, pg, ring_full + at);
           if (scales) {
             const uint32_t sd = smem_addr(sm + P::kOffScale) + ((j % P::kScaleSlots) * 2 * kTT + lane * box) * 4;
-            bulk_in(sd, A.kv.scale_at(false, pg, head, tok & page_mask), box * 4, ring_full + at);
-            bulk_in(sd + kTT * 4, A.kv.scale_at(true, pg, head, tok & page_mask), box * 4, ring_full + at);
+            bulk_g2s_addr(sd, A.kv.scale_at(false, pg, head, tok & page_mask), box * 4, ring_full + at);
+            bulk_g2s_addr(sd + kTT * 4, A.kv.scale_at(true, pg, head, tok & page_mask), box * 4, ring_full + at);
           }
         }
         __syncwarp();
@@ -373,15 +359,13 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
   };
 
   // ---------------- widening warps (8-bit): codes -> float16 operands ----------------
-  // V's scale goes into V here, relative to a power of two at or above every V scale so far (vref, from
-  // 2^-100 up, kept beside the tile's scales for the softmax) and times 2^7, which leaves the largest
-  // code within float16: rows whose scale is 2^-21 of the largest are still held to 2^-11.
+  // The softmax multiplies V's scales into its weights; so that float16 holds the products, it takes its
+  // reference point relative to vref, a power of two at or above every V scale so far (from 2^-60 up).
   auto widen = [&]() {
     const int lt = tid - 32 * P::kWidenWarp;
     constexpr int kPieces = P::kRawStage / 16 / 128;  // 16-byte pieces of codes per thread and stage
     constexpr int kRowPieces = P::kInner / 16;
-    float vref = 7.888609052210118e-31f, vprev = vref;  // after K(j_last) and before it
-    int j_last = -1;
+    float vref = 8.673617379884035e-19f;
     const int total = items * P::kPer;
     for (int k = 0; k < total && !*stop; ++k) {
       bool value;
@@ -407,12 +391,10 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
         }
         mx = __reduce_max_sync(kFullMask, mx);
         const float top = __uint_as_float(mx > 0x7e800000u ? 0x7f000000u : (mx + 0x7fffffu) & 0x7f800000u);  // up to a power of two
-        vprev = vref;
         vref = fmaxf(vref, top);
-        j_last = j;
         if (lt == 0) reinterpret_cast<float*>(sm + P::kOffRef)[j % P::kScaleSlots] = vref;
+        if (!R.seen_by_any(j0 + lt)) sc[kTT + lt] = 0.0f;  // (its weight is 0; the page may hold a NaN)
       }
-      const float vinv = kVUp / (j == j_last ? vref : vprev);  // (K runs at most one tile ahead of V)
       const int toks = value ? P::kVTok : P::kKTok;
       const int jt = j0 + (value ? h * P::kVTok : 0);
       const bool edge = jt + toks > R.hi || (jt < R.lo && jt + toks > R.sink);  // some token no row sees
@@ -424,13 +406,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
         const int cb = rowid / toks, tr = rowid % toks;  // column block of kInner codes, token
         const uint4 x = *reinterpret_cast<const uint4*>(src + id * 16);
         uint2 q[4] = {widen_half<FMT>(x.x), widen_half<FMT>(x.y), widen_half<FMT>(x.z), widen_half<FMT>(x.w)};
-        if (value) {
-          const float f = sc[kTT + h * P::kVTok + tr] * vinv;
-          const uint32_t f2 = half2_of(f, f);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) q[i].x = half2_mul(q[i].x, f2), q[i].y = half2_mul(q[i].y, f2);
-          if (edge && !R.seen_by_any(jt + tr)) q[0] = q[1] = q[2] = q[3] = make_uint2(0u, 0u);
-        }
+        if (value && edge && !R.seen_by_any(jt + tr)) q[0] = q[1] = q[2] = q[3] = make_uint2(0u, 0u);
         const int hc = cb * (P::kInner / 64) + (ch >> 2);  // 64-column operand block
         const int c0 = (ch & 3) * 2, odd = hc & 1;
         unsigned char* rowp = dst + hc * (toks * 128) + tr * 128;
@@ -463,7 +439,8 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
     const uint32_t o_at = lane_base + 256u + static_cast<uint32_t>(s * D);
     float m = -INFINITY;
     float2 l2 = make_float2(0.0f, 0.0f);
-    float vref = 1.0f;  // (8-bit) what O is relative to
+    float vref = 1.0f;  // (8-bit) weights, sums and O are in units of vref / 2^7
+    float unit = 0.0f;  // log2 of 1 over that
     for (int j = 0; j < n && !*stop; ++j) {
       const int buf = NQ == 2 ? s : (j & 1);
       const uint32_t ph = static_cast<uint32_t>((j / SB) & 1);
@@ -507,8 +484,12 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
         float al = m == -INFINITY ? 0.0f : ex2((m - mn) * c);
         m = mn;
         l2.x *= al, l2.y *= al;
-        al *= vref / vnew;
-        vref = vnew;
+        if constexpr (!P::kBf) {
+          al *= vref / vnew;
+          l2.x *= vref / vnew, l2.y *= vref / vnew;
+          vref = vnew;
+          unit = 7.0f - log2f(vref);
+        }
         if (j > 0) {
           bool ok = true;
           if constexpr (SB == 2) ok = mbar_wait(o_done, static_cast<uint32_t>((j - 1) & 1), kWaitNs);
@@ -528,14 +509,20 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
           }
         }
       }
-      const float mc = m == -INFINITY ? 0.0f : -m * c;
+      const float mc = (m == -INFINITY ? 0.0f : -m * c) + unit;
       uint32_t* w = reinterpret_cast<uint32_t*>(x);
 #pragma unroll
       for (int i = 0; i < 128; i += 2) {
         float2 t = __ffma2_rn(make_float2(x[i], x[i + 1]), make_float2(c, c), make_float2(mc, mc));
         t.x = ex2(t.x), t.y = ex2(t.y);
         l2 = __fadd2_rn(l2, t);
-        w[i >> 1] = P::kBf ? bf16x2(t.x, t.y) : half2_of(t.x, t.y);
+        if constexpr (P::kBf) {
+          w[i >> 1] = bf16x2(t.x, t.y);
+        } else {
+          const float2 v2 = *reinterpret_cast<const float2*>(sc + kTT + i);
+          t = __fmul2_rn(t, v2);
+          w[i >> 1] = half2_of(t.x, t.y);
+        }
       }
       tm_st32(s_at, w);
       tm_st32(s_at + 32, w + 32);
@@ -559,8 +546,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
       const bool live = r < R.rows;
       const int64_t t = R.q0 + row / A.group;
       const int hq = head * A.group + row % A.group;
-      const float ounit = P::kBf ? 1.0f : vref / kVUp;  // what O is in units of
-      const float inv = l == 0.0f ? 0.0f : ounit / l;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       const int64_t part = ((static_cast<int64_t>(b) * gridDim.y + rb * A.kv.kv_heads + head) * A.splits + split) * P::kRows + r;
 #pragma unroll
       for (int q = 0; q < D / 32; ++q) {
@@ -582,11 +568,11 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
           float4* dst = reinterpret_cast<float4*>(A.part_o + part * D + 32 * q);
 #pragma unroll
           for (int i = 0; i < 8; ++i)
-            dst[i] = make_float4(o[4 * i] * ounit, o[4 * i + 1] * ounit, o[4 * i + 2] * ounit, o[4 * i + 3] * ounit);
+            dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
         }
       }
       if (live) {
-        const float mc = m * c;  // (log2 units)
+        const float mc = m * c - unit;  // (log2 units)
         if (nsplit == 1) {
           if (A.lse) A.lse[t * A.q_heads + hq] = l == 0.0f ? -INFINITY : (mc + log2f(l)) * 0.6931471805599453f;
         } else {
@@ -769,7 +755,7 @@ cudaError_t launch_attn_tile(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) 
 // The pools as (head_dim, page token, head, page) tensors, boxes of at most 128 bytes of a row (bf16:
 // one swizzle row) by as many tokens as a page and a stage share.
 const char* make_attn_maps(gs_kv_cache* c) {
-  static_assert(sizeof(TileMaps) <= sizeof(c->maps), "room for two tensor maps");
+  static_assert(4 * sizeof(CUtensorMap) <= sizeof(c->maps), "room for the tensor maps");
   const gs_kv_cache_desc& d = c->d;
   const bool bf16 = d.format == GS_DTYPE_BF16;
   const cuuint64_t el = bf16 ? 2 : 1;
@@ -781,19 +767,24 @@ const char* make_attn_maps(gs_kv_cache* c) {
   auto encode = reinterpret_cast<CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill)>(fn);
-  TileMaps* m = reinterpret_cast<TileMaps*>(c->maps);
-  for (int v = 0; v < 2; ++v) {
+  CUtensorMap* maps = reinterpret_cast<CUtensorMap*>(c->maps);
+  const int inner = bf16 ? 64 : d.head_dim < 128 ? 64 : 128;  // elements of a box row: 128 bytes, or 64
+  for (int i = 0; i < 4; ++i) {
+    const bool v = (i & 1) != 0, rows = i >= 2;
     const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d.head_dim), static_cast<cuuint64_t>(d.page_size),
                                 static_cast<cuuint64_t>(d.kv_heads), static_cast<cuuint64_t>(d.pages)};
     const cuuint64_t strides[3] = {static_cast<cuuint64_t>(v ? d.v_token_stride : d.k_token_stride) * el,
                                    static_cast<cuuint64_t>(v ? d.v_head_stride : d.k_head_stride) * el,
                                    static_cast<cuuint64_t>(v ? d.v_page_stride : d.k_page_stride) * el};
-    const int most = v && d.head_dim == 256 ? 64 : kTT;
-    const cuuint32_t box[4] = {static_cast<cuuint32_t>(bf16 ? 64 : d.head_dim < 128 ? 64 : 128), static_cast<cuuint32_t>(d.page_size < most ? d.page_size : most), 1, 1};
+    const int most = rows ? 16 : v && d.head_dim == 256 ? 64 : kTT;
+    const cuuint32_t box[4] = {static_cast<cuuint32_t>(inner), static_cast<cuuint32_t>(d.page_size < most ? d.page_size : most), 1, 1};
     const cuuint32_t ones[4] = {1, 1, 1, 1};
-    const CUresult r = encode(v ? &m->v : &m->k, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, v ? d.v : d.k, dims, strides, box, ones,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, bf16 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    // operands of the tensor cores and of ldmatrix are swizzled; codes to be widened are read row by row
+    const CUtensorMapSwizzle swizzle = !rows && !bf16 ? CU_TENSOR_MAP_SWIZZLE_NONE
+                                       : inner * el == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+    const CUresult r = encode(maps + i, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, v ? d.v : d.k,
+                              dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return "KV cache: these strides do not make a tensor map";
   }
   return nullptr;

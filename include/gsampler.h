@@ -366,7 +366,7 @@ gs_status gs_kv_cache_destroy(gs_kv_cache* c);
 const char* gs_kv_cache_last_error(const gs_kv_cache* c);
 /* Errors that the kernels found in device data since the last check (synchronising):
  * a slot past the cache (skipped), a page-table entry outside [0, pages) or past the
- * table's columns (its tokens read as zeros), a sequence longer than max_q / max_kv (cut
+ * table's columns (page 0 is read in its place), a sequence longer than max_q / max_kv (cut
  * off).  GS_EINVAL when any bit is set; GS_ETIMEOUT when a bounded wait ran out. */
 #define GS_KV_ERR_SLOT 1
 #define GS_KV_ERR_PAGE 2
