@@ -15,7 +15,7 @@ struct gs_kv_cache {
   int page_shift = 0;
   int32_t* flag = nullptr;       // device: GS_KV_ERR_* bits
   unsigned char* ws = nullptr;   // the context's attention workspace (kAttnWsBytes)
-  alignas(64) unsigned char maps[512] = {};  // tensor maps of the pools: many-row kernel's, few-row kernel's
+  alignas(64) unsigned char maps[768] = {};  // tensor maps of the pools: many-row kernel's, few-row kernel's, two-block kernel's
   std::string err;
 };
 

@@ -34,21 +34,25 @@ namespace {
 
 constexpr int kTT = 128;  // context tokens per tile
 
-template <int D, int FMT>
+// CG: blocks that share a context's tiles (tcgen05 cta_group).  Two blocks of a cluster each hold half of
+// every K tile (tokens) and V tile (columns), and one product covers the query rows of both: half the L2
+// reads, shared memory traffic and widening per row.
+template <int D, int FMT, int CG>
 struct TilePlan {
   static constexpr bool kBf = FMT == GS_DTYPE_BF16;
   static constexpr int NQ = D == 256 ? 1 : 2;   // query tiles of 128 rows
   static constexpr int SB = D == 256 ? 2 : 1;   // score buffers per query tile
-  static constexpr int kRows = 128 * NQ;
-  static constexpr int kPer = D == 256 ? 2 : 1;               // stages per K or V tile
-  static constexpr int kKTok = kTT, kKCols = D == 256 ? 128 : D;   // one K stage: tokens x columns
-  static constexpr int kVTok = D == 256 ? 64 : kTT, kVCols = D;    // one V stage
+  static constexpr int kRows = 128 * NQ;        // query rows of a block
+  static constexpr int kPer = D == 256 && CG == 1 ? 2 : 1;                   // stages per K or V tile
+  static constexpr int kKTok = kTT / CG, kKCols = kPer == 2 ? 128 : D;       // one K stage: tokens x columns
+  static constexpr int kVTok = kPer == 2 ? 64 : kTT, kVCols = D / CG;        // one V stage
   static constexpr int kStage = kKTok * kKCols * 2;
-  static constexpr int kStages = kBf ? (D == 64 ? 8 : 5) : (D == 64 ? 6 : 3);
+  static constexpr int kStages = kBf ? (D == 64 ? 8 : kStage == 16384 ? 10 : 5) : (D == 64 ? 6 : kStage == 16384 ? 5 : 3);
   static constexpr int kEl = kBf ? 2 : 1;
-  static constexpr int kInner = D * kEl < 128 ? D * kEl : 128;  // bytes of a row in one TMA box
+  static constexpr int kKInner = kKCols * kEl < 128 ? kKCols * kEl : 128;  // bytes of a row in one TMA box
+  static constexpr int kVInner = kVCols * kEl < 128 ? kVCols * kEl : 128;
   static constexpr int kRawStage = kBf ? 0 : kStage / 2;        // codes of one stage
-  static constexpr int kRawStages = kBf ? 0 : D == 64 ? 6 : 3;
+  static constexpr int kRawStages = kBf ? 0 : kStage == 16384 ? 6 : 3;
   // Tiles whose scales are held: K(j + 8) is loaded only after the codes of an earlier V were taken
   // (raw and operand stages reach at most 6 tiles ahead of the products).
   static constexpr int kScaleSlots = 8;
@@ -57,7 +61,7 @@ struct TilePlan {
   static constexpr int kOffRaw = kOffStage + kStages * kStage;
   static constexpr int kOffScale = kOffRaw + kRawStages * kRawStage;       // [slot][K, V][kTT] float
   static constexpr int kOffQf = kOffScale + (kBf ? 0 : kScaleSlots * 2 * kTT * 4);  // [kRows] float
-  static constexpr int kOffRef = kOffQf + (kBf ? 0 : kRows * 4);           // [slot] float
+  static constexpr int kOffRef = kOffQf + (kBf ? 0 : kRows * 4);           // [slot][widening warp] float
   static constexpr int kOffBar = kOffRef + (kBf ? 0 : 128);
   static constexpr int kSmem = kOffBar + 512 + 1024;  // barriers, alignment slack
   // Warpgroups: softmax (NQ), then the MMA issuer with the TMA loader beside it, then the widening
@@ -75,12 +79,13 @@ struct TilePlan {
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
-// tcgen05.mma kind::f16: f32 accumulators, bf16 or f16 operands (both the same), M = 128.
-template <bool BF16>
-constexpr uint32_t kIdescQK = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
-template <int D, bool BF16>
+// tcgen05.mma kind::f16: f32 accumulators, bf16 or f16 operands (both the same), M = 128
+// rows a block.
+template <bool BF16, int CG>
+constexpr uint32_t kIdescQK = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | ((128u >> 3) << 17) | ((128u * CG >> 4) << 24);
+template <int D, bool BF16, int CG>
 constexpr uint32_t kIdescPV = (1u << 4) | (BF16 ? (1u << 7) | (1u << 10) : 0u) | (1u << 16) |
-                              ((static_cast<uint32_t>(D) >> 3) << 17) | ((128u >> 4) << 24);  // bit 16: B MN-major (V's token rows)
+                              ((static_cast<uint32_t>(D) >> 3) << 17) | ((128u * CG >> 4) << 24);  // bit 16: B MN-major (V's token rows)
 
 // 128-byte swizzled operands.  K-major: 8-row groups 1024 bytes apart (stride offset).  MN-major:
 // blocks of 64 columns `lead` bytes apart (leading offset), 8-token groups 1024 bytes apart.
@@ -88,23 +93,68 @@ __device__ __forceinline__ uint64_t desc_sw128(uint32_t saddr, uint32_t lead) {
   return static_cast<uint64_t>((saddr >> 4) & 0x3FFFu) | (static_cast<uint64_t>(lead >> 4) << 16) |
          (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
+#define GS_TC_MMA(GROUP, A_OPERAND)                                                                                   \
+  "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::" GROUP ".kind::f16 [%0], " A_OPERAND    \
+  ", %2, %3, p;\n\t}\n"
+template <int CG>
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
+  if constexpr (CG == 1) asm volatile(GS_TC_MMA("1", "%1")::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+  else asm volatile(GS_TC_MMA("2", "%1")::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
 }
+template <int CG>
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(acc)
-      : "memory");
+  if constexpr (CG == 1) asm volatile(GS_TC_MMA("1", "[%1]")::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+  else asm volatile(GS_TC_MMA("2", "[%1]")::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
 }
+// Completion of the products issued so far, on the barrier of every block of the group.
+template <int CG>
 __device__ __forceinline__ void commit_to(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+  if constexpr (CG == 1)
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+  else
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(smem_addr(bar)),
+                 "h"(static_cast<uint16_t>(3))
+                 : "memory");
 }
 __device__ __forceinline__ void arrive_on(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+// Arrival on the first block's barrier (the one that issues the products).
+template <int CG>
+__device__ __forceinline__ void arrive_first(uint64_t* bar) {
+  if constexpr (CG == 1) {
+    arrive_on(bar);
+  } else {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_addr(bar)));
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
+  }
+}
+// Bounded wait on a barrier that the other block may have arrived on.
+template <int CG>
+__device__ __forceinline__ bool wait_group(uint64_t* bar, uint32_t parity) {
+  if constexpr (CG == 1) {
+    return mbar_wait(bar, parity, kWaitNs);
+  } else {
+    uint64_t t0 = 0;
+    for (;;) {
+      uint32_t done;
+      asm volatile(
+          "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+          : "=r"(done)
+          : "r"(smem_addr(bar)), "r"(parity)
+          : "memory");
+      if (done) return true;
+      const uint64_t t = globaltimer_ns();
+      if (t0 == 0) t0 = t;
+      else if (t - t0 > kWaitNs) return false;
+    }
+  }
+}
+template <int CG>
+__device__ __forceinline__ void group_sync() {
+  if constexpr (CG == 1) __syncthreads();
+  else asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -177,10 +227,10 @@ struct TileMaps {
   CUtensorMap k, v;
 };
 
-template <int D, int FMT>
-__global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
+template <int D, int FMT, int CG>
+__global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     attn_tile_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ TileMaps maps) {
-  using P = TilePlan<D, FMT>;
+  using P = TilePlan<D, FMT, CG>;
   constexpr int NQ = P::NQ, SB = P::SB;
   extern __shared__ unsigned char smem_raw[];
   const uint32_t raw = smem_addr(smem_raw);
@@ -194,6 +244,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
   uint64_t* m_done = o_done + 2;
   uint64_t* raw_full = m_done + 2;                  // [kRawStages]
   uint64_t* raw_free = raw_full + P::kRawStages;    // [kRawStages]
+  uint64_t* peer_full = raw_free + P::kRawStages;   // [kStages] (CG 2, first block): the other block's stage is there
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(m_done + 1);
   volatile int* stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -202,12 +253,13 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
   const int blocks = gridDim.y / A.kv.kv_heads;
   const int head = blockIdx.y / blocks;
   const int rb = blocks - 1 - static_cast<int>(blockIdx.y % blocks);  // longest contexts first
-  const int r0 = rb * P::kRows;
-  const RowRange R = row_range<kTT>(A, b, r0, P::kRows);
-  if (R.rows == 0) return;
+  const int rank = CG == 1 ? 0 : static_cast<int>(blockIdx.x) & 1;  // (clusters of CG blocks along x)
+  const int r0 = rb * (CG * P::kRows);  // the group's first row; this block's are rank · kRows further on
+  const RowRange R = row_range<kTT>(A, b, r0, CG * P::kRows);
+  if (R.rows == 0) return;  // (the whole group)
   int nsplit = (R.tiles + A.chunk_tiles - 1) / A.chunk_tiles;
   nsplit = nsplit < 1 ? 1 : nsplit > A.splits ? A.splits : nsplit;
-  const int split = blockIdx.x;
+  const int split = static_cast<int>(blockIdx.x) / CG;
   if (split >= nsplit) return;
   const int t_begin = split * A.chunk_tiles;
   const int t_end = split == nsplit - 1 ? R.tiles : t_begin + A.chunk_tiles;
@@ -220,10 +272,12 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(s_full + s, 1);
-      mbar_init(p_full + s, 128);
+      mbar_init(p_full + s, 4 * CG);
       mbar_init(o_done + s, 1);
     }
     mbar_init(m_done, 1);
+    if constexpr (CG == 2)
+      for (int s = 0; s < P::kStages; ++s) mbar_init(peer_full + s, 1);
     for (int s = 0; s < P::kRawStages; ++s) {
       mbar_init(raw_full + s, 1);
       mbar_init(raw_free + s, 128);
@@ -231,8 +285,13 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
     *stop = 0;
   }
   if (warp == P::kMmaWarp) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(tmem_slot)) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    if constexpr (CG == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(tmem_slot)) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(tmem_slot)) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
   }
   // ---- Q: [query tile][64-column block][128 rows][128 bytes], swizzled; rows past the block zero
   {
@@ -241,8 +300,8 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
     for (int id = tid; id < P::kRows * kCh; id += P::kThreads) {
       const int r = id / kCh, ch = id % kCh;
       uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (r < R.rows) {
-        const int row = r0 + r;
+      if (rank * P::kRows + r < R.rows) {
+        const int row = r0 + rank * P::kRows + r;
         x = *reinterpret_cast<const uint4*>(A.q + (R.q0 + row / A.group) * A.q_token + (head * A.group + row % A.group) * A.q_head + ch * 8);
         x.x ^= flip, x.y ^= flip, x.z ^= flip, x.w ^= flip;
       }
@@ -269,7 +328,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
     fence_async();
   }
   fence_before();
-  __syncthreads();
+  group_sync<CG>();
   fence_after();
   const uint32_t tmem = *tmem_slot;
   auto give_up = [&]() {
@@ -289,19 +348,20 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
     else value = true, j = k - (n - SB > 0 ? n - SB : 0);
   };
 
+  const int32_t* table = A.table + b * A.table_stride;
+  const int shift = A.kv.page_shift, page_mask = (1 << shift) - 1;
+  auto page_of = [&](int tok) {  // the page of a context token, checked
+    const int col = tok >> shift;
+    int pg = col < A.table_cols ? __ldg(table + col) : -1;
+    if (pg < 0 || pg >= A.kv.pages) {
+      atomicOr(A.flag, GS_KV_ERR_PAGE);
+      pg = 0;
+    }
+    return pg;
+  };
+
   // ---------------- loaders ----------------
   auto load = [&]() {
-    const int32_t* table = A.table + b * A.table_stride;
-    const int shift = A.kv.page_shift, page_mask = (1 << shift) - 1;
-    auto page_of = [&](int tok) {  // the page of a context token, checked
-      const int col = tok >> shift;
-      int pg = col < A.table_cols ? __ldg(table + col) : -1;
-      if (pg < 0 || pg >= A.kv.pages) {
-        atomicOr(A.flag, GS_KV_ERR_PAGE);
-        pg = 0;
-      }
-      return pg;
-    };
     // The stages of a bf16 cache are the operands themselves; of an 8-bit one the codes, which the
     // widening warps turn into operands.
     constexpr int kRing = P::kBf ? P::kStages : P::kRawStages;
@@ -320,32 +380,28 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
         if (round > 0) ok = __all_sync(kFullMask, mbar_wait(ring_free + at, static_cast<uint32_t>((round - 1) & 1), kWaitNs));
         if (!ok) break;
         const int toks = value ? P::kVTok : P::kKTok;
+        const int inner = value ? P::kVInner : P::kKInner;
         const int box = min(1 << shift, toks);  // tokens per box
         const int groups = toks / box;
-        const int cols = (value ? P::kVCols : P::kKCols) * P::kEl / P::kInner;
-        const int j0 = R.tile(t_begin + j) * kTT + (value ? h * P::kVTok : 0);
+        const int cols = (value ? P::kVCols : P::kKCols) * P::kEl / inner;
+        const int j0 = R.tile(t_begin + j) * kTT + (value ? h * P::kVTok : rank * P::kKTok);
         // lane g: token group g (at most 8); a group past every row's last token stays as it is
         const int tok = j0 + lane * box;
         const bool real = lane < groups && tok < R.hi;
         const int pg = real ? page_of(tok) : 0;
-        const bool scales = !P::kBf && !value && h == 0;  // both scales of a tile come with its K codes
         const unsigned live = __ballot_sync(kFullMask, real);
-        const uint32_t bytes = static_cast<uint32_t>(__popc(live) * box * (cols * P::kInner + (scales ? 8 : 0)));
+        const uint32_t bytes = static_cast<uint32_t>(__popc(live) * box * cols * inner);
         if (lane == 0) {
           if (bytes) mbar_expect_tx(ring_full + at, bytes);
           else arrive_on(ring_full + at);
         }
         __syncwarp();
         if (real) {
-          const uint32_t dst = smem_addr(ring + at * kRingStage) + lane * box * P::kInner;
+          const uint32_t dst = smem_addr(ring + at * kRingStage) + lane * box * inner;
+          const int x0 = value ? rank * P::kVCols : h * P::kKCols;
           for (int cb = 0; cb < cols; ++cb)
-            tma_box(dst + cb * toks * P::kInner, value ? &maps.v : &maps.k, cb * (P::kInner / P::kEl) + (value ? 0 : h * P::kKCols),
-                    tok & page_mask, head, pg, ring_full + at);
-          if (scales) {
-            const uint32_t sd = smem_addr(sm + P::kOffScale) + ((j % P::kScaleSlots) * 2 * kTT + lane * box) * 4;
-            bulk_g2s_addr(sd, A.kv.scale_at(false, pg, head, tok & page_mask), box * 4, ring_full + at);
-            bulk_g2s_addr(sd + kTT * 4, A.kv.scale_at(true, pg, head, tok & page_mask), box * 4, ring_full + at);
-          }
+            tma_box(dst + cb * toks * inner, value ? &maps.v : &maps.k, x0 + cb * (inner / P::kEl), tok & page_mask, head, pg,
+                    ring_full + at);
         }
         __syncwarp();
         ++issued;
@@ -364,8 +420,19 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
   auto widen = [&]() {
     const int lt = tid - 32 * P::kWidenWarp;
     constexpr int kPieces = P::kRawStage / 16 / 128;  // 16-byte pieces of codes per thread and stage
-    constexpr int kRowPieces = P::kInner / 16;
     float vref = 8.673617379884035e-19f;
+    // the scales of token lt of the tile after this one, in flight
+    float next_k = 0.0f, next_v = 0.0f;
+    auto fetch_scales = [&](int j) {
+      const int tok = R.tile(t_begin + j) * kTT + lt;
+      next_k = next_v = 0.0f;  // (a hidden token's weight is 0; its page may hold a NaN)
+      if (R.seen_by_any(tok)) {
+        const int pg = page_of(tok), off = tok & page_mask;
+        next_k = __ldg(A.kv.scale_at(false, pg, head, off));
+        next_v = __ldg(A.kv.scale_at(true, pg, head, off));
+      }
+    };
+    if (n > 0) fetch_scales(0);
     const int total = items * P::kPer;
     for (int k = 0; k < total && !*stop; ++k) {
       bool value;
@@ -382,39 +449,44 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
       const int j0 = R.tile(t_begin + j) * kTT;
       float* sc = reinterpret_cast<float*>(sm + P::kOffScale) + (j % P::kScaleSlots) * (2 * kTT);
       if (!value && h == 0) {
-        // every warp takes the tile's largest V scale of visible tokens (bits of positive floats in order)
-        uint32_t mx = 0;
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const float v = sc[kTT + lane + 32 * u];
-          if (R.seen_by_any(j0 + lane + 32 * u) && v < INFINITY) mx = max(mx, __float_as_uint(fmaxf(v, 0.0f)));
-        }
-        mx = __reduce_max_sync(kFullMask, mx);
+        // The tile's largest V scale (bits of positive floats in order), by way of this warp's maximum of
+        // the 32 tokens it holds: vref only has to be at or above the scales that were seen with it, so each
+        // warp keeps one of its own.
+        sc[lt] = next_k;
+        sc[kTT + lt] = next_v;
+        const uint32_t mx = __reduce_max_sync(kFullMask, next_v > 0.0f && next_v < INFINITY ? __float_as_uint(next_v) : 0u);
         const float top = __uint_as_float(mx > 0x7e800000u ? 0x7f000000u : (mx + 0x7fffffu) & 0x7f800000u);  // up to a power of two
         vref = fmaxf(vref, top);
-        if (lt == 0) reinterpret_cast<float*>(sm + P::kOffRef)[j % P::kScaleSlots] = vref;
-        if (!R.seen_by_any(j0 + lt)) sc[kTT + lt] = 0.0f;  // (its weight is 0; the page may hold a NaN)
+        if (lane == 0) reinterpret_cast<float*>(sm + P::kOffRef)[(j % P::kScaleSlots) * 4 + (warp & 3)] = vref;
+        if (j + 1 < n) fetch_scales(j + 1);
       }
       const int toks = value ? P::kVTok : P::kKTok;
-      const int jt = j0 + (value ? h * P::kVTok : 0);
+      const int jt = j0 + (value ? h * P::kVTok : rank * P::kKTok);
       const bool edge = jt + toks > R.hi || (jt < R.lo && jt + toks > R.sink);  // some token no row sees
       const unsigned char* src = sm + P::kOffRaw + rs * P::kRawStage;
       unsigned char* dst = sm + P::kOffStage + at * P::kStage;
+      // TOKS tokens in column blocks of INNER codes
+      auto turn = [&](auto v_, auto toks_, auto inner_) {
+        constexpr bool V = decltype(v_)::value;
+        constexpr int TOKS = decltype(toks_)::value, INNER = decltype(inner_)::value;
 #pragma unroll
-      for (int u = 0; u < kPieces; ++u) {
-        const int id = lt + 128 * u, ch = id % kRowPieces, rowid = id / kRowPieces;
-        const int cb = rowid / toks, tr = rowid % toks;  // column block of kInner codes, token
-        const uint4 x = *reinterpret_cast<const uint4*>(src + id * 16);
-        uint2 q[4] = {widen_half<FMT>(x.x), widen_half<FMT>(x.y), widen_half<FMT>(x.z), widen_half<FMT>(x.w)};
-        if (value && edge && !R.seen_by_any(jt + tr)) q[0] = q[1] = q[2] = q[3] = make_uint2(0u, 0u);
-        const int hc = cb * (P::kInner / 64) + (ch >> 2);  // 64-column operand block
-        const int c0 = (ch & 3) * 2, odd = hc & 1;
-        unsigned char* rowp = dst + hc * (toks * 128) + tr * 128;
-        // (lanes of the two blocks store their halves in opposite order: no two in one bank)
-        const uint4 lo = make_uint4(q[0].x, q[0].y, q[1].x, q[1].y), hi = make_uint4(q[2].x, q[2].y, q[3].x, q[3].y);
-        *reinterpret_cast<uint4*>(rowp + (((c0 + odd) ^ (tr & 7)) << 4)) = odd ? hi : lo;
-        *reinterpret_cast<uint4*>(rowp + (((c0 + 1 - odd) ^ (tr & 7)) << 4)) = odd ? lo : hi;
-      }
+        for (int u = 0; u < kPieces; ++u) {
+          const int id = lt + 128 * u, ch = id % (INNER / 16), rowid = id / (INNER / 16);
+          const int cb = rowid / TOKS, tr = rowid % TOKS;  // column block, token
+          const uint4 x = *reinterpret_cast<const uint4*>(src + id * 16);
+          uint2 q[4] = {widen_half<FMT>(x.x), widen_half<FMT>(x.y), widen_half<FMT>(x.z), widen_half<FMT>(x.w)};
+          if (V && edge && !R.seen_by_any(jt + tr)) q[0] = q[1] = q[2] = q[3] = make_uint2(0u, 0u);
+          const int hc = (cb * INNER + ch * 16) / 64;  // 64-column operand block
+          const int c0 = (ch & 3) * 2, odd = INNER == 64 ? (tr >> 1) & 1 : hc & 1;
+          unsigned char* rowp = dst + hc * (TOKS * 128) + tr * 128;
+          // (the lanes of a store's quarter warp take their halves in opposite orders: no two in one bank)
+          const uint4 lo = make_uint4(q[0].x, q[0].y, q[1].x, q[1].y), hi = make_uint4(q[2].x, q[2].y, q[3].x, q[3].y);
+          *reinterpret_cast<uint4*>(rowp + (((c0 + odd) ^ (tr & 7)) << 4)) = odd ? hi : lo;
+          *reinterpret_cast<uint4*>(rowp + (((c0 + 1 - odd) ^ (tr & 7)) << 4)) = odd ? lo : hi;
+        }
+      };
+      if (value) turn(std::true_type{}, std::integral_constant<int, P::kVTok>{}, std::integral_constant<int, P::kVInner>{});
+      else turn(std::false_type{}, std::integral_constant<int, P::kKTok>{}, std::integral_constant<int, P::kKInner>{});
       fence_async();
       arrive_on(raw_free + rs);
       arrive_on(full + at);
@@ -428,7 +500,8 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
     const int s = NQ == 2 ? warp >> 2 : 0;  // query tile
     const int quad = warp & 3;
     const int r = s * 128 + quad * 32 + lane;
-    const int row = r0 + min(r, R.rows - 1);
+    const int gr = rank * P::kRows + r;  // row of the group
+    const int row = r0 + min(gr, R.rows - 1);
     const int p = R.p0 + row / A.group;
     const int lo = A.window ? max(p - A.window + 1, 0) : 0;
     float c = fabsf(A.scale_log2);
@@ -478,7 +551,10 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
       const float tm = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       const bool move = tm > m + slack || (m == -INFINITY && tm > m);
       float vnew = vref;
-      if constexpr (!P::kBf) vnew = reinterpret_cast<const float*>(sm + P::kOffRef)[j % P::kScaleSlots];
+      if constexpr (!P::kBf) {
+        const float4 v4 = reinterpret_cast<const float4*>(sm + P::kOffRef)[j % P::kScaleSlots];
+        vnew = fmaxf(fmaxf(v4.x, v4.y), fmaxf(v4.z, v4.w));
+      }
       if (__any_sync(kFullMask, move || vnew != vref)) {
         const float mn = move ? tm : m;
         float al = m == -INFINITY ? 0.0f : ex2((m - mn) * c);
@@ -528,7 +604,8 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
       tm_st32(s_at + 32, w + 32);
       tm_wait_st();
       fence_before();
-      arrive_on(p_full + buf);
+      __syncwarp();
+      if (lane == 0) arrive_first<CG>(p_full + buf);
     }
     // ---- epilogue
     const float l = l2.x + l2.y;
@@ -543,11 +620,11 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
     ok = __all_sync(kFullMask, ok);
     if (ok) {
       fence_after();
-      const bool live = r < R.rows;
+      const bool live = gr < R.rows;
       const int64_t t = R.q0 + row / A.group;
       const int hq = head * A.group + row % A.group;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      const int64_t part = ((static_cast<int64_t>(b) * gridDim.y + rb * A.kv.kv_heads + head) * A.splits + split) * P::kRows + r;
+      const int64_t part = ((static_cast<int64_t>(b) * gridDim.y + rb * A.kv.kv_heads + head) * A.splits + split) * (CG * P::kRows) + gr;
 #pragma unroll
       for (int q = 0; q < D / 32; ++q) {
         float o[32];
@@ -587,8 +664,11 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
     // ---------------- MMA issuer ----------------
     const bool leader = elected();
     int cnt = 0;  // stages consumed
-    auto stage_ready = [&](int at) {
+    auto stage_ready = [&](int at) {  // this block's half
       return __all_sync(kFullMask, mbar_wait(full + at % P::kStages, static_cast<uint32_t>((at / P::kStages) & 1), kWaitNs));
+    };
+    auto peer_ready = [&](int at) {  // the other's
+      return CG == 1 || __all_sync(kFullMask, wait_group<CG>(peer_full + at % P::kStages, static_cast<uint32_t>((at / P::kStages) & 1)));
     };
     // S(query tile s, buffer buf) = Q K^T over stages at .. at + kPer - 1
     auto scores = [&](int s, int buf, int at) {
@@ -598,10 +678,9 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
           const uint32_t ka = smem_addr(sm + P::kOffStage + ((at + h) % P::kStages) * P::kStage);
           const uint32_t qa = smem_addr(sm + s * (D / 64) * 16384 + h * (P::kKCols / 64) * 16384);
 #pragma unroll
-          for (int k = 0; k < P::kKCols / 16; ++k) {
-            const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-            mma_ss(tmem + buf * 128, desc_sw128(qa + off, 16), desc_sw128(ka + off, 16), kIdescQK<P::kBf>, (h | k) != 0 ? 1u : 0u);
-          }
+          for (int k = 0; k < P::kKCols / 16; ++k)
+            mma_ss<CG>(tmem + buf * 128, desc_sw128(qa + (k >> 2) * 16384 + (k & 3) * 32, 16),
+                       desc_sw128(ka + (k >> 2) * (P::kKTok * 128) + (k & 3) * 32, 16), kIdescQK<P::kBf, CG>, (h | k) != 0 ? 1u : 0u);
         }
       }
       __syncwarp();
@@ -613,8 +692,8 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
       const bool hidden = j0 + P::kVTok > R.hi || (j0 < R.lo && j0 + P::kVTok > R.sink);
       if (!P::kBf || !hidden) return;
       unsigned char* st = sm + P::kOffStage + (at % P::kStages) * P::kStage;
-      for (int id = lane; id < P::kVTok * (D / 8); id += 32) {
-        const int tr = id / (D / 8), ch = id % (D / 8);
+      for (int id = lane; id < P::kVTok * (P::kVCols / 8); id += 32) {
+        const int tr = id / (P::kVCols / 8), ch = id % (P::kVCols / 8);
         if (!R.seen_by_any(j0 + tr))
           *reinterpret_cast<uint4*>(st + (ch >> 3) * (P::kVTok * 128) + tr * 128 + ((ch & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
       }
@@ -622,22 +701,38 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
       __syncwarp();
     };
     bool ok = true;
-    for (int i = 0; ok && i < SB && i < n; ++i) {
-      for (int h = 0; ok && h < P::kPer; ++h) ok = stage_ready(cnt + h);
+    if (CG == 2 && rank == 1) {
+      // second block: tells the first when a stage of its own is there (and clean)
+      for (int i = 0; ok && i < items && !*stop; ++i) {
+        bool value;
+        int j;
+        item(i, value, j);
+        for (int h = 0; ok && h < P::kPer; ++h, ++cnt) {
+          ok = stage_ready(cnt);
+          if (!ok) break;
+          if (value) clean(cnt, j, h);
+          if (lane == 0) arrive_first<CG>(peer_full + cnt % P::kStages);
+          __syncwarp();
+        }
+      }
+    }
+    const bool issues = CG == 1 || rank == 0;
+    for (int i = 0; issues && ok && i < SB && i < n; ++i) {
+      for (int h = 0; ok && h < P::kPer; ++h) ok = stage_ready(cnt + h) && peer_ready(cnt + h);
       if (!ok) break;
       fence_after();
       for (int s = 0; s < NQ; ++s) {
         scores(s, NQ == 2 ? s : i, cnt);
         if (leader) {
-          commit_to(s_full + (NQ == 2 ? s : i));
+          commit_to<CG>(s_full + (NQ == 2 ? s : i));
           if (s == NQ - 1)
-            for (int h = 0; h < P::kPer; ++h) commit_to(freeb + (cnt + h) % P::kStages);
+            for (int h = 0; h < P::kPer; ++h) commit_to<CG>(freeb + (cnt + h) % P::kStages);
         }
         __syncwarp();
       }
       cnt += P::kPer;
     }
-    for (int j = 0; ok && j < n && !*stop; ++j) {
+    for (int j = 0; issues && ok && j < n && !*stop; ++j) {
       const int v_at = cnt, k_at = cnt + P::kPer;
       const bool more = j + SB < n;
       for (int s = 0; ok && s < NQ; ++s) {
@@ -646,8 +741,9 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
           for (int h = 0; ok && h < P::kPer; ++h) {
             ok = stage_ready(v_at + h);
             if (ok) clean(v_at + h, j, h);
+            ok = ok && peer_ready(v_at + h);
           }
-        ok = ok && __all_sync(kFullMask, mbar_wait(p_full + buf, static_cast<uint32_t>((j / SB) & 1), kWaitNs));
+        ok = ok && __all_sync(kFullMask, wait_group<CG>(p_full + buf, static_cast<uint32_t>((j / SB) & 1)));
         if (!ok) break;
         fence_after();
         if (leader) {
@@ -656,24 +752,24 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
             const uint32_t va = smem_addr(sm + P::kOffStage + ((v_at + h) % P::kStages) * P::kStage);
 #pragma unroll
             for (int k = 0; k < P::kVTok / 16; ++k)
-              mma_ts(tmem + 256 + s * D, tmem + buf * 128 + (h * P::kVTok + k * 16) / 2, desc_sw128(va + k * 2048, P::kVTok * 128),
-                     kIdescPV<D, P::kBf>, (j | h | k) != 0 ? 1u : 0u);
+              mma_ts<CG>(tmem + 256 + s * D, tmem + buf * 128 + (h * P::kVTok + k * 16) / 2, desc_sw128(va + k * 2048, P::kVTok * 128),
+                         kIdescPV<D, P::kBf, CG>, (j | h | k) != 0 ? 1u : 0u);
           }
-          commit_to(o_done + s);
+          commit_to<CG>(o_done + s);
           if (s == NQ - 1)
-            for (int h = 0; h < P::kPer; ++h) commit_to(freeb + (v_at + h) % P::kStages);
+            for (int h = 0; h < P::kPer; ++h) commit_to<CG>(freeb + (v_at + h) % P::kStages);
         }
         __syncwarp();
         if (more) {
           if (s == 0)
-            for (int h = 0; ok && h < P::kPer; ++h) ok = stage_ready(k_at + h);
+            for (int h = 0; ok && h < P::kPer; ++h) ok = stage_ready(k_at + h) && peer_ready(k_at + h);
           if (!ok) break;
           fence_after();
           scores(s, buf, k_at);
           if (leader) {
-            commit_to(s_full + buf);
+            commit_to<CG>(s_full + buf);
             if (s == NQ - 1)
-              for (int h = 0; h < P::kPer; ++h) commit_to(freeb + (k_at + h) % P::kStages);
+              for (int h = 0; h < P::kPer; ++h) commit_to<CG>(freeb + (k_at + h) % P::kStages);
           }
           __syncwarp();
         }
@@ -682,7 +778,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
     }
     if (!ok) give_up();
     // every product has completed before tensor memory is freed
-    if (leader) commit_to(m_done);
+    if (leader && issues) commit_to<CG>(m_done);
     __syncwarp();
     if (!__all_sync(kFullMask, mbar_wait(m_done, 0, kWaitNs))) give_up();
    } else if (warp == P::kLoadWarp) {
@@ -693,24 +789,26 @@ __global__ void __launch_bounds__(TilePlan<D, FMT>::kThreads, 1)
    widen();
   }
   fence_before();
-  __syncthreads();
+  group_sync<CG>();  // (no block leaves while the other's products may read its shared memory)
   if (warp == P::kMmaWarp) {
     fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if constexpr (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
   }
 }
 
-template <int D, int FMT>
+template <int D, int FMT, int CG>
 cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
-  using P = TilePlan<D, FMT>;
-  const int blocks = static_cast<int>((static_cast<int64_t>(a.max_q) * a.group + P::kRows - 1) / P::kRows);
+  using P = TilePlan<D, FMT, CG>;
+  constexpr int kRows = CG * P::kRows;  // rows of a group of blocks
+  const int blocks = static_cast<int>((static_cast<int64_t>(a.max_q) * a.group + kRows - 1) / kRows);
   const int64_t items = static_cast<int64_t>(a.seqs) * a.kv.kv_heads * blocks;
-  const int64_t tiles = most_tiles(a, kTT, P::kRows);
+  const int64_t tiles = most_tiles(a, kTT, kRows);
   // Splits: only while the blocks do not fill the SMs, each of at least 8 tiles, within the workspace.
-  int64_t splits = c->num_sms / items;
+  int64_t splits = c->num_sms / CG / items;
   const int64_t by_len = tiles / 8;
   splits = splits > by_len ? by_len : splits;
-  const int64_t slot = static_cast<int64_t>(P::kRows) * (D + 2) * 4;
+  const int64_t slot = static_cast<int64_t>(kRows) * (D + 2) * 4;
   const int64_t by_ws = static_cast<int64_t>(kAttnWsBytes) / (items * slot);
   splits = splits > by_ws ? by_ws : splits;
   if (splits < 1) splits = 1;
@@ -718,31 +816,53 @@ cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
   a.chunk_tiles = static_cast<int32_t>(chunk);
   a.splits = static_cast<int32_t>(tiles > 0 ? (tiles + chunk - 1) / chunk : 1);
   a.part_o = reinterpret_cast<float*>(c->ws);
-  a.part_ml = a.part_o + items * a.splits * P::kRows * D;
+  a.part_ml = a.part_o + items * a.splits * kRows * D;
   static std::atomic<uint64_t> done{0};
   if (device_todo(done)) {
     cudaFuncAttributes at;
-    cudaError_t e = cudaFuncGetAttributes(&at, attn_tile_kernel<D, FMT>);
+    cudaError_t e = cudaFuncGetAttributes(&at, attn_tile_kernel<D, FMT, CG>);
     // (the warpgroups' shares must not exceed what the block is launched with)
     if (e == cudaSuccess && P::kSoftRegs != P::kRegs && at.numRegs != P::kRegs) e = cudaErrorInvalidKernelImage;
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(attn_tile_kernel<D, FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, P::kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(attn_tile_kernel<D, FMT, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, P::kSmem);
     if (e != cudaSuccess) return e;
     mark_device_done(done);
   }
-  const dim3 grid(static_cast<unsigned>(a.splits), static_cast<unsigned>(a.kv.kv_heads * blocks), static_cast<unsigned>(a.seqs));
-  if (grid.y > 65535) return cudaErrorInvalidConfiguration;
-  attn_tile_kernel<D, FMT><<<grid, P::kThreads, P::kSmem, st>>>(a, *reinterpret_cast<const TileMaps*>(c->maps));
-  cudaError_t e = cudaGetLastError();
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.splits * CG), static_cast<unsigned>(a.kv.kv_heads * blocks), static_cast<unsigned>(a.seqs));
+  if (cfg.gridDim.y > 65535) return cudaErrorInvalidConfiguration;
+  cfg.blockDim = dim3(P::kThreads);
+  cfg.dynamicSmemBytes = P::kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = CG;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = CG > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_tile_kernel<D, FMT, CG>, a,
+                                           *reinterpret_cast<const TileMaps*>(c->maps + (CG == 1 ? 0 : 512)));
   if (e != cudaSuccess || a.splits == 1) return e;
-  return launch_attn_join(a, D, P::kRows, blocks, kTT, st);
+  return launch_attn_join(a, D, kRows, blocks, kTT, st);
+}
+
+template <int D, int FMT>
+cudaError_t go_cg(const gs_kv_cache* c, const AttnArgs& a, cudaStream_t st) {
+  // Two blocks a group at head_dim 256, where one block's 128 rows read K and V faster than L2 gives them
+  // (2048 x 16384 tokens, 16 / 8 heads: bf16 627 -> 483 us, e4m3 871 -> 573 us).  At head_dim 128 a block has
+  // 256 rows of its own, and the round trips between the blocks cost more than the halved reads save
+  // (32 / 8 heads: bf16 485 -> 718 us, e4m3 727 -> 873 us).
+  if constexpr (D == 256) {
+    if (static_cast<int64_t>(a.max_q) * a.group > TilePlan<D, FMT, 1>::kRows) return go<D, FMT, 2>(c, a, st);
+  }
+  return go<D, FMT, 1>(c, a, st);
 }
 
 template <int D>
 cudaError_t go_fmt(const gs_kv_cache* c, const AttnArgs& a, cudaStream_t st) {
   switch (c->d.format) {
-    case GS_DTYPE_BF16: return go<D, GS_DTYPE_BF16>(c, a, st);
-    case GS_DTYPE_E4M3: return go<D, GS_DTYPE_E4M3>(c, a, st);
-    default: return go<D, GS_DTYPE_INT8>(c, a, st);
+    case GS_DTYPE_BF16: return go_cg<D, GS_DTYPE_BF16>(c, a, st);
+    case GS_DTYPE_E4M3: return go_cg<D, GS_DTYPE_E4M3>(c, a, st);
+    default: return go_cg<D, GS_DTYPE_INT8>(c, a, st);
   }
 }
 
@@ -755,7 +875,7 @@ cudaError_t launch_attn_tile(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) 
 // The pools as (head_dim, page token, head, page) tensors, boxes of at most 128 bytes of a row (bf16:
 // one swizzle row) by as many tokens as a page and a stage share.
 const char* make_attn_maps(gs_kv_cache* c) {
-  static_assert(4 * sizeof(CUtensorMap) <= sizeof(c->maps), "room for the tensor maps");
+  static_assert(6 * sizeof(CUtensorMap) <= sizeof(c->maps), "room for the tensor maps");
   const gs_kv_cache_desc& d = c->d;
   const bool bf16 = d.format == GS_DTYPE_BF16;
   const cuuint64_t el = bf16 ? 2 : 1;
@@ -768,17 +888,20 @@ const char* make_attn_maps(gs_kv_cache* c) {
                                               const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill)>(fn);
   CUtensorMap* maps = reinterpret_cast<CUtensorMap*>(c->maps);
-  const int inner = bf16 ? 64 : d.head_dim < 128 ? 64 : 128;  // elements of a box row: 128 bytes, or 64
-  for (int i = 0; i < 4; ++i) {
-    const bool v = (i & 1) != 0, rows = i >= 2;
+  for (int i = 0; i < 6; ++i) {  // K and V of the one-block kernel, the few-row kernel, the two-block kernel
+    const bool v = (i & 1) != 0, rows = i / 2 == 1, two = i / 2 == 2;
     const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d.head_dim), static_cast<cuuint64_t>(d.page_size),
                                 static_cast<cuuint64_t>(d.kv_heads), static_cast<cuuint64_t>(d.pages)};
     const cuuint64_t strides[3] = {static_cast<cuuint64_t>(v ? d.v_token_stride : d.k_token_stride) * el,
                                    static_cast<cuuint64_t>(v ? d.v_head_stride : d.k_head_stride) * el,
                                    static_cast<cuuint64_t>(v ? d.v_page_stride : d.k_page_stride) * el};
-    const int most = rows ? 16 : v && d.head_dim == 256 ? 64 : kTT;
+    // a box row: 128 bytes, or the whole (half) row where that is less
+    const int row = v && two ? d.head_dim / 2 : d.head_dim;
+    const int inner = row * static_cast<int>(el) < 128 ? row : 128 / static_cast<int>(el);
+    const int most = rows ? 16 : two ? (v ? kTT : kTT / 2) : v && d.head_dim == 256 ? 64 : kTT;
     const cuuint32_t box[4] = {static_cast<cuuint32_t>(inner), static_cast<cuuint32_t>(d.page_size < most ? d.page_size : most), 1, 1};
     const cuuint32_t ones[4] = {1, 1, 1, 1};
+    if (two && d.head_dim != 256) break;
     // operands of the tensor cores and of ldmatrix are swizzled; codes to be widened are read row by row
     const CUtensorMapSwizzle swizzle = !rows && !bf16 ? CU_TENSOR_MAP_SWIZZLE_NONE
                                        : inner * el == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
