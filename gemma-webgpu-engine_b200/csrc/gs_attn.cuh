@@ -56,11 +56,12 @@ struct AttnArgs {
   const int32_t* q_start;
   const int32_t* kv_len;
   const int32_t* table;
-  int64_t q_token, q_head, o_token, o_head;  // element strides
+  int32_t q_token, q_head, o_token, o_head;  // element strides
   int64_t table_stride;
   int64_t tokens;
   int32_t table_cols;
   int32_t seqs, q_heads, group;
+  float inv_group;      // 1 / group
   int32_t max_q, max_kv;
   int32_t window, sinks;
   float scale_log2;     // scale · log2(e): scores in log2 units
@@ -83,10 +84,35 @@ struct RowRange {
   int32_t hi;       // tokens >= hi are hidden from every row
   int32_t lo;       // tokens in [sink, lo) are hidden from every row (0 without a window)
   int32_t sink;     // tokens below stay visible (0 without a window)
+  int32_t t0, g0;   // new token and head of the block's row 0
   int32_t sink_tiles, first_tile, tiles;  // context tiles: [0, sink_tiles), then from first_tile
   __device__ __forceinline__ int tile(int i) const { return i < sink_tiles ? i : first_tile + i - sink_tiles; }
+  // New token and head of the group of row i of the block.  (g0 + i + 1/2) / group stays 1 / (2 group) away from
+  // every whole number, which the float product's error does not reach below 2^21.
+  __device__ __forceinline__ int token_of(const AttnArgs& A, int i, int& g) const {
+    const int x = g0 + i, t = static_cast<int>((static_cast<float>(x) + 0.5f) * A.inv_group);
+    g = x - t * A.group;
+    return t0 + t;
+  }
   __device__ __forceinline__ bool seen_by_any(int j) const { return j < hi && (j >= lo || j < sink); }
 };
+
+__device__ __forceinline__ const __nv_bfloat16* q_row(const AttnArgs& A, const RowRange& R, int head, int t, int g) {
+  return A.q + static_cast<int64_t>(R.q0 + t) * A.q_token + static_cast<int64_t>(head * A.group + g) * A.q_head;
+}
+__device__ __forceinline__ __nv_bfloat16* o_row(const AttnArgs& A, const RowRange& R, int head, int t, int g) {
+  return A.out + static_cast<int64_t>(R.q0 + t) * A.o_token + static_cast<int64_t>(head * A.group + g) * A.o_head;
+}
+// Power of two that brings a row into [1, 2) at its largest component (all bits of `top`, the largest
+// magnitude's bf16 pattern), as the factor down and the factor back; 1 for a row of zeros or not finite.
+__device__ __forceinline__ void row_power(uint32_t top, float& down, float& up) {
+  int e = static_cast<int>(top >> 7) - 127;
+  e = top == 0u || e > 127 ? 0 : min(max(e, -120), 120);
+  down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+  up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+}
+// Larger magnitudes of two bf16 pairs, and of a pair's halves (patterns without sign order as values do).
+__device__ __forceinline__ uint32_t pair_max(uint32_t a, uint32_t b) { return __vmaxu2(a & 0x7fff7fffu, b & 0x7fff7fffu); }
 
 // Rows [r0, r0 + cap) of sequence b, context tiles of kTile tokens.
 template <int kTile>
@@ -103,6 +129,8 @@ __device__ __forceinline__ RowRange row_range(const AttnArgs& A, int b, int r0, 
   R.p0 = R.len - R.nq;
   R.nq = min(R.nq, A.max_q);
   R.rows = min(cap, R.nq * A.group - r0);
+  R.t0 = r0 / A.group;
+  R.g0 = r0 - R.t0 * A.group;
   if (R.rows <= 0) {
     R.rows = 0;
     R.tiles = 0;
@@ -110,7 +138,7 @@ __device__ __forceinline__ RowRange row_range(const AttnArgs& A, int b, int r0, 
     return R;
   }
   if (bad && threadIdx.x == 0) atomicOr(A.flag, GS_KV_ERR_LENGTH);
-  const int pf = R.p0 + r0 / A.group, pl = R.p0 + (r0 + R.rows - 1) / A.group;
+  const int pf = R.p0 + R.t0, pl = R.p0 + (r0 + R.rows - 1) / A.group;
   R.hi = max(pl + 1, 0);
   R.lo = A.window ? max(pf - A.window + 1, 0) : 0;
   R.lo = min(R.lo, R.hi);

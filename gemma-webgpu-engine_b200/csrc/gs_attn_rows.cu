@@ -263,8 +263,9 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
   for (int nb = warp; nb < NB; nb += kRowsWarps) {
     const int r = 8 * nb + g;
     const bool live = r < R.rows;
-    const int row = r0 + (live ? r : 0);
-    const __nv_bfloat16* q = A.q + (R.q0 + row / A.group) * A.q_token + (head * A.group + row % A.group) * A.q_head;
+    int gq;
+    const int tq = R.token_of(A, live ? r : 0, gq);
+    const __nv_bfloat16* q = q_row(A, R, head, tq, gq);
     uint32_t w[KS][2];
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
@@ -275,19 +276,13 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
     }
     float f = 1.0f;
     if constexpr (!kBf) {
-      float mx = 0.0f;
+      uint32_t mx = 0;
 #pragma unroll
-      for (int k = 0; k < KS; ++k)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) mx = fmaxf(mx, fmaxf(fabsf(bf16_lo(w[k][h])), fabsf(bf16_hi(w[k][h]))));
-      mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, 2));
-      // 2^-e with 2^e <= mx < 2^(e + 1); exponents clamped so that both factors are normal
-      int e = static_cast<int>((__float_as_uint(mx) >> 23) & 0xffu) - 127;
-      e = mx == 0.0f || e > 127 ? 0 : max(e, -120);
-      e = min(e, 120);
-      const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-      f = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+      for (int k = 0; k < KS; ++k) mx = __vmaxu2(mx, pair_max(w[k][0], w[k][1]));
+      mx = __vmaxu2(mx, __shfl_xor_sync(kFullMask, mx, 1));
+      mx = __vmaxu2(mx, __shfl_xor_sync(kFullMask, mx, 2));
+      float down;
+      row_power(max(mx & 0xffffu, mx >> 16), down, f);
 #pragma unroll
       for (int k = 0; k < KS; ++k)
 #pragma unroll
@@ -316,9 +311,10 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
     for (int h = 0; h < 2; ++h) {
       const int r = 8 * nb + 2 * c + h;
       qf[nb][h] = s_qf[r];
-      pos[nb][h] = R.p0 + (r0 + min(r, R.rows - 1)) / A.group;
+      int gq;
+      pos[nb][h] = R.p0 + R.token_of(A, min(r, R.rows - 1), gq);
     }
-  const int p_min = R.p0 + r0 / A.group, p_max = R.hi - 1;
+  const int p_min = R.p0 + R.t0, p_max = R.hi - 1;
 
   float o[NB][KS][4];
   float m[NB][2], l[NB][2];
@@ -548,13 +544,12 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
   // the (m, l, O) of one row piece to where it goes: the result, or this cluster's partial one
   auto put = [&](int r, int d, float M, float L, float4 acc) {
     if (A.splits == 1) {
-      const int row = r0 + r;
-      const int64_t t = R.q0 + row / A.group;
-      const int hq = head * A.group + row % A.group;
+      int gq;
+      const int t = R.token_of(A, r, gq);
       const float inv = L == 0.0f ? 0.0f : 1.0f / L;
       const uint2 w = make_uint2(bf16x2(acc.x * inv, acc.y * inv), bf16x2(acc.z * inv, acc.w * inv));
-      *reinterpret_cast<uint2*>(A.out + t * A.o_token + hq * A.o_head + d) = w;
-      if (A.lse && d == 0) A.lse[t * A.q_heads + hq] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+      *reinterpret_cast<uint2*>(o_row(A, R, head, t, gq) + d) = w;
+      if (A.lse && d == 0) A.lse[static_cast<int64_t>(R.q0 + t) * A.q_heads + head * A.group + gq] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
     } else {
       *reinterpret_cast<float4*>(A.part_o + (part * kRows + r) * D + d) = acc;
       if (d == 0) *reinterpret_cast<float2*>(A.part_ml + (part * kRows + r) * 2) = make_float2(M, L);
@@ -669,13 +664,12 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
     acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
   }
   L = s_lse[0] + s_lse[1] + s_lse[2] + s_lse[3];
-  const int row = r0 + r;
-  const int64_t t = R.q0 + row / A.group;
-  const int hq = head * A.group + row % A.group;
+  int gq;
+  const int t = R.token_of(A, r, gq);
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-  *reinterpret_cast<uint2*>(A.out + t * A.o_token + hq * A.o_head + d) =
+  *reinterpret_cast<uint2*>(o_row(A, R, head, t, gq) + d) =
       make_uint2(bf16x2(acc.x * inv, acc.y * inv), bf16x2(acc.z * inv, acc.w * inv));
-  if (A.lse && d == 0) A.lse[t * A.q_heads + hq] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+  if (A.lse && d == 0) A.lse[static_cast<int64_t>(R.q0 + t) * A.q_heads + head * A.group + gq] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
 
 template <int D, int FMT, int NB>

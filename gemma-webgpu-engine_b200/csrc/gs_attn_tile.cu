@@ -242,7 +242,8 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
   uint64_t* p_full = s_full + 2;           // [2]
   uint64_t* o_done = p_full + 2;           // [NQ]
   uint64_t* m_done = o_done + 2;
-  uint64_t* raw_full = m_done + 2;                  // [kRawStages]
+  uint64_t* q_full = m_done + 2;                    // every query tile of the group is in shared memory
+  uint64_t* raw_full = q_full + 1;                  // [kRawStages]
   uint64_t* raw_free = raw_full + P::kRawStages;    // [kRawStages]
   uint64_t* peer_full = raw_free + P::kRawStages;   // [kStages] (CG 2, first block): the other block's stage is there
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(m_done + 1);
@@ -276,6 +277,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       mbar_init(o_done + s, 1);
     }
     mbar_init(m_done, 1);
+    mbar_init(q_full, 4 * NQ * CG);
     if constexpr (CG == 2)
       for (int s = 0; s < P::kStages; ++s) mbar_init(peer_full + s, 1);
     for (int s = 0; s < P::kRawStages; ++s) {
@@ -292,40 +294,6 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(tmem_slot)) : "memory");
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
     }
-  }
-  // ---- Q: [query tile][64-column block][128 rows][128 bytes], swizzled; rows past the block zero
-  {
-    constexpr int kCh = D / 8;
-    const uint32_t flip = A.scale_log2 < 0.0f ? 0x80008000u : 0u;  // (a negative scale: -q and |scale|)
-    for (int id = tid; id < P::kRows * kCh; id += P::kThreads) {
-      const int r = id / kCh, ch = id % kCh;
-      uint4 x = make_uint4(0u, 0u, 0u, 0u);
-      if (rank * P::kRows + r < R.rows) {
-        const int row = r0 + rank * P::kRows + r;
-        x = *reinterpret_cast<const uint4*>(A.q + (R.q0 + row / A.group) * A.q_token + (head * A.group + row % A.group) * A.q_head + ch * 8);
-        x.x ^= flip, x.y ^= flip, x.z ^= flip, x.w ^= flip;
-      }
-      if constexpr (!P::kBf) {
-        // float16 by a power of two per row (bf16 has fewer mantissa bits: exact except for components
-        // below 2^-17 of the row's largest); the lanes of a row are neighbours
-        uint32_t w[4] = {x.x, x.y, x.z, x.w};
-        float mx = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(fabsf(bf16_lo(w[i])), fabsf(bf16_hi(w[i]))));
-#pragma unroll
-        for (int o = kCh >> 1; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(kFullMask, mx, o));
-        int e = static_cast<int>((__float_as_uint(mx) >> 23) & 0xffu) - 127;
-        e = mx == 0.0f || e > 127 ? 0 : min(max(e, -120), 120);
-        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = half2_of(bf16_lo(w[i]) * down, bf16_hi(w[i]) * down);
-        x = make_uint4(w[0], w[1], w[2], w[3]);
-        if (ch == 0) reinterpret_cast<float*>(sm + P::kOffQf)[r] = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-      }
-      const int rr = r & 127, blk = (r >> 7) * (D / 64) + (ch >> 3), c = ch & 7;
-      *reinterpret_cast<uint4*>(sm + blk * 16384 + rr * 128 + ((c ^ (rr & 7)) << 4)) = x;
-    }
-    fence_async();
   }
   fence_before();
   group_sync<CG>();
@@ -498,16 +466,57 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     // ---------------- softmax: one query row per thread ----------------
     set_regs<P::kRegs, P::kSoftRegs>();
     const int s = NQ == 2 ? warp >> 2 : 0;  // query tile
+    // ---- Q: [query tile][64-column block][128 rows][128 bytes], swizzled; rows past the group zero.  Each
+    // warpgroup brings its own tile, sixteen bytes a lane, eight loads at a time, while the loaders start.
+    {
+      constexpr int kCh = D / 8, kRowsAt = 128 / kCh;  // pieces of a row; rows a warpgroup covers at once
+      constexpr int kBatch = 8;
+      const uint32_t flip = A.scale_log2 < 0.0f ? 0x80008000u : 0u;  // (a negative scale: -q and |scale|)
+      const int qt = tid & 127, ch = qt % kCh;
+      unsigned char* tile = sm + s * (D / 64) * 16384 + (ch >> 3) * 16384;
+      for (int i0 = 0; i0 < kCh; i0 += kBatch) {
+        uint4 x[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int rr = (i0 + i) * kRowsAt + qt / kCh, gq = rank * P::kRows + s * 128 + rr;
+          x[i] = make_uint4(0u, 0u, 0u, 0u);
+          int g;
+          const int t = R.token_of(A, gq, g);
+          if (gq < R.rows) x[i] = *reinterpret_cast<const uint4*>(q_row(A, R, head, t, g) + ch * 8);
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int rr = (i0 + i) * kRowsAt + qt / kCh;
+          uint32_t w[4] = {x[i].x ^ flip, x[i].y ^ flip, x[i].z ^ flip, x[i].w ^ flip};
+          if constexpr (!P::kBf) {
+            // float16 by a power of two per row (bf16 has fewer mantissa bits: exact except for components
+            // below 2^-17 of the row's largest); the lanes of a row are neighbours
+            uint32_t mx = pair_max(pair_max(w[0], w[1]), pair_max(w[2], w[3]));
+#pragma unroll
+            for (int o = kCh >> 1; o > 0; o >>= 1) mx = __vmaxu2(mx, __shfl_xor_sync(kFullMask, mx, o));
+            float down, up;
+            row_power(max(mx & 0xffffu, mx >> 16), down, up);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) w[u] = half2_of(bf16_lo(w[u]) * down, bf16_hi(w[u]) * down);
+            if (ch == 0) reinterpret_cast<float*>(sm + P::kOffQf)[s * 128 + rr] = up;
+          }
+          *reinterpret_cast<uint4*>(tile + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+      fence_async();
+      __syncwarp();
+      if (lane == 0) arrive_first<CG>(q_full);
+    }
     const int quad = warp & 3;
     const int r = s * 128 + quad * 32 + lane;
     const int gr = rank * P::kRows + r;  // row of the group
-    const int row = r0 + min(gr, R.rows - 1);
-    const int p = R.p0 + row / A.group;
+    int hq;
+    const int tq = R.token_of(A, min(gr, R.rows - 1), hq);
+    hq += head * A.group;
+    const int p = R.p0 + tq;
     const int lo = A.window ? max(p - A.window + 1, 0) : 0;
-    float c = fabsf(A.scale_log2);
-    if constexpr (!P::kBf) c *= reinterpret_cast<const float*>(sm + P::kOffQf)[r];
-    c = fmaxf(c, 1e-30f);  // (0 would turn a hidden score's -inf into NaN)
-    const float slack = 8.0f / c;
+    float c = fmaxf(fabsf(A.scale_log2), 1e-30f);  // (0 would turn a hidden score's -inf into NaN)
+    float slack = 8.0f / c;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const uint32_t o_at = lane_base + 256u + static_cast<uint32_t>(s * D);
     float m = -INFINITY;
@@ -524,6 +533,12 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         break;
       }
       fence_after();
+      if constexpr (!P::kBf) {
+        if (j == 0) {  // (every warp's Q is in place: the products have read it)
+          c = fmaxf(fabsf(A.scale_log2) * reinterpret_cast<const float*>(sm + P::kOffQf)[r], 1e-30f);
+          slack = 8.0f / c;
+        }
+      }
       float x[128];
 #pragma unroll
       for (int q = 0; q < 4; ++q) tm_ld32(s_at + 32 * q, x + 32 * q);
@@ -621,37 +636,61 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     if (ok) {
       fence_after();
       const bool live = gr < R.rows;
-      const int64_t t = R.q0 + row / A.group;
-      const int hq = head * A.group + row % A.group;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       const int64_t part = ((static_cast<int64_t>(b) * gridDim.y + rb * A.kv.kv_heads + head) * A.splits + split) * (CG * P::kRows) + gr;
+      if (nsplit == 1) {
+        // by way of shared memory (the query tile's, which no product reads any more): whole rows leave in
+        // 16-byte pieces of neighbouring lanes
+        constexpr int kCh = D / 8;
+        unsigned char* st = sm + s * (D / 64) * 16384 + quad * 32 * D * 2;
 #pragma unroll
-      for (int q = 0; q < D / 32; ++q) {
-        float o[32];
-        if (n > 0) {
-          tm_ld32(o_at + 32 * q, o);
-          tm_wait_ld();
-        } else {
+        for (int q = 0; q < D / 32; ++q) {
+          float o[32];
+          if (n > 0) {
+            tm_ld32(o_at + 32 * q, o);
+            tm_wait_ld();
+          } else {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0.0f;
-        }
-        if (live && nsplit == 1) {
-          uint4* dst = reinterpret_cast<uint4*>(A.out + t * A.o_token + hq * A.o_head + 32 * q);
+            for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+          }
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            dst[i] = make_uint4(bf16x2(o[8 * i] * inv, o[8 * i + 1] * inv), bf16x2(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
-                                bf16x2(o[8 * i + 4] * inv, o[8 * i + 5] * inv), bf16x2(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
-        } else if (live) {
-          float4* dst = reinterpret_cast<float4*>(A.part_o + part * D + 32 * q);
+            *reinterpret_cast<uint4*>(st + lane * D * 2 + (((4 * q + i) ^ (lane & 7)) << 4)) =
+                make_uint4(bf16x2(o[8 * i] * inv, o[8 * i + 1] * inv), bf16x2(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
+                           bf16x2(o[8 * i + 4] * inv, o[8 * i + 5] * inv), bf16x2(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
+        }
+        __syncwarp();
+        const int base = rank * P::kRows + s * 128 + quad * 32;  // the warp's first row of the group
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+        for (int i = 0; i < kCh; ++i) {
+          const int rr = (i * 32 + lane) / kCh, ch = (i * 32 + lane) % kCh;
+          int g;
+          const int t = R.token_of(A, base + rr, g);
+          if (base + rr < R.rows)
+            *reinterpret_cast<uint4*>(o_row(A, R, head, t, g) + ch * 8) = *reinterpret_cast<const uint4*>(st + rr * D * 2 + ((ch ^ (rr & 7)) << 4));
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < D / 32; ++q) {
+          float o[32];
+          if (n > 0) {
+            tm_ld32(o_at + 32 * q, o);
+            tm_wait_ld();
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+          }
+          if (live) {
+            float4* dst = reinterpret_cast<float4*>(A.part_o + part * D + 32 * q);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) dst[i] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+          }
         }
       }
       if (live) {
         const float mc = m * c - unit;  // (log2 units)
         if (nsplit == 1) {
-          if (A.lse) A.lse[t * A.q_heads + hq] = l == 0.0f ? -INFINITY : (mc + log2f(l)) * 0.6931471805599453f;
+          if (A.lse) A.lse[static_cast<int64_t>(R.q0 + tq) * A.q_heads + hq] = l == 0.0f ? -INFINITY : (mc + log2f(l)) * 0.6931471805599453f;
         } else {
           *reinterpret_cast<float2*>(A.part_ml + part * 2) = make_float2(m == -INFINITY ? m : mc, l);
         }
@@ -717,6 +756,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       }
     }
     const bool issues = CG == 1 || rank == 0;
+    if (issues && n > 0) ok = ok && __all_sync(kFullMask, wait_group<CG>(q_full, 0));
     for (int i = 0; issues && ok && i < SB && i < n; ++i) {
       for (int h = 0; ok && h < P::kPer; ++h) ok = stage_ready(cnt + h) && peer_ready(cnt + h);
       if (!ok) break;

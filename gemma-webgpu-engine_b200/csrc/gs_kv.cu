@@ -384,7 +384,7 @@ gs_status gs_attention(gs_kv_cache* c, const gs_attention_args* p, void* stream)
   if (!p->q || !p->out || !p->kv_len || !p->page_table)
     return kfail(c, GS_EINVAL, "q, out, kv_len and page_table are required");
   if (!p->q_start && p->tokens != p->seqs) return kfail(c, GS_EINVAL, "without q_start every sequence has one token");
-  if (p->q_heads < 1 || p->q_heads % c->d.kv_heads != 0)
+  if (p->q_heads < 1 || p->q_heads > (1 << 20) || p->q_heads % c->d.kv_heads != 0)
     return kfail(c, GS_EINVAL, "q_heads must be a multiple of the cache's kv_heads");
   if (p->max_q < 1 || p->max_kv < 0) return kfail(c, GS_EINVAL, "max_q >= 1 and max_kv >= 0 are required");
   if (!p->q_start && p->max_q != 1) return kfail(c, GS_EINVAL, "without q_start max_q is 1");
@@ -398,7 +398,8 @@ gs_status gs_attention(gs_kv_cache* c, const gs_attention_args* p, void* stream)
     return kfail(c, GS_EUNSUPPORTED, "tokens and page table columns are at most 2^31 - 1");
   const int64_t st[4] = {p->q_token_stride, p->q_head_stride, p->out_token_stride, p->out_head_stride};
   for (int64_t s : st)
-    if (s < c->d.head_dim || s % 8 != 0) return kfail(c, GS_EINVAL, "q and out strides must be >= head_dim and multiples of 8");
+    if (s < c->d.head_dim || s % 8 != 0 || s > 0x7fffffffll)
+      return kfail(c, GS_EINVAL, "q and out strides must be >= head_dim, multiples of 8 and below 2^31");
   if (reinterpret_cast<uintptr_t>(p->q) % 16 || reinterpret_cast<uintptr_t>(p->out) % 16)
     return kfail(c, GS_EINVAL, "q and out must be 16-byte aligned");
   const int64_t group = p->q_heads / c->d.kv_heads;
@@ -414,13 +415,15 @@ gs_status gs_attention(gs_kv_cache* c, const gs_attention_args* p, void* stream)
   a.q_start = p->q_start;
   a.kv_len = p->kv_len;
   a.table = p->page_table;
-  a.q_token = st[0], a.q_head = st[1], a.o_token = st[2], a.o_head = st[3];
+  a.q_token = static_cast<int32_t>(st[0]), a.q_head = static_cast<int32_t>(st[1]);
+  a.o_token = static_cast<int32_t>(st[2]), a.o_head = static_cast<int32_t>(st[3]);
   a.table_stride = p->page_table_stride;
   a.table_cols = static_cast<int32_t>(p->page_table_cols);
   a.tokens = p->tokens;
   a.seqs = p->seqs;
   a.q_heads = p->q_heads;
   a.group = static_cast<int32_t>(group);
+  a.inv_group = 1.0f / static_cast<float>(group);
   a.max_q = p->max_q;
   a.max_kv = p->max_kv;
   // (a window that covers max_kv tokens hides nothing)
