@@ -71,9 +71,9 @@ struct TilePlan {
   static constexpr int kGroups = NQ + (kBf ? 1 : 2);
   static constexpr int kThreads = 128 * kGroups;
   static constexpr int kRegs = kGroups == 2 ? 248 : kGroups == 3 ? 168 : 128;
-  static constexpr int kSoftRegs = kGroups == 2 ? 248 : kBf ? 200 : NQ == 1 ? 224 : 176;
-  static constexpr int kMmaRegs = kGroups == 2 ? 248 : kBf ? 104 : NQ == 1 ? 96 : 64;
-  static constexpr int kLoadRegs = kBf ? 0 : NQ == 1 ? 184 : 96;  // (widening warps)
+  static constexpr int kSoftRegs = kGroups == 2 ? 248 : kBf ? 200 : NQ == 1 ? 224 : 192;
+  static constexpr int kMmaRegs = kGroups == 2 ? 248 : kBf ? 104 : NQ == 1 ? 96 : 48;
+  static constexpr int kLoadRegs = kBf ? 0 : NQ == 1 ? 184 : 80;  // (widening warps)
   static_assert(NQ * kSoftRegs + kMmaRegs + kLoadRegs == kGroups * kRegs, "register shares");
   static_assert(kVTok * kVCols * 2 == kStage, "K and V stages are one size");
   static_assert(kSmem <= 227 * 1024, "shared memory");
@@ -467,10 +467,10 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     set_regs<P::kRegs, P::kSoftRegs>();
     const int s = NQ == 2 ? warp >> 2 : 0;  // query tile
     // ---- Q: [query tile][64-column block][128 rows][128 bytes], swizzled; rows past the group zero.  Each
-    // warpgroup brings its own tile, sixteen bytes a lane, eight loads at a time, while the loaders start.
+    // warpgroup brings its own tile, sixteen bytes a lane, 8 or 16 loads at a time, while the loaders start.
     {
       constexpr int kCh = D / 8, kRowsAt = 128 / kCh;  // pieces of a row; rows a warpgroup covers at once
-      constexpr int kBatch = 8;
+      constexpr int kBatch = kCh < 16 ? 8 : 16;
       const uint32_t flip = A.scale_log2 < 0.0f ? 0x80008000u : 0u;  // (a negative scale: -q and |scale|)
       const int qt = tid & 127, ch = qt % kCh;
       unsigned char* tile = sm + s * (D / 64) * 16384 + (ch >> 3) * 16384;
@@ -548,7 +548,9 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
 #pragma unroll
         for (int i = 0; i < 128; i += 4) {
           const float4 k4 = *reinterpret_cast<const float4*>(sc + i);
-          x[i] *= k4.x, x[i + 1] *= k4.y, x[i + 2] *= k4.z, x[i + 3] *= k4.w;
+          const float2 a = __fmul2_rn(make_float2(x[i], x[i + 1]), make_float2(k4.x, k4.y));
+          const float2 b2 = __fmul2_rn(make_float2(x[i + 2], x[i + 3]), make_float2(k4.z, k4.w));
+          x[i] = a.x, x[i + 1] = a.y, x[i + 2] = b2.x, x[i + 3] = b2.y;
         }
       }
       const bool whole = j0 + kTT - 1 <= p && (j0 >= lo || j0 + kTT <= R.sink);
@@ -602,19 +604,26 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       }
       const float mc = (m == -INFINITY ? 0.0f : -m * c) + unit;
       uint32_t* w = reinterpret_cast<uint32_t*>(x);
+      float2 l3 = make_float2(0.0f, 0.0f);  // (two chains of the sum)
 #pragma unroll
-      for (int i = 0; i < 128; i += 2) {
+      for (int i = 0; i < 128; i += 4) {
         float2 t = __ffma2_rn(make_float2(x[i], x[i + 1]), make_float2(c, c), make_float2(mc, mc));
-        t.x = ex2(t.x), t.y = ex2(t.y);
+        float2 u = __ffma2_rn(make_float2(x[i + 2], x[i + 3]), make_float2(c, c), make_float2(mc, mc));
+        t.x = ex2(t.x), t.y = ex2(t.y), u.x = ex2(u.x), u.y = ex2(u.y);
         l2 = __fadd2_rn(l2, t);
+        l3 = __fadd2_rn(l3, u);
         if constexpr (P::kBf) {
           w[i >> 1] = bf16x2(t.x, t.y);
+          w[(i >> 1) + 1] = bf16x2(u.x, u.y);
         } else {
-          const float2 v2 = *reinterpret_cast<const float2*>(sc + kTT + i);
-          t = __fmul2_rn(t, v2);
+          const float4 v4 = *reinterpret_cast<const float4*>(sc + kTT + i);
+          t = __fmul2_rn(t, make_float2(v4.x, v4.y));
+          u = __fmul2_rn(u, make_float2(v4.z, v4.w));
           w[i >> 1] = half2_of(t.x, t.y);
+          w[(i >> 1) + 1] = half2_of(u.x, u.y);
         }
       }
+      l2 = __fadd2_rn(l2, l3);
       tm_st32(s_at, w);
       tm_st32(s_at + 32, w + 32);
       tm_wait_st();
