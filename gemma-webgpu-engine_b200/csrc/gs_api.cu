@@ -125,10 +125,13 @@ gs_status ensure_plans_slot(gs_ctx* c, int k, size_t n) {
 namespace gs {
 int ctx_device(const gs_ctx* c) { return c->device; }
 void ctx_set_error(gs_ctx* c, const char* msg) { c->err = msg; }
-cudaError_t ctx_attn_workspace(gs_ctx* c, size_t bytes, unsigned char** out) {
+cudaError_t ctx_attn_workspace(gs_ctx* c, size_t bytes, size_t zeroed_tail, unsigned char** out) {
   cudaError_t e = cudaSuccess;
-  if (!c->attn_ws) e = cudaMalloc(&c->attn_ws, bytes);
-  if (e != cudaSuccess) c->attn_ws = nullptr;
+  if (!c->attn_ws) {
+    e = cudaMalloc(&c->attn_ws, bytes);
+    if (e != cudaSuccess) c->attn_ws = nullptr;
+    else e = cudaMemset(c->attn_ws + bytes - zeroed_tail, 0, zeroed_tail);
+  }
   *out = c->attn_ws;
   return e;
 }

@@ -24,6 +24,7 @@ namespace gs {
 // Workspace of split-context partial results: [partial][rows][head_dim] float32 outputs and
 // [partial][rows][2] maxima and sums.  The planner never asks for more.
 constexpr size_t kAttnWsBytes = 64u << 20;
+constexpr size_t kAttnTicketBytes = 16u << 10;  // behind it, zero between calls
 
 struct KvPool {
   const unsigned char* k;
@@ -68,6 +69,9 @@ struct AttnArgs {
   int32_t chunk_tiles;  // context tiles per split (0: every context in `splits` even parts)
   int32_t splits;       // partial results per (sequence, head, row block)
   int32_t cluster;      // blocks per partial result (few-row kernel)
+  int32_t row_blocks;   // (many-row kernel) blocks of query rows per sequence and head
+  int32_t units;        // (many-row kernel, balanced) sequences times row blocks
+  unsigned* tickets;    // [groups][8] finished pieces of the item that begins in a group, per warp; zero between calls
   float* part_o;        // [seq][row block][kv head][split][rows][head_dim]
   float* part_ml;       // [..][rows][2]: running maximum (log2 units) and sum
   int32_t* flag;

@@ -63,7 +63,8 @@ struct TilePlan {
   static constexpr int kOffQf = kOffScale + (kBf ? 0 : kScaleSlots * 2 * kTT * 4);  // [kRows] float
   static constexpr int kOffRef = kOffQf + (kBf ? 0 : kRows * 4);           // [slot][widening warp] float
   static constexpr int kOffBar = kOffRef + (kBf ? 0 : 128);
-  static constexpr int kSmem = kOffBar + 512 + 1024;  // barriers, alignment slack
+  static constexpr int kOffWalk = kOffBar + 512;                           // (bf16) a Walk per warp
+  static constexpr int kSmem = kOffWalk + (kBf ? 1536 : 0) + 1024;         // alignment slack
   // Warpgroups: softmax (NQ), then the MMA issuer with the TMA loader beside it, then the widening
   // loaders.  Registers a thread: a row of 128 scores lives in its softmax thread; the shares add
   // up to what the block is launched with.
@@ -227,7 +228,109 @@ struct TileMaps {
   CUtensorMap k, v;
 };
 
-template <int D, int FMT, int CG>
+// One stretch of context tiles of one item (sequence, key/value head, query rows of a group of blocks).
+struct Piece {
+  RowRange R;
+  int b, head;
+  int t_begin, n;  // context tiles
+  int part;        // partial-result slot, or -1: the whole context is here
+  int first, pieces;  // (balanced, pieces > 0) first group with a piece of the item, and how many have one
+};
+
+// The pieces of a group of blocks.  Fixed: grid (split, head and row block, sequence), one
+// piece.  Balanced: the items in a row (head by head, sequence by sequence), measured in tiles, are cut into as many equal stretches as there are groups; a group walks its stretch, and an
+// item cut in two or more is joined by whoever finishes its last piece.
+struct Cursor {
+  int64_t x, x1, total;
+  int head, b, rb, off;
+  int me, groups, blocks;
+  __device__ __forceinline__ int group_of(int64_t at) const { return static_cast<int>(((at + 1) * groups - 1) / total); }
+};
+
+// Cursor and piece of a warp lie in shared memory (a softmax thread has no registers for them); the whole warp
+// takes the step and one lane writes it down.
+struct Walk {
+  Cursor cursor;
+  Piece piece;
+};
+
+template <int ROWS, bool BAL>
+__device__ __forceinline__ bool next_piece(const AttnArgs& A, Cursor& c, Piece& p) {
+  if constexpr (!BAL) {
+    if (c.x >= c.x1) return false;
+    c.x = c.x1;
+    p.R = row_range<kTT>(A, c.b, c.rb * ROWS, ROWS);
+    int nsplit = (p.R.tiles + A.chunk_tiles - 1) / A.chunk_tiles;
+    nsplit = nsplit < 1 ? 1 : nsplit > A.splits ? A.splits : nsplit;
+    if (p.R.rows == 0 || c.off >= nsplit) return false;
+    p.b = c.b, p.head = c.head;
+    p.t_begin = c.off * A.chunk_tiles;
+    p.n = (c.off == nsplit - 1 ? p.R.tiles : p.t_begin + A.chunk_tiles) - p.t_begin;
+    p.part = nsplit == 1 ? -1 : ((c.b * c.blocks + c.rb) * A.kv.kv_heads + c.head) * A.splits + c.off;
+    p.pieces = 0;
+    return true;
+  }
+  while (c.x < c.x1 && c.head < A.kv.kv_heads) {
+    p.R = row_range<kTT>(A, c.b, c.rb * ROWS, ROWS);
+    const int w = p.R.rows == 0 ? 0 : max(p.R.tiles, 1);
+    const int take = static_cast<int>(min(static_cast<int64_t>(w - c.off), c.x1 - c.x));
+    const bool got = take > 0;
+    if (got) {
+      p.b = c.b, p.head = c.head;
+      p.t_begin = c.off;
+      p.n = min(take, p.R.tiles);
+      p.part = -1;
+      p.pieces = 0;
+      if (take < w) {
+        const int64_t start = c.x - c.off;
+        p.first = c.group_of(start);
+        p.pieces = c.group_of(start + w - 1) - p.first + 1;
+        p.part = 2 * c.me + (c.me == p.first ? 1 : 0);  // the stretch's last item, or its first
+      }
+      c.x += take;
+      c.off += take;
+    }
+    if (c.off >= w) {
+      c.off = 0;
+      if (++c.rb == c.blocks) {
+        c.rb = 0;
+        if (++c.b == A.seqs) c.b = 0, ++c.head;
+      }
+    }
+    if (got) return true;
+  }
+  return false;
+}
+
+template <int ROWS>
+__device__ __forceinline__ bool next_piece(const AttnArgs& A, Walk* walk, int lane) {
+  __syncwarp();
+  Cursor c = walk->cursor;
+  Piece p;
+  const bool got = next_piece<ROWS, true>(A, c, p);
+  __syncwarp();
+  if (lane == 0) {
+    walk->cursor = c;
+    if (got) walk->piece = p;
+  }
+  __syncwarp();
+  return got;
+}
+
+// Item i of the stage order of n tiles: K(0) .. K(SB - 1), then V(j), K(j + SB) in turn.
+template <int SB>
+__device__ __forceinline__ void stage_item(int i, int n, bool& value, int& j) {
+  const int lead = SB < n ? SB : n;
+  if (i < lead) {
+    value = false, j = i;
+    return;
+  }
+  const int k = i - lead;
+  if (k < 2 * (n - SB)) value = (k & 1) == 0, j = value ? k >> 1 : (k >> 1) + SB;
+  else value = true, j = k - (n - SB > 0 ? n - SB : 0);
+}
+
+template <int D, int FMT, int CG, bool BAL>
 __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     attn_tile_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ TileMaps maps) {
   using P = TilePlan<D, FMT, CG>;
@@ -250,21 +353,85 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
   volatile int* stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int b = blockIdx.z;
-  const int blocks = gridDim.y / A.kv.kv_heads;
-  const int head = blockIdx.y / blocks;
-  const int rb = blocks - 1 - static_cast<int>(blockIdx.y % blocks);  // longest contexts first
+  constexpr int kGroupRows = CG * P::kRows;
   const int rank = CG == 1 ? 0 : static_cast<int>(blockIdx.x) & 1;  // (clusters of CG blocks along x)
-  const int r0 = rb * (CG * P::kRows);  // the group's first row; this block's are rank · kRows further on
-  const RowRange R = row_range<kTT>(A, b, r0, CG * P::kRows);
-  if (R.rows == 0) return;  // (the whole group)
-  int nsplit = (R.tiles + A.chunk_tiles - 1) / A.chunk_tiles;
-  nsplit = nsplit < 1 ? 1 : nsplit > A.splits ? A.splits : nsplit;
-  const int split = static_cast<int>(blockIdx.x) / CG;
-  if (split >= nsplit) return;
-  const int t_begin = split * A.chunk_tiles;
-  const int t_end = split == nsplit - 1 ? R.tiles : t_begin + A.chunk_tiles;
-  const int n = t_end - t_begin;
+  Cursor start;
+  start.blocks = A.row_blocks;
+  start.me = static_cast<int>(blockIdx.x) / CG;
+  start.groups = static_cast<int>(gridDim.x) / CG;
+  if constexpr (!BAL) {
+    start.b = blockIdx.z;
+    start.head = blockIdx.y / A.row_blocks;
+    start.rb = A.row_blocks - 1 - static_cast<int>(blockIdx.y % A.row_blocks);  // longest contexts first
+    start.off = start.me;  // (the split)
+    start.x = 0, start.x1 = 1, start.total = 1;
+  } else {
+    // every unit's (sequence, row block) tiles, their running sum, and where this group's stretch begins
+    int* sums = reinterpret_cast<int*>(sm + P::kOffStage);  // [units + 1]
+    for (int u = tid; u < A.units; u += P::kThreads) {
+      const RowRange R = row_range<kTT>(A, u / A.row_blocks, u % A.row_blocks * kGroupRows, kGroupRows);
+      sums[u] = R.rows == 0 ? 0 : max(R.tiles, 1);
+    }
+    __syncthreads();
+    if (warp == 0) {
+      int carry = 0;
+      for (int u0 = 0; u0 < A.units; u0 += 32) {
+        const int v = u0 + lane < A.units ? sums[u0 + lane] : 0;
+        int x = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(kFullMask, x, o);
+          if (lane >= o) x += y;
+        }
+        if (u0 + lane < A.units) sums[u0 + lane] = carry + x - v;
+        carry += __shfl_sync(kFullMask, x, 31);
+      }
+      if (lane == 0) sums[A.units] = carry;
+    }
+    __syncthreads();
+    const int per_head = sums[A.units];
+    start.total = static_cast<int64_t>(per_head) * A.kv.kv_heads;
+    start.x = start.me * start.total / start.groups;
+    start.x1 = (start.me + 1) * start.total / start.groups;
+    int at = 0;
+    start.head = 0;
+    start.off = 0;
+    if (start.x < start.x1) {
+      start.head = static_cast<int>(start.x / per_head);
+      const int rem = static_cast<int>(start.x - static_cast<int64_t>(start.head) * per_head);
+      int lo = 0, hi = A.units;  // the last unit whose sum is at most rem
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (sums[mid] <= rem) lo = mid;
+        else hi = mid;
+      }
+      at = lo;
+      start.off = rem - sums[at];
+    }
+    start.b = at / A.row_blocks;
+    start.rb = at % A.row_blocks;
+    fence_async();  // (the loads that overwrite the sums)
+  }
+  // (balanced: a Walk per warp in shared memory, two warps idle; fixed: the one piece in registers)
+  Walk* walk = reinterpret_cast<Walk*>(sm + P::kOffWalk) + (warp <= P::kLoadWarp ? warp : warp - 2);
+  Piece only;
+  {
+    Cursor c = start;
+    if (!next_piece<kGroupRows, BAL>(A, c, only)) return;  // (the whole group)
+  }
+  if constexpr (BAL) {
+    static_assert(P::kBf && sizeof(Walk) * (P::kThreads / 32 - 2) <= 1536, "a Walk per warp");
+    if (lane == 0 && warp <= P::kLoadWarp) walk->cursor = start;
+    __syncwarp();
+  }
+  const Piece& pc = BAL ? walk->piece : only;
+  bool begun = false;
+  auto more_pieces = [&]() {
+    if constexpr (BAL) return next_piece<kGroupRows>(A, walk, lane);
+    const bool first = !begun;
+    begun = true;
+    return first;
+  };
 
   if (tid == 0) {
     for (int s = 0; s < P::kStages; ++s) {
@@ -304,23 +471,10 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     atomicOr(A.flag, GS_KV_ERR_TIMEOUT);
   };
 
-  // item i of the stage order: K(0) .. K(SB - 1), then V(j), K(j + SB) in turn
-  const int items = 2 * n;
-  auto item = [&](int i, bool& value, int& j) {
-    if (i < (SB < n ? SB : n)) {
-      value = false, j = i;
-      return;
-    }
-    const int k = i - (SB < n ? SB : n);
-    if (k < 2 * (n - SB)) value = (k & 1) == 0, j = value ? k >> 1 : (k >> 1) + SB;
-    else value = true, j = k - (n - SB > 0 ? n - SB : 0);
-  };
-
-  const int32_t* table = A.table + b * A.table_stride;
   const int shift = A.kv.page_shift, page_mask = (1 << shift) - 1;
-  auto page_of = [&](int tok) {  // the page of a context token, checked
+  auto page_of = [&](int b, int tok) {  // the page of a context token, checked
     const int col = tok >> shift;
-    int pg = col < A.table_cols ? __ldg(table + col) : -1;
+    int pg = col < A.table_cols ? __ldg(A.table + b * A.table_stride + col) : -1;
     if (pg < 0 || pg >= A.kv.pages) {
       atomicOr(A.flag, GS_KV_ERR_PAGE);
       pg = 0;
@@ -339,10 +493,13 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     unsigned char* ring = sm + (P::kBf ? P::kOffStage : P::kOffRaw);
     int issued = 0;
     bool ok = true;
-    for (int i = 0; i < items && ok && !*stop; ++i) {
+    while (ok && !*stop && more_pieces()) {
+     const RowRange& R = pc.R;
+     const int head = pc.head;
+     for (int i = 0; i < 2 * pc.n && ok && !*stop; ++i) {
       bool value;
       int j;
-      item(i, value, j);
+      stage_item<SB>(i, pc.n, value, j);
       for (int h = 0; h < P::kPer; ++h) {
         const int at = issued % kRing, round = issued / kRing;
         if (round > 0) ok = __all_sync(kFullMask, mbar_wait(ring_free + at, static_cast<uint32_t>((round - 1) & 1), kWaitNs));
@@ -352,11 +509,11 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         const int box = min(1 << shift, toks);  // tokens per box
         const int groups = toks / box;
         const int cols = (value ? P::kVCols : P::kKCols) * P::kEl / inner;
-        const int j0 = R.tile(t_begin + j) * kTT + (value ? h * P::kVTok : rank * P::kKTok);
+        const int j0 = R.tile(pc.t_begin + j) * kTT + (value ? h * P::kVTok : rank * P::kKTok);
         // lane g: token group g (at most 8); a group past every row's last token stays as it is
         const int tok = j0 + lane * box;
         const bool real = lane < groups && tok < R.hi;
-        const int pg = real ? page_of(tok) : 0;
+        const int pg = real ? page_of(pc.b, tok) : 0;
         const unsigned live = __ballot_sync(kFullMask, real);
         const uint32_t bytes = static_cast<uint32_t>(__popc(live) * box * cols * inner);
         if (lane == 0) {
@@ -374,6 +531,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         __syncwarp();
         ++issued;
       }
+     }
     }
     if (!ok) give_up();
     if (*stop)  // copies in flight land before the block ends
@@ -388,6 +546,10 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
   auto widen = [&]() {
     const int lt = tid - 32 * P::kWidenWarp;
     constexpr int kPieces = P::kRawStage / 16 / 128;  // 16-byte pieces of codes per thread and stage
+    int k0 = 0, g0 = 0;  // stages and tiles of the pieces before
+    while (!*stop && more_pieces()) {
+    const RowRange& R = pc.R;
+    const int head = pc.head, n = pc.n, t_begin = pc.t_begin;
     float vref = 8.673617379884035e-19f;
     // the scales of token lt of the tile after this one, in flight
     float next_k = 0.0f, next_v = 0.0f;
@@ -395,27 +557,27 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       const int tok = R.tile(t_begin + j) * kTT + lt;
       next_k = next_v = 0.0f;  // (a hidden token's weight is 0; its page may hold a NaN)
       if (R.seen_by_any(tok)) {
-        const int pg = page_of(tok), off = tok & page_mask;
+        const int pg = page_of(pc.b, tok), off = tok & page_mask;
         next_k = __ldg(A.kv.scale_at(false, pg, head, off));
         next_v = __ldg(A.kv.scale_at(true, pg, head, off));
       }
     };
     if (n > 0) fetch_scales(0);
-    const int total = items * P::kPer;
+    const int total = 2 * n * P::kPer;
     for (int k = 0; k < total && !*stop; ++k) {
       bool value;
       int j;
-      item(k / P::kPer, value, j);
-      const int h = k % P::kPer;
-      const int rs = k % P::kRawStages, at = k % P::kStages;
-      bool ok = mbar_wait(raw_full + rs, static_cast<uint32_t>((k / P::kRawStages) & 1), kWaitNs);
-      if (k >= P::kStages) ok = ok && mbar_wait(freeb + at, static_cast<uint32_t>((k / P::kStages - 1) & 1), kWaitNs);
+      stage_item<SB>(k / P::kPer, n, value, j);
+      const int h = k % P::kPer, kk = k0 + k;
+      const int rs = kk % P::kRawStages, at = kk % P::kStages;
+      bool ok = mbar_wait(raw_full + rs, static_cast<uint32_t>((kk / P::kRawStages) & 1), kWaitNs);
+      if (kk >= P::kStages) ok = ok && mbar_wait(freeb + at, static_cast<uint32_t>((kk / P::kStages - 1) & 1), kWaitNs);
       if (!__all_sync(kFullMask, ok)) {
         give_up();
         break;
       }
       const int j0 = R.tile(t_begin + j) * kTT;
-      float* sc = reinterpret_cast<float*>(sm + P::kOffScale) + (j % P::kScaleSlots) * (2 * kTT);
+      float* sc = reinterpret_cast<float*>(sm + P::kOffScale) + ((g0 + j) % P::kScaleSlots) * (2 * kTT);
       if (!value && h == 0) {
         // The tile's largest V scale (bits of positive floats in order), by way of this warp's maximum of
         // the 32 tokens it holds: vref only has to be at or above the scales that were seen with it, so each
@@ -425,7 +587,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         const uint32_t mx = __reduce_max_sync(kFullMask, next_v > 0.0f && next_v < INFINITY ? __float_as_uint(next_v) : 0u);
         const float top = __uint_as_float(mx > 0x7e800000u ? 0x7f000000u : (mx + 0x7fffffu) & 0x7f800000u);  // up to a power of two
         vref = fmaxf(vref, top);
-        if (lane == 0) reinterpret_cast<float*>(sm + P::kOffRef)[(j % P::kScaleSlots) * 4 + (warp & 3)] = vref;
+        if (lane == 0) reinterpret_cast<float*>(sm + P::kOffRef)[((g0 + j) % P::kScaleSlots) * 4 + (warp & 3)] = vref;
         if (j + 1 < n) fetch_scales(j + 1);
       }
       const int toks = value ? P::kVTok : P::kKTok;
@@ -459,6 +621,9 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       arrive_on(raw_free + rs);
       arrive_on(full + at);
     }
+    k0 += total;
+    g0 += n;
+    }
     __syncwarp();
   };
 
@@ -466,9 +631,18 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     // ---------------- softmax: one query row per thread ----------------
     set_regs<P::kRegs, P::kSoftRegs>();
     const int s = NQ == 2 ? warp >> 2 : 0;  // query tile
+    const int quad = warp & 3;
+    const int r = s * 128 + quad * 32 + lane;
+    const int gr = rank * P::kRows + r;  // row of the group
+    const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16);
+    const uint32_t o_at = lane_base + 256u + static_cast<uint32_t>(s * D);
+    int g0 = 0;  // tiles of the pieces before
+    while (!*stop && more_pieces()) {
+    const RowRange& R = pc.R;
+    const int head = pc.head, n = pc.n;
     // ---- Q: [query tile][64-column block][128 rows][128 bytes], swizzled; rows past the group zero.  Each
     // warpgroup brings its own tile, sixteen bytes a lane, 8 or 16 loads at a time, while the loaders start.
-    {
+    if (n > 0) {
       constexpr int kCh = D / 8, kRowsAt = 128 / kCh;  // pieces of a row; rows a warpgroup covers at once
       constexpr int kBatch = kCh < 16 ? 8 : 16;
       const uint32_t flip = A.scale_log2 < 0.0f ? 0x80008000u : 0u;  // (a negative scale: -q and |scale|)
@@ -507,9 +681,6 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       __syncwarp();
       if (lane == 0) arrive_first<CG>(q_full);
     }
-    const int quad = warp & 3;
-    const int r = s * 128 + quad * 32 + lane;
-    const int gr = rank * P::kRows + r;  // row of the group
     int hq;
     const int tq = R.token_of(A, min(gr, R.rows - 1), hq);
     hq += head * A.group;
@@ -517,17 +688,16 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     const int lo = A.window ? max(p - A.window + 1, 0) : 0;
     float c = fmaxf(fabsf(A.scale_log2), 1e-30f);  // (0 would turn a hidden score's -inf into NaN)
     float slack = 8.0f / c;
-    const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16);
-    const uint32_t o_at = lane_base + 256u + static_cast<uint32_t>(s * D);
     float m = -INFINITY;
     float2 l2 = make_float2(0.0f, 0.0f);
     float vref = 1.0f;  // (8-bit) weights, sums and O are in units of vref / 2^7
     float unit = 0.0f;  // log2 of 1 over that
     for (int j = 0; j < n && !*stop; ++j) {
-      const int buf = NQ == 2 ? s : (j & 1);
-      const uint32_t ph = static_cast<uint32_t>((j / SB) & 1);
+      const int gt = g0 + j;  // tile number of this block
+      const int buf = NQ == 2 ? s : (gt & 1);
+      const uint32_t ph = static_cast<uint32_t>((gt / SB) & 1);
       const uint32_t s_at = lane_base + static_cast<uint32_t>(buf * 128);
-      const int j0 = R.tile(t_begin + j) * kTT;
+      const int j0 = R.tile(pc.t_begin + j) * kTT;
       if (!__all_sync(kFullMask, mbar_wait(s_full + buf, ph, kWaitNs))) {
         give_up();
         break;
@@ -543,7 +713,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
 #pragma unroll
       for (int q = 0; q < 4; ++q) tm_ld32(s_at + 32 * q, x + 32 * q);
       tm_wait_ld();
-      const float* sc = reinterpret_cast<const float*>(sm + P::kOffScale) + (j % P::kScaleSlots) * (2 * kTT);
+      const float* sc = reinterpret_cast<const float*>(sm + P::kOffScale) + (gt % P::kScaleSlots) * (2 * kTT);
       if constexpr (!P::kBf) {
 #pragma unroll
         for (int i = 0; i < 128; i += 4) {
@@ -569,7 +739,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       const bool move = tm > m + slack || (m == -INFINITY && tm > m);
       float vnew = vref;
       if constexpr (!P::kBf) {
-        const float4 v4 = reinterpret_cast<const float4*>(sm + P::kOffRef)[j % P::kScaleSlots];
+        const float4 v4 = reinterpret_cast<const float4*>(sm + P::kOffRef)[gt % P::kScaleSlots];
         vnew = fmaxf(fmaxf(v4.x, v4.y), fmaxf(v4.z, v4.w));
       }
       if (__any_sync(kFullMask, move || vnew != vref)) {
@@ -585,7 +755,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         }
         if (j > 0) {
           bool ok = true;
-          if constexpr (SB == 2) ok = mbar_wait(o_done, static_cast<uint32_t>((j - 1) & 1), kWaitNs);
+          if constexpr (SB == 2) ok = mbar_wait(o_done, static_cast<uint32_t>((gt - 1) & 1), kWaitNs);
           if (!__all_sync(kFullMask, ok)) {
             give_up();
             break;
@@ -628,26 +798,102 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       tm_st32(s_at + 32, w + 32);
       tm_wait_st();
       fence_before();
+      if (SB == 2 && j > 0 && j == n - 1) {
+        // (the product before the last has to be over before the last one may start: a wait by parity that
+        // finds two phases passed would never end)
+        if (!__all_sync(kFullMask, mbar_wait(o_done, static_cast<uint32_t>((gt - 1) & 1), kWaitNs))) {
+          give_up();
+          break;
+        }
+      }
       __syncwarp();
       if (lane == 0) arrive_first<CG>(p_full + buf);
     }
     // ---- epilogue
-    const float l = l2.x + l2.y;
+    float l = l2.x + l2.y;
+    float ml = m == -INFINITY ? m : m * c - unit;  // (log2 units)
     bool ok = *stop == 0;
     if (n > 0 && ok) {
-      // (two score buffers: the product before the last may still run, and a wait by parity must not
-      // be a phase ahead)
-      if (SB == 2 && n > 1) ok = mbar_wait(o_done, static_cast<uint32_t>((n - 2) & 1), kWaitNs);
-      ok = ok && mbar_wait(o_done + s, static_cast<uint32_t>((n - 1) & 1), kWaitNs);
+      ok = mbar_wait(o_done + s, static_cast<uint32_t>((g0 + n - 1) & 1), kWaitNs);
       if (!ok) give_up();
     }
     ok = __all_sync(kFullMask, ok);
-    if (ok) {
+    bool finish = pc.part < 0;  // whether the result leaves from here
+    if (BAL && ok && pc.pieces > 0) {
+      // A piece of an item that other groups have the rest of: its (m, l, O) to the workspace, warp by warp,
+      // column quads of the 32 rows side by side.  The same 32 rows are the same warp's in every piece, so a
+      // counter per warp tells who is last (nothing waits), and the last one adds the others' to its own.
+      fence_after();
+      const int64_t warp_at = static_cast<int64_t>(rank * P::kRows + s * 128 + quad * 32);
+      auto part_o = [&](int slot) { return reinterpret_cast<float4*>(A.part_o) + (static_cast<int64_t>(slot) * kGroupRows + warp_at) * (D / 4) + lane; };
+      auto part_ml = [&](int slot) { return reinterpret_cast<float2*>(A.part_ml) + static_cast<int64_t>(slot) * kGroupRows + warp_at + lane; };
+#pragma unroll
+      for (int q = 0; q < D / 32; ++q) {
+        float o[32];
+        tm_ld32(o_at + 32 * q, o);
+        tm_wait_ld();
+        float4* dst = part_o(pc.part) + q * 8 * 32;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) __stcg(dst + i * 32, make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
+      }
+      __stcg(part_ml(pc.part), make_float2(ml, l));
+      __threadfence();
+      __syncwarp();
+      unsigned* ticket = A.tickets + pc.first * 8 + static_cast<int>(warp_at / 32);
+      unsigned old = 0;
+      if (lane == 0) old = atomicAdd(ticket, 1u);
+      finish = __shfl_sync(kFullMask, old, 0) == static_cast<unsigned>(pc.pieces - 1);
+      if (finish) {
+        __threadfence();
+        if (lane == 0) *ticket = 0u;  // (for the next call)
+        auto slot = [&](int k) { return k == 0 ? 2 * pc.first + 1 : 2 * (pc.first + k); };
+        float M = -INFINITY, L = 0.0f;
+        for (int k = 0; k < pc.pieces; ++k) M = max_nan(M, __ldcg(part_ml(slot(k))).x);
+        const float ref = M == -INFINITY ? 0.0f : M;
+        for (int k = 0; k < pc.pieces; ++k) {
+          const float2 v = __ldcg(part_ml(slot(k)));
+          L += ex2(v.x - ref) * v.y;
+        }
+        float fo = ex2(ml - ref);
+        for (int k = 0; k < pc.pieces; ++k) {
+          if (slot(k) == pc.part) continue;
+          const float f = ex2(__ldcg(part_ml(slot(k))).x - ref);
+          const float4* src = part_o(slot(k));
+          float4 x[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = __ldcg(src + i * 32);
+#pragma unroll
+          for (int q = 0; q < D / 32; ++q) {
+            float4 y[8];  // (the next columns, in flight)
+            if (q + 1 < D / 32) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) y[i] = __ldcg(src + ((q + 1) * 8 + i) * 32);
+            }
+            float o[32];
+            tm_ld32(o_at + 32 * q, o);
+            tm_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              o[4 * i] = o[4 * i] * fo + f * x[i].x, o[4 * i + 1] = o[4 * i + 1] * fo + f * x[i].y;
+              o[4 * i + 2] = o[4 * i + 2] * fo + f * x[i].z, o[4 * i + 3] = o[4 * i + 3] * fo + f * x[i].w;
+            }
+            tm_st32(o_at + 32 * q, reinterpret_cast<uint32_t*>(o));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = y[i];
+          }
+          tm_wait_st();
+          fo = 1.0f;
+        }
+        ml = M;
+        l = L;
+      }
+    }
+    if (ok && (finish || pc.pieces == 0)) {
       fence_after();
       const bool live = gr < R.rows;
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      const int64_t part = ((static_cast<int64_t>(b) * gridDim.y + rb * A.kv.kv_heads + head) * A.splits + split) * (CG * P::kRows) + gr;
-      if (nsplit == 1) {
+      const int64_t part = static_cast<int64_t>(pc.part) * kGroupRows + gr;
+      if (finish) {
         // by way of shared memory (the query tile's, which no product reads any more): whole rows leave in
         // 16-byte pieces of neighbouring lanes
         constexpr int kCh = D / 8;
@@ -697,21 +943,24 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         }
       }
       if (live) {
-        const float mc = m * c - unit;  // (log2 units)
-        if (nsplit == 1) {
-          if (A.lse) A.lse[static_cast<int64_t>(R.q0 + tq) * A.q_heads + hq] = l == 0.0f ? -INFINITY : (mc + log2f(l)) * 0.6931471805599453f;
+        if (finish) {
+          if (A.lse) A.lse[static_cast<int64_t>(R.q0 + tq) * A.q_heads + hq] = l == 0.0f ? -INFINITY : (ml + log2f(l)) * 0.6931471805599453f;
         } else {
-          *reinterpret_cast<float2*>(A.part_ml + part * 2) = make_float2(m == -INFINITY ? m : mc, l);
+          *reinterpret_cast<float2*>(A.part_ml + part * 2) = make_float2(ml, l);
         }
       }
     }
     fence_before();
+    g0 += n;
+    }
   } else if (warp < P::kMmaWarp + 4) {
    set_regs<P::kRegs, P::kMmaRegs>();
    if (warp == P::kMmaWarp) {
     // ---------------- MMA issuer ----------------
     const bool leader = elected();
     int cnt = 0;  // stages consumed
+    int g0 = 0;   // tiles of the pieces before
+    uint32_t q_phase = 0;
     auto stage_ready = [&](int at) {  // this block's half
       return __all_sync(kFullMask, mbar_wait(full + at % P::kStages, static_cast<uint32_t>((at / P::kStages) & 1), kWaitNs));
     };
@@ -736,7 +985,8 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     // zeros in the rows of a V stage that no query row of the block sees: their weights are 0,
     // and what the pages hold there may be a NaN
     auto clean = [&](int at, int j, int h) {
-      const int j0 = R.tile(t_begin + j) * kTT + h * P::kVTok;
+      const RowRange& R = pc.R;
+      const int j0 = R.tile(pc.t_begin + j) * kTT + h * P::kVTok;
       const bool hidden = j0 + P::kVTok > R.hi || (j0 < R.lo && j0 + P::kVTok > R.sink);
       if (!P::kBf || !hidden) return;
       unsigned char* st = sm + P::kOffStage + (at % P::kStages) * P::kStage;
@@ -749,12 +999,15 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       __syncwarp();
     };
     bool ok = true;
+    const bool issues = CG == 1 || rank == 0;
+    while (ok && !*stop && more_pieces()) {
+    const int n = pc.n;
     if (CG == 2 && rank == 1) {
       // second block: tells the first when a stage of its own is there (and clean)
-      for (int i = 0; ok && i < items && !*stop; ++i) {
+      for (int i = 0; ok && i < 2 * n && !*stop; ++i) {
         bool value;
         int j;
-        item(i, value, j);
+        stage_item<SB>(i, n, value, j);
         for (int h = 0; ok && h < P::kPer; ++h, ++cnt) {
           ok = stage_ready(cnt);
           if (!ok) break;
@@ -764,16 +1017,18 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         }
       }
     }
-    const bool issues = CG == 1 || rank == 0;
-    if (issues && n > 0) ok = ok && __all_sync(kFullMask, wait_group<CG>(q_full, 0));
+    if (issues && n > 0) {
+      ok = ok && __all_sync(kFullMask, wait_group<CG>(q_full, q_phase));
+      q_phase ^= 1;
+    }
     for (int i = 0; issues && ok && i < SB && i < n; ++i) {
       for (int h = 0; ok && h < P::kPer; ++h) ok = stage_ready(cnt + h) && peer_ready(cnt + h);
       if (!ok) break;
       fence_after();
       for (int s = 0; s < NQ; ++s) {
-        scores(s, NQ == 2 ? s : i, cnt);
+        scores(s, NQ == 2 ? s : (g0 + i) & 1, cnt);
         if (leader) {
-          commit_to<CG>(s_full + (NQ == 2 ? s : i));
+          commit_to<CG>(s_full + (NQ == 2 ? s : (g0 + i) & 1));
           if (s == NQ - 1)
             for (int h = 0; h < P::kPer; ++h) commit_to<CG>(freeb + (cnt + h) % P::kStages);
         }
@@ -785,14 +1040,14 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       const int v_at = cnt, k_at = cnt + P::kPer;
       const bool more = j + SB < n;
       for (int s = 0; ok && s < NQ; ++s) {
-        const int buf = NQ == 2 ? s : (j & 1);
+        const int buf = NQ == 2 ? s : ((g0 + j) & 1);
         if (s == 0)
           for (int h = 0; ok && h < P::kPer; ++h) {
             ok = stage_ready(v_at + h);
             if (ok) clean(v_at + h, j, h);
             ok = ok && peer_ready(v_at + h);
           }
-        ok = ok && __all_sync(kFullMask, wait_group<CG>(p_full + buf, static_cast<uint32_t>((j / SB) & 1)));
+        ok = ok && __all_sync(kFullMask, wait_group<CG>(p_full + buf, static_cast<uint32_t>(((g0 + j) / SB) & 1)));
         if (!ok) break;
         fence_after();
         if (leader) {
@@ -825,6 +1080,8 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       }
       cnt += more ? 2 * P::kPer : P::kPer;
     }
+    g0 += n;
+    }
     if (!ok) give_up();
     // every product has completed before tensor memory is freed
     if (leader && issues) commit_to<CG>(m_done);
@@ -846,39 +1103,27 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
   }
 }
 
-template <int D, int FMT, int CG>
-cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
+// Units (sequence, row block) whose tile counts a block sums up at the start of a balanced call, and the
+// blocks whose partial results the workspace holds.
+constexpr int64_t kBalancedUnits = 2048;
+constexpr int64_t kMaxGroups = 240;
+
+template <int D, int FMT, int CG, bool BAL>
+cudaError_t run(const gs_kv_cache* c, const AttnArgs& a, dim3 grid, cudaStream_t st) {
   using P = TilePlan<D, FMT, CG>;
-  constexpr int kRows = CG * P::kRows;  // rows of a group of blocks
-  const int blocks = static_cast<int>((static_cast<int64_t>(a.max_q) * a.group + kRows - 1) / kRows);
-  const int64_t items = static_cast<int64_t>(a.seqs) * a.kv.kv_heads * blocks;
-  const int64_t tiles = most_tiles(a, kTT, kRows);
-  // Splits: only while the blocks do not fill the SMs, each of at least 8 tiles, within the workspace.
-  int64_t splits = c->num_sms / CG / items;
-  const int64_t by_len = tiles / 8;
-  splits = splits > by_len ? by_len : splits;
-  const int64_t slot = static_cast<int64_t>(kRows) * (D + 2) * 4;
-  const int64_t by_ws = static_cast<int64_t>(kAttnWsBytes) / (items * slot);
-  splits = splits > by_ws ? by_ws : splits;
-  if (splits < 1) splits = 1;
-  const int64_t chunk = tiles > 0 ? (tiles + splits - 1) / splits : 1;
-  a.chunk_tiles = static_cast<int32_t>(chunk);
-  a.splits = static_cast<int32_t>(tiles > 0 ? (tiles + chunk - 1) / chunk : 1);
-  a.part_o = reinterpret_cast<float*>(c->ws);
-  a.part_ml = a.part_o + items * a.splits * kRows * D;
+  auto kern = attn_tile_kernel<D, FMT, CG, BAL>;
   static std::atomic<uint64_t> done{0};
   if (device_todo(done)) {
     cudaFuncAttributes at;
-    cudaError_t e = cudaFuncGetAttributes(&at, attn_tile_kernel<D, FMT, CG>);
+    cudaError_t e = cudaFuncGetAttributes(&at, kern);
     // (the warpgroups' shares must not exceed what the block is launched with)
     if (e == cudaSuccess && P::kSoftRegs != P::kRegs && at.numRegs != P::kRegs) e = cudaErrorInvalidKernelImage;
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(attn_tile_kernel<D, FMT, CG>, cudaFuncAttributeMaxDynamicSharedMemorySize, P::kSmem);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, P::kSmem);
     if (e != cudaSuccess) return e;
     mark_device_done(done);
   }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.splits * CG), static_cast<unsigned>(a.kv.kv_heads * blocks), static_cast<unsigned>(a.seqs));
-  if (cfg.gridDim.y > 65535) return cudaErrorInvalidConfiguration;
+  cfg.gridDim = grid;
   cfg.blockDim = dim3(P::kThreads);
   cfg.dynamicSmemBytes = P::kSmem;
   cfg.stream = st;
@@ -888,8 +1133,53 @@ cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = CG > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_tile_kernel<D, FMT, CG>, a,
-                                           *reinterpret_cast<const TileMaps*>(c->maps + (CG == 1 ? 0 : 512)));
+  return cudaLaunchKernelEx(&cfg, kern, a, *reinterpret_cast<const TileMaps*>(c->maps + (CG == 1 ? 0 : 512)));
+}
+
+template <int D, int FMT, int CG>
+cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
+  using P = TilePlan<D, FMT, CG>;
+  constexpr int kRows = CG * P::kRows;  // rows of a group of blocks
+  const int blocks = static_cast<int>((static_cast<int64_t>(a.max_q) * a.group + kRows - 1) / kRows);
+  const int64_t items = static_cast<int64_t>(a.seqs) * a.kv.kv_heads * blocks;
+  const int64_t tiles = most_tiles(a, kTT, kRows);
+  const int64_t groups = c->num_sms / CG;
+  const int64_t units = static_cast<int64_t>(a.seqs) * blocks;
+  a.row_blocks = blocks;
+  a.part_o = reinterpret_cast<float*>(c->ws);
+  if constexpr (P::kBf && P::NQ == 2) {
+    // Balanced: every block takes an equal stretch of all items' tiles.  Against the rounds of a fixed grid
+    // this saves the last round's idle blocks and costs a block about one more beginning and end (about 5
+    // tiles' time) and the joining of what is cut (as much again): 2048 tokens over 16384 in 1.73 rounds, head_dim
+    // 128: 476 -> 446 us, head_dim 64: 419 -> 387 us; 1024-token windows (10 tiles): 70 -> 86 us, so not there.
+    // (Beside 8-bit caches the walk's registers cost more than the rounds: 696 -> 806 us; at head_dim 256 there
+    // are half as many groups and it gains nothing: 474 -> 498 us.)
+    const int64_t rounds = (items + groups - 1) / groups;
+    const bool gains = rounds * groups * (tiles + 5) > items * tiles + (items + 2 * groups) * 5;
+    if (2 * items > groups && gains && units <= kBalancedUnits && groups <= kMaxGroups) {
+      static_assert(2 * kMaxGroups * static_cast<int64_t>(kRows) * (D + 2) * 4 <= static_cast<int64_t>(kAttnWsBytes), "partial results");
+      a.tickets = reinterpret_cast<unsigned*>(c->ws + kAttnWsBytes);
+      a.units = static_cast<int32_t>(units);
+      a.part_ml = a.part_o + 2 * groups * kRows * D;
+      return run<D, FMT, CG, true>(c, a, dim3(static_cast<unsigned>(groups)), st);
+    }
+  }
+  // Fixed: a block (or two) an item.  Where the items do not fill the SMs each is split evenly, in pieces of at
+  // least 8 tiles, and a second launch joins them.
+  int64_t splits = groups / items;
+  const int64_t by_len = tiles / 8;
+  splits = splits > by_len ? by_len : splits;
+  const int64_t slot = static_cast<int64_t>(kRows) * (D + 2) * 4;
+  const int64_t by_ws = static_cast<int64_t>(kAttnWsBytes) / (items * slot);
+  splits = splits > by_ws ? by_ws : splits;
+  if (splits < 1) splits = 1;
+  const int64_t chunk = tiles > 0 ? (tiles + splits - 1) / splits : 1;
+  a.chunk_tiles = static_cast<int32_t>(chunk);
+  a.splits = static_cast<int32_t>(tiles > 0 ? (tiles + chunk - 1) / chunk : 1);
+  a.part_ml = a.part_o + items * a.splits * kRows * D;
+  const dim3 grid(static_cast<unsigned>(a.splits * CG), static_cast<unsigned>(a.kv.kv_heads * blocks), static_cast<unsigned>(a.seqs));
+  if (grid.y > 65535) return cudaErrorInvalidConfiguration;
+  const cudaError_t e = run<D, FMT, CG, false>(c, a, grid, st);
   if (e != cudaSuccess || a.splits == 1) return e;
   return launch_attn_join(a, D, kRows, blocks, kTT, st);
 }

@@ -148,7 +148,7 @@ inline void mark_device_done(std::atomic<uint64_t>& seen) {
 }
 int ctx_device(const gs_ctx* c);                 // the device a context is bound to
 void ctx_set_error(gs_ctx* c, const char* msg);  // the message gs_last_error returns
-cudaError_t ctx_attn_workspace(gs_ctx* c, size_t bytes, unsigned char** out);  // one fixed size for every caller
+cudaError_t ctx_attn_workspace(gs_ctx* c, size_t bytes, size_t zeroed_tail, unsigned char** out);  // one size for every caller
 size_t stream_smem_bytes(int64_t chunk, int kc);
 cudaError_t launch_finalize(const FinalizeArgs& a, int dtype, int rows, size_t smem, cudaStream_t st);
 // Warp-per-row merge (topK <= 128, history stride <= 512, not a shard call).

@@ -328,7 +328,7 @@ gs_status gs_kv_cache_create(gs_ctx* ctx, const gs_kv_cache_desc* d, gs_kv_cache
   DeviceScope scope(c->device);
   cudaError_t er = cudaMalloc(&c->flag, 4);
   if (er == cudaSuccess) er = cudaMemset(c->flag, 0, 4);
-  if (er == cudaSuccess) er = ctx_attn_workspace(ctx, kAttnWsBytes, &c->ws);
+  if (er == cudaSuccess) er = ctx_attn_workspace(ctx, kAttnWsBytes + kAttnTicketBytes, kAttnTicketBytes, &c->ws);
   if (er == cudaSuccess) er = cudaDeviceGetAttribute(&c->num_sms, cudaDevAttrMultiProcessorCount, c->device);
   if (er != cudaSuccess) {
     ctx_set_error(ctx, cudaGetErrorString(er));
@@ -366,6 +366,7 @@ gs_status gs_kv_cache_check(gs_kv_cache* c, int32_t* bits) {
   if (e == cudaSuccess && f) e = cudaMemset(c->flag, 0, 4);
   if (e != cudaSuccess) return kfail(c, GS_ECUDA, cudaGetErrorString(e));
   *bits = f;
+  if (f & GS_KV_ERR_TIMEOUT) cudaMemset(c->ws + kAttnWsBytes, 0, kAttnTicketBytes);  // (a piece may not have counted)
   if (f & GS_KV_ERR_TIMEOUT) return kfail(c, GS_ETIMEOUT, "a bounded wait inside the attention kernel ran out");
   if (f & GS_KV_ERR_SLOT) return kfail(c, GS_EINVAL, "a slot lies past the cache");
   if (f & GS_KV_ERR_PAGE) return kfail(c, GS_EINVAL, "a page-table entry is outside the cache");

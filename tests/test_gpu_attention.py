@@ -230,3 +230,43 @@ def test_refusals(pkg, sampler):
         with pytest.raises(ValueError):
             c.cache.attend(**{**ok, **change})
     c.cache.attend(**ok)
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("lens,heads,window", [([(300, 900), (70, 2000), (513, 513)], 4, 0), ([(1000, 1500)], 8, 200)])
+def test_many_rows_repeated(pkg, sampler, form, dim, lens, heads, window):
+    """Whole grids of the many-row kernel, many times over: the same bits, and no wait that runs out."""
+    c = Case(sampler, pkg, lens, heads, 2, dim, 32, form, seed=dim, window=window, sinks=2 if window else 0)
+    want, want_lse = c.check()
+    outs = []
+    for _ in range(40):
+        outs.append(c.cache.attend(c.q, c.q_start, c.kv_len, c.table, max_q=c.max_q, max_kv=c.max_kv, scale=c.scale,
+                                   window=c.window, sinks=c.sinks, lse=True))
+    torch.cuda.synchronize()
+    c.cache.check()
+    for out, lse in outs:
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lens,heads,group", [([(700, 3000), (1, 1), (0, 5), (40, 0), (300, 1200)], 16, 4),
+                                              ([(64, 2500)] * 9 + [(3, 2)], 16, 8), ([(512, 2049)], 20, 4)])
+def test_balanced_over_items(pkg, sampler, dim, lens, heads, group):
+    """More items than SMs: the blocks' stretches begin and end inside items, which are then joined."""
+    c = Case(sampler, pkg, lens, heads, group, dim, 64, "bf16", seed=dim, poison=float("nan"))
+    out, lse = c.run()
+    again, lse2 = c.run()
+    # the float64 form token by token takes long at these sizes: every 37th token
+    tokens = list(range(0, c.q.shape[0], 37))
+    keep, starts = [], []
+    for b, (nq, n) in enumerate(c.lens):
+        for t in range(c.starts[b], c.starts[b + 1]):
+            if t in tokens:
+                keep.append((t, b, n - nq + (t - c.starts[b])))
+    ref = [R.attend(c.q[t:t + 1], [0, 1], [max(p + 1, 0)], c.table[b:b + 1], c.kd, c.vd, c.page, c.scale, 0, 0) for t, b, p in keep]
+    ref = [torch.cat(x) for x in zip(*ref)]
+    idx = [t for t, _, _ in keep]
+    R.check_attend(out[idx], lse[idx], ref)
+    # which piece of an item comes last is a matter of time: joined results agree to the rounding of one more sum
+    assert ((out.double() - again.double()).abs() <= 2.0 ** -7 * out.double().abs() + 1e-6).all()
