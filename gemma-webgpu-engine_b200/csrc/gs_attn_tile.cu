@@ -418,19 +418,19 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
   {
     Cursor c = start;
     if (!next_piece<kGroupRows, BAL>(A, c, only)) return;  // (the whole group)
-  }
-  if constexpr (BAL) {
-    static_assert(P::kBf && sizeof(Walk) * (P::kThreads / 32 - 2) <= 1536, "a Walk per warp");
-    if (lane == 0 && warp <= P::kLoadWarp) walk->cursor = start;
-    __syncwarp();
+    if constexpr (BAL) {
+      static_assert(P::kBf && sizeof(Walk) * (P::kThreads / 32 - 2) <= 1536, "a Walk per warp");
+      if (lane == 0 && warp <= P::kLoadWarp) {
+        walk->cursor = c;
+        walk->piece = only;
+      }
+      __syncwarp();
+    }
   }
   const Piece& pc = BAL ? walk->piece : only;
-  bool begun = false;
-  auto more_pieces = [&]() {
-    if constexpr (BAL) return next_piece<kGroupRows>(A, walk, lane);
-    const bool first = !begun;
-    begun = true;
-    return first;
+  auto another = [&]() {  // the next piece, once a warp is done with this one
+    if constexpr (BAL) return *stop == 0 && next_piece<kGroupRows>(A, walk, lane);
+    else return false;
   };
 
   if (tid == 0) {
@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     unsigned char* ring = sm + (P::kBf ? P::kOffStage : P::kOffRaw);
     int issued = 0;
     bool ok = true;
-    while (ok && !*stop && more_pieces()) {
+    do {
      const RowRange& R = pc.R;
      const int head = pc.head;
      for (int i = 0; i < 2 * pc.n && ok && !*stop; ++i) {
@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         ++issued;
       }
      }
-    }
+    } while (ok && another());
     if (!ok) give_up();
     if (*stop)  // copies in flight land before the block ends
       for (int k = max(0, issued - kRing); k < issued; ++k)
@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     const int lt = tid - 32 * P::kWidenWarp;
     constexpr int kPieces = P::kRawStage / 16 / 128;  // 16-byte pieces of codes per thread and stage
     int k0 = 0, g0 = 0;  // stages and tiles of the pieces before
-    while (!*stop && more_pieces()) {
+    do {
     const RowRange& R = pc.R;
     const int head = pc.head, n = pc.n, t_begin = pc.t_begin;
     float vref = 8.673617379884035e-19f;
@@ -623,7 +623,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     }
     k0 += total;
     g0 += n;
-    }
+    } while (another());
     __syncwarp();
   };
 
@@ -637,7 +637,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const uint32_t o_at = lane_base + 256u + static_cast<uint32_t>(s * D);
     int g0 = 0;  // tiles of the pieces before
-    while (!*stop && more_pieces()) {
+    do {
     const RowRange& R = pc.R;
     const int head = pc.head, n = pc.n;
     // ---- Q: [query tile][64-column block][128 rows][128 bytes], swizzled; rows past the group zero.  Each
@@ -952,7 +952,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     }
     fence_before();
     g0 += n;
-    }
+    } while (another());
   } else if (warp < P::kMmaWarp + 4) {
    set_regs<P::kRegs, P::kMmaRegs>();
    if (warp == P::kMmaWarp) {
@@ -1000,7 +1000,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     };
     bool ok = true;
     const bool issues = CG == 1 || rank == 0;
-    while (ok && !*stop && more_pieces()) {
+    do {
     const int n = pc.n;
     if (CG == 2 && rank == 1) {
       // second block: tells the first when a stage of its own is there (and clean)
@@ -1081,7 +1081,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       cnt += more ? 2 * P::kPer : P::kPer;
     }
     g0 += n;
-    }
+    } while (ok && another());
     if (!ok) give_up();
     // every product has completed before tensor memory is freed
     if (leader && issues) commit_to<CG>(m_done);
