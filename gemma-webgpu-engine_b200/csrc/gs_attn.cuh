@@ -21,8 +21,8 @@ struct gs_kv_cache {
 
 namespace gs {
 
-// Workspace of split-context partial results: [partial][rows][head_dim] float32 outputs and
-// [partial][rows][2] maxima and sums.  The planner never asks for more.
+// Workspace of split-context partial results, float32 outputs and their maxima and sums.  The planners never
+// ask for more.
 constexpr size_t kAttnWsBytes = 64u << 20;
 constexpr size_t kAttnTicketBytes = 16u << 10;  // behind it, zero between calls
 
@@ -66,14 +66,14 @@ struct AttnArgs {
   int32_t max_q, max_kv;
   int32_t window, sinks;
   float scale_log2;     // scale · log2(e): scores in log2 units
-  int32_t chunk_tiles;  // context tiles per split (0: every context in `splits` even parts)
+  int32_t chunk_tiles;  // (many-row kernel) context tiles per split
   int32_t splits;       // partial results per (sequence, head, row block)
   int32_t cluster;      // blocks per partial result (few-row kernel)
   int32_t row_blocks;   // (many-row kernel) blocks of query rows per sequence and head
   int32_t units;        // (many-row kernel, balanced) sequences times row blocks
-  unsigned* tickets;    // [groups][8] finished pieces of the item that begins in a group, per warp; zero between calls
-  float* part_o;        // [seq][row block][kv head][split][rows][head_dim]
-  float* part_ml;       // [..][rows][2]: running maximum (log2 units) and sum
+  unsigned* tickets;    // finished parts of a context, per warp that holds the same rows of each; zero between calls
+  float* part_o;        // partial results: outputs
+  float* part_ml;       // and running maxima (log2 units) and sums
   int32_t* flag;
 };
 
@@ -169,8 +169,4 @@ cudaError_t launch_attn_rows(const gs_kv_cache* c, AttnArgs a, cudaStream_t st);
 // Many-row kernel (tcgen05), and the tensor maps both read a cache by (an error text, or nullptr).
 cudaError_t launch_attn_tile(const gs_kv_cache* c, AttnArgs a, cudaStream_t st);
 const char* make_attn_maps(gs_kv_cache* c);
-// Joins the partial results of a split context.  rows_per_block and tile as in the kernel
-// that wrote them.
-cudaError_t launch_attn_join(const AttnArgs& a, int head_dim, int rows_per_block, int row_blocks, int tile, cudaStream_t st);
-
 }  // namespace gs

@@ -1,5 +1,4 @@
-// Attention of few query rows over the paged cache (one decoded token, a few drafted ones),
-// and the join of split contexts.
+// Attention of few query rows over the paged cache (one decoded token, a few drafted ones).
 //
 // Per row, over the visible tokens j in tiles of 16, with the running maximum m and sum l
 // (log2 units, s_j = scale · log2(e) · q·k_j):
@@ -21,8 +20,8 @@
 // Values of tokens hidden from every row of the block are set to zero before they are used.
 //
 // A context is shared evenly by the blocks of a cluster (up to 8), which join their (m, l, O) through
-// distributed shared memory; several clusters per context write partial results, joined by a second
-// launch.
+// distributed shared memory; of several clusters per context the last to finish joins their partial
+// results.
 //
 // 8-bit codes are widened to float16 (exact for e4m3 and int8) in registers, K's scale
 // multiplies the finished score, V's scale the weight: 2^(s - m) · (scale / largest scale so
@@ -51,7 +50,7 @@ struct RowsPlan {
   static constexpr int kInner = kRow < 128 ? kRow : 128;     // bytes of a row in one TMA box
   static constexpr int kCols = kRow / kInner;                // boxes across a row
   static constexpr int kTileBytes = kRT * kRow;              // K or V of one tile
-  static constexpr int kSub = kTileBytes <= 2048 ? 2 : 1;    // tiles per stage
+  static constexpr int kSub = kTileBytes <= 1024 ? 2 : 1;    // tiles per stage
   static constexpr int kStage = kSub * 2 * kTileBytes;
   static constexpr int kStages = 3;
   static constexpr int kRing = kRowsWarps * kStages * kStage;
@@ -540,20 +539,15 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
   __syncthreads();
   float* oj = reinterpret_cast<float*>(smem);
   const bool alone = A.cluster == 1;
-  const int64_t part = (static_cast<int64_t>(b) * gridDim.y + blockIdx.y) * A.splits + blockIdx.x / A.cluster;
-  // the (m, l, O) of one row piece to where it goes: the result, or this cluster's partial one
+  // the (m, l, O) of a row's four values as the result
   auto put = [&](int r, int d, float M, float L, float4 acc) {
-    if (A.splits == 1) {
-      int gq;
-      const int t = R.token_of(A, r, gq);
-      const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-      const uint2 w = make_uint2(bf16x2(acc.x * inv, acc.y * inv), bf16x2(acc.z * inv, acc.w * inv));
-      *reinterpret_cast<uint2*>(o_row(A, R, head, t, gq) + d) = w;
-      if (A.lse && d == 0) A.lse[static_cast<int64_t>(R.q0 + t) * A.q_heads + head * A.group + gq] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
-    } else {
-      *reinterpret_cast<float4*>(A.part_o + (part * kRows + r) * D + d) = acc;
-      if (d == 0) *reinterpret_cast<float2*>(A.part_ml + (part * kRows + r) * 2) = make_float2(M, L);
-    }
+    int gq;
+    const int t = R.token_of(A, r, gq);
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    const uint2 w = make_uint2(bf16x2(acc.x * inv, acc.y * inv), bf16x2(acc.z * inv, acc.w * inv));
+    *reinterpret_cast<uint2*>(o_row(A, R, head, t, gq) + d) = w;
+    if (A.lse && d == 0)
+      A.lse[static_cast<int64_t>(R.q0 + t) * A.q_heads + head * A.group + gq] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
   };
   for (int e = tid; e < R.rows * (D / 4); e += kRowsThreads) {
     const int r = e / (D / 4), d = (e % (D / 4)) * 4;
@@ -580,12 +574,13 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
     }
   }
   if (alone) return;
-  // ---- join the cluster: its blocks take the row pieces in turn
+  // ---- join the cluster: four values of a row per thread of its blocks (8 blocks have one for each)
   cluster_sync();
   const uint32_t rank = cluster_rank();
   const uint32_t o_at = smem_addr(oj), ml_at = smem_addr(&s_ml[0][0]);
-  for (int e = static_cast<int>(rank) * kRowsThreads + tid; e < R.rows * (D / 4); e += A.cluster * kRowsThreads) {
-    const int r = e / (D / 4), d = (e % (D / 4)) * 4;
+  for (int e = static_cast<int>(rank) * kRowsThreads + tid; e - lane < R.rows * (D / 4); e += A.cluster * kRowsThreads) {
+    const bool has = e < R.rows * (D / 4);
+    const int r = has ? e / (D / 4) : 0, d = (e % (D / 4)) * 4;
     float2 ml[8];
     float4 x[8];
 #pragma unroll
@@ -608,68 +603,59 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
         L += f * ml[k].y;
         acc.x += f * x[k].x, acc.y += f * x[k].y, acc.z += f * x[k].z, acc.w += f * x[k].w;
       }
+    if (A.splits == 1) {
+      if (has) put(r, d, M, L, acc);
+      continue;
+    }
+    // ---- several clusters (of 8: one turn of this loop): partial results to the workspace, each thread's
+    // four values with their row's maximum and sum.  The same values are the same thread's in every cluster,
+    // so a counter per warp tells which cluster's is last (nothing waits), and that one joins them.
+    const int item = b * gridDim.y + blockIdx.y;
+    auto part = [&](int k) { return (static_cast<int64_t>(item * A.splits + k) * kRows + r) * (D / 4) + d / 4; };
+    if (has) {
+      const int64_t at = part(blockIdx.x / A.cluster);
+      __stcg(reinterpret_cast<float4*>(A.part_o) + at, acc);
+      __stcg(reinterpret_cast<float2*>(A.part_ml) + at, make_float2(M, L));
+    }
+    __threadfence();
+    __syncwarp();
+    unsigned* ticket = A.tickets + item * 32 + static_cast<int>(rank) * kRowsWarps + warp;
+    unsigned old = 0;
+    if (lane == 0) old = atomicAdd(ticket, 1u);
+    if (__shfl_sync(kFullMask, old, 0) != static_cast<unsigned>(A.splits - 1)) continue;
+    __threadfence();
+    if (lane == 0) *ticket = 0u;  // (for the next call)
+    if (!has) continue;
+    // (eight parts' loads together)
+    M = -INFINITY;
+    L = 0.0f;
+    acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int k0 = 0; k0 < A.splits; k0 += 8) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k0 + k < A.splits) {
+          ml[k] = __ldcg(reinterpret_cast<const float2*>(A.part_ml) + part(k0 + k));
+          x[k] = __ldcg(reinterpret_cast<const float4*>(A.part_o) + part(k0 + k));
+        }
+      float mx = M;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k0 + k < A.splits) mx = max_nan(mx, ml[k].x);
+      const float at = mx == -INFINITY ? 0.0f : mx, back = ex2(M - at);
+      L *= back;
+      acc.x *= back, acc.y *= back, acc.z *= back, acc.w *= back;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (k0 + k < A.splits) {
+          const float f = ex2(ml[k].x - at);
+          L += f * ml[k].y;
+          acc.x += f * x[k].x, acc.y += f * x[k].y, acc.z += f * x[k].z, acc.w += f * x[k].w;
+        }
+      M = mx;
+    }
     put(r, d, M, L, acc);
   }
   cluster_sync();  // (no block leaves while its shared memory is read)
-}
-
-// One block per query row: its splits' (m, l, O) joined as the warps' are above.  kTile, rows per block
-// and chunk_tiles as in the kernel that wrote them, so that the number of splits agrees.
-template <int D, int kTile>
-__global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ AttnArgs A, int rows_per_block) {
-  constexpr int kVec = D / 4, kParts = 128 / kVec;  // threads across head_dim, splits in parallel
-  __shared__ float4 s_acc[128];
-  __shared__ float s_red[4], s_lse[4];
-  const int b = blockIdx.z, head = blockIdx.y % A.kv.kv_heads, rb = blockIdx.y / A.kv.kv_heads;
-  const int r = blockIdx.x, r0 = rb * rows_per_block, tid = threadIdx.x;
-  const RowRange R = row_range<kTile>(A, b, r0, rows_per_block);
-  if (r >= R.rows) return;
-  int nsplit = A.splits;  // (the few-row kernel writes every partial result)
-  if (A.chunk_tiles > 0) {
-    nsplit = (R.tiles + A.chunk_tiles - 1) / A.chunk_tiles;
-    nsplit = nsplit < 1 ? 1 : nsplit > A.splits ? A.splits : nsplit;
-  }
-  if (nsplit == 1) return;
-  const int64_t part0 = (static_cast<int64_t>(b) * gridDim.y + blockIdx.y) * A.splits;
-  const float* ml = A.part_ml + (part0 * rows_per_block + r) * 2;
-  const int64_t step = static_cast<int64_t>(rows_per_block);
-  float M = -INFINITY;
-  for (int s = tid; s < nsplit; s += 128) M = max_nan(M, ml[s * step * 2]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) M = max_nan(M, __shfl_xor_sync(kFullMask, M, o));
-  if ((tid & 31) == 0) s_red[tid >> 5] = M;
-  __syncthreads();
-  M = max_nan(max_nan(s_red[0], s_red[1]), max_nan(s_red[2], s_red[3]));
-  const float ref = M == -INFINITY ? 0.0f : M;
-  float L = 0.0f;
-  for (int s = tid; s < nsplit; s += 128) {
-    const float2 v = *reinterpret_cast<const float2*>(ml + s * step * 2);
-    L += ex2(v.x - ref) * v.y;
-  }
-  L = warp_sum_f(L);
-  if ((tid & 31) == 0) s_lse[tid >> 5] = L;
-  const int pv = tid / kVec, d = (tid % kVec) * 4;
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int s = pv; s < nsplit; s += kParts) {
-    const float f = ex2(ml[s * step * 2] - ref);
-    const float4 x = *reinterpret_cast<const float4*>(A.part_o + ((part0 + s) * rows_per_block + r) * D + d);
-    acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
-  }
-  s_acc[tid] = acc;
-  __syncthreads();
-  if (tid >= kVec) return;
-#pragma unroll
-  for (int p = 1; p < kParts; ++p) {
-    const float4 x = s_acc[p * kVec + tid];
-    acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
-  }
-  L = s_lse[0] + s_lse[1] + s_lse[2] + s_lse[3];
-  int gq;
-  const int t = R.token_of(A, r, gq);
-  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-  *reinterpret_cast<uint2*>(o_row(A, R, head, t, gq) + d) =
-      make_uint2(bf16x2(acc.x * inv, acc.y * inv), bf16x2(acc.z * inv, acc.w * inv));
-  if (A.lse && d == 0) A.lse[static_cast<int64_t>(R.q0 + t) * A.q_heads + head * A.group + gq] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
 
 template <int D, int FMT, int NB>
@@ -679,25 +665,27 @@ cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
   constexpr int smem = RowsSmem<D, FMT, NB>::kTotal;
   const int blocks = static_cast<int>((static_cast<int64_t>(a.max_q) * a.group + kRows - 1) / kRows);
   const int64_t items = static_cast<int64_t>(a.seqs) * a.kv.kv_heads * blocks;
-  // Blocks per context: enough for two rounds of the SMs (contexts are ragged), each of at least two
-  // stages a warp.  Up to 8 are one cluster; more are clusters of 8 whose partial results are joined.
+  // Blocks per context: one round of what the SMs hold, each block with at least two stages a warp.  (Two
+  // sequences of 131072 tokens, 4 heads of 128: bf16 86 us in one round, 102 in two; e4m3 59 and 87.)
+  // Up to 8 blocks are one cluster; more are clusters of 8 whose partial results are joined.
   const int64_t tiles = most_tiles(a, kRT, kRows);
   const int64_t slots = static_cast<int64_t>(c->num_sms) * rows_occupancy<D, FMT, NB>();
-  int64_t want = 2 * slots / items;
+  int64_t want = slots / items;
   const int64_t by_len = (tiles + 2 * kRowsWarps * P::kSub - 1) / (2 * kRowsWarps * P::kSub);
   want = want > by_len ? by_len : want;
   int cluster = 1;
   while (cluster < 8 && cluster * 2 <= want) cluster *= 2;
   int64_t splits = want / cluster;
-  const int64_t slot = static_cast<int64_t>(kRows) * (D + 2) * 4;
-  const int64_t by_ws = static_cast<int64_t>(kAttnWsBytes) / (items * slot);
+  const int64_t by_ws = static_cast<int64_t>(kAttnWsBytes) / (items * kRows * (D / 4) * 24);
   splits = splits > by_ws ? by_ws : splits;
-  if (splits < 1 || cluster < 8) splits = 1;
+  // (8 blocks of 128 threads have a thread for each four values of a block's rows)
+  static_assert(kRows * (D / 4) <= 8 * kRowsThreads, "one turn of the join");
+  if (splits < 1 || cluster < 8 || items * 32 * 4 > static_cast<int64_t>(kAttnTicketBytes)) splits = 1;
   a.cluster = cluster;
-  a.chunk_tiles = 0;
   a.splits = static_cast<int32_t>(splits);
   a.part_o = reinterpret_cast<float*>(c->ws);
   a.part_ml = a.part_o + items * splits * kRows * D;
+  a.tickets = reinterpret_cast<unsigned*>(c->ws + kAttnWsBytes);
   static std::atomic<uint64_t> done{0};
   if (device_todo(done)) {
     const cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<D, FMT, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -716,9 +704,7 @@ cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, attn_rows_kernel<D, FMT, NB>, a, *reinterpret_cast<const RowsMaps*>(c->maps + 256));
-  if (e != cudaSuccess || splits == 1) return e;
-  return launch_attn_join(a, D, kRows, blocks, kRT, st);
+  return cudaLaunchKernelEx(&cfg, attn_rows_kernel<D, FMT, NB>, a, *reinterpret_cast<const RowsMaps*>(c->maps + 256));
 }
 
 template <int D, int FMT>
@@ -742,19 +728,6 @@ cudaError_t go_fmt(const gs_kv_cache* c, const AttnArgs& a, cudaStream_t st) {
 
 cudaError_t launch_attn_rows(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
   return c->d.head_dim == 64 ? go_fmt<64>(c, a, st) : c->d.head_dim == 128 ? go_fmt<128>(c, a, st) : go_fmt<256>(c, a, st);
-}
-
-cudaError_t launch_attn_join(const AttnArgs& a, int head_dim, int rows_per_block, int row_blocks, int tile, cudaStream_t st) {
-  const dim3 grid(static_cast<unsigned>(rows_per_block), static_cast<unsigned>(a.kv.kv_heads * row_blocks),
-                  static_cast<unsigned>(a.seqs));
-  auto run = [&](auto kern) {
-    kern<<<grid, 128, 0, st>>>(a, rows_per_block);
-    return cudaGetLastError();
-  };
-  if (tile == 16) {
-    return head_dim == 64 ? run(attn_join_kernel<64, 16>) : head_dim == 128 ? run(attn_join_kernel<128, 16>) : run(attn_join_kernel<256, 16>);
-  }
-  return head_dim == 64 ? run(attn_join_kernel<64, 128>) : head_dim == 128 ? run(attn_join_kernel<128, 128>) : run(attn_join_kernel<256, 128>);
 }
 
 }  // namespace gs

@@ -1103,6 +1103,61 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
   }
 }
 
+// One block per query row of a split context: the splits' (m, l, O) joined.
+template <int D>
+__global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ AttnArgs A, int rows_per_block) {
+  constexpr int kVec = D / 4, kParts = 128 / kVec;  // threads across head_dim, splits in parallel
+  __shared__ float4 s_acc[128];
+  __shared__ float s_red[4], s_lse[4];
+  const int b = blockIdx.z, head = blockIdx.y % A.kv.kv_heads, rb = blockIdx.y / A.kv.kv_heads;
+  const int r = blockIdx.x, r0 = rb * rows_per_block, tid = threadIdx.x;
+  const RowRange R = row_range<kTT>(A, b, r0, rows_per_block);
+  if (r >= R.rows) return;
+  int nsplit = (R.tiles + A.chunk_tiles - 1) / A.chunk_tiles;
+  nsplit = nsplit < 1 ? 1 : nsplit > A.splits ? A.splits : nsplit;
+  if (nsplit == 1) return;
+  const int64_t part0 = (static_cast<int64_t>(b) * gridDim.y + blockIdx.y) * A.splits;
+  const float* ml = A.part_ml + (part0 * rows_per_block + r) * 2;
+  const int64_t step = static_cast<int64_t>(rows_per_block);
+  float M = -INFINITY;
+  for (int s = tid; s < nsplit; s += 128) M = max_nan(M, ml[s * step * 2]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = max_nan(M, __shfl_xor_sync(kFullMask, M, o));
+  if ((tid & 31) == 0) s_red[tid >> 5] = M;
+  __syncthreads();
+  M = max_nan(max_nan(s_red[0], s_red[1]), max_nan(s_red[2], s_red[3]));
+  const float ref = M == -INFINITY ? 0.0f : M;
+  float L = 0.0f;
+  for (int s = tid; s < nsplit; s += 128) {
+    const float2 v = *reinterpret_cast<const float2*>(ml + s * step * 2);
+    L += ex2(v.x - ref) * v.y;
+  }
+  L = warp_sum_f(L);
+  if ((tid & 31) == 0) s_lse[tid >> 5] = L;
+  const int pv = tid / kVec, d = (tid % kVec) * 4;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int s = pv; s < nsplit; s += kParts) {
+    const float f = ex2(ml[s * step * 2] - ref);
+    const float4 x = *reinterpret_cast<const float4*>(A.part_o + ((part0 + s) * rows_per_block + r) * D + d);
+    acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
+  }
+  s_acc[tid] = acc;
+  __syncthreads();
+  if (tid >= kVec) return;
+#pragma unroll
+  for (int p = 1; p < kParts; ++p) {
+    const float4 x = s_acc[p * kVec + tid];
+    acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+  }
+  L = s_lse[0] + s_lse[1] + s_lse[2] + s_lse[3];
+  int gq;
+  const int t = R.token_of(A, r, gq);
+  const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  *reinterpret_cast<uint2*>(o_row(A, R, head, t, gq) + d) =
+      make_uint2(bf16x2(acc.x * inv, acc.y * inv), bf16x2(acc.z * inv, acc.w * inv));
+  if (A.lse && d == 0) A.lse[static_cast<int64_t>(R.q0 + t) * A.q_heads + head * A.group + gq] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+}
+
 // Units (sequence, row block) whose tile counts a block sums up at the start of a balanced call, and the
 // blocks whose partial results the workspace holds.
 constexpr int64_t kBalancedUnits = 2048;
@@ -1181,7 +1236,8 @@ cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
   if (grid.y > 65535) return cudaErrorInvalidConfiguration;
   const cudaError_t e = run<D, FMT, CG, false>(c, a, grid, st);
   if (e != cudaSuccess || a.splits == 1) return e;
-  return launch_attn_join(a, D, kRows, blocks, kTT, st);
+  attn_join_kernel<D><<<dim3(kRows, static_cast<unsigned>(a.kv.kv_heads * blocks), static_cast<unsigned>(a.seqs)), 128, 0, st>>>(a, kRows);
+  return cudaGetLastError();
 }
 
 template <int D, int FMT>
