@@ -665,13 +665,33 @@ cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
   constexpr int smem = RowsSmem<D, FMT, NB>::kTotal;
   const int blocks = static_cast<int>((static_cast<int64_t>(a.max_q) * a.group + kRows - 1) / kRows);
   const int64_t items = static_cast<int64_t>(a.seqs) * a.kv.kv_heads * blocks;
-  // Blocks per context: one round of what the SMs hold, each block with at least two stages a warp.  (Two
-  // sequences of 131072 tokens, 4 heads of 128: bf16 86 us in one round, 102 in two; e4m3 59 and 87.)
-  // Up to 8 blocks are one cluster; more are clusters of 8 whose partial results are joined.
+  static std::atomic<uint64_t> done{0};
+  static std::atomic<int> held{0};  // clusters of 8 that the device holds at once (a GPU process runs on one kind of device)
+  if (device_todo(done)) {
+    cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<D, FMT, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t q{};
+    cudaLaunchAttribute at{};
+    q.gridDim = dim3(8 * 1024);
+    q.blockDim = dim3(kRowsThreads);
+    q.dynamicSmemBytes = smem;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = 8, at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    q.attrs = &at;
+    q.numAttrs = 1;
+    int n = 0;
+    e = cudaOccupancyMaxActiveClusters(&n, attn_rows_kernel<D, FMT, NB>, &q);
+    if (e != cudaSuccess) return e;
+    held.store(n > 0 ? n : 1);
+    mark_device_done(done);
+  }
+  // Blocks per context: one round of what the device holds (in clusters of 8, which have to find their SMs
+  // in one GPC: fewer than the SMs alone would), each block with at least a stage a warp.  (Two sequences of 131072 tokens, 4 heads
+  // of 128: bf16 86 us in one round, 102 in two.)  Up to 8 blocks are one cluster; more are
+  // clusters of 8 whose partial results are joined.
   const int64_t tiles = most_tiles(a, kRT, kRows);
-  const int64_t slots = static_cast<int64_t>(c->num_sms) * rows_occupancy<D, FMT, NB>();
-  int64_t want = slots / items;
-  const int64_t by_len = (tiles + 2 * kRowsWarps * P::kSub - 1) / (2 * kRowsWarps * P::kSub);
+  int64_t want = 8ll * held.load() / items;
+  const int64_t by_len = (tiles + kRowsWarps * P::kSub - 1) / (kRowsWarps * P::kSub);
   want = want > by_len ? by_len : want;
   int cluster = 1;
   while (cluster < 8 && cluster * 2 <= want) cluster *= 2;
@@ -686,12 +706,6 @@ cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
   a.part_o = reinterpret_cast<float*>(c->ws);
   a.part_ml = a.part_o + items * splits * kRows * D;
   a.tickets = reinterpret_cast<unsigned*>(c->ws + kAttnWsBytes);
-  static std::atomic<uint64_t> done{0};
-  if (device_todo(done)) {
-    const cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<D, FMT, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    mark_device_done(done);
-  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(splits * cluster), static_cast<unsigned>(a.kv.kv_heads * blocks), static_cast<unsigned>(a.seqs));
   if (cfg.gridDim.y > 65535) return cudaErrorInvalidConfiguration;
