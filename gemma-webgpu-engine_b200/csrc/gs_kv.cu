@@ -2,8 +2,8 @@
 //
 // write  a = max(max|x|, 2^-64) over head_dim, code = round(x · (M / a)), scale = a / M
 // read   value = code · scale, rounded once
-// A row (one token and head) is head_dim / 8 neighbouring lanes of 8 elements each, so its
-// maximum is a shuffle reduction and every access is 16 bytes (8 for codes); one launch
+// A row (one token and head) is a few neighbouring lanes of 8 or 16 elements each, so its
+// maximum is a shuffle reduction and every access is 16 bytes; one launch
 // covers keys and values.  Both directions move 3 bytes an element (bf16 beside codes) and
 // are bound by HBM for long chunks, by launch latency for one step.
 #include <cmath>
@@ -59,18 +59,24 @@ __device__ __forceinline__ void store8(void* p, const float (&x)[8]) {
   }
 }
 
-// U tokens per group of lanes, `step` apart, their loads issued together: one row (16 bytes a thread)
-// keeps too few bytes in flight for a long chunk, and a step's few rows are better spread.
+// Elements of a row per lane: eight beside a bf16 pool, else twice eight, half a row apart, so that neighbouring
+// lanes' 16-byte pieces (8 of codes) are neighbours.
+template <int FMT, bool VEC>
+constexpr int row_piece() {
+  return FMT == GS_DTYPE_BF16 || !VEC ? 8 : 16;
+}
+
+// A group of lanes takes the key and the value of U tokens (`step` apart) of one head, all loads together: one
+// row keeps too few bytes in flight for a long chunk, and a step's few rows are better spread.  (The kernels
+// are bound by issue slots about as much as by HBM: what a row costs beside its data is shared where it can be.)
 template <int D, int FMT, bool BF16, bool VEC, int U>
 __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ KvRowsArgs A, uint32_t step) {
-  constexpr int kLanes = D / 8;
+  constexpr int E = row_piece<FMT, VEC>(), kLanes = D / E, kWords = E / (BF16 ? 8 : 4);
   const uint32_t row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
   const uint32_t token0 = row / static_cast<uint32_t>(A.kv.kv_heads);
   const int head = static_cast<int>(row - token0 * A.kv.kv_heads);
   const int at = (threadIdx.x % kLanes) * 8;
-  const bool value = blockIdx.y != 0;
-  constexpr int kWords = BF16 ? 1 : 2;
-  uint4 raw[U][kWords];
+  uint4 raw[U][2][kWords];
   SlotAt s[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -79,117 +85,138 @@ __global__ void __launch_bounds__(256) kv_write_kernel(const __grid_constant__ K
     if (token0 < step && token < A.tokens) s[u] = slot_at(A, token);
   }
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
+  for (int u = 0; u < U; ++u)
 #pragma unroll
-    for (int i = 0; i < kWords; ++i) raw[u][i] = make_uint4(0u, 0u, 0u, 0u);
-    if (!s[u].ok) continue;
-    const unsigned char* src = (value ? A.v : A.k) + (row_at(A, value, token0 + u * step, head) + at) * (BF16 ? 2 : 4);
-    if constexpr (VEC) {
+    for (int v = 0; v < 2; ++v) {
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) raw[u][i] = reinterpret_cast<const uint4*>(src)[i];
-    } else if constexpr (BF16) {
-      const unsigned short* h = reinterpret_cast<const unsigned short*>(src);
-      raw[u][0] = make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
-    } else {
-      const uint32_t* h = reinterpret_cast<const uint32_t*>(src);
-      raw[u][0] = make_uint4(h[0], h[1], h[2], h[3]);
-      raw[u][kWords - 1] = make_uint4(h[4], h[5], h[6], h[7]);
-    }
-  }
+      for (int i = 0; i < kWords; ++i) raw[u][v][i] = make_uint4(0u, 0u, 0u, 0u);
+      if (!s[u].ok) continue;
+      const unsigned char* src = (v ? A.v : A.k) + (row_at(A, v, token0 + u * step, head) + at) * (BF16 ? 2 : 4);
+      if constexpr (VEC) {
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    float v[8];
-    load_row<8, BF16>(raw[u], v);
-    unsigned char* pool = const_cast<unsigned char*>(A.kv.at(value, s[u].page, head, s[u].off));
-    if constexpr (FMT == GS_DTYPE_BF16) {
-      if (s[u].ok) store_row<8, true>(pool + at * 2, v);
-    } else {
-      constexpr float kMax = FMT == GS_DTYPE_E4M3 ? kE4m3Max : kInt8Max;
-      float m = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(v[i]));
-#pragma unroll
-      for (int o = kLanes >> 1; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(kFullMask, m, o));
-      const float inv = quant_inv(m, kMax);
-      if (s[u].ok) {
-        uint2 c;
-        if constexpr (FMT == GS_DTYPE_E4M3) {
-          c.x = e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-          c.y = e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
-        } else {
-          c.x = int8x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-          c.y = int8x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+        for (int i = 0; i < kWords; ++i) {
+          constexpr int kPer = BF16 ? 1 : 2;  // words of eight elements
+          raw[u][v][i] = ld_stream_u4(reinterpret_cast<const uint4*>(src + (i / kPer) * (D / 2) * (BF16 ? 2 : 4)) + i % kPer);
         }
-        *reinterpret_cast<uint2*>(pool + at) = c;
-        if (at == 0) *const_cast<float*>(A.kv.scale_at(value, s[u].page, head, s[u].off)) = quant_scale(m, kMax);
+      } else if constexpr (BF16) {
+        const unsigned short* h = reinterpret_cast<const unsigned short*>(src);
+        raw[u][v][0] = make_uint4(h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16));
+      } else {
+        const uint32_t* h = reinterpret_cast<const uint32_t*>(src);
+        raw[u][v][0] = make_uint4(h[0], h[1], h[2], h[3]);
+        raw[u][v][kWords - 1] = make_uint4(h[4], h[5], h[6], h[7]);
       }
     }
-  }
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      float x[E];
+#pragma unroll
+      for (int i = 0; i < E / 8; ++i) load_row<8, BF16>(&raw[u][v][i * (BF16 ? 1 : 2)], *reinterpret_cast<float(*)[8]>(x + 8 * i));
+      unsigned char* pool = const_cast<unsigned char*>(A.kv.at(v, s[u].page, head, s[u].off));
+      if constexpr (FMT == GS_DTYPE_BF16) {
+        if (s[u].ok) store_row<8, true>(pool + at * 2, *reinterpret_cast<float(*)[8]>(x));
+      } else {
+        constexpr float kMax = FMT == GS_DTYPE_E4M3 ? kE4m3Max : kInt8Max;
+        float m = 0.0f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) m = max_nan(m, fabsf(x[i]));
+#pragma unroll
+        for (int o = kLanes >> 1; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(kFullMask, m, o));
+        const float inv = quant_inv(m, kMax);
+        if (!s[u].ok) continue;
+        uint32_t c[E / 4];
+#pragma unroll
+        for (int i = 0; i < E / 4; ++i) {
+          const float y0 = x[4 * i] * inv, y1 = x[4 * i + 1] * inv, y2 = x[4 * i + 2] * inv, y3 = x[4 * i + 3] * inv;
+          c[i] = FMT == GS_DTYPE_E4M3 ? e4m3x4(y0, y1, y2, y3) : int8x4(y0, y1, y2, y3);
+        }
+#pragma unroll
+        for (int i = 0; i < E / 8; ++i) *reinterpret_cast<uint2*>(pool + at + i * (D / 2)) = make_uint2(c[2 * i], c[2 * i + 1]);
+        if (at == 0) *const_cast<float*>(A.kv.scale_at(v, s[u].page, head, s[u].off)) = quant_scale(m, kMax);
+      }
+    }
 }
 
 template <int D, int FMT, bool BF16, bool VEC, int U>
 __global__ void __launch_bounds__(256) kv_read_kernel(const __grid_constant__ KvRowsArgs A, uint32_t step) {
-  constexpr int kLanes = D / 8;
+  constexpr int E = row_piece<FMT, VEC>(), kLanes = D / E;
   const uint32_t row = blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
   const uint32_t token0 = row / static_cast<uint32_t>(A.kv.kv_heads);
   const int head = static_cast<int>(row - token0 * A.kv.kv_heads);
   if (token0 >= step) return;
   const int at = (threadIdx.x % kLanes) * 8;
-  const bool value = blockIdx.y != 0;
-  uint4 raw[U];  // 8 elements: bf16, or codes in .x and .y
-  float sc[U];
+  uint4 raw[U][2];  // the piece as it lies in the pool
+  float sc[U][2];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const uint32_t token = token0 + u * step;
-    raw[u] = make_uint4(0u, 0u, 0u, 0u);
-    sc[u] = 0.0f;
-    if (token >= A.tokens) continue;
-    const SlotAt s = slot_at(A, token);
-    if (!s.ok) continue;
-    const unsigned char* pool = A.kv.at(value, s.page, head, s.off);
-    if constexpr (FMT == GS_DTYPE_BF16) {
-      raw[u] = *reinterpret_cast<const uint4*>(pool + at * 2);
-    } else {
-      const uint2 c = *reinterpret_cast<const uint2*>(pool + at);
-      raw[u].x = c.x, raw[u].y = c.y;
-      sc[u] = *A.kv.scale_at(value, s.page, head, s.off);
+    SlotAt s{0, 0, false};
+    if (token < A.tokens) s = slot_at(A, token);
+#pragma unroll
+    for (int v = 0; v < 2; ++v) {
+      raw[u][v] = make_uint4(0u, 0u, 0u, 0u);
+      sc[u][v] = 0.0f;
+      if (!s.ok) continue;
+      const unsigned char* pool = A.kv.at(v, s.page, head, s.off);
+      if constexpr (FMT == GS_DTYPE_BF16) {
+        raw[u][v] = ld_stream_u4(reinterpret_cast<const uint4*>(pool + at * 2));
+      } else {
+        const uint2 c = *reinterpret_cast<const uint2*>(pool + at);
+        raw[u][v].x = c.x, raw[u][v].y = c.y;
+        if constexpr (E == 16) {
+          const uint2 d = *reinterpret_cast<const uint2*>(pool + at + D / 2);
+          raw[u][v].z = d.x, raw[u][v].w = d.y;
+        }
+        sc[u][v] = *A.kv.scale_at(v, s.page, head, s.off);
+      }
     }
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     const uint32_t token = token0 + u * step;
     if (token >= A.tokens) continue;
-    float x[8];
-    if constexpr (FMT == GS_DTYPE_BF16) {
-      const uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[2 * i] = bf16_lo(w[i]), x[2 * i + 1] = bf16_hi(w[i]);
-    } else {
-      const uint32_t w[2] = {raw[u].x, raw[u].y};
+    for (int v = 0; v < 2; ++v) {
+      unsigned char* dst = (v ? A.v : A.k) + (row_at(A, v, token, head) + at) * (BF16 ? 2 : 4);
+      const uint32_t w[4] = {raw[u][v].x, raw[u][v].y, raw[u][v].z, raw[u][v].w};
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        if constexpr (FMT == GS_DTYPE_E4M3) {
-          const float2 a = half2_float2(e4m3x2_half2(w[i] & 0xffffu)), b = half2_float2(e4m3x2_half2(w[i] >> 16));
-          x[4 * i] = a.x * sc[u], x[4 * i + 1] = a.y * sc[u], x[4 * i + 2] = b.x * sc[u], x[4 * i + 3] = b.y * sc[u];
+      for (int i = 0; i < E / 8; ++i) {
+        float x[8];
+        if constexpr (FMT == GS_DTYPE_BF16) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[2 * k] = bf16_lo(w[k]), x[2 * k + 1] = bf16_hi(w[k]);
         } else {
+          const float2 f = make_float2(sc[u][v], sc[u][v]);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            x[4 * i + k] = static_cast<float>(static_cast<int8_t>((w[i] >> (8 * k)) & 0xffu)) * sc[u];
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t c = w[2 * i + k];
+            float2 a, b;
+            if constexpr (FMT == GS_DTYPE_E4M3) {
+              a = half2_float2(e4m3x2_half2(c & 0xffffu)), b = half2_float2(e4m3x2_half2(c >> 16));
+            } else {
+              a = make_float2(static_cast<float>(static_cast<int8_t>(c & 0xffu)), static_cast<float>(static_cast<int8_t>((c >> 8) & 0xffu)));
+              b = make_float2(static_cast<float>(static_cast<int8_t>((c >> 16) & 0xffu)), static_cast<float>(static_cast<int8_t>(c >> 24)));
+            }
+            a = __fmul2_rn(a, f), b = __fmul2_rn(b, f);
+            x[4 * k] = a.x, x[4 * k + 1] = a.y, x[4 * k + 2] = b.x, x[4 * k + 3] = b.y;
+          }
         }
+        store8<BF16, VEC>(dst + i * (D / 2) * (BF16 ? 2 : 4), x);
       }
     }
-    store8<BF16, VEC>((value ? A.v : A.k) + (row_at(A, value, token, head) + at) * (BF16 ? 2 : 4), x);
   }
 }
 
 template <int D, int FMT, bool BF16, bool VEC>
 cudaError_t launch_rows3(const KvRowsArgs& a, bool write, cudaStream_t st) {
-  constexpr int64_t per = 256 / (D / 8);
-  constexpr int U = 4;
-  // (four rows a thread from about two blocks an SM on)
+  constexpr int64_t per = 256 / (D / row_piece<FMT, VEC>());
+  constexpr int U = 2;
+  // (two tokens a thread from about two blocks an SM on)
   const bool many = VEC && a.tokens * a.kv.kv_heads >= 148 * 2 * per * U;
   const uint32_t step = static_cast<uint32_t>(many ? (a.tokens + U - 1) / U : a.tokens);
-  const dim3 grid(static_cast<unsigned>((static_cast<int64_t>(step) * a.kv.kv_heads + per - 1) / per), 2);
+  const unsigned grid = static_cast<unsigned>((static_cast<int64_t>(step) * a.kv.kv_heads + per - 1) / per);
   if (write) {
     if (VEC && many) kv_write_kernel<D, FMT, BF16, VEC, VEC ? U : 1><<<grid, 256, 0, st>>>(a, step);
     else kv_write_kernel<D, FMT, BF16, VEC, 1><<<grid, 256, 0, st>>>(a, step);

@@ -30,9 +30,10 @@ struct NormArgs {
   int64_t ld_x, ld_residual, ld_residual_out, ld_out;
   int32_t hidden;
   int32_t group;   // columns per scale (hidden when one scale a row)
+  int32_t shift;   // log2(group) where a row has several scales
   int32_t groups;  // scales per row
   int32_t weight_bf16;
-  float eps, offset, srq_scale;
+  float eps, offset, srq_scale, inv_hidden;
 };
 
 enum { kOutF32 = 0, kOutBf16 = 1, kOutE4m3 = 2, kOutSrq = 3 };
@@ -117,6 +118,9 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(const __grid_constant__ Norm
   const int wid = threadIdx.y * warps + (t >> 5), lane = t & 31;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y;
   const bool live = row < A.rows;
+  bool in[PIECES];  // whether this thread's pieces lie in the row
+#pragma unroll
+  for (int p = 0; p < PIECES; ++p) in[p] = live && (t + p * tpr) * V < A.hidden;
   using T = typename std::conditional<BF16, unsigned short, float>::type;
   float h[PIECES][V];
   float2 sq2 = make_float2(0.0f, 0.0f);
@@ -126,13 +130,13 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(const __grid_constant__ Norm
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
       const int col = (t + p * tpr) * V;
-      if (col < A.hidden) load_row<V, BF16>(x + col, h[p]);
+      if (in[p]) load_row<V, BF16>(x + col, h[p]);
     }
     if (r) {
 #pragma unroll
       for (int p = 0; p < PIECES; ++p) {
         const int col = (t + p * tpr) * V;
-        if (col < A.hidden) {
+        if (in[p]) {
           float b[V];
           load_row<V, BF16>(r + col, b);
           add_row(h[p], b);
@@ -142,7 +146,7 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(const __grid_constant__ Norm
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
       const int col = (t + p * tpr) * V;
-      if (col < A.hidden) {
+      if (in[p]) {
         if (A.residual_out) store_row<V, BF16>(static_cast<T*>(A.residual_out) + row * A.ld_residual_out + col, h[p]);
         square_row(h[p], sq2);
       }
@@ -152,14 +156,13 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(const __grid_constant__ Norm
   if (warps > 1) {
     if (lane == 0) red[wid] = sq;
     __syncthreads();
-    sq = 0.0f;
-    for (int w = 0; w < warps; ++w) sq += red[threadIdx.y * warps + w];
+    sq = warp_sum_f(lane < warps ? red[threadIdx.y * warps + lane] : 0.0f);
   }
-  const float rstd = 1.0f / sqrtf(sq / static_cast<float>(A.hidden) + A.eps);
+  const float rstd = rsqrtf(sq * A.inv_hidden + A.eps);
 #pragma unroll
   for (int p = 0; p < PIECES; ++p) {
     const int col = (t + p * tpr) * V;
-    if (col < A.hidden && live) {
+    if (in[p]) {
       float w[V];
       load_weight<V>(A, col, w);
       scale_row(h[p], rstd);
@@ -170,7 +173,7 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(const __grid_constant__ Norm
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
       const int col = (t + p * tpr) * V;
-      if (col < A.hidden && live) {
+      if (in[p]) {
         using O = typename std::conditional<OUT == kOutBf16, unsigned short, float>::type;
         store_row<V, OUT == kOutBf16>(static_cast<O*>(A.out) + row * A.ld_out + col, h[p]);
       }
@@ -180,7 +183,7 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(const __grid_constant__ Norm
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
       const int col = (t + p * tpr) * V;
-      if (col < A.hidden && live) {
+      if (in[p]) {
         float o[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
@@ -195,8 +198,7 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(const __grid_constant__ Norm
     if (warps > 1) {
       if (lane == 0) redi[wid] = qs;
       __syncthreads();
-      qs = 0;
-      for (int w = 0; w < warps; ++w) qs += redi[threadIdx.y * warps + w];
+      qs = warp_sum_i(lane < warps ? redi[threadIdx.y * warps + lane] : 0);
     }
     if (t == 0 && live && A.row_sum) A.row_sum[row] = __fmul_rn(static_cast<float>(qs), A.srq_scale);
   } else {
@@ -207,7 +209,7 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(const __grid_constant__ Norm
     for (int p = 0; p < PIECES; ++p) {
       gm[p] = 0.0f;
       const int col = (t + p * tpr) * V;
-      if (col < A.hidden && live)
+      if (in[p])
 #pragma unroll
         for (int i = 0; i < V; ++i) gm[p] = max_nan(gm[p], fabsf(h[p][i]));
     }
@@ -219,8 +221,7 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(const __grid_constant__ Norm
       if (warps > 1) {
         if (lane == 0) red2[wid] = m;
         __syncthreads();
-        m = 0.0f;
-        for (int w = 0; w < warps; ++w) m = max_nan(m, red2[threadIdx.y * warps + w]);
+        m = warp_max_bits(lane < warps ? red2[threadIdx.y * warps + lane] : 0.0f);
       }
 #pragma unroll
       for (int p = 0; p < PIECES; ++p) gm[p] = m;
@@ -230,10 +231,13 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(const __grid_constant__ Norm
       const int span = A.group >> 3;
 #pragma unroll
       for (int p = 0; p < PIECES; ++p) {
-        for (int o = span >> 1; o > 0; o >>= 1) gm[p] = max_nan(gm[p], __shfl_xor_sync(kFullMask, gm[p], o));
+        gm[p] = max_nan(gm[p], __shfl_xor_sync(kFullMask, gm[p], 1));
+        gm[p] = max_nan(gm[p], __shfl_xor_sync(kFullMask, gm[p], 2));
+        if (span > 4) gm[p] = max_nan(gm[p], __shfl_xor_sync(kFullMask, gm[p], 4));
+        if (span > 8) gm[p] = max_nan(gm[p], __shfl_xor_sync(kFullMask, gm[p], 8));
         const int col = (t + p * tpr) * V;
         if (col < A.hidden && live && (lane & (span - 1)) == 0)
-          scales[col / A.group] = quant_floor(gm[p]) * (1.0f / kE4m3Max);
+          scales[col >> A.shift] = quant_floor(gm[p]) * (1.0f / kE4m3Max);
       }
     } else {
       int* gr = gmax + threadIdx.y * A.groups;
@@ -244,13 +248,13 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(const __grid_constant__ Norm
         // a warp's 32 columns lie in one group (groups are multiples of 32 columns)
         const int col = t + p * tpr;
         const int m = __float_as_int(warp_max_bits(gm[p]));
-        if (lane == 0 && col < A.hidden) atomicMax(gr + col / A.group, m);
+        if (lane == 0 && col < A.hidden) atomicMax(gr + (col >> A.shift), m);
       }
       __syncthreads();
 #pragma unroll
       for (int p = 0; p < PIECES; ++p) {
         const int col = (t + p * tpr) * V;
-        if (col < A.hidden && live) gm[p] = __int_as_float(gr[col / A.group]);
+        if (in[p]) gm[p] = __int_as_float(gr[col >> A.shift]);
       }
       if (live)
         for (int g = t; g < A.groups; g += tpr) scales[g] = quant_scale(__int_as_float(gr[g]), kE4m3Max);
@@ -258,7 +262,7 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(const __grid_constant__ Norm
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
       const int col = (t + p * tpr) * V;
-      if (col < A.hidden && live) {
+      if (in[p]) {
         const float inv = norm_inv(gm[p]);
         if constexpr (V == 8) {
           uint2 c;
@@ -363,10 +367,12 @@ extern "C" gs_status gs_rms_norm(gs_ctx* ctx, const gs_rms_norm_args* p, void* s
   a.hidden = static_cast<int32_t>(p->hidden);
   a.group = p->group ? p->group : a.hidden;
   a.groups = (a.hidden + a.group - 1) / a.group;
+  a.shift = p->group == 32 ? 5 : p->group == 64 ? 6 : 7;
   a.weight_bf16 = p->weight_dtype == GS_DTYPE_BF16;
   a.eps = p->eps;
   a.offset = p->weight_offset;
   a.srq_scale = p->srq_scale;
+  a.inv_hidden = static_cast<float>(1.0 / static_cast<double>(p->hidden));
   // 16-byte accesses need every row to start on 16 bytes (8 for codes) and whole pieces
   auto fits = [&](const void* ptr, int64_t ld, int dtype) {
     if (!ptr) return true;
