@@ -13,8 +13,8 @@
 // S^T's accumulators become the B operand of the second product by one 8x8 transpose each.
 //
 // Every warp walks its own tiles (every fourth of the block's share) through a private ring of
-// shared-memory stages that one lane fills by TMA boxes of 16 tokens in the swizzled layout ldmatrix
-// reads without bank conflicts: the loop has no block barrier, and 64 to 128 KB are in flight per SM.
+// shared-memory stages that one lane fills by TMA boxes of 16 tokens in the swizzled layout
+// ldmatrix reads without bank conflicts: the loop has no block barrier, and 100 to 190 KB are in flight per SM.
 // A row's reference point m moves only when a score passes it by 2^8 (as V's reference scale does
 // when a larger one comes), so the usual tile needs one vote instead of reductions and rescaling.
 // Values of tokens hidden from every row of the block are set to zero before they are used.
@@ -51,7 +51,12 @@ struct RowsPlan {
   static constexpr int kCols = kRow / kInner;                // boxes across a row
   static constexpr int kTileBytes = kRT * kRow;              // K or V of one tile
   static constexpr int kSub = kTileBytes <= 1024 ? 2 : 1;    // tiles per stage
-  static constexpr int kStage = kSub * 2 * kTileBytes;
+  // A stage holds K and V of its tiles, or, where those are 16 KB, one of them, in turn: three stages of 8 KB a warp
+  // then leave room for a second block on the SM (32 rows, 8 sequences of 4000 tokens, 8 heads of 256: 78 -> 48 us), at the
+  // price of two waits and two fetches a tile (narrower rows lose by it: heads of 64 161 -> 187 us).
+  static constexpr bool kHalves = kTileBytes >= 8192;
+  static constexpr int kParts = kHalves ? 1 : 2;
+  static constexpr int kStage = kSub * kParts * kTileBytes;
   static constexpr int kStages = 3;
   static constexpr int kRing = kRowsWarps * kStages * kStage;
   static constexpr int kScale = kBf ? 0 : kSub * 2 * kRT * 4;  // scales of a stage
@@ -200,7 +205,8 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
   if (lane < P::kStages) mbar_init(&s_bar[warp][lane], 1);
   __syncwarp();
 
-  // ---- the warp's ring: stage n holds tiles i_begin + (n · 4 + warp) · kSub ..
+  // ---- the warp's ring: stage i holds the warp's step i, tiles i_begin + (i · 4 + warp) · kSub .., or (halves)
+  // K (i even) or V of step i / 2
   const uint32_t ring = smem_addr(smem) + warp * (P::kStages * P::kStage);
   const uint32_t scales = smem_addr(smem + S::kOffScale) + warp * (P::kStages * P::kScale);
   const int32_t* table = A.table + b * A.table_stride;
@@ -208,11 +214,11 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
   const int page_mask = (1 << A.kv.page_shift) - 1;
   const int first = i_begin + warp * P::kSub;
   constexpr int kStep = kRowsWarps * P::kSub;
-  const int n_stages = i_end > first ? (i_end - first + kStep - 1) / kStep : 0;
+  const int n_steps = i_end > first ? (i_end - first + kStep - 1) / kStep : 0;
   int pages = 0;       // table entries of the warp's next 32 tiles
   int pages_at = -1;   // which 32
-  auto fetch = [&](int n) {
-    const int t = n * P::kSub;  // the warp's tile number
+  auto fetch = [&](int i, int slot) {
+    const int n = P::kHalves ? i >> 1 : i, t = n * P::kSub;  // step, the warp's tile number
     if ((t >> 5) != pages_at) {
       pages_at = t >> 5;
       const int tl = (pages_at << 5) + lane;
@@ -230,24 +236,30 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
     int pg[P::kSub];
 #pragma unroll
     for (int u = 0; u < P::kSub; ++u) pg[u] = __shfl_sync(kFullMask, pages, (t + u) & 31);
-    if (lane == 0 && n < n_stages) {
-      const int st = n % P::kStages;
-      uint64_t* bar = &s_bar[warp][st];
+    if (lane == 0 && n < n_steps) {
+      uint64_t* bar = &s_bar[warp][slot];
       const int i0 = first + n * kStep;
       const int live = P::kSub == 1 || i0 + 1 < i_end ? P::kSub : 1;
-      mbar_expect_tx(bar, live * (2 * P::kTileBytes + (kBf ? 0 : 2 * kRT * 4)));
+      mbar_expect_tx(bar, live * (P::kParts * P::kTileBytes + (kBf ? 0 : 2 * kRT * 4)));
 #pragma unroll
       for (int u = 0; u < P::kSub; ++u) {
         if (u >= live) break;
         const int off = (R.tile(i0 + u) * kRT) & page_mask;
-        const uint32_t ks = ring + st * P::kStage + u * 2 * P::kTileBytes;
+        const uint32_t at = ring + slot * P::kStage + u * P::kParts * P::kTileBytes;
 #pragma unroll
         for (int cb = 0; cb < P::kCols; ++cb) {
-          box_in(ks + cb * (kRT * P::kInner), &maps.k, cb * (P::kInner / P::kEl), off, head, pg[u], bar);
-          box_in(ks + P::kTileBytes + cb * (kRT * P::kInner), &maps.v, cb * (P::kInner / P::kEl), off, head, pg[u], bar);
+          const int x = cb * (P::kInner / P::kEl);
+          const uint32_t to = at + cb * (kRT * P::kInner);
+          if constexpr (P::kHalves) {
+            box_in(to, i & 1 ? &maps.v : &maps.k, x, off, head, pg[u], bar);
+          } else {
+            box_in(to, &maps.k, x, off, head, pg[u], bar);
+            box_in(to + P::kTileBytes, &maps.v, x, off, head, pg[u], bar);
+          }
         }
         if constexpr (!kBf) {
-          const uint32_t sd = scales + st * P::kScale + u * (2 * kRT * 4);
+          static_assert(kBf || !P::kHalves, "scales come with both");
+          const uint32_t sd = scales + slot * P::kScale + u * (2 * kRT * 4);
           bulk_g2s_addr(sd, A.kv.scale_at(false, pg[u], head, off), kRT * 4, bar);
           bulk_g2s_addr(sd + kRT * 4, A.kv.scale_at(true, pg[u], head, off), kRT * 4, bar);
         }
@@ -256,7 +268,7 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
     __syncwarp();
   };
 #pragma unroll
-  for (int s = 0; s < P::kStages - 1; ++s) fetch(s);
+  for (int i = 0; i < P::kStages; ++i) fetch(i, i);
 
   // ---- Q fragments (B operand: k = 2c.. of row n = g), once
   for (int nb = warp; nb < NB; nb += kRowsWarps) {
@@ -328,39 +340,33 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
   }
   float vref = 0.0f, vinv = 0.0f;  // (8-bit) largest V scale so far, kPScale over it
 
-  int stage = 0;
+  int slot = 0;  // of the next stage
   uint32_t phase = 0;
-  for (int n = 0; n < n_stages; ++n) {
-    if (!mbar_wait(&s_bar[warp][stage], phase, kWaitNs)) {
-      // (bounded: the other copies in flight get the same limit once more before the block ends)
-      atomicOr(A.flag, GS_KV_ERR_TIMEOUT);
-      for (int k = n + 1; k < n + P::kStages - 1 && k < n_stages; ++k)
-        mbar_wait(&s_bar[warp][k % P::kStages], static_cast<uint32_t>((k / P::kStages) & 1), kWaitNs);
-      break;
+  auto wait = [&](int s_, uint32_t p_) {
+    const bool ok = mbar_wait(&s_bar[warp][s_], p_, kWaitNs);
+    if (!ok) atomicOr(A.flag, GS_KV_ERR_TIMEOUT);
+    return __all_sync(kFullMask, ok);
+  };
+  bool ok = true;
+  for (int n = 0; n < n_steps; ++n) {
+    const int k_slot = slot;
+    const uint32_t k_phase = phase;
+    if (++slot == P::kStages) slot = 0, phase ^= 1;
+    const int v_slot = P::kHalves ? slot : k_slot;
+    const uint32_t v_phase = phase;  // (halves)
+    if constexpr (P::kHalves) {
+      if (++slot == P::kStages) slot = 0, phase ^= 1;
     }
-    __syncwarp();  // every lane is done with the stage before this one: it is the next fetch's
-    fetch(n + P::kStages - 1);
     const int i0 = first + n * kStep;
+    ok = wait(k_slot, k_phase);
+    if (!ok) break;
 #pragma unroll
     for (int sub = 0; sub < P::kSub; ++sub) {
-      if (P::kSub > 1 && sub > 0 && i0 + sub >= i_end) break;
-      const uint32_t ks = ring + stage * P::kStage + sub * 2 * P::kTileBytes, vs = ks + P::kTileBytes;
+      const bool last = sub == P::kSub - 1 || (P::kSub > 1 && i0 + sub + 1 >= i_end);
+      const uint32_t ks = ring + k_slot * P::kStage + sub * P::kParts * P::kTileBytes;
+      const uint32_t vs = P::kHalves ? ring + v_slot * P::kStage : ks + P::kTileBytes;
       const int j0 = R.tile(i0 + sub) * kRT;
       const bool whole = j0 + kRT - 1 <= p_min && (!A.window || j0 > p_max - A.window || j0 + kRT <= A.sinks);
-      if (!whole) {
-        // tokens no row sees (past the context, before every window): their pages may hold anything
-        constexpr int kPc = P::kRow / 16;
-        bool wrote = false;
-        for (int id = lane; id < kRT * kPc; id += 32) {
-          const int r = id / kPc, ch = id % kPc;
-          if (!R.seen_by_any(j0 + r)) {
-            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vs + piece<P::kInner>(r, ch)), "r"(0u) : "memory");
-            wrote = true;
-          }
-        }
-        if (wrote) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (before the stage's next copy)
-        __syncwarp();
-      }
       // ---- S^T = K Q^T
       float s[NB][4];
       {
@@ -406,12 +412,32 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
       // ---- scores in log2 units; lane: tokens j0 + g, j0 + g + 8, rows 2c, 2c + 1
       float ksc[2] = {1.0f, 1.0f}, vsc[2] = {1.0f, 1.0f};
       if constexpr (!kBf) {
-        const float* sc = reinterpret_cast<const float*>(smem + S::kOffScale) + ((warp * P::kStages + stage) * P::kSub + sub) * 2 * kRT;
+        const float* sc = reinterpret_cast<const float*>(smem + S::kOffScale) + ((warp * P::kStages + k_slot) * P::kSub + sub) * 2 * kRT;
         ksc[0] = sc[g], ksc[1] = sc[g + 8], vsc[0] = sc[16 + g], vsc[1] = sc[24 + g];
         if (!whole) {
           if (!R.seen_by_any(j0 + g)) vsc[0] = 0.0f;
           if (!R.seen_by_any(j0 + g + 8)) vsc[1] = 0.0f;
         }
+      }
+      if constexpr (P::kHalves) {
+        __syncwarp();  // (every lane has read the stage)
+        fetch(2 * n + P::kStages, k_slot);
+        ok = wait(v_slot, v_phase);
+        if (!ok) break;
+      }
+      if (!whole) {
+        // tokens no row sees (past the context, before every window): their pages may hold anything
+        constexpr int kPc = P::kRow / 16;
+        bool wrote = false;
+        for (int id = lane; id < kRT * kPc; id += 32) {
+          const int r = id / kPc, ch = id % kPc;
+          if (!R.seen_by_any(j0 + r)) {
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vs + piece<P::kInner>(r, ch)), "r"(0u) : "memory");
+            wrote = true;
+          }
+        }
+        if (wrote) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (before the stage's next copy)
+        __syncwarp();
       }
       bool move = !kBf && fmaxf(vsc[0], vsc[1]) > vref;
 #pragma unroll
@@ -508,8 +534,18 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
           }
         }
       }
+      if (last) {
+        __syncwarp();
+        fetch((P::kHalves ? 2 * n + 1 : n) + P::kStages, v_slot);
+        break;
+      }
     }
-    if (++stage == P::kStages) stage = 0, phase ^= 1;
+    if (!ok) break;
+  }
+  if (!ok) {
+    // (bounded: what is in flight gets the same limit once more before the block ends)
+    for (int s_ = 0; s_ < P::kStages; ++s_)
+      for (uint32_t p_ = 0; p_ < 2; ++p_) mbar_wait(&s_bar[warp][s_], p_, kWaitNs / 8);
   }
   __syncthreads();  // (the rings are done with)
 

@@ -243,8 +243,10 @@ cudaError_t launch_rows(const KvRowsArgs& a, int fmt, bool write, bool bf16, boo
   }
 }
 
-// Rows (new tokens × heads of a group) up to which the few-row kernel is taken.
-constexpr int64_t kFewRows = 32;
+// Rows (new tokens × heads of a group) up to which the few-row kernel is taken (8 sequences of 4000 tokens, 8
+// heads, few rows against many: 64 rows of 128: 50 and 60 us bf16, 59 and 77 us int8, 128 rows: 83 and 66,
+// 102 and 84; 32 rows of 256: 64 and 83 us int8, 64 rows: 110 and 87).
+int64_t few_rows(int head_dim) { return head_dim == 256 ? 32 : 64; }
 
 gs_status kfail(gs_kv_cache* c, gs_status s, const char* m) {
   c->err = m;
@@ -461,7 +463,7 @@ gs_status gs_attention(gs_kv_cache* c, const gs_attention_args* p, void* stream)
   a.flag = c->flag;
   DeviceScope scope(c->device);
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = most_rows > kFewRows ? launch_attn_tile(c, a, cs) : launch_attn_rows(c, a, cs);
+  const cudaError_t e = most_rows > few_rows(c->d.head_dim) ? launch_attn_tile(c, a, cs) : launch_attn_rows(c, a, cs);
   if (e != cudaSuccess) return kfail(c, GS_ECUDA, cudaGetErrorString(e));
   return GS_OK;
 }
