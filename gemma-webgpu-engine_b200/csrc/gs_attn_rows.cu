@@ -579,7 +579,12 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
   auto put = [&](int r, int d, float M, float L, float4 acc) {
     int gq;
     const int t = R.token_of(A, r, gq);
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    float inv = L == 0.0f ? 0.0f : 1.0f / L;
+    if (!finite4(acc) && L == L) {  // (its maximum and sum do not come from V)
+      float2 ml;
+      attn_by_row<FMT>(A, b, head, q_row(A, R, head, t, gq), R.p0 + t, D, d, &acc, &ml);
+      inv = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;
+    }
     const uint2 w = make_uint2(bf16x2(acc.x * inv, acc.y * inv), bf16x2(acc.z * inv, acc.w * inv));
     *reinterpret_cast<uint2*>(o_row(A, R, head, t, gq) + d) = w;
     if (A.lse && d == 0)

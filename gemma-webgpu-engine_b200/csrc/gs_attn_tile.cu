@@ -822,7 +822,8 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     if (BAL && ok && pc.pieces > 0) {
       // A piece of an item that other groups have the rest of: its (m, l, O) to the workspace, warp by warp,
       // column quads of the 32 rows side by side.  The same 32 rows are the same warp's in every piece, so a
-      // counter per warp tells who is last (nothing waits), and the last one adds the others' to its own.
+      // counter per warp tells who is last (nothing waits), and the last one adds them up, its own too, in
+      // the pieces' order: which of them came last changes no bit of the result.
       fence_after();
       const int64_t warp_at = static_cast<int64_t>(rank * P::kRows + s * 128 + quad * 32);
       auto part_o = [&](int slot) { return reinterpret_cast<float4*>(A.part_o) + (static_cast<int64_t>(slot) * kGroupRows + warp_at) * (D / 4) + lane; };
@@ -854,9 +855,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
           const float2 v = __ldcg(part_ml(slot(k)));
           L += ex2(v.x - ref) * v.y;
         }
-        float fo = ex2(ml - ref);
         for (int k = 0; k < pc.pieces; ++k) {
-          if (slot(k) == pc.part) continue;
           const float f = ex2(__ldcg(part_ml(slot(k))).x - ref);
           const float4* src = part_o(slot(k));
           float4 x[8];
@@ -870,19 +869,23 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
               for (int i = 0; i < 8; ++i) y[i] = __ldcg(src + ((q + 1) * 8 + i) * 32);
             }
             float o[32];
-            tm_ld32(o_at + 32 * q, o);
-            tm_wait_ld();
+            if (k == 0) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+            } else {
+              tm_ld32(o_at + 32 * q, o);
+              tm_wait_ld();
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              o[4 * i] = o[4 * i] * fo + f * x[i].x, o[4 * i + 1] = o[4 * i + 1] * fo + f * x[i].y;
-              o[4 * i + 2] = o[4 * i + 2] * fo + f * x[i].z, o[4 * i + 3] = o[4 * i + 3] * fo + f * x[i].w;
+              o[4 * i] += f * x[i].x, o[4 * i + 1] += f * x[i].y;
+              o[4 * i + 2] += f * x[i].z, o[4 * i + 3] += f * x[i].w;
             }
             tm_st32(o_at + 32 * q, reinterpret_cast<uint32_t*>(o));
 #pragma unroll
             for (int i = 0; i < 8; ++i) x[i] = y[i];
           }
           tm_wait_st();
-          fo = 1.0f;
         }
         ml = M;
         l = L;
@@ -898,6 +901,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         // 16-byte pieces of neighbouring lanes
         constexpr int kCh = D / 8;
         unsigned char* st = sm + s * (D / 64) * 16384 + quad * 32 * D * 2;
+        uint32_t top = 0u;  // largest magnitudes, as patterns
 #pragma unroll
         for (int q = 0; q < D / 32; ++q) {
           float o[32];
@@ -909,11 +913,14 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
             for (int i = 0; i < 32; ++i) o[i] = 0.0f;
           }
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<uint4*>(st + lane * D * 2 + (((4 * q + i) ^ (lane & 7)) << 4)) =
-                make_uint4(bf16x2(o[8 * i] * inv, o[8 * i + 1] * inv), bf16x2(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
-                           bf16x2(o[8 * i + 4] * inv, o[8 * i + 5] * inv), bf16x2(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
+          for (int i = 0; i < 4; ++i) {
+            const uint4 w = make_uint4(bf16x2(o[8 * i] * inv, o[8 * i + 1] * inv), bf16x2(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
+                                       bf16x2(o[8 * i + 4] * inv, o[8 * i + 5] * inv), bf16x2(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
+            top = __vmaxu2(top, __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
+            *reinterpret_cast<uint4*>(st + lane * D * 2 + (((4 * q + i) ^ (lane & 7)) << 4)) = w;
+          }
         }
+        if (live && ((top & 0xffffu) >= 0x7f80u || (top >> 16) >= 0x7f80u)) A.mend[0] = 1u;  // (attn_mend_kernel)
         __syncwarp();
         const int base = rank * P::kRows + s * 128 + quad * 32;  // the warp's first row of the group
 #pragma unroll
@@ -1153,9 +1160,60 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
   int gq;
   const int t = R.token_of(A, r, gq);
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+  if (!finite4(make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv))) A.mend[0] = 1u;  // (attn_mend_kernel)
   *reinterpret_cast<uint2*>(o_row(A, R, head, t, gq) + d) =
       make_uint2(bf16x2(acc.x * inv, acc.y * inv), bf16x2(acc.z * inv, acc.w * inv));
   if (A.lse && d == 0) A.lse[static_cast<int64_t>(R.q0 + t) * A.q_heads + head * A.group + gq] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
+}
+
+// After the many-row kernel, and nothing to do unless that wrote a result that is not finite: those, four values a
+// thread, computed again from what their rows see alone.  It is launched while the kernel before it still runs and waits
+// for its end on the device, and costs a call about a microsecond.
+template <int FMT>
+__global__ void __launch_bounds__(128) attn_mend_kernel(const __grid_constant__ AttnArgs A, int head_dim) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (__ldcg(A.mend) == 0u) return;
+  const int pieces = head_dim / 4;
+  for (int u = blockIdx.x; u < A.seqs * A.kv.kv_heads; u += gridDim.x) {
+    const int b = u / A.kv.kv_heads, head = u % A.kv.kv_heads;
+    const RowRange R = row_range<kTT>(A, b, 0, 0x7fffffff);
+    for (int64_t e = threadIdx.x + static_cast<int64_t>(blockIdx.y) * 128; e < static_cast<int64_t>(R.rows) * pieces; e += gridDim.y * 128) {
+      const int r = static_cast<int>(e / pieces), d = static_cast<int>(e % pieces) * 4, t = r / A.group, g = r % A.group;
+      uint2* at = reinterpret_cast<uint2*>(o_row(A, R, head, t, g) + d);
+      const uint2 w = *at;
+      if (finite4(make_float4(bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y)))) continue;
+      float4 o;
+      float2 ml;
+      attn_by_row<FMT>(A, b, head, q_row(A, R, head, t, g), R.p0 + t, head_dim, d, &o, &ml);
+      const float inv = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;
+      *at = make_uint2(bf16x2(o.x * inv, o.y * inv), bf16x2(o.z * inv, o.w * inv));
+      // (beside an 8-bit cache an infinite V scale takes the row's sum with it)
+      if (A.lse && d == 0)
+        A.lse[static_cast<int64_t>(R.q0 + t) * A.q_heads + head * A.group + g] = ml.y == 0.0f ? -INFINITY : (ml.x + log2f(ml.y)) * 0.6931471805599453f;
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    // (all have read the flag when the last one comes here)
+    if (atomicAdd(A.mend + 1, 1u) == gridDim.x * gridDim.y - 1u) A.mend[0] = 0u, A.mend[1] = 0u;
+  }
+}
+
+template <int FMT>
+cudaError_t mend(const gs_kv_cache* c, const AttnArgs& a, cudaStream_t st) {
+  const int64_t heads = static_cast<int64_t>(a.seqs) * a.kv.kv_heads, most = 4ll * c->num_sms;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim.x = static_cast<unsigned>(heads < most ? heads : most);
+  cfg.gridDim.y = static_cast<unsigned>((most + heads - 1) / heads);
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attn_mend_kernel<FMT>, a, c->d.head_dim);
 }
 
 // Units (sequence, row block) whose tile counts a block sums up at the start of a balanced call, and the
@@ -1264,7 +1322,10 @@ cudaError_t go_fmt(const gs_kv_cache* c, const AttnArgs& a, cudaStream_t st) {
 }  // namespace
 
 cudaError_t launch_attn_tile(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
-  return c->d.head_dim == 64 ? go_fmt<64>(c, a, st) : c->d.head_dim == 128 ? go_fmt<128>(c, a, st) : go_fmt<256>(c, a, st);
+  const cudaError_t e = c->d.head_dim == 64 ? go_fmt<64>(c, a, st) : c->d.head_dim == 128 ? go_fmt<128>(c, a, st) : go_fmt<256>(c, a, st);
+  if (e != cudaSuccess) return e;
+  return c->d.format == GS_DTYPE_BF16   ? mend<GS_DTYPE_BF16>(c, a, st)
+         : c->d.format == GS_DTYPE_E4M3 ? mend<GS_DTYPE_E4M3>(c, a, st) : mend<GS_DTYPE_INT8>(c, a, st);
 }
 
 // The pools as (head_dim, page token, head, page) tensors, boxes of at most 128 bytes of a row (bf16:

@@ -357,7 +357,7 @@ gs_status gs_kv_cache_create(gs_ctx* ctx, const gs_kv_cache_desc* d, gs_kv_cache
   DeviceScope scope(c->device);
   cudaError_t er = cudaMalloc(&c->flag, 4);
   if (er == cudaSuccess) er = cudaMemset(c->flag, 0, 4);
-  if (er == cudaSuccess) er = ctx_attn_workspace(ctx, kAttnWsBytes + kAttnTicketBytes, kAttnTicketBytes, &c->ws);
+  if (er == cudaSuccess) er = ctx_attn_workspace(ctx, kAttnWsBytes + kAttnTicketBytes + kAttnMendBytes, kAttnTicketBytes + kAttnMendBytes, &c->ws);
   if (er == cudaSuccess) er = cudaDeviceGetAttribute(&c->num_sms, cudaDevAttrMultiProcessorCount, c->device);
   if (er != cudaSuccess) {
     ctx_set_error(ctx, cudaGetErrorString(er));
@@ -395,7 +395,7 @@ gs_status gs_kv_cache_check(gs_kv_cache* c, int32_t* bits) {
   if (e == cudaSuccess && f) e = cudaMemset(c->flag, 0, 4);
   if (e != cudaSuccess) return kfail(c, GS_ECUDA, cudaGetErrorString(e));
   *bits = f;
-  if (f & GS_KV_ERR_TIMEOUT) cudaMemset(c->ws + kAttnWsBytes, 0, kAttnTicketBytes);  // (a piece may not have counted)
+  if (f & GS_KV_ERR_TIMEOUT) cudaMemset(c->ws + kAttnWsBytes, 0, kAttnTicketBytes + kAttnMendBytes);  // (a piece may not have counted)
   if (f & GS_KV_ERR_TIMEOUT) return kfail(c, GS_ETIMEOUT, "a bounded wait inside the attention kernel ran out");
   if (f & GS_KV_ERR_SLOT) return kfail(c, GS_EINVAL, "a slot lies past the cache");
   if (f & GS_KV_ERR_PAGE) return kfail(c, GS_EINVAL, "a page-table entry is outside the cache");
@@ -461,6 +461,7 @@ gs_status gs_attention(gs_kv_cache* c, const gs_attention_args* p, void* stream)
   a.sinks = a.window ? (p->sinks < p->max_kv ? p->sinks : p->max_kv) : 0;
   a.scale_log2 = static_cast<float>(static_cast<double>(p->scale) * 1.4426950408889634);
   a.flag = c->flag;
+  a.mend = reinterpret_cast<unsigned*>(c->ws + kAttnWsBytes + kAttnTicketBytes);
   DeviceScope scope(c->device);
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   const cudaError_t e = most_rows > few_rows(c->d.head_dim) ? launch_attn_tile(c, a, cs) : launch_attn_rows(c, a, cs);

@@ -270,3 +270,58 @@ def test_balanced_over_items(pkg, sampler, dim, lens, heads, group):
     R.check_attend(out[idx], lse[idx], ref)
     # which piece of an item comes last is a matter of time: joined results agree to the rounding of one more sum
     assert ((out.double() - again.double()).abs() <= 2.0 ** -7 * out.double().abs() + 1e-6).all()
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 3)])
+@pytest.mark.parametrize("dim,lens,group", [(64, [(20, 300), (3, 130), (1, 65)], 2), (128, [(9, 700), (9, 9)], 6),
+                                            (256, [(7, 2100)], 2), (64, [(60, 300), (200, 260), (1, 65)], 4),
+                                            (128, [(300, 900), (5, 5)], 2), (256, [(200, 500), (40, 333)], 3)])
+@pytest.mark.parametrize("form", FORMS)
+def test_values_that_only_some_rows_see(pkg, sampler, form, dim, lens, group, window, sinks, value):
+    """An infinity or a NaN in the cached values of one new token and of one at the windows' edge: the rows that do not
+    see it give the formula's finite result, the others none."""
+    c = Case(sampler, pkg, lens, 2, group, dim, 16, form, seed=dim, window=window, sinks=sinks)
+    bad = set()
+    for b, (nq, n) in enumerate(lens):
+        # from a quarter before the last new token on; up to a quarter after the first
+        for j in [n - 1 - nq // 4] + ([max(sinks, n - nq + nq // 4 - window + 1)] if window else []):
+            bad.add((b, j))
+            pg, off = int(c.table[b, j // 16]), j % 16
+            if form == "bf16":
+                c.cache.v[pg, :, off, 3] = value
+                c.vd[pg, :, off, 3] = value
+            else:
+                c.cache.v_scale[pg, :, off] = value
+                c.vd[pg, :, off] = value
+    out, lse = c.run()
+    ref = list(c.reference())
+    clean = torch.ones(out.shape[0], dtype=torch.bool, device="cuda")
+    for b, (nq, n) in enumerate(lens):
+        for t in range(nq):
+            p = n - nq + t
+            for b2, j in bad:
+                if b2 == b and j <= p and (not window or j > p - window or j < sinks):
+                    clean[c.starts[b] + t] = False
+    assert clean.any() and not clean.all()
+    R.check_attend(out[clean], lse[clean], [x[clean] for x in ref])
+    assert not out[~clean][..., 3].isfinite().any()
+    rest = [x[~clean].clone() for x in ref]
+    if form == "bf16":  # (the token's other values are finite)
+        got = out[~clean].clone()
+        got[..., 3] = 0
+        rest[0][..., 3] = 0
+        rest[2][..., 3] = 0
+        R.check_attend(got, lse[~clean], rest)
+    again, lse2 = c.run()
+    assert torch.equal(out[clean], again[clean]) and torch.equal(lse[clean], lse2[clean])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_balanced_join_has_one_order(pkg, sampler, dim):
+    """Which piece of a shared item comes last changes no bit."""
+    c = Case(sampler, pkg, [(64, 2500)] * 9 + [(3, 2)], 16, 8, dim, 64, "bf16", seed=dim)
+    out, lse = c.run()
+    for _ in range(20):
+        again, lse2 = c.run()
+        assert torch.equal(out, again) and torch.equal(lse, lse2)
