@@ -325,3 +325,60 @@ def test_balanced_join_has_one_order(pkg, sampler, dim):
     for _ in range(20):
         again, lse2 = c.run()
         assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.11, 2.0 ** -40])
+@pytest.mark.parametrize("dim,lens", [(64, [(2, 200), (1, 3)]), (128, [(50, 300), (2, 2)]), (256, [(40, 150)])])
+@pytest.mark.parametrize("form", FORMS)
+def test_scales_of_any_sign(pkg, sampler, form, dim, lens, scale):
+    c = Case(sampler, pkg, lens, 2, 4, dim, 16, form, seed=dim, window=90, sinks=2)
+    c.scale = scale
+    c.check()
+
+
+@pytest.mark.parametrize("group,heads", [(1, 5), (7, 3), (33, 1), (71, 1)])
+@pytest.mark.parametrize("form,dim", [("bf16", 128), ("e4m3", 64), ("int8", 256)])
+def test_odd_groups(pkg, sampler, form, dim, group, heads):
+    """Row blocks that begin and end inside a token's heads."""
+    Case(sampler, pkg, [(1, 333), (3, 64), (11, 200)], heads, group, dim, 32, form, seed=group).check()
+
+
+@pytest.mark.parametrize("lens", [[(1, 200), (1, 150), (2, 170)], [(40, 200), (33, 180)]])
+def test_shared_pages(pkg, sampler, lens):
+    """Sequences whose first pages are the same ones."""
+    c = Case(sampler, pkg, lens, 2, 4, 128, 32, "bf16", seed=4)
+    c.table[1:, :4] = c.table[0, :4]
+    c.check()
+
+
+@pytest.mark.parametrize("form,dim", [("bf16", 128), ("e4m3", 256)])
+def test_pools_past_32_bit_offsets(pkg, sampler, form, dim):
+    """Pages whose byte offsets pass 2^32 and 2^33: written, read back and attended over."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    typ = R.TYPES[form]
+    page, heads = 64, 2
+    per_page = heads * page * dim * torch.empty((), dtype=typ).element_size()
+    pages = 2 ** 33 // per_page + 8
+    k, v = (torch.empty((pages, heads, page, dim), dtype=typ, device="cuda") for _ in range(2))
+    scales = [None, None] if form == "bf16" else [torch.zeros((pages, heads, page), device="cuda") for _ in range(2)]
+    cache = pkg.GpuKvCache(sampler, k, v, *scales)
+    low = 2 ** 32 // per_page
+    table = torch.tensor([[pages - 1, 0, low, pages - 2], [low + 1, pages - 3, 1, 2]], dtype=torch.int32, device="cuda")
+    lens = [(60, 250), (1, 130)]
+    x = [torch.randn((256 + 256, heads, dim), generator=gen, device="cuda").to(torch.bfloat16) for _ in range(2)]
+    slots = (table.reshape(-1).long()[:, None] * page + torch.arange(page, device="cuda")).reshape(-1)
+    cache.write(x[0], x[1], slots.to(torch.int32))
+    want = x if form == "bf16" else [R.pool_values(*R.quantise(t, form)).to(torch.bfloat16) for t in x]
+    for got, w in zip(cache.read(slots.to(torch.int32)), want):
+        assert torch.equal(got, w)
+    q = torch.randn((61, 4, dim), generator=gen, device="cuda").to(torch.bfloat16)
+    for starts, rows, q_ in (([0, 60, 61], lens, q), ([0, 1, 2], [(1, 250), (1, 130)], q[:2])):
+        out, lse = cache.attend(q_, torch.tensor(starts, dtype=torch.int32, device="cuda"),
+                                torch.tensor([n for _, n in rows], dtype=torch.int32, device="cuda"), table,
+                                max_q=rows[0][0], max_kv=256, scale=dim ** -0.5, lse=True)
+        small = table.clone()  # the same tokens in a small pool: page i of it is entry i of the table
+        small[:] = torch.arange(8, device="cuda", dtype=torch.int32).view(2, 4)
+        vals = [(t if form == "bf16" else R.pool_values(*R.quantise(t, form))).double().view(8, page, heads, dim).transpose(1, 2) for t in x]
+        ref = R.attend(q_, starts, [n for _, n in rows], small, vals[0], vals[1], page, dim ** -0.5, 0, 0)
+        R.check_attend(out, lse, ref)
+    cache.check()
