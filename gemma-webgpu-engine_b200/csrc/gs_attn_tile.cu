@@ -128,7 +128,7 @@ __device__ __forceinline__ void arrive_first(uint64_t* bar) {
   } else {
     uint32_t a;
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_addr(bar)));
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(a) : "memory");
   }
 }
 // Bounded wait on a barrier that the other block may have arrived on.
@@ -141,7 +141,7 @@ __device__ __forceinline__ bool wait_group(uint64_t* bar, uint32_t parity) {
     for (;;) {
       uint32_t done;
       asm volatile(
-          "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+          "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
           : "=r"(done)
           : "r"(smem_addr(bar)), "r"(parity)
           : "memory");

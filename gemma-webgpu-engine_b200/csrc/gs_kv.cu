@@ -345,7 +345,7 @@ gs_status gs_kv_cache_create(gs_ctx* ctx, const gs_kv_cache_desc* d, gs_kv_cache
                               d->v_page_stride, d->v_head_stride, d->v_token_stride};
   for (int64_t s : strides)
     if (s < d->head_dim || (s * e) % 16 != 0 || s >= (1ll << 35))
-      return bad(GS_EINVAL, "KV cache: strides must be at least head_dim, whole 16-byte pieces and below 2^35");
+      return bad(GS_EINVAL, "KV cache: strides must be at least head_dim, whole 16-byte pieces and below 2^35 elements");
   if (reinterpret_cast<uintptr_t>(d->k) % 16 || reinterpret_cast<uintptr_t>(d->v) % 16)
     return bad(GS_EINVAL, "KV cache: k and v must be 16-byte aligned");
   auto* c = new (std::nothrow) gs_kv_cache();
@@ -434,8 +434,9 @@ gs_status gs_attention(gs_kv_cache* c, const gs_attention_args* p, void* stream)
     return kfail(c, GS_EINVAL, "q and out must be 16-byte aligned");
   const int64_t group = p->q_heads / c->d.kv_heads;
   const int64_t most_rows = static_cast<int64_t>(p->max_q) * group;
-  if (most_rows > (1ll << 24) || most_rows / 8 * c->d.kv_heads > 0x7fffffffll)
-    return kfail(c, GS_EUNSUPPORTED, "max_q * (q_heads / kv_heads) is at most 2^24");
+  // (the many-row grid's second dimension holds blocks of at least 128 rows for every head)
+  if (most_rows > (1ll << 23) || (most_rows + 127) / 128 * c->d.kv_heads > 65535)
+    return kfail(c, GS_EUNSUPPORTED, "max_q * (q_heads / kv_heads) times kv_heads is at most 2^23 - 128");
   if (p->seqs > 65535) return kfail(c, GS_EUNSUPPORTED, "at most 65535 sequences per call");
   AttnArgs a{};
   a.kv = pool_of(c);

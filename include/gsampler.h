@@ -342,8 +342,9 @@ gs_status gs_rms_norm(gs_ctx* ctx, const gs_rms_norm_args* args, void* stream);
  * step whose logits are sampled.)  The caller owns the memory: `pages` pages of page_size
  * tokens, each [kv_heads][page_size][head_dim] by default (any strides whose rows of
  * head_dim are contiguous and 16-byte aligned), and for 8-bit formats one float32 scale
- * per page, head and token, contiguous [pages][kv_heads][page_size].  A slot is
- * page · page_size + offset. */
+ * per page, head and token, contiguous [pages][kv_heads][page_size], 16-byte aligned.
+ * A slot is page · page_size + offset.  Strides are below 2^35 elements; destroy the handle
+ * before its context. */
 typedef struct gs_kv_cache_desc {
   void* k;                  /* device */
   void* v;
@@ -398,11 +399,13 @@ gs_status gs_kv_read(gs_kv_cache* c, const gs_kv_rows* rows, void* stream);
  * page_table[b · page_table_stride + j / page_size].  Query head g reads key/value head
  * g / (q_heads / kv_heads).  Per row, with s_j = scale · q·k_j over the tokens it sees:
  *   lse = log Σ e^(s_j),  out = Σ e^(s_j - lse) v_j
- * rounded once to bf16.  A row that sees nothing gives out 0 and lse -inf.  What no row of
- * a call sees (tokens past kv_len, before every window) is not read.
+ * rounded once to bf16.  A row that sees nothing gives out 0 and lse -inf.  A token that a
+ * row does not see changes none of its bits, infinities and NaN included.
  * Scores, maxima, sums and the accumulated output are float32; a row's weights
- * e^(s_j - running max), times the value's scale, are rounded to bf16 (float16 beside an
- * 8-bit cache in the few-row kernel) for the second product.
+ * e^(s_j - running max) are rounded to bf16 for the second product, beside an 8-bit cache
+ * their product with the value's scale to float16.  (Beside an 8-bit cache q enters the first
+ * product as float16 after an exact power of two per row: components below 2^-24 of the row's
+ * largest are lost.)  The same call gives the same bits every time.
  * The calls of one context use its workspace: order them on the GPU (one stream, or
  * events between streams), as for gs_sample. */
 typedef struct gs_attention_args {
@@ -412,10 +415,11 @@ typedef struct gs_attention_args {
   const int32_t* q_start;   /* device [seqs + 1], or NULL (tokens == seqs, one each) */
   const int32_t* kv_len;    /* device [seqs] */
   const int32_t* page_table;/* device [seqs][page_table_stride] */
-  int64_t tokens, q_token_stride, q_head_stride, out_token_stride, out_head_stride; /* elements */
-  int64_t page_table_stride, page_table_cols;
+  int64_t tokens, q_token_stride, q_head_stride, out_token_stride, out_head_stride; /* elements: multiples of 8 below 2^31 */
+  int64_t page_table_stride, page_table_cols; /* columns for max_kv tokens */
   int32_t seqs, q_heads;
-  int32_t max_q;            /* bound on a sequence's new tokens (host knowledge: it sizes the launch) */
+  int32_t max_q;            /* bound on a sequence's new tokens (host knowledge: it sizes the launch);
+                             * max_q * q_heads < 2^23 - 2^17 */
   int32_t max_kv;           /* bound on kv_len */
   int32_t window, sinks;    /* 0: no window.  sinks only beside a window */
   float scale;
