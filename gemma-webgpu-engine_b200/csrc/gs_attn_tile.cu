@@ -69,13 +69,15 @@ struct TilePlan {
   // loaders.  Registers a thread: a row of 128 scores lives in its softmax thread; the shares add
   // up to what the block is launched with.
   static constexpr int kSoftWarps = 4 * NQ, kMmaWarp = kSoftWarps, kLoadWarp = kSoftWarps + 1, kWidenWarp = kSoftWarps + 4;
-  static constexpr int kGroups = NQ + (kBf ? 1 : 2);
+  // (At head_dim 256 eight warps widen: four take 1400 cycles a stage and the products wait for them.)
+  static constexpr int kWidenGroups = kBf ? 0 : NQ == 1 ? 2 : 1, kWideners = kBf ? 128 : 128 * kWidenGroups;
+  static constexpr int kGroups = NQ + 1 + kWidenGroups;
   static constexpr int kThreads = 128 * kGroups;
   static constexpr int kRegs = kGroups == 2 ? 248 : kGroups == 3 ? 168 : 128;
   static constexpr int kSoftRegs = kGroups == 2 ? 248 : kBf ? 200 : NQ == 1 ? 224 : 192;
-  static constexpr int kMmaRegs = kGroups == 2 ? 248 : kBf ? 104 : NQ == 1 ? 96 : 48;
-  static constexpr int kLoadRegs = kBf ? 0 : NQ == 1 ? 184 : 80;  // (widening warps)
-  static_assert(NQ * kSoftRegs + kMmaRegs + kLoadRegs == kGroups * kRegs, "register shares");
+  static constexpr int kMmaRegs = kGroups == 2 ? 248 : kBf ? 104 : NQ == 1 ? 64 : 48;
+  static constexpr int kLoadRegs = kBf ? 0 : NQ == 1 ? 112 : 80;  // (widening warps)
+  static_assert(NQ * kSoftRegs + kMmaRegs + kWidenGroups * kLoadRegs == kGroups * kRegs, "register shares");
   static_assert(kVTok * kVCols * 2 == kStage, "K and V stages are one size");
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
@@ -435,7 +437,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
 
   if (tid == 0) {
     for (int s = 0; s < P::kStages; ++s) {
-      mbar_init(full + s, P::kBf ? 1 : 128);
+      mbar_init(full + s, P::kBf ? 1 : P::kWideners);
       mbar_init(freeb + s, 1);
     }
     for (int s = 0; s < 2; ++s) {
@@ -449,7 +451,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       for (int s = 0; s < P::kStages; ++s) mbar_init(peer_full + s, 1);
     for (int s = 0; s < P::kRawStages; ++s) {
       mbar_init(raw_full + s, 1);
-      mbar_init(raw_free + s, 128);
+      mbar_init(raw_free + s, P::kWideners);
     }
     *stop = 0;
   }
@@ -545,7 +547,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
   // reference point relative to vref, a power of two at or above every V scale so far (from 2^-60 up).
   auto widen = [&]() {
     const int lt = tid - 32 * P::kWidenWarp;
-    constexpr int kPieces = P::kRawStage / 16 / 128;  // 16-byte pieces of codes per thread and stage
+    constexpr int kPieces = P::kRawStage / 16 / P::kWideners;  // 16-byte pieces of codes per thread and stage
     int k0 = 0, g0 = 0;  // stages and tiles of the pieces before
     do {
     const RowRange& R = pc.R;
@@ -562,7 +564,8 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         next_v = __ldg(A.kv.scale_at(true, pg, head, off));
       }
     };
-    if (n > 0) fetch_scales(0);
+    const bool scales = lt < kTT;  // (a token each)
+    if (scales && n > 0) fetch_scales(0);
     const int total = 2 * n * P::kPer;
     for (int k = 0; k < total && !*stop; ++k) {
       bool value;
@@ -578,7 +581,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       }
       const int j0 = R.tile(t_begin + j) * kTT;
       float* sc = reinterpret_cast<float*>(sm + P::kOffScale) + ((g0 + j) % P::kScaleSlots) * (2 * kTT);
-      if (!value && h == 0) {
+      if (scales && !value && h == 0) {
         // The tile's largest V scale (bits of positive floats in order), by way of this warp's maximum of
         // the 32 tokens it holds: vref only has to be at or above the scales that were seen with it, so each
         // warp keeps one of its own.
@@ -586,7 +589,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         sc[kTT + lt] = next_v;
         const uint32_t mx = __reduce_max_sync(kFullMask, next_v > 0.0f && next_v < INFINITY ? __float_as_uint(next_v) : 0u);
         const float top = __uint_as_float(mx > 0x7e800000u ? 0x7f000000u : (mx + 0x7fffffu) & 0x7f800000u);  // up to a power of two
-        vref = fmaxf(vref, top);
+        if (top > vref) vref = fminf(2.0f * top, 1.7014118346046923e38f);  // (a power of two of room: each move costs a pass over O)
         if (lane == 0) reinterpret_cast<float*>(sm + P::kOffRef)[((g0 + j) % P::kScaleSlots) * 4 + (warp & 3)] = vref;
         if (j + 1 < n) fetch_scales(j + 1);
       }
@@ -601,7 +604,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         constexpr int TOKS = decltype(toks_)::value, INNER = decltype(inner_)::value;
 #pragma unroll
         for (int u = 0; u < kPieces; ++u) {
-          const int id = lt + 128 * u, ch = id % (INNER / 16), rowid = id / (INNER / 16);
+          const int id = lt + P::kWideners * u, ch = id % (INNER / 16), rowid = id / (INNER / 16);
           const int cb = rowid / TOKS, tr = rowid % TOKS;  // column block, token
           const uint4 x = *reinterpret_cast<const uint4*>(src + id * 16);
           uint2 q[4] = {widen_half<FMT>(x.x), widen_half<FMT>(x.y), widen_half<FMT>(x.z), widen_half<FMT>(x.w)};
