@@ -644,41 +644,49 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     const RowRange& R = pc.R;
     const int head = pc.head, n = pc.n;
     // ---- Q: [query tile][64-column block][128 rows][128 bytes], swizzled; rows past the group zero.  Each
-    // warpgroup brings its own tile, sixteen bytes a lane, 8 or 16 loads at a time, while the loaders start.
+    // warpgroup brings its own tile, sixteen bytes a lane, all its loads at once, while the loaders start.  A lane works
+    // out the address of one of the warp's rows for all (an item of 10 tiles spends 6 us here at head_dim 256
+    // where every lane does so for each piece).
     if (n > 0) {
       constexpr int kCh = D / 8, kRowsAt = 128 / kCh;  // pieces of a row; rows a warpgroup covers at once
-      constexpr int kBatch = kCh < 16 ? 8 : 16;
+      constexpr int kPerWarp = 32 / kCh;               // and a warp
       const uint32_t flip = A.scale_log2 < 0.0f ? 0x80008000u : 0u;  // (a negative scale: -q and |scale|)
-      const int qt = tid & 127, ch = qt % kCh;
+      const int ch = lane % kCh;
       unsigned char* tile = sm + s * (D / 64) * 16384 + (ch >> 3) * 16384;
-      for (int i0 = 0; i0 < kCh; i0 += kBatch) {
-        uint4 x[kBatch];
+      const uint4* mine = nullptr;
+      {
+        const int gq = rank * P::kRows + s * 128 + (lane / kPerWarp) * kRowsAt + quad * kPerWarp + lane % kPerWarp;
+        int g;
+        const int t = R.token_of(A, gq, g);
+        if (gq < R.rows) mine = reinterpret_cast<const uint4*>(q_row(A, R, head, t, g));
+      }
+      uint4 x[kCh];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int rr = (i0 + i) * kRowsAt + qt / kCh, gq = rank * P::kRows + s * 128 + rr;
-          x[i] = make_uint4(0u, 0u, 0u, 0u);
-          int g;
-          const int t = R.token_of(A, gq, g);
-          if (gq < R.rows) x[i] = *reinterpret_cast<const uint4*>(q_row(A, R, head, t, g) + ch * 8);
-        }
+      for (int i = 0; i < kCh; ++i) {
+        const uint4* row = reinterpret_cast<const uint4*>(__shfl_sync(kFullMask, reinterpret_cast<uint64_t>(mine), i * kPerWarp + lane / kCh));
+        x[i] = row ? row[ch] : make_uint4(0u, 0u, 0u, 0u);
+      }
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i) {
-          const int rr = (i0 + i) * kRowsAt + qt / kCh;
-          uint32_t w[4] = {x[i].x ^ flip, x[i].y ^ flip, x[i].z ^ flip, x[i].w ^ flip};
-          if constexpr (!P::kBf) {
-            // float16 by a power of two per row (bf16 has fewer mantissa bits: exact except for components
-            // below 2^-17 of the row's largest); the lanes of a row are neighbours
-            uint32_t mx = pair_max(pair_max(w[0], w[1]), pair_max(w[2], w[3]));
+      for (int i = 0; i < kCh; ++i) {
+        const int rr = i * kRowsAt + quad * kPerWarp + lane / kCh;
+        uint32_t w[4] = {x[i].x ^ flip, x[i].y ^ flip, x[i].z ^ flip, x[i].w ^ flip};
+        if constexpr (!P::kBf) {
+          // float16 by a power of two per row (bf16 has fewer mantissa bits: exact except for components
+          // below 2^-17 of the row's largest); the lanes of a row are neighbours
+          uint32_t mx = pair_max(pair_max(w[0], w[1]), pair_max(w[2], w[3]));
+          if constexpr (kCh == 32) {
+            mx = __reduce_max_sync(kFullMask, max(mx & 0xffffu, mx >> 16));
+          } else {
 #pragma unroll
             for (int o = kCh >> 1; o > 0; o >>= 1) mx = __vmaxu2(mx, __shfl_xor_sync(kFullMask, mx, o));
-            float down, up;
-            row_power(max(mx & 0xffffu, mx >> 16), down, up);
-#pragma unroll
-            for (int u = 0; u < 4; ++u) w[u] = half2_of(bf16_lo(w[u]) * down, bf16_hi(w[u]) * down);
-            if (ch == 0) reinterpret_cast<float*>(sm + P::kOffQf)[s * 128 + rr] = up;
           }
-          *reinterpret_cast<uint4*>(tile + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          float down, up;
+          row_power(max(mx & 0xffffu, mx >> 16), down, up);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) w[u] = half2_of(bf16_lo(w[u]) * down, bf16_hi(w[u]) * down);
+          if (ch == 0) reinterpret_cast<float*>(sm + P::kOffQf)[s * 128 + rr] = up;
         }
+        *reinterpret_cast<uint4*>(tile + rr * 128 + (((ch & 7) ^ (rr & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
       }
       fence_async();
       __syncwarp();
@@ -728,9 +736,21 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       }
       const bool whole = j0 + kTT - 1 <= p && (j0 >= lo || j0 + kTT <= R.sink);
       if (!__all_sync(kFullMask, whole)) {
+        // One bound where one is enough: a causal edge, a window's edge past the sinks (6 sequences of windows of
+        // 1024 at head_dim 256: 226 -> 222 us e4m3; not with two query tiles beside an 8-bit cache, whose
+        // softmax has no registers left for it: 735 -> 797 us at head_dim 128).
+        constexpr bool kEdges = P::kBf || NQ == 1;
         const int hi_c = p + 1 - j0, lo_c = lo - j0, sk_c = R.sink - j0;
+        if (kEdges && __all_sync(kFullMask, lo_c <= 0)) {
 #pragma unroll
-        for (int i = 0; i < 128; ++i) x[i] = (i < hi_c && (i >= lo_c || i < sk_c)) ? x[i] : -INFINITY;
+          for (int i = 0; i < 128; ++i) x[i] = i < hi_c ? x[i] : -INFINITY;
+        } else if (kEdges && sk_c <= 0 && __all_sync(kFullMask, hi_c >= kTT)) {
+#pragma unroll
+          for (int i = 0; i < 128; ++i) x[i] = i >= lo_c ? x[i] : -INFINITY;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 128; ++i) x[i] = (i < hi_c && (i >= lo_c || i < sk_c)) ? x[i] : -INFINITY;
+        }
       }
       float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
@@ -925,14 +945,12 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         }
         if (live && ((top & 0xffffu) >= 0x7f80u || (top >> 16) >= 0x7f80u)) A.mend[0] = 1u;  // (attn_mend_kernel)
         __syncwarp();
-        const int base = rank * P::kRows + s * 128 + quad * 32;  // the warp's first row of the group
+        uint4* mine = live ? reinterpret_cast<uint4*>(o_row(A, R, head, tq, hq - head * A.group)) : nullptr;  // (lane = row)
 #pragma unroll
         for (int i = 0; i < kCh; ++i) {
           const int rr = (i * 32 + lane) / kCh, ch = (i * 32 + lane) % kCh;
-          int g;
-          const int t = R.token_of(A, base + rr, g);
-          if (base + rr < R.rows)
-            *reinterpret_cast<uint4*>(o_row(A, R, head, t, g) + ch * 8) = *reinterpret_cast<const uint4*>(st + rr * D * 2 + ((ch ^ (rr & 7)) << 4));
+          uint4* row = reinterpret_cast<uint4*>(__shfl_sync(kFullMask, reinterpret_cast<uint64_t>(mine), rr));
+          if (row) row[ch] = *reinterpret_cast<const uint4*>(st + rr * D * 2 + ((ch ^ (rr & 7)) << 4));
         }
       } else {
 #pragma unroll
