@@ -74,9 +74,9 @@ struct TilePlan {
   static constexpr int kGroups = NQ + 1 + kWidenGroups;
   static constexpr int kThreads = 128 * kGroups;
   static constexpr int kRegs = kGroups == 2 ? 248 : kGroups == 3 ? 168 : 128;
-  static constexpr int kSoftRegs = kGroups == 2 ? 248 : kBf ? 200 : NQ == 1 ? 224 : 192;
-  static constexpr int kMmaRegs = kGroups == 2 ? 248 : kBf ? 104 : NQ == 1 ? 64 : 48;
-  static constexpr int kLoadRegs = kBf ? 0 : NQ == 1 ? 112 : 80;  // (widening warps)
+  static constexpr int kSoftRegs = kGroups == 2 ? 248 : kBf ? 216 : NQ == 1 ? 224 : 200;
+  static constexpr int kMmaRegs = kGroups == 2 ? 248 : kBf ? 72 : NQ == 1 ? 64 : 40;
+  static constexpr int kLoadRegs = kBf ? 0 : NQ == 1 ? 112 : 72;  // (widening warps)
   static_assert(NQ * kSoftRegs + kMmaRegs + kWidenGroups * kLoadRegs == kGroups * kRegs, "register shares");
   static_assert(kVTok * kVCols * 2 == kStage, "K and V stages are one size");
   static_assert(kSmem <= 227 * 1024, "shared memory");
