@@ -736,6 +736,11 @@ cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
   want = want > by_len ? by_len : want;
   int cluster = 1;
   while (cluster < 8 && cluster * 2 <= want) cluster *= 2;
+  // More contexts than blocks at once: two blocks each all the same where a warp still has 32 tiles, since shorter blocks
+  // leave a shorter last round (64 sequences of up to 8192 tokens, 8 heads, ragged: heads of 128 189 -> 185 us bf16, 122 ->
+  // 120 e4m3, of 256 366 -> 354, 222 -> 209; all alike 308 -> 306, 188 -> 180, but 596 -> 601, 326 -> 341; 128 of 2000 tokens
+  // 94 -> 100 us).
+  if (cluster < 2 && tiles >= 2 * kRowsWarps * 32) cluster = 2;
   int64_t splits = want / cluster;
   const int64_t by_ws = static_cast<int64_t>(kAttnWsBytes) / (items * kRows * (D / 4) * 24);
   splits = splits > by_ws ? by_ws : splits;

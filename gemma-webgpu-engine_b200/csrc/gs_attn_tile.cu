@@ -1322,9 +1322,8 @@ cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
 template <int D, int FMT>
 cudaError_t go_cg(const gs_kv_cache* c, const AttnArgs& a, cudaStream_t st) {
   // Two blocks a group at head_dim 256, where one block's 128 rows read K and V faster than L2 gives them
-  // (2048 x 16384 tokens, 16 / 8 heads: bf16 627 -> 483 us, e4m3 871 -> 573 us).  At head_dim 128 a block has
-  // 256 rows of its own, and the round trips between the blocks cost more than the halved reads save
-  // (32 / 8 heads: bf16 485 -> 718 us, e4m3 727 -> 873 us).
+  // (2048 x 16384 tokens, 16 / 8 heads: bf16 627 -> 402 us, e4m3 871 -> 484 us).  At head_dim 128 a block has
+  // 256 rows of its own, and two of them gain nothing (32 / 8 heads: e4m3 665 -> 673 us, int8 704 -> 682 us).
   if constexpr (D == 256) {
     if (static_cast<int64_t>(a.max_q) * a.group > TilePlan<D, FMT, 1>::kRows) return go<D, FMT, 2>(c, a, st);
   }
