@@ -23,6 +23,13 @@
 // distributed shared memory; of several clusters per context the last to finish joins their partial
 // results.
 //
+// Measured (one token a sequence, 32 query heads on 8 of 128): 64 sequences of 8192 tokens bf16 304 us,
+// 7.1 TB/s, e4m3 179 us, 6.2 TB/s, ragged 184 and 119 us; two of 131072 tokens (4 heads) 89 us, 6.0 TB/s;
+// one of 777 tokens (2 heads of 256) 7.5 us: launch, table and query loads, one round of tiles, join.
+// Beside 8-bit codes the widening keeps the issue slots half busy and the ragged last round is the
+// other loss; 20 rows of 256 (16 windows of 1028 tokens, int8, 25 us) take two passes of 16 rows at 1.5 us
+// a tile and warp: bound by the products' latency, not by bytes.
+//
 // 8-bit codes are widened to float16 (exact for e4m3 and int8) in registers, K's scale
 // multiplies the finished score, V's scale the weight: 2^(s - m) · (scale / largest scale so
 // far) · 2^7, at most 2^15, which float16 holds to 11 bits down to 2^-21 of the largest; the factor is

@@ -15,6 +15,13 @@
 // as long as the softmax and the output alone fills half of tensor memory: one query tile, two
 // score buffers.
 //
+// Measured (2048 new tokens over 16384): 32 / 8 heads of 128 bf16 438 us, 1177 TFLOP/s, both the tensor pipe and
+// the 2^x unit 55 % busy (back to back at the 1000 W cap and 1.7 GHz: 508 us, 1014 TFLOP/s; starting the
+// second product at three quarters of P gained nothing: 440 -> 446 us); of 64 378 us; 16 / 8 heads of 256
+// 402 us, 1281 TFLOP/s, bound by what L2 delivers of K and V (6.3 TB/s); e4m3 of 128 665 us, of 256 475 us: widening
+// and softmax share the issue slots and shared memory.  Six ragged chunks of up to 1500 tokens, windows of 1024,
+// heads of 256: e4m3 222 us, bf16 193 us; an item's 11 tiles take 25 of its 38 us, query loads from HBM 4, output 3.
+//
 // Tensor memory (512 columns): S0 at 0, S1 at 128, O0 at 256, O1 at 256 + D.
 // Warps: softmax warpgroup(s) first (warp % 4 = its tensor-memory lanes), then the MMA issuer and the
 // loader (TMA boxes; bf16 pages go straight to the swizzled operand layout), then, beside an 8-bit
@@ -63,8 +70,10 @@ struct TilePlan {
   static constexpr int kOffQf = kOffScale + (kBf ? 0 : kScaleSlots * 2 * kTT * 4);  // [kRows] float
   static constexpr int kOffRef = kOffQf + (kBf ? 0 : kRows * 4);           // [slot][widening warp] float
   static constexpr int kOffBar = kOffRef + (kBf ? 0 : 128);
-  static constexpr int kOffWalk = kOffBar + 512;                           // (bf16) a Walk per warp
-  static constexpr int kSmem = kOffWalk + (kBf ? 1536 : 0) + 1024;         // alignment slack
+  static constexpr int kOffWalk = kOffBar + 512;                           // (balanced) a Walk per warp
+  static constexpr bool kBalance = NQ == 2 && (kBf || D == 64);
+  static constexpr int kWalks = !kBalance ? 0 : kBf ? 1536 : 2304;
+  static constexpr int kSmem = kOffWalk + kWalks + 1024;         // alignment slack
   // Warpgroups: softmax (NQ), then the MMA issuer with the TMA loader beside it, then the widening
   // loaders.  Registers a thread: a row of 128 scores lives in its softmax thread; the shares add
   // up to what the block is launched with.
@@ -122,7 +131,10 @@ __device__ __forceinline__ void commit_to(uint64_t* bar) {
 __device__ __forceinline__ void arrive_on(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
-// Arrival on the first block's barrier (the one that issues the products).
+// Arrival on the first block's barrier (the one that issues the products).  It releases at block scope: what the products
+// read lies in the arriving block's own shared memory, handed to the async proxy by its writers before, or in tensor
+// memory, ordered by the tcgen05 fences.  At cluster scope each arrival waits for all of the thread's memory traffic, 1000
+// clocks a tile (2048 x 16384 tokens, heads of 256: 402 -> 480 us).
 template <int CG>
 __device__ __forceinline__ void arrive_first(uint64_t* bar) {
   if constexpr (CG == 1) {
@@ -421,8 +433,8 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     Cursor c = start;
     if (!next_piece<kGroupRows, BAL>(A, c, only)) return;  // (the whole group)
     if constexpr (BAL) {
-      static_assert(P::kBf && sizeof(Walk) * (P::kThreads / 32 - 2) <= 1536, "a Walk per warp");
-      if (lane == 0 && warp <= P::kLoadWarp) {
+      static_assert(static_cast<int>(sizeof(Walk)) * (P::kThreads / 32 - 2) <= P::kWalks, "a Walk per warp");
+      if (lane == 0 && (warp <= P::kLoadWarp || warp >= P::kWidenWarp)) {
         walk->cursor = c;
         walk->piece = only;
       }
@@ -1281,12 +1293,12 @@ cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
   const int64_t units = static_cast<int64_t>(a.seqs) * blocks;
   a.row_blocks = blocks;
   a.part_o = reinterpret_cast<float*>(c->ws);
-  if constexpr (P::kBf && P::NQ == 2) {
+  if constexpr (P::kBalance) {
     // Balanced: every block takes an equal stretch of all items' tiles.  Against the rounds of a fixed grid
     // this saves the last round's idle blocks and costs a block about one more beginning and end (about 5
     // tiles' time) and the joining of what is cut (as much again): 2048 tokens over 16384 in 1.73 rounds, head_dim
     // 128: 476 -> 446 us, head_dim 64: 419 -> 387 us; 1024-token windows (10 tiles): 70 -> 86 us, so not there.
-    // (Beside 8-bit caches the walk's registers cost more than the rounds: 696 -> 806 us; at head_dim 256 there
+    // (8-bit at head_dim 64: e4m3 553 -> 497 us; at 128 the softmax spills for it, 665 -> 820 us; at head_dim 256 there
     // are half as many groups and it gains nothing: 474 -> 498 us.)
     const int64_t rounds = (items + groups - 1) / groups;
     const bool gains = rounds * groups * (tiles + 5) > items * tiles + (items + 2 * groups) * 5;

