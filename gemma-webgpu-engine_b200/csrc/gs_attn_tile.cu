@@ -516,8 +516,6 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       stage_item<SB>(i, pc.n, value, j);
       for (int h = 0; h < P::kPer; ++h) {
         const int at = issued % kRing, round = issued / kRing;
-        if (round > 0) ok = __all_sync(kFullMask, mbar_wait(ring_free + at, static_cast<uint32_t>((round - 1) & 1), kWaitNs));
-        if (!ok) break;
         const int toks = value ? P::kVTok : P::kKTok;
         const int inner = value ? P::kVInner : P::kKInner;
         const int box = min(1 << shift, toks);  // tokens per box
@@ -527,7 +525,9 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         // lane g: token group g (at most 8); a group past every row's last token stays as it is
         const int tok = j0 + lane * box;
         const bool real = lane < groups && tok < R.hi;
-        const int pg = real ? page_of(pc.b, tok) : 0;
+        const int pg = real ? page_of(pc.b, tok) : 0;  // (on its way while the stage is awaited)
+        if (round > 0) ok = __all_sync(kFullMask, mbar_wait(ring_free + at, static_cast<uint32_t>((round - 1) & 1), kWaitNs));
+        if (!ok) break;
         const unsigned live = __ballot_sync(kFullMask, real);
         const uint32_t bytes = static_cast<uint32_t>(__popc(live) * box * cols * inner);
         if (lane == 0) {
