@@ -80,11 +80,18 @@ __device__ __forceinline__ void square_row(const float (&a)[V], float2& s) {
       s = __ffma2_rn(x, x, s);
     }
 }
-// 448 / a for a >= 2^-64 by the approximate reciprocal (1 ulp; a code differs from the quotient's only
-// where the product lies that near a rounding boundary), which is 0 from 2^126 on: there the quotient.
+// 448 / a for a >= 2^-64 by the approximate reciprocal and one step that takes up its remainder (the
+// reciprocal is 0 from 2^126 on: there the quotient), and a / 448 by the same step.  Without the step each is an
+// ulp off now and then, and a twentieth more codes fall on the other side of a rounding boundary than with the quotients.
 __device__ __forceinline__ float norm_inv(float a) {
   const float f = quant_floor(a);
-  return f < 8.0e37f ? kE4m3Max * __fdividef(1.0f, f) : __fdiv_rn(kE4m3Max, f);
+  if (!(f < 8.0e37f)) return __fdiv_rn(kE4m3Max, f);
+  const float r = __fdividef(1.0f, f), q = kE4m3Max * r;
+  return fmaf(fmaf(-q, f, kE4m3Max), r, q);
+}
+__device__ __forceinline__ float norm_scale(float a) {
+  const float f = quant_floor(a), q = f * (1.0f / kE4m3Max);
+  return f < INFINITY ? fmaf(fmaf(-q, kE4m3Max, f), 1.0f / kE4m3Max, q) : q;
 }
 
 template <int V>
@@ -240,7 +247,7 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(const __grid_constant__ Norm
         if (span > 8) gm[p] = max_nan(gm[p], __shfl_xor_sync(kFullMask, gm[p], 8));
         const int col = (t + p * tpr) * V;
         if (col < A.hidden && live && (lane & (span - 1)) == 0)
-          scales[col >> A.shift] = quant_floor(gm[p]) * (1.0f / kE4m3Max);
+          scales[col >> A.shift] = norm_scale(gm[p]);
       }
     } else {
       int* gr = gmax + threadIdx.y * A.groups;
