@@ -292,7 +292,9 @@ template <bool BF16, int OUT, int V>
 cudaError_t launch_norm_v(const NormArgs& a, cudaStream_t st) {
   const int pieces = (a.hidden + V - 1) / V;
   int tpr = 32;
-  const int want = a.rows <= 296 ? 1 : V == 8 ? 2 : 4;
+  // (one element a piece: blocks of 512 threads overlap better than of 1024: 4118 rows of 3834 f32 117 -> 91 us, 8000 of 1111
+  // 32 -> 29, but 20000 of 333 27 -> 29)
+  const int want = a.rows <= 296 ? 1 : V == 8 ? 2 : pieces > 512 ? 8 : 4;
   while (tpr < 1024 && tpr * want < pieces) tpr <<= 1;
   const int rpb = tpr >= 256 ? 1 : 256 / tpr;
   const int per = (pieces + tpr - 1) / tpr;
