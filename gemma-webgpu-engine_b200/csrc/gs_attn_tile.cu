@@ -442,6 +442,9 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     }
   }
   const Piece& pc = BAL ? walk->piece : only;
+  // (A piece of at most 128 rows leaves the second query tile out: 8 sequences of 4000 tokens, 128 rows of 128: 66 -> 60 us
+  // bf16, 84 -> 69 int8; the counting costs chunks over 8-bit caches with heads of 64 3%.)
+  auto query_tiles = [&]() { return NQ == 2 && pc.R.rows <= 128 ? 1 : NQ; };  // (with rows of the piece)
   auto another = [&]() {  // the next piece, once a warp is done with this one
     if constexpr (BAL) return *stop == 0 && next_piece<kGroupRows>(A, walk, lane);
     else return false;
@@ -651,7 +654,8 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     const int gr = rank * P::kRows + r;  // row of the group
     const uint32_t lane_base = tmem + (static_cast<uint32_t>(quad * 32) << 16);
     const uint32_t o_at = lane_base + 256u + static_cast<uint32_t>(s * D);
-    int g0 = 0;  // tiles of the pieces before
+    uint32_t q_turn = 0;
+    int g0 = 0, gp = 0;  // tiles of the pieces before, and those of them this query tile had a part in
     do {
     const RowRange& R = pc.R;
     const int head = pc.head, n = pc.n;
@@ -704,6 +708,13 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       __syncwarp();
       if (lane == 0) arrive_first<CG>(q_full);
     }
+    q_turn ^= n > 0 ? 1u : 0u;
+    if (s >= query_tiles()) {
+      // No rows of the piece.  (Its barrier has to be through: arrivals of the next piece would count in it.)
+      if (BAL && n > 0 && !__all_sync(kFullMask, mbar_wait(q_full, q_turn ^ 1u, kWaitNs))) give_up();
+      g0 += n;
+      continue;
+    }
     int hq;
     const int tq = R.token_of(A, min(gr, R.rows - 1), hq);
     hq += head * A.group;
@@ -718,7 +729,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     for (int j = 0; j < n && !*stop; ++j) {
       const int gt = g0 + j;  // tile number of this block
       const int buf = NQ == 2 ? s : (gt & 1);
-      const uint32_t ph = static_cast<uint32_t>((gt / SB) & 1);
+      const uint32_t ph = static_cast<uint32_t>(((gp + j) / SB) & 1);
       const uint32_t s_at = lane_base + static_cast<uint32_t>(buf * 128);
       const int j0 = R.tile(pc.t_begin + j) * kTT;
       if (!__all_sync(kFullMask, mbar_wait(s_full + buf, ph, kWaitNs))) {
@@ -849,7 +860,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     float ml = m == -INFINITY ? m : m * c - unit;  // (log2 units)
     bool ok = *stop == 0;
     if (n > 0 && ok) {
-      ok = mbar_wait(o_done + s, static_cast<uint32_t>((g0 + n - 1) & 1), kWaitNs);
+      ok = mbar_wait(o_done + s, static_cast<uint32_t>((gp + n - 1) & 1), kWaitNs);
       if (!ok) give_up();
     }
     ok = __all_sync(kFullMask, ok);
@@ -992,6 +1003,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     }
     fence_before();
     g0 += n;
+    gp += n;
     } while (another());
   } else if (warp < P::kMmaWarp + 4) {
    set_regs<P::kRegs, P::kMmaRegs>();
@@ -1000,6 +1012,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     const bool leader = elected();
     int cnt = 0;  // stages consumed
     int g0 = 0;   // tiles of the pieces before
+    int g1 = 0;   // those of them with a second query tile
     uint32_t q_phase = 0;
     auto stage_ready = [&](int at) {  // this block's half
       return __all_sync(kFullMask, mbar_wait(full + at % P::kStages, static_cast<uint32_t>((at / P::kStages) & 1), kWaitNs));
@@ -1041,7 +1054,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     bool ok = true;
     const bool issues = CG == 1 || rank == 0;
     do {
-    const int n = pc.n;
+    const int n = pc.n, nq = query_tiles();
     if (CG == 2 && rank == 1) {
       // second block: tells the first when a stage of its own is there (and clean)
       for (int i = 0; ok && i < 2 * n && !*stop; ++i) {
@@ -1065,11 +1078,11 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       for (int h = 0; ok && h < P::kPer; ++h) ok = stage_ready(cnt + h) && peer_ready(cnt + h);
       if (!ok) break;
       fence_after();
-      for (int s = 0; s < NQ; ++s) {
+      for (int s = 0; s < nq; ++s) {
         scores(s, NQ == 2 ? s : (g0 + i) & 1, cnt);
         if (leader) {
           commit_to<CG>(s_full + (NQ == 2 ? s : (g0 + i) & 1));
-          if (s == NQ - 1)
+          if (s == nq - 1)
             for (int h = 0; h < P::kPer; ++h) commit_to<CG>(freeb + (cnt + h) % P::kStages);
         }
         __syncwarp();
@@ -1079,7 +1092,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     for (int j = 0; issues && ok && j < n && !*stop; ++j) {
       const int v_at = cnt, k_at = cnt + P::kPer;
       const bool more = j + SB < n;
-      for (int s = 0; ok && s < NQ; ++s) {
+      for (int s = 0; ok && s < nq; ++s) {
         const int buf = NQ == 2 ? s : ((g0 + j) & 1);
         if (s == 0)
           for (int h = 0; ok && h < P::kPer; ++h) {
@@ -1087,7 +1100,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
             if (ok) clean(v_at + h, j, h);
             ok = ok && peer_ready(v_at + h);
           }
-        ok = ok && __all_sync(kFullMask, wait_group<CG>(p_full + buf, static_cast<uint32_t>(((g0 + j) / SB) & 1)));
+        ok = ok && __all_sync(kFullMask, wait_group<CG>(p_full + buf, static_cast<uint32_t>((((s == 0 ? g0 : g1) + j) / SB) & 1)));
         if (!ok) break;
         fence_after();
         if (leader) {
@@ -1100,7 +1113,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
                          kIdescPV<D, P::kBf, CG>, (j | h | k) != 0 ? 1u : 0u);
           }
           commit_to<CG>(o_done + s);
-          if (s == NQ - 1)
+          if (s == nq - 1)
             for (int h = 0; h < P::kPer; ++h) commit_to<CG>(freeb + (v_at + h) % P::kStages);
         }
         __syncwarp();
@@ -1112,7 +1125,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
           scores(s, buf, k_at);
           if (leader) {
             commit_to<CG>(s_full + buf);
-            if (s == NQ - 1)
+            if (s == nq - 1)
               for (int h = 0; h < P::kPer; ++h) commit_to<CG>(freeb + (k_at + h) % P::kStages);
           }
           __syncwarp();
@@ -1121,6 +1134,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       cnt += more ? 2 * P::kPer : P::kPer;
     }
     g0 += n;
+    if (nq == 2) g1 += n;
     } while (ok && another());
     if (!ok) give_up();
     // every product has completed before tensor memory is freed

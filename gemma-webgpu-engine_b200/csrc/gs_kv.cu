@@ -247,8 +247,9 @@ cudaError_t launch_rows(const KvRowsArgs& a, int fmt, bool write, bool bf16, boo
 }
 
 // Rows (new tokens × heads of a group) up to which the few-row kernel is taken (8 sequences of 4000 tokens, 8
-// heads, few rows against many: 64 rows of 128: 50 and 60 us bf16, 59 and 77 us int8, 128 rows: 83 and 66,
-// 102 and 84; 32 rows of 256: 64 and 83 us int8, 64 rows: 110 and 87).
+// heads, few rows against many: 64 rows of 128: 47 and 53 us bf16, 58 and 63 us int8, 128 rows: 83 and 60,
+// 102 and 69; 32 rows of 256: 64 and 83 us int8, 64 rows: 110 and 87; where contexts fill the device the lines cross
+// earlier: 26 sequences of 4000, 55 rows of 128, int8 101 and 90).
 int64_t few_rows(int head_dim) { return head_dim == 256 ? 32 : 64; }
 
 gs_status kfail(gs_kv_cache* c, gs_status s, const char* m) {
@@ -416,6 +417,7 @@ gs_status gs_attention(gs_kv_cache* c, const gs_attention_args* p, void* stream)
   if (p->seqs == 0 || p->tokens == 0) return GS_OK;
   if (!p->q || !p->out || !p->kv_len || !p->page_table)
     return kfail(c, GS_EINVAL, "q, out, kv_len and page_table are required");
+  if (p->q == p->out) return kfail(c, GS_EINVAL, "out must not be q");
   if (!p->q_start && p->tokens != p->seqs) return kfail(c, GS_EINVAL, "without q_start every sequence has one token");
   if (p->q_heads < 1 || p->q_heads > (1 << 20) || p->q_heads % c->d.kv_heads != 0)
     return kfail(c, GS_EINVAL, "q_heads must be a multiple of the cache's kv_heads");

@@ -411,7 +411,7 @@ gs_status gs_kv_read(gs_kv_cache* c, const gs_kv_rows* rows, void* stream);
  * events between streams), as for gs_sample. */
 typedef struct gs_attention_args {
   const void* q;            /* device bf16 [tokens][q_heads][head_dim] by the strides below */
-  void* out;                /* device bf16, same shape */
+  void* out;                /* device bf16, same shape; must not overlap q */
   float* lse;               /* device [tokens][q_heads], or NULL */
   const int32_t* q_start;   /* device [seqs + 1], or NULL (tokens == seqs, one each) */
   const int32_t* kv_len;    /* device [seqs] */

@@ -251,7 +251,8 @@ def test_many_rows_repeated(pkg, sampler, form, dim, lens, heads, window):
 
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("lens,heads,group", [([(700, 3000), (1, 1), (0, 5), (40, 0), (300, 1200)], 16, 4),
-                                              ([(64, 2500)] * 9 + [(3, 2)], 16, 8), ([(512, 2049)], 20, 4)])
+                                              ([(64, 2500)] * 9 + [(3, 2)], 16, 8), ([(512, 2049)], 20, 4),
+                                              ([(64, 2500), (20, 2400)] * 5, 16, 4)])
 @pytest.mark.parametrize("form", FORMS)
 def test_balanced_over_items(pkg, sampler, dim, lens, heads, group, form):
     """More items than SMs: the blocks' stretches begin and end inside items, which are then joined."""
@@ -326,6 +327,12 @@ def test_balanced_join_has_one_order(pkg, sampler, dim, form):
     for _ in range(20):
         again, lse2 = c.run()
         assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+def test_result_in_place_of_the_query_is_refused(pkg, sampler):
+    c = Case(sampler, pkg, [(1, 30)], 2, 2, 64, 16, "bf16")
+    with pytest.raises(ValueError, match="out must not be q"):
+        c.run(out=c.q)
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.11, 2.0 ** -40])
