@@ -1312,7 +1312,7 @@ cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
     // this saves the last round's idle blocks and costs a block about one more beginning and end (about 5
     // tiles' time) and the joining of what is cut (as much again): 2048 tokens over 16384 in 1.73 rounds, head_dim
     // 128: 476 -> 446 us, head_dim 64: 419 -> 387 us; 1024-token windows (10 tiles): 70 -> 86 us, so not there.
-    // (8-bit at head_dim 64: e4m3 553 -> 497 us; at 128 the softmax spills for it, 665 -> 820 us; at head_dim 256 there
+    // (8-bit at head_dim 64: e4m3 553 -> 512 us; at 128 the softmax spills for it, 665 -> 820 us; at head_dim 256 there
     // are half as many groups and it gains nothing: 474 -> 498 us.)
     const int64_t rounds = (items + groups - 1) / groups;
     const bool gains = rounds * groups * (tiles + 5) > items * tiles + (items + 2 * groups) * 5;
