@@ -331,6 +331,14 @@ __device__ __forceinline__ bool next_piece(const AttnArgs& A, Walk* walk, int la
   return got;
 }
 
+// Row of its query tile that warp `quad` brings as its i-th of 32: a few neighbouring rows at a time (as many as the
+// 32 lanes hold 16-byte pieces of), the four warps in turn.
+template <int D>
+__device__ __forceinline__ constexpr int q_slot(int quad, int i) {
+  constexpr int kPerWarp = 256 / D;
+  return i / kPerWarp * (4 * kPerWarp) + quad * kPerWarp + i % kPerWarp;
+}
+
 // Item i of the stage order of n tiles: K(0) .. K(SB - 1), then V(j), K(j + SB) in turn.
 template <int SB>
 __device__ __forceinline__ void stage_item(int i, int n, bool& value, int& j) {
@@ -664,14 +672,14 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     // out the address of one of the warp's rows for all (an item of 10 tiles spends 6 us here at head_dim 256
     // where every lane does so for each piece).
     if (n > 0) {
-      constexpr int kCh = D / 8, kRowsAt = 128 / kCh;  // pieces of a row; rows a warpgroup covers at once
-      constexpr int kPerWarp = 32 / kCh;               // and a warp
+      constexpr int kCh = D / 8;          // pieces of a row
+      constexpr int kPerWarp = 32 / kCh;  // rows a warp covers at once
       const uint32_t flip = A.scale_log2 < 0.0f ? 0x80008000u : 0u;  // (a negative scale: -q and |scale|)
       const int ch = lane % kCh;
       unsigned char* tile = sm + s * (D / 64) * 16384 + (ch >> 3) * 16384;
       const uint4* mine = nullptr;
       {
-        const int gq = rank * P::kRows + s * 128 + (lane / kPerWarp) * kRowsAt + quad * kPerWarp + lane % kPerWarp;
+        const int gq = rank * P::kRows + s * 128 + q_slot<D>(quad, lane);
         int g;
         const int t = R.token_of(A, gq, g);
         if (gq < R.rows) mine = reinterpret_cast<const uint4*>(q_row(A, R, head, t, g));
@@ -684,7 +692,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       }
 #pragma unroll
       for (int i = 0; i < kCh; ++i) {
-        const int rr = i * kRowsAt + quad * kPerWarp + lane / kCh;
+        const int rr = q_slot<D>(quad, i * kPerWarp + lane / kCh);
         uint32_t w[4] = {x[i].x ^ flip, x[i].y ^ flip, x[i].z ^ flip, x[i].w ^ flip};
         if constexpr (!P::kBf) {
           // float16 by a power of two per row (bf16 has fewer mantissa bits: exact except for components
@@ -944,9 +952,10 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       const int64_t part = static_cast<int64_t>(pc.part) * kGroupRows + gr;
       if (finish) {
         // by way of shared memory (the query tile's, which no product reads any more): whole rows leave in
-        // 16-byte pieces of neighbouring lanes
+        // 16-byte pieces of neighbouring lanes.  A warp stages its 32 rows where it brings its 32 rows of the next
+        // item's Q (q_slot), and no other warp of the tile writes there: the four are not ordered between one item and the next.
         constexpr int kCh = D / 8;
-        unsigned char* st = sm + s * (D / 64) * 16384 + quad * 32 * D * 2;
+        unsigned char* st = sm + s * (D / 64) * 16384;
         uint32_t top = 0u;  // largest magnitudes, as patterns
 #pragma unroll
         for (int q = 0; q < D / 32; ++q) {
@@ -963,7 +972,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
             const uint4 w = make_uint4(bf16x2(o[8 * i] * inv, o[8 * i + 1] * inv), bf16x2(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
                                        bf16x2(o[8 * i + 4] * inv, o[8 * i + 5] * inv), bf16x2(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
             top = __vmaxu2(top, __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
-            *reinterpret_cast<uint4*>(st + lane * D * 2 + (((4 * q + i) ^ (lane & 7)) << 4)) = w;
+            *reinterpret_cast<uint4*>(st + q_slot<D>(quad, lane) * 128 + ((4 * q + i) >> 3) * 16384 + ((((4 * q + i) ^ lane) & 7) << 4)) = w;
           }
         }
         if (live && ((top & 0xffffu) >= 0x7f80u || (top >> 16) >= 0x7f80u)) A.mend[0] = 1u;  // (attn_mend_kernel)
@@ -973,7 +982,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         for (int i = 0; i < kCh; ++i) {
           const int rr = (i * 32 + lane) / kCh, ch = (i * 32 + lane) % kCh;
           uint4* row = reinterpret_cast<uint4*>(__shfl_sync(kFullMask, reinterpret_cast<uint64_t>(mine), rr));
-          if (row) row[ch] = *reinterpret_cast<const uint4*>(st + rr * D * 2 + ((ch ^ (rr & 7)) << 4));
+          if (row) row[ch] = *reinterpret_cast<const uint4*>(st + q_slot<D>(quad, rr) * 128 + (ch >> 3) * 16384 + (((ch ^ rr) & 7) << 4));
         }
       } else {
 #pragma unroll

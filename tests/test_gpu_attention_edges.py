@@ -1,0 +1,43 @@
+"""GpuKvCache.attend where its masks, pools and lengths are unusual: signs of the scales, pages that are gone, values
+that are not finite, contexts of few tiles, offsets out of order."""
+import pytest
+import torch
+
+import operator_refs as R
+from test_gpu_attention import FORMS, Case
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("lens,heads,group", [([(64, 2500)] * 9 + [(3, 2)], 16, 8), ([(20, 1500)] * 40, 8, 4)])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form", FORMS)
+def test_shared_items_beside_another_context(pkg, sampler, form, dim, lens, heads, group):
+    """Blocks that walk several items, started late and at odd times because another context's calls hold
+    their SMs: a block's warps leave an item far apart, and none may touch what another still needs of it."""
+    c = Case(sampler, pkg, lens, heads, group, dim, 64, form, seed=dim)
+    want, want_lse = c.run()
+    assert torch.equal(c.run()[0], want)
+    other = pkg.GpuSampler(0)
+    beside = Case(other, pkg, [(30, 700), (1, 900), (90, 500)], 8, 4, dim, 32, form, seed=1)
+    side = torch.cuda.Stream()
+    outs = []
+    for i in range(30):
+        with torch.cuda.stream(side):
+            for _ in range(1 + i % 3):
+                beside.cache.attend(beside.q, beside.q_start, beside.kv_len, beside.table, max_q=beside.max_q,
+                                    max_kv=beside.max_kv, scale=beside.scale)
+        outs.append(c.cache.attend(c.q, c.q_start, c.kv_len, c.table, max_q=c.max_q, max_kv=c.max_kv, scale=c.scale, lse=True))
+    torch.cuda.synchronize()
+    c.cache.check()
+    beside.cache.check()
+    for out, lse in outs:
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    tokens = list(range(0, c.q.shape[0], 97))
+    seq = [next(b for b in range(len(lens)) if t < c.starts[b + 1]) for t in tokens]
+    ref = [R.attend(c.q[t:t + 1], [0, 1], [lens[b][1] - lens[b][0] + t - c.starts[b] + 1], c.table[b:b + 1], c.kd, c.vd,
+                    c.page, c.scale, 0, 0) for t, b in zip(tokens, seq) if lens[b][1] >= lens[b][0]]
+    keep = [t for t, b in zip(tokens, seq) if lens[b][1] >= lens[b][0]]
+    R.check_attend(want[keep], want_lse[keep], [torch.cat(x) for x in zip(*ref)])
+    beside.cache.close()
+    other.close()
