@@ -413,8 +413,11 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     __syncthreads();
     const int per_head = sums[A.units];
     start.total = static_cast<int64_t>(per_head) * A.kv.kv_heads;
+    // (The host chose the path by the bounds max_q and max_kv.  Of fewer tiles than groups each goes to one group and the
+    // groups past them have nothing: a group in between without a tile would be counted among an item's pieces.)
+    start.groups = static_cast<int>(min(static_cast<int64_t>(start.groups), max(start.total, static_cast<int64_t>(1))));
     start.x = start.me * start.total / start.groups;
-    start.x1 = (start.me + 1) * start.total / start.groups;
+    start.x1 = start.me < start.groups ? (start.me + 1) * start.total / start.groups : start.x;
     int at = 0;
     start.head = 0;
     start.off = 0;

@@ -41,3 +41,34 @@ def test_shared_items_beside_another_context(pkg, sampler, form, dim, lens, head
     R.check_attend(want[keep], want_lse[keep], [torch.cat(x) for x in zip(*ref)])
     beside.cache.close()
     other.close()
+
+
+@pytest.mark.parametrize("lens,heads,group,bound", [([(20, 2500)] + [(20, 100)] * 79, 1, 4, 0),
+                                                    ([(20, 100), (17, 250), (20, 30), (5, 5), (20, 200)], 16, 4, 16384),
+                                                    ([(20, 0)] * 6, 16, 4, 16384)])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form", FORMS)
+def test_fewer_tiles_than_blocks(pkg, sampler, form, dim, lens, heads, group, bound):
+    """Many items of few tokens, by their lengths or under a max_kv far above them, on the path that divides all
+    items' tiles over the SMs: every row is written, and the counters of the context's workspace are zero again."""
+    c = Case(sampler, pkg, lens, heads, group, dim, 64, form, seed=dim, poison=float("nan"))
+    if bound:
+        c.table = torch.nn.functional.pad(c.table, (0, bound // 64 - c.table.shape[1]), value=-1)
+        c.max_kv = bound
+    out = torch.full_like(c.q, 7.0)
+    c.check(out=out)
+    again, _ = c.run()
+    assert torch.equal(out, again)
+    # contexts cut into pieces right after, in both kernels
+    Case(sampler, pkg, [(1, 9000)], 1, 2, dim, 64, form, poison=float("nan")).check()
+    c.check()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_tokens_of_no_sequence_stay_as_they_are(pkg, sampler, dim):
+    c = Case(sampler, pkg, [(20, 100)] * 5, 16, 4, dim, 64, "bf16")
+    c.table = torch.nn.functional.pad(c.table, (0, 254), value=-1)
+    c.q_start.zero_()
+    out = torch.full_like(c.q, 7.0)
+    c.run(out=out, max_kv=16384)
+    assert (out == 7).all()
