@@ -31,7 +31,7 @@
 // a tile and warp: bound by the products' latency, not by bytes.
 //
 // 8-bit codes are widened to float16 (exact for e4m3 and int8) in registers, K's scale
-// multiplies the finished score, V's scale the weight: 2^(s - m) · (scale / largest scale so
+// multiplies the finished score, V's scale the weight: 2^(s - m) · (scale / largest magnitude of one so
 // far) · 2^7, at most 2^15, which float16 holds to 11 bits down to 2^-21 of the largest; the factor is
 // taken out of O at the end.  q is brought into float16's range by a power of two per row
 // (bfloat16 has fewer mantissa bits: exact except for components below 2^-17 of the row's
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
 #pragma unroll
       for (int u = 0; u < 4; ++u) o[nb][k][u] = 0.0f;
   }
-  float vref = 0.0f, vinv = 0.0f;  // (8-bit) largest V scale so far, kPScale over it
+  float vref = 0.0f, vinv = 0.0f;  // (8-bit) largest V scale's magnitude so far, kPScale over it
 
   int slot = 0;  // of the next stage
   uint32_t phase = 0;
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
         if (wrote) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (before the stage's next copy)
         __syncwarp();
       }
-      bool move = !kBf && fmaxf(vsc[0], vsc[1]) > vref;
+      bool move = !kBf && fmaxf(fabsf(vsc[0]), fabsf(vsc[1])) > vref;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
@@ -466,7 +466,7 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
         // new references: every row's largest score so far, the largest V scale so far
         float vfac = 1.0f;
         if constexpr (!kBf) {
-          float vm = fmaxf(vref, fmaxf(vsc[0], vsc[1]));
+          float vm = fmaxf(vref, fmaxf(fabsf(vsc[0]), fabsf(vsc[1])));
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) vm = fmaxf(vm, __shfl_xor_sync(kFullMask, vm, d));
           vfac = vm > vref ? vref / vm : 1.0f;

@@ -570,7 +570,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
 
   // ---------------- widening warps (8-bit): codes -> float16 operands ----------------
   // The softmax multiplies V's scales into its weights; so that float16 holds the products, it takes its
-  // reference point relative to vref, a power of two at or above every V scale so far (from 2^-60 up).
+  // reference point relative to vref, a power of two at or above every V scale's magnitude so far (from 2^-60 up).
   auto widen = [&]() {
     const int lt = tid - 32 * P::kWidenWarp;
     constexpr int kPieces = P::kRawStage / 16 / P::kWideners;  // 16-byte pieces of codes per thread and stage
@@ -608,12 +608,13 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       const int j0 = R.tile(t_begin + j) * kTT;
       float* sc = reinterpret_cast<float*>(sm + P::kOffScale) + ((g0 + j) % P::kScaleSlots) * (2 * kTT);
       if (scales && !value && h == 0) {
-        // The tile's largest V scale (bits of positive floats in order), by way of this warp's maximum of
+        // The tile's largest magnitude of a V scale (bits of positive floats in order), by way of this warp's maximum of
         // the 32 tokens it holds: vref only has to be at or above the scales that were seen with it, so each
         // warp keeps one of its own.
         sc[lt] = next_k;
         sc[kTT + lt] = next_v;
-        const uint32_t mx = __reduce_max_sync(kFullMask, next_v > 0.0f && next_v < INFINITY ? __float_as_uint(next_v) : 0u);
+        const uint32_t mag = __float_as_uint(next_v) & 0x7fffffffu;
+        const uint32_t mx = __reduce_max_sync(kFullMask, mag < 0x7f800000u ? mag : 0u);
         const float top = __uint_as_float(mx > 0x7e800000u ? 0x7f000000u : (mx + 0x7fffffu) & 0x7f800000u);  // up to a power of two
         if (top > vref) vref = fminf(2.0f * top, 1.7014118346046923e38f);  // (a power of two of room: each move costs a pass over O)
         if (lane == 0) reinterpret_cast<float*>(sm + P::kOffRef)[((g0 + j) % P::kScaleSlots) * 4 + (warp & 3)] = vref;

@@ -341,8 +341,9 @@ gs_status gs_rms_norm(gs_ctx* ctx, const gs_rms_norm_args* args, void* stream);
  * (No entry of its own in the reference's sampling path: this is the state of the decode
  * step whose logits are sampled.)  The caller owns the memory: `pages` pages of page_size
  * tokens, each [kv_heads][page_size][head_dim] by default (any strides whose rows of
- * head_dim are contiguous and 16-byte aligned), and for 8-bit formats one float32 scale
- * per page, head and token, contiguous [pages][kv_heads][page_size], 16-byte aligned.
+ * head_dim are contiguous and 16-byte aligned), and for 8-bit formats one float32 scale (of any
+ * sign; a value is code · scale) per page, head and token, contiguous [pages][kv_heads][page_size],
+ * 16-byte aligned.
  * A slot is page · page_size + offset.  Strides are below 2^35 elements; destroy the handle
  * before its context. */
 typedef struct gs_kv_cache_desc {

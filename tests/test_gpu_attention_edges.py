@@ -72,3 +72,23 @@ def test_tokens_of_no_sequence_stay_as_they_are(pkg, sampler, dim):
     out = torch.full_like(c.q, 7.0)
     c.run(out=out, max_kv=16384)
     assert (out == 7).all()
+
+
+FEW, MANY = [(1, 300), (2, 130), (1, 17)], [(70, 300), (40, 130), (1, 17)]
+
+
+@pytest.mark.parametrize("lens", [FEW, MANY])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("form", ["e4m3", "int8"])
+@pytest.mark.parametrize("signs", ["negative", "mixed"])
+def test_cache_scales_of_any_sign(pkg, sampler, form, dim, lens, signs):
+    """The pools are the caller's: a value is code times scale, whatever the scale's sign."""
+    c = Case(sampler, pkg, lens, 2, 3, dim, 16, form, seed=dim)
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    for pool, scale, name in ((c.cache.k, c.cache.k_scale, "kd"), (c.cache.v, c.cache.v_scale, "vd")):
+        if signs == "negative":
+            scale.neg_()
+        else:
+            scale.mul_(torch.randint(0, 2, scale.shape, generator=gen, device="cuda").float() * 2 - 1)
+        setattr(c, name, R.pool_values(pool, scale))
+    c.check()
