@@ -94,6 +94,9 @@ __device__ __forceinline__ float norm_scale(float a) {
   return f < INFINITY ? fmaf(fmaf(-q, kE4m3Max, f), 1.0f / kE4m3Max, q) : q;
 }
 
+// x within [lo, hi]; a NaN stays one (fminf and fmaxf alone would make it a code like any other).
+__device__ __forceinline__ float clamp_nan(float x, float lo, float hi) { return x != x ? x : fminf(fmaxf(x, lo), hi); }
+
 template <int V>
 __device__ __forceinline__ void load_weight(const NormArgs& A, int col, float (&w)[V]) {
   if (!A.weight) {
@@ -121,7 +124,6 @@ __device__ __forceinline__ float warp_max_bits(float v) {
 template <bool BF16, int OUT, int V, int PIECES, int MAXT>
 __global__ void __launch_bounds__(MAXT) norm_kernel(const __grid_constant__ NormArgs A) {
   __shared__ float red[32];
-  __shared__ int redi[32];
   __shared__ float red2[32];
   extern __shared__ int gmax[];  // V = 1, several groups: [blockDim.y][groups] bits of max|y|
   const int t = threadIdx.x, tpr = blockDim.x, warps = tpr >> 5;
@@ -189,7 +191,8 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(const __grid_constant__ Norm
       }
     }
   } else if constexpr (OUT == kOutSrq) {
-    int qs = 0;
+    // (The sum of codes in float32: at most 2^15 codes of at most 2^7, exact in any order, and a NaN stays one.)
+    float qs = 0.0f;
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
       const int col = (t + p * tpr) * V;
@@ -197,20 +200,20 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(const __grid_constant__ Norm
         float o[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float q = fminf(fmaxf(rintf(__fdiv_rn(h[p][i], A.srq_scale)), -128.0f), 127.0f);
-          qs += static_cast<int>(q);
+          const float q = clamp_nan(rintf(__fdiv_rn(h[p][i], A.srq_scale)), -128.0f, 127.0f);
+          qs += q;
           o[i] = __fmul_rn(q, A.srq_scale);
         }
         store_row<V, false>(static_cast<float*>(A.out) + row * A.ld_out + col, o);
       }
     }
-    qs = warp_sum_i(qs);
+    qs = warp_sum_f(qs);
     if (warps > 1) {
-      if (lane == 0) redi[wid] = qs;
+      if (lane == 0) red2[wid] = qs;
       __syncthreads();
-      qs = warp_sum_i(lane < warps ? redi[threadIdx.y * warps + lane] : 0);
+      qs = warp_sum_f(lane < warps ? red2[threadIdx.y * warps + lane] : 0.0f);
     }
-    if (t == 0 && live && A.row_sum) A.row_sum[row] = __fmul_rn(static_cast<float>(qs), A.srq_scale);
+    if (t == 0 && live && A.row_sum) A.row_sum[row] = __fmul_rn(qs, A.srq_scale);
   } else {
     unsigned char* out = static_cast<unsigned char*>(A.out) + row * A.ld_out;
     float* scales = A.out_scale + row * A.groups;

@@ -316,7 +316,8 @@ gs_status gs_lm_head_set_route(gs_lm_head* h, int32_t route);
  *                 over each group of `group` columns (0: the whole row; the last group of
  *                 a row may be short).  out_scale is [rows][ceil(hidden / group)].
  * A NaN or infinity in a row makes that row's mean, and so its y, NaN (or 0 where h is
- * finite and the mean infinite), as the formula does; its scales follow. */
+ * finite and the mean infinite), as the formula does; its scales follow.  On the srq grid a NaN y
+ * stays a NaN, and so does its row's row_sum, which is a term of each of the row's logits. */
 typedef struct gs_rms_norm_args {
   const void* x;            /* device [rows][ld_x] of `dtype` */
   const void* residual;     /* device [rows][ld_residual] of `dtype`, or NULL (h = x) */
