@@ -536,9 +536,11 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         const int groups = toks / box;
         const int cols = (value ? P::kVCols : P::kKCols) * P::kEl / inner;
         const int j0 = R.tile(pc.t_begin + j) * kTT + (value ? h * P::kVTok : rank * P::kKTok);
-        // lane g: token group g (at most 8); a group past every row's last token stays as it is
+        // lane g: token group g (at most 8), of one page.  A group that no row sees a token of stays as it is, and so does its table
+        // entry: past the last position, or behind the window, where a server may have freed the page.  (K's scores there
+        // are masked, V's rows set to zero.)
         const int tok = j0 + lane * box;
-        const bool real = lane < groups && tok < R.hi;
+        const bool real = lane < groups && tok < R.hi && (tok + box > R.lo || tok < R.sink);
         const int pg = real ? page_of(pc.b, tok) : 0;  // (on its way while the stage is awaited)
         if (round > 0) ok = __all_sync(kFullMask, mbar_wait(ring_free + at, static_cast<uint32_t>((round - 1) & 1), kWaitNs));
         if (!ok) break;

@@ -92,3 +92,37 @@ def test_cache_scales_of_any_sign(pkg, sampler, form, dim, lens, signs):
             scale.mul_(torch.randint(0, 2, scale.shape, generator=gen, device="cuda").float() * 2 - 1)
         setattr(c, name, R.pool_values(pool, scale))
     c.check()
+
+
+def free_hidden_pages(c):
+    """-1 in the table for every page of which no row of the sequence sees a token; how many there are."""
+    gone = 0
+    for b, (nq, n) in enumerate(c.lens):
+        lo = max(0, n - nq - c.window + 1)
+        for i in range(-(-n // c.page)):
+            if not any(j >= lo or j < c.sinks for j in range(i * c.page, min((i + 1) * c.page, n))):
+                c.table[b, i] = -1
+                gone += 1
+    return gone
+
+
+@pytest.mark.parametrize("lens", [[(1, 700), (3, 500)], [(40, 900), (90, 700)]])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("form", FORMS)
+def test_pages_behind_the_window_may_be_gone(pkg, sampler, form, page, dim, lens):
+    """A server frees what no token can see any more: neither kernel looks there."""
+    c = Case(sampler, pkg, lens, 2, 3, dim, page, form, seed=dim, poison=float("nan"), window=100, sinks=4)
+    want, want_lse = c.run()
+    assert free_hidden_pages(c) > 0
+    out, lse = c.check()
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("form,dim", [("bf16", 64), ("bf16", 128), ("e4m3", 64)])
+def test_pages_behind_the_window_may_be_gone_from_shared_items(pkg, sampler, form, dim):
+    c = Case(sampler, pkg, [(40, 2500), (30, 1900)] * 5, 16, 4, dim, 16, form, seed=dim, poison=float("nan"), window=1700, sinks=4)
+    want, want_lse = c.run()
+    assert free_hidden_pages(c) > 0
+    out, lse = c.run()
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
