@@ -73,7 +73,7 @@ struct AttnArgs {
   int32_t row_blocks;   // (many-row kernel) blocks of query rows per sequence and head
   int32_t units;        // (many-row kernel, balanced) sequences times row blocks
   unsigned* tickets;    // finished parts of a context, per warp that holds the same rows of each; zero between calls
-  unsigned* mend;       // (many-row kernel) whether a result is not finite; blocks that have mended theirs
+  unsigned* mend;       // (many-row kernel) whether values were left out of a product; blocks that have seen to it
   float* part_o;        // partial results: outputs
   float* part_ml;       // and running maxima (log2 units) and sums
   int32_t* flag;
@@ -101,6 +101,10 @@ struct RowRange {
     return t0 + t;
   }
   __device__ __forceinline__ bool seen_by_any(int j) const { return j < hi && (j >= lo || j < sink); }
+  // Whether every row sees the tokens j .. j + n - 1.
+  __device__ __forceinline__ bool seen_by_all(const AttnArgs& A, int j, int n = 1) const {
+    return j + n - 1 <= p0 + t0 && (!A.window || j > hi - 1 - A.window || j + n <= sink);
+  }
 };
 
 __device__ __forceinline__ const __nv_bfloat16* q_row(const AttnArgs& A, const RowRange& R, int head, int t, int g) {
@@ -166,67 +170,25 @@ inline int64_t most_tiles(const AttnArgs& a, int tile, int rows_per_block) {
 
 __device__ __forceinline__ float ex2(float x) { return ex2_approx(x); }
 
-__device__ __forceinline__ bool finite4(float4 x) {
-  return fabsf(x.x) < INFINITY && fabsf(x.y) < INFINITY && fabsf(x.z) < INFINITY && fabsf(x.w) < INFINITY;
-}
-
-// Values d .. d + 3 of one row's result by the formula, token by token over what the row sees, in float32 by one
-// thread: (O, not yet divided by the sum) and (m in log2 units, sum).  The kernels' second product runs over whole tiles, where a
-// hidden token's weight is 0; when its value is an infinity or a NaN, 0 times that is a NaN in rows that never see
-// the token.  So a result that is not finite is computed again here, which the sums of finite values never pay for.
+// Values that are not finite.  The kernels' second product runs over whole tiles, where a token hidden from a row has the weight
+// 0 in it, and 0 times an infinity is a NaN.  Tokens that no row of a block sees are zeroed before the product.  Of tokens that
+// some rows see and others do not (at the causal edge and at the window's, as many as a block has new tokens) the elements
+// that are not finite are zeroed, and added to the rows that do see them apart from the product.  (Beside an 8-bit cache a scale that is not
+// finite counts for all of its row.)  Tokens that all rows see go through the product as they are.
+//
+// The elements of a word of a cached row that are not finite, all bits of each.
 template <int FMT>
-__device__ __noinline__ void attn_by_row(const AttnArgs& A, int b, int head, const __nv_bfloat16* q, int pos, int head_dim, int d, float4* o,
-                                         float2* ml) {
-  constexpr int kEl = FMT == GS_DTYPE_BF16 ? 2 : 1;
-  const int32_t* table = A.table + b * A.table_stride;
-  const int lo = A.window ? max(pos - A.window + 1, 0) : 0, mask = (1 << A.kv.page_shift) - 1;
-  auto four = [](const unsigned char* p) {
-    if constexpr (FMT == GS_DTYPE_BF16) {
-      const uint2 w = *reinterpret_cast<const uint2*>(p);
-      return make_float4(bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y));
-    } else {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
-      if constexpr (FMT == GS_DTYPE_E4M3) {
-        const float2 x = half2_float2(e4m3x2_half2(w & 0xffffu)), y = half2_float2(e4m3x2_half2(w >> 16));
-        return make_float4(x.x, x.y, y.x, y.y);
-      } else {
-        return make_float4(static_cast<float>(static_cast<signed char>(w)), static_cast<float>(static_cast<signed char>(w >> 8)),
-                           static_cast<float>(static_cast<signed char>(w >> 16)), static_cast<float>(static_cast<signed char>(w >> 24)));
-      }
-    }
-  };
-  float M = -INFINITY, L = 0.0f;
-  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (int j = A.sinks > 0 ? 0 : lo; j <= pos; ++j) {
-    if (j >= A.sinks && j < lo) j = lo;
-    const int col = j >> A.kv.page_shift, off = j & mask;
-    int page = col < A.table_cols ? __ldg(table + col) : 0;
-    if (page < 0 || page >= A.kv.pages) page = 0;  // (noted by the kernel that came here)
-    const unsigned char* k = A.kv.at(false, page, head, off);
-    float s = 0.0f;
-    for (int i = 0; i < head_dim; i += 4) {
-      const float4 x = four(k + i * kEl);
-      const uint2 w = *reinterpret_cast<const uint2*>(q + i);
-      s += bf16_lo(w.x) * x.x, s += bf16_hi(w.x) * x.y, s += bf16_lo(w.y) * x.z, s += bf16_hi(w.y) * x.w;
-    }
-    s *= A.scale_log2;
-    float vs = 1.0f;
-    if constexpr (FMT != GS_DTYPE_BF16) {
-      s *= *A.kv.scale_at(false, page, head, off);
-      vs = *A.kv.scale_at(true, page, head, off);
-    }
-    const float mx = max_nan(M, s), at = mx == -INFINITY ? 0.0f : mx, back = ex2(M - at), p = ex2(s - at);
-    const float4 x = four(A.kv.at(true, page, head, off) + d * kEl);
-    M = mx;
-    L = L * back + p;
-    acc.x = acc.x * back + p * (x.x * vs), acc.y = acc.y * back + p * (x.y * vs);
-    acc.z = acc.z * back + p * (x.z * vs), acc.w = acc.w * back + p * (x.w * vs);
-    if (L != L) break;  // (a score that is no number: all of the row is none)
-  }
-  if (L != L) acc = make_float4(L, L, L, L);
-  *o = acc;
-  *ml = make_float2(M, L);
+__device__ __forceinline__ uint32_t not_finite_in(uint32_t w) {
+  if constexpr (FMT == GS_DTYPE_BF16) return __vcmpeq2(w & 0x7f807f80u, 0x7f807f80u);
+  else if constexpr (FMT == GS_DTYPE_E4M3) return __vcmpeq4(w & 0x7f7f7f7fu, 0x7f7f7f7fu);
+  else return 0u;
 }
+template <int FMT>
+__device__ __forceinline__ uint4 not_finite_in(uint4 w) {
+  return make_uint4(not_finite_in<FMT>(w.x), not_finite_in<FMT>(w.y), not_finite_in<FMT>(w.z), not_finite_in<FMT>(w.w));
+}
+__device__ __forceinline__ bool any4(uint4 m) { return (m.x | m.y | m.z | m.w) != 0u; }
+__device__ __forceinline__ uint4 without4(uint4 w, uint4 m) { return make_uint4(w.x & ~m.x, w.y & ~m.y, w.z & ~m.z, w.w & ~m.w); }
 
 // Few-row kernel (mma.sync, one 16-token tile per warp): any number of rows in blocks.
 cudaError_t launch_attn_rows(const gs_kv_cache* c, AttnArgs a, cudaStream_t st);

@@ -17,7 +17,8 @@
 // ldmatrix reads without bank conflicts: the loop has no block barrier, and 100 to 190 KB are in flight per SM.
 // A row's reference point m moves only when a score passes it by 2^8 (as V's reference scale does
 // when a larger one comes), so the usual tile needs one vote instead of reductions and rescaling.
-// Values of tokens hidden from every row of the block are set to zero before they are used.
+// Values of tokens hidden from every row of the block are set to zero before they are used, and so is what is not finite in
+// those hidden from some, which is added to the other rows' output as it stands.
 //
 // A context is shared evenly by the blocks of a cluster (up to 8), which join their (m, l, O) through
 // distributed shared memory; of several clusters per context the last to finish joins their partial
@@ -101,6 +102,16 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
   return r;
+}
+__device__ __forceinline__ uint4 ld_shared4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t ld_shared1(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
 }
 template <bool BF16>
 __device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -433,13 +444,63 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
         if (!ok) break;
       }
       if (!whole) {
-        // tokens no row sees (past the context, before every window): their pages may hold anything
+        // tokens no row sees (past the context, before every window): their pages may hold anything; of tokens that some rows
+        // see, what is not finite (rows of one token all see the same ones)
         constexpr int kPc = P::kRow / 16;
         bool wrote = false;
+        unsigned odd = 0u;  // tokens with such values
         for (int id = lane; id < kRT * kPc; id += 32) {
           const int r = id / kPc, ch = id % kPc;
+          const uint32_t at = vs + piece<P::kInner>(r, ch);
           if (!R.seen_by_any(j0 + r)) {
-            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vs + piece<P::kInner>(r, ch)), "r"(0u) : "memory");
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
+            wrote = true;
+          } else if (FMT != GS_DTYPE_INT8 && A.max_q > 1 && !R.seen_by_all(A, j0 + r)) {
+            if (any4(not_finite_in<FMT>(ld_shared4(at)))) odd |= 1u << r;
+          }
+        }
+        bool scale_odd[2] = {false, false};  // (8-bit) of this lane's two tokens
+        if constexpr (!kBf) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            scale_odd[h] = !(fabsf(vsc[h]) < INFINITY) && A.max_q > 1 && !R.seen_by_all(A, j0 + g + 8 * h);
+            if (scale_odd[h]) odd |= 1u << (g + 8 * h), vsc[h] = 0.0f;
+          }
+        }
+        odd = __reduce_or_sync(kFullMask, odd);
+        if (odd) {
+          for (unsigned rest = odd; rest; rest &= rest - 1) {
+            const int r = __ffs(rest) - 1, j = j0 + r;
+            bool seen[NB][2];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) seen[nb][h] = j <= pos[nb][h] && (!A.window || j > pos[nb][h] - A.window || j < A.sinks);
+            const bool all = __shfl_sync(kFullMask, (r < 8 ? scale_odd[0] : scale_odd[1]) ? 1 : 0, (r & 7) * 4) != 0;
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int at = (kBf ? 16 * k + g + 8 * h : 16 * k + 2 * g + h) * P::kEl;  // (this lane's value of O's column)
+                const uint32_t w = ld_shared1(vs + piece<P::kInner>(r, at / 16) + (at & 12));
+                const uint32_t el = kBf ? (w >> (at & 2) * 8) << 16 : (w >> (at & 3) * 8) & 0xffu;
+                const float x = kBf ? __uint_as_float(el) : all || (FMT == GS_DTYPE_E4M3 && (el & 0x7fu) == 0x7fu) ? NAN : 0.0f;
+                if (!(fabsf(x) < INFINITY)) {
+#pragma unroll
+                  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+                      if (seen[nb][u]) o[nb][k][2 * h + u] += x;
+                }
+              }
+          }
+          __syncwarp();
+          for (int id = lane; id < kRT * kPc; id += 32) {
+            const int r = id / kPc, ch = id % kPc;
+            if (!(odd >> r & 1u)) continue;
+            const uint32_t at = vs + piece<P::kInner>(r, ch);
+            const uint4 w = ld_shared4(at), x = without4(w, not_finite_in<FMT>(w));
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
             wrote = true;
           }
         }
@@ -586,12 +647,7 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
   auto put = [&](int r, int d, float M, float L, float4 acc) {
     int gq;
     const int t = R.token_of(A, r, gq);
-    float inv = L == 0.0f ? 0.0f : 1.0f / L;
-    if (!finite4(acc) && L == L) {  // (its maximum and sum do not come from V)
-      float2 ml;
-      attn_by_row<FMT>(A, b, head, q_row(A, R, head, t, gq), R.p0 + t, D, d, &acc, &ml);
-      inv = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;
-    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
     const uint2 w = make_uint2(bf16x2(acc.x * inv, acc.y * inv), bf16x2(acc.z * inv, acc.w * inv));
     *reinterpret_cast<uint2*>(o_row(A, R, head, t, gq) + d) = w;
     if (A.lse && d == 0)

@@ -39,7 +39,8 @@
 namespace gs {
 namespace {
 
-constexpr int kTT = 128;  // context tokens per tile
+constexpr int kTT = 128;        // context tokens per tile
+constexpr int kMostRows = 256;  // query rows of a group of blocks, at most
 
 // CG: blocks that share a context's tiles (tcgen05 cta_group).  Two blocks of a cluster each hold half of
 // every K tile (tokens) and V tile (columns), and one product covers the query rows of both: half the L2
@@ -590,6 +591,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         const int pg = page_of(pc.b, tok), off = tok & page_mask;
         next_k = __ldg(A.kv.scale_at(false, pg, head, off));
         next_v = __ldg(A.kv.scale_at(true, pg, head, off));
+        if (!(fabsf(next_v) < INFINITY) && !R.seen_by_all(A, tok)) next_v = 0.0f, A.mend[0] = 1u;  // (attn_mend_kernel)
       }
     };
     const bool scales = lt < kTT;  // (a token each)
@@ -624,7 +626,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       }
       const int toks = value ? P::kVTok : P::kKTok;
       const int jt = j0 + (value ? h * P::kVTok : rank * P::kKTok);
-      const bool edge = jt + toks > R.hi || (jt < R.lo && jt + toks > R.sink);  // some token no row sees
+      const bool edge = !R.seen_by_all(A, jt, toks);
       const unsigned char* src = sm + P::kOffRaw + rs * P::kRawStage;
       unsigned char* dst = sm + P::kOffStage + at * P::kStage;
       // TOKS tokens in column blocks of INNER codes
@@ -635,7 +637,14 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         for (int u = 0; u < kPieces; ++u) {
           const int id = lt + P::kWideners * u, ch = id % (INNER / 16), rowid = id / (INNER / 16);
           const int cb = rowid / TOKS, tr = rowid % TOKS;  // column block, token
-          const uint4 x = *reinterpret_cast<const uint4*>(src + id * 16);
+          uint4 x = *reinterpret_cast<const uint4*>(src + id * 16);
+          if (FMT == GS_DTYPE_E4M3 && V && edge && !R.seen_by_all(A, jt + tr)) {
+            const uint4 m = not_finite_in<FMT>(x);
+            if (any4(m)) {
+              x = without4(x, m);
+              if (R.seen_by_any(jt + tr)) A.mend[0] = 1u;  // (attn_mend_kernel)
+            }
+          }
           uint2 q[4] = {widen_half<FMT>(x.x), widen_half<FMT>(x.y), widen_half<FMT>(x.z), widen_half<FMT>(x.w)};
           if (V && edge && !R.seen_by_any(jt + tr)) q[0] = q[1] = q[2] = q[3] = make_uint2(0u, 0u);
           const int hc = (cb * INNER + ch * 16) / 64;  // 64-column operand block
@@ -962,7 +971,6 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         // item's Q (q_slot), and no other warp of the tile writes there: the four are not ordered between one item and the next.
         constexpr int kCh = D / 8;
         unsigned char* st = sm + s * (D / 64) * 16384;
-        uint32_t top = 0u;  // largest magnitudes, as patterns
 #pragma unroll
         for (int q = 0; q < D / 32; ++q) {
           float o[32];
@@ -977,11 +985,9 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
           for (int i = 0; i < 4; ++i) {
             const uint4 w = make_uint4(bf16x2(o[8 * i] * inv, o[8 * i + 1] * inv), bf16x2(o[8 * i + 2] * inv, o[8 * i + 3] * inv),
                                        bf16x2(o[8 * i + 4] * inv, o[8 * i + 5] * inv), bf16x2(o[8 * i + 6] * inv, o[8 * i + 7] * inv));
-            top = __vmaxu2(top, __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu)));
             *reinterpret_cast<uint4*>(st + q_slot<D>(quad, lane) * 128 + ((4 * q + i) >> 3) * 16384 + ((((4 * q + i) ^ lane) & 7) << 4)) = w;
           }
         }
-        if (live && ((top & 0xffffu) >= 0x7f80u || (top >> 16) >= 0x7f80u)) A.mend[0] = 1u;  // (attn_mend_kernel)
         __syncwarp();
         uint4* mine = live ? reinterpret_cast<uint4*>(o_row(A, R, head, tq, hq - head * A.group)) : nullptr;  // (lane = row)
 #pragma unroll
@@ -1050,19 +1056,27 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       }
       __syncwarp();
     };
-    // zeros in the rows of a V stage that no query row of the block sees: their weights are 0,
-    // and what the pages hold there may be a NaN
+    // Zeros in the rows of a V stage that no query row of the block sees (their weights are 0, and what the pages hold there may
+    // be a NaN), and in place of what is not finite in rows that only some see (attn_mend_kernel adds it to those).
+    // This runs while the softmax works on the same tile's scores.
     auto clean = [&](int at, int j, int h) {
       const RowRange& R = pc.R;
       const int j0 = R.tile(pc.t_begin + j) * kTT + h * P::kVTok;
-      const bool hidden = j0 + P::kVTok > R.hi || (j0 < R.lo && j0 + P::kVTok > R.sink);
-      if (!P::kBf || !hidden) return;
+      if (!P::kBf || R.seen_by_all(A, j0, P::kVTok)) return;
       unsigned char* st = sm + P::kOffStage + (at % P::kStages) * P::kStage;
+      bool odd = false;
+#pragma unroll 4
       for (int id = lane; id < P::kVTok * (P::kVCols / 8); id += 32) {
         const int tr = id / (P::kVCols / 8), ch = id % (P::kVCols / 8);
-        if (!R.seen_by_any(j0 + tr))
-          *reinterpret_cast<uint4*>(st + (ch >> 3) * (P::kVTok * 128) + tr * 128 + ((ch & 7) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+        uint4* piece = reinterpret_cast<uint4*>(st + (ch >> 3) * (P::kVTok * 128) + tr * 128 + ((ch & 7) << 4));
+        if (!R.seen_by_any(j0 + tr)) {
+          *piece = make_uint4(0u, 0u, 0u, 0u);
+        } else if (!R.seen_by_all(A, j0 + tr)) {
+          const uint4 w = *piece, m = not_finite_in<FMT>(w);
+          if (any4(m)) *piece = without4(w, m), odd = true;
+        }
       }
+      if (odd) A.mend[0] = 1u;
       fence_async();
       __syncwarp();
     };
@@ -1222,36 +1236,61 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
   int gq;
   const int t = R.token_of(A, r, gq);
   const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-  if (!finite4(make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv))) A.mend[0] = 1u;  // (attn_mend_kernel)
   *reinterpret_cast<uint2*>(o_row(A, R, head, t, gq) + d) =
       make_uint2(bf16x2(acc.x * inv, acc.y * inv), bf16x2(acc.z * inv, acc.w * inv));
   if (A.lse && d == 0) A.lse[static_cast<int64_t>(R.q0 + t) * A.q_heads + head * A.group + gq] = L == 0.0f ? -INFINITY : (M + log2f(L)) * 0.6931471805599453f;
 }
 
-// After the many-row kernel, and nothing to do unless that wrote a result that is not finite: those, four values a
-// thread, computed again from what their rows see alone.  It is launched while the kernel before it still runs and waits
-// for its end on the device, and costs a call about a microsecond.
+// After the many-row kernel, and nothing to do unless that left values out of a product: tokens that some rows of a
+// block see and others do not, and whose values are not finite.  A row that sees such a token lies at most a block's new tokens
+// behind it, or the token lies as little behind the beginning of the row's window: those tokens are asked, four columns a
+// thread, and what is not finite is added to the result.  (Where a token was not left out it is in the result
+// already, which adding it again does not change.)  Launched while the kernel before it still runs and waiting for its end on the
+// device, it costs a call about a microsecond.
 template <int FMT>
 __global__ void __launch_bounds__(128) attn_mend_kernel(const __grid_constant__ AttnArgs A, int head_dim) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (__ldcg(A.mend) == 0u) return;
-  const int pieces = head_dim / 4;
+  constexpr int kEl = FMT == GS_DTYPE_BF16 ? 2 : 1;
+  const int pieces = head_dim / 4, mask = (1 << A.kv.page_shift) - 1;
+  const int span = (kMostRows + A.group - 2) / A.group + 1;  // tokens that a block's rows are of, at most
   for (int u = blockIdx.x; u < A.seqs * A.kv.kv_heads; u += gridDim.x) {
     const int b = u / A.kv.kv_heads, head = u % A.kv.kv_heads;
     const RowRange R = row_range<kTT>(A, b, 0, 0x7fffffff);
+    const int32_t* table = A.table + b * A.table_stride;
     for (int64_t e = threadIdx.x + static_cast<int64_t>(blockIdx.y) * 128; e < static_cast<int64_t>(R.rows) * pieces; e += gridDim.y * 128) {
       const int r = static_cast<int>(e / pieces), d = static_cast<int>(e % pieces) * 4, t = r / A.group, g = r % A.group;
+      const int pos = R.p0 + t, lo = A.window ? max(pos - A.window + 1, 0) : 0;
+      float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      auto ask = [&](int j0, int end) {
+#pragma unroll 8
+        for (int j = j0; j < end; ++j) {
+          const int col = j >> A.kv.page_shift, off = j & mask;
+          int page = col < A.table_cols ? __ldg(table + col) : 0;
+          if (page < 0 || page >= A.kv.pages) page = 0;  // (noted by the kernel that came here)
+          const unsigned char* v = A.kv.at(true, page, head, off) + d * kEl;
+          if constexpr (FMT == GS_DTYPE_BF16) {
+            const uint2 w = *reinterpret_cast<const uint2*>(v);
+            const float x[4] = {bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y)};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) add[i] += fabsf(x[i]) < INFINITY ? 0.0f : x[i];
+          } else {
+            const uint32_t m = fabsf(*A.kv.scale_at(true, page, head, off)) < INFINITY ? not_finite_in<FMT>(*reinterpret_cast<const uint32_t*>(v)) : ~0u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) add[i] = m >> (8 * i) & 1u ? NAN : add[i];
+          }
+        }
+      };
+      const int recent = max(max(pos - span + 1, lo), 0);
+      ask(recent, pos + 1);
+      if (A.window) {
+        ask(max(recent - span, 0), min(recent, min(A.sinks, lo)));  // (a sink among them that the window has left behind)
+        ask(lo, min(lo + span, recent));
+      }
+      if (add[0] == 0.0f && add[1] == 0.0f && add[2] == 0.0f && add[3] == 0.0f) continue;
       uint2* at = reinterpret_cast<uint2*>(o_row(A, R, head, t, g) + d);
       const uint2 w = *at;
-      if (finite4(make_float4(bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y)))) continue;
-      float4 o;
-      float2 ml;
-      attn_by_row<FMT>(A, b, head, q_row(A, R, head, t, g), R.p0 + t, head_dim, d, &o, &ml);
-      const float inv = ml.y == 0.0f ? 0.0f : 1.0f / ml.y;
-      *at = make_uint2(bf16x2(o.x * inv, o.y * inv), bf16x2(o.z * inv, o.w * inv));
-      // (beside an 8-bit cache an infinite V scale takes the row's sum with it)
-      if (A.lse && d == 0)
-        A.lse[static_cast<int64_t>(R.q0 + t) * A.q_heads + head * A.group + g] = ml.y == 0.0f ? -INFINITY : (ml.x + log2f(ml.y)) * 0.6931471805599453f;
+      *at = make_uint2(bf16x2(bf16_lo(w.x) + add[0], bf16_hi(w.x) + add[1]), bf16x2(bf16_lo(w.y) + add[2], bf16_hi(w.y) + add[3]));
     }
   }
   __syncthreads();
@@ -1315,6 +1354,7 @@ template <int D, int FMT, int CG>
 cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
   using P = TilePlan<D, FMT, CG>;
   constexpr int kRows = CG * P::kRows;  // rows of a group of blocks
+  static_assert(kRows <= kMostRows, "rows by which attn_mend_kernel asks");
   const int blocks = static_cast<int>((static_cast<int64_t>(a.max_q) * a.group + kRows - 1) / kRows);
   const int64_t items = static_cast<int64_t>(a.seqs) * a.kv.kv_heads * blocks;
   const int64_t tiles = most_tiles(a, kTT, kRows);

@@ -402,8 +402,9 @@ gs_status gs_kv_read(gs_kv_cache* c, const gs_kv_rows* rows, void* stream);
  * g / (q_heads / kv_heads).  Per row, with s_j = scale · q·k_j over the tokens it sees:
  *   lse = log Σ e^(s_j),  out = Σ e^(s_j - lse) v_j
  * rounded once to bf16.  A row that sees nothing gives out 0 and lse -inf.  A token that a
- * row does not see does not enter its result, even if it holds infinities or NaN.  (Results
- * that come out not finite are formed a second time, token by token: such a call takes longer.)
+ * row does not see does not enter its result, even if it holds infinities or NaN; one that it does
+ * see makes the result not finite (an infinity or a NaN) in the columns where it is not.  (A call in
+ * which new tokens beside one another see and do not see such a value takes up to 1.8 times as long.)
  * Scores, maxima, sums and the accumulated output are float32; a row's weights
  * e^(s_j - running max) are rounded to bf16 for the second product, beside an 8-bit cache
  * their product with the value's scale to float16.  (Beside an 8-bit cache q enters the first

@@ -126,3 +126,49 @@ def test_pages_behind_the_window_may_be_gone_from_shared_items(pkg, sampler, for
     assert free_hidden_pages(c) > 0
     out, lse = c.run()
     assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+def milliseconds(f, reps=3):
+    f()
+    t = []
+    for _ in range(reps):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        f()
+        b.record()
+        b.synchronize()
+        t.append(a.elapsed_time(b))
+    return min(t)
+
+
+@pytest.mark.parametrize("lens,token,most", [([(1, 60000)], 0, 4), ([(300, 8000)], 0, 4), ([(6, 20000)], -1, 8),
+                                             ([(300, 8000)], -1, 8)])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("form", FORMS)
+def test_cost_of_a_value_that_is_not_finite(pkg, sampler, form, dim, lens, token, most):
+    """An infinite value that every row sees, or only the last one: no such call takes many times the usual one's time."""
+    c = Case(sampler, pkg, lens, 2, 4, dim, 64, form, seed=dim)
+    call = dict(max_q=c.max_q, max_kv=c.max_kv, scale=c.scale)
+
+    def run():
+        return c.cache.attend(c.q, c.q_start, c.kv_len, c.table, **call)[0]
+    want = run()
+    plain = milliseconds(run)
+    j = token % lens[0][1]
+    pg, off = int(c.table[0, j // 64]), j % 64
+    if form == "bf16":
+        c.cache.v[pg, :, off, 5] = float("inf")
+    else:
+        c.cache.v_scale[pg, :, off] = float("inf")
+    out = run()
+    seen = out if token == 0 else out[-1:]
+    assert not seen[..., 5].isfinite().any()
+    if form == "bf16":
+        seen[..., 5] = want[-seen.shape[0]:][..., 5]
+        assert torch.equal(seen, want[-seen.shape[0]:])
+    if token != 0:
+        assert out[:-1].isfinite().all()
+        err = (out[:-1].float() - want[:-1].float()).abs()
+        assert (err <= 2.0 ** -7 * want[:-1].float().abs() + 2.0 ** -7 * c.vd.abs().nan_to_num(posinf=0.0).max().item()).all()
+    slow = milliseconds(run)
+    assert slow < most * plain, f"{plain * 1e3:.0f} -> {slow * 1e3:.0f} us"
