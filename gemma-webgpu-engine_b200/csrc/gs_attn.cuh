@@ -187,7 +187,14 @@ template <int FMT>
 __device__ __forceinline__ uint4 not_finite_in(uint4 w) {
   return make_uint4(not_finite_in<FMT>(w.x), not_finite_in<FMT>(w.y), not_finite_in<FMT>(w.z), not_finite_in<FMT>(w.w));
 }
-__device__ __forceinline__ bool any4(uint4 m) { return (m.x | m.y | m.z | m.w) != 0u; }
+// Whether there are any among four words: the next larger exponent (e4m3: code) carries into the sign's place.
+template <int FMT>
+__device__ __forceinline__ bool any_not_finite(uint4 w) {
+  if constexpr (FMT == GS_DTYPE_INT8) return false;
+  constexpr uint32_t kField = FMT == GS_DTYPE_BF16 ? 0x7f807f80u : 0x7f7f7f7fu, kOne = FMT == GS_DTYPE_BF16 ? 0x00800080u : 0x01010101u;
+  const uint32_t m = ((w.x & kField) + kOne) | ((w.y & kField) + kOne) | ((w.z & kField) + kOne) | ((w.w & kField) + kOne);
+  return (m & (FMT == GS_DTYPE_BF16 ? 0x80008000u : 0x80808080u)) != 0u;
+}
 __device__ __forceinline__ uint4 without4(uint4 w, uint4 m) { return make_uint4(w.x & ~m.x, w.y & ~m.y, w.z & ~m.z, w.w & ~m.w); }
 
 // Few-row kernel (mma.sync, one 16-token tile per warp): any number of rows in blocks.

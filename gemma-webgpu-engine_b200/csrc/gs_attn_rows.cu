@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
             asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
             wrote = true;
           } else if (FMT != GS_DTYPE_INT8 && A.max_q > 1 && !R.seen_by_all(A, j0 + r)) {
-            if (any4(not_finite_in<FMT>(ld_shared4(at)))) odd |= 1u << r;
+            if (any_not_finite<FMT>(ld_shared4(at))) odd |= 1u << r;
           }
         }
         bool scale_odd[2] = {false, false};  // (8-bit) of this lane's two tokens

@@ -591,7 +591,6 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         const int pg = page_of(pc.b, tok), off = tok & page_mask;
         next_k = __ldg(A.kv.scale_at(false, pg, head, off));
         next_v = __ldg(A.kv.scale_at(true, pg, head, off));
-        if (!(fabsf(next_v) < INFINITY) && !R.seen_by_all(A, tok)) next_v = 0.0f, A.mend[0] = 1u;  // (attn_mend_kernel)
       }
     };
     const bool scales = lt < kTT;  // (a token each)
@@ -617,8 +616,12 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         // warp keeps one of its own.
         sc[lt] = next_k;
         sc[kTT + lt] = next_v;
-        const uint32_t mag = __float_as_uint(next_v) & 0x7fffffffu;
-        const uint32_t mx = __reduce_max_sync(kFullMask, mag < 0x7f800000u ? mag : 0u);
+        uint32_t mag = __float_as_uint(next_v) & 0x7fffffffu;
+        if (mag >= 0x7f800000u) {
+          if (!R.seen_by_all(A, j0 + lt)) sc[kTT + lt] = 0.0f, A.mend[0] = 1u;  // (attn_mend_kernel)
+          mag = 0u;
+        }
+        const uint32_t mx = __reduce_max_sync(kFullMask, mag);
         const float top = __uint_as_float(mx > 0x7e800000u ? 0x7f000000u : (mx + 0x7fffffu) & 0x7f800000u);  // up to a power of two
         if (top > vref) vref = fminf(2.0f * top, 1.7014118346046923e38f);  // (a power of two of room: each move costs a pass over O)
         if (lane == 0) reinterpret_cast<float*>(sm + P::kOffRef)[((g0 + j) % P::kScaleSlots) * 4 + (warp & 3)] = vref;
@@ -626,27 +629,19 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       }
       const int toks = value ? P::kVTok : P::kKTok;
       const int jt = j0 + (value ? h * P::kVTok : rank * P::kKTok);
-      const bool edge = !R.seen_by_all(A, jt, toks);
       const unsigned char* src = sm + P::kOffRaw + rs * P::kRawStage;
       unsigned char* dst = sm + P::kOffStage + at * P::kStage;
-      // TOKS tokens in column blocks of INNER codes
-      auto turn = [&](auto v_, auto toks_, auto inner_) {
-        constexpr bool V = decltype(v_)::value;
+      // TOKS tokens in column blocks of INNER codes.  MIXED: a V stage with tokens that not every row sees: those that no row sees are
+      // zeros, and where there are codes that are not finite (looked for in all pieces at once: a branch in
+      // each costs 4% of a call of short windows) their pieces are taken again without them.
+      auto turn = [&](auto mixed_, auto toks_, auto inner_) {
+        constexpr bool MIXED = decltype(mixed_)::value;
         constexpr int TOKS = decltype(toks_)::value, INNER = decltype(inner_)::value;
-#pragma unroll
-        for (int u = 0; u < kPieces; ++u) {
-          const int id = lt + P::kWideners * u, ch = id % (INNER / 16), rowid = id / (INNER / 16);
+        auto put = [&](int id, uint4 x, bool hide) {
+          const int ch = id % (INNER / 16), rowid = id / (INNER / 16);
           const int cb = rowid / TOKS, tr = rowid % TOKS;  // column block, token
-          uint4 x = *reinterpret_cast<const uint4*>(src + id * 16);
-          if (FMT == GS_DTYPE_E4M3 && V && edge && !R.seen_by_all(A, jt + tr)) {
-            const uint4 m = not_finite_in<FMT>(x);
-            if (any4(m)) {
-              x = without4(x, m);
-              if (R.seen_by_any(jt + tr)) A.mend[0] = 1u;  // (attn_mend_kernel)
-            }
-          }
           uint2 q[4] = {widen_half<FMT>(x.x), widen_half<FMT>(x.y), widen_half<FMT>(x.z), widen_half<FMT>(x.w)};
-          if (V && edge && !R.seen_by_any(jt + tr)) q[0] = q[1] = q[2] = q[3] = make_uint2(0u, 0u);
+          if (MIXED && hide) q[0] = q[1] = q[2] = q[3] = make_uint2(0u, 0u);
           const int hc = (cb * INNER + ch * 16) / 64;  // 64-column operand block
           const int c0 = (ch & 3) * 2, odd = INNER == 64 ? (tr >> 1) & 1 : hc & 1;
           unsigned char* rowp = dst + hc * (TOKS * 128) + tr * 128;
@@ -654,10 +649,28 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
           const uint4 lo = make_uint4(q[0].x, q[0].y, q[1].x, q[1].y), hi = make_uint4(q[2].x, q[2].y, q[3].x, q[3].y);
           *reinterpret_cast<uint4*>(rowp + (((c0 + odd) ^ (tr & 7)) << 4)) = odd ? hi : lo;
           *reinterpret_cast<uint4*>(rowp + (((c0 + 1 - odd) ^ (tr & 7)) << 4)) = odd ? lo : hi;
+        };
+        bool any = false;
+#pragma unroll
+        for (int u = 0; u < kPieces; ++u) {
+          const int id = lt + P::kWideners * u;
+          const uint4 x = *reinterpret_cast<const uint4*>(src + id * 16);
+          if constexpr (MIXED) any |= any_not_finite<FMT>(x);
+          put(id, x, MIXED && !R.seen_by_any(jt + id / (INNER / 16) % TOKS));
+        }
+        if (MIXED && any) {
+          for (int u = 0; u < kPieces; ++u) {
+            const int id = lt + P::kWideners * u, tok = jt + id / (INNER / 16) % TOKS;
+            const uint4 x = *reinterpret_cast<const uint4*>(src + id * 16);
+            if (!any_not_finite<FMT>(x) || !R.seen_by_any(tok) || R.seen_by_all(A, tok)) continue;
+            put(id, without4(x, not_finite_in<FMT>(x)), false);
+            A.mend[0] = 1u;  // (attn_mend_kernel)
+          }
         }
       };
-      if (value) turn(std::true_type{}, std::integral_constant<int, P::kVTok>{}, std::integral_constant<int, P::kVInner>{});
-      else turn(std::false_type{}, std::integral_constant<int, P::kKTok>{}, std::integral_constant<int, P::kKInner>{});
+      if (!value) turn(std::false_type{}, std::integral_constant<int, P::kKTok>{}, std::integral_constant<int, P::kKInner>{});
+      else if (R.seen_by_all(A, jt, toks)) turn(std::false_type{}, std::integral_constant<int, P::kVTok>{}, std::integral_constant<int, P::kVInner>{});
+      else turn(std::true_type{}, std::integral_constant<int, P::kVTok>{}, std::integral_constant<int, P::kVInner>{});
       fence_async();
       arrive_on(raw_free + rs);
       arrive_on(full + at);
@@ -1064,18 +1077,34 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       const int j0 = R.tile(pc.t_begin + j) * kTT + h * P::kVTok;
       if (!P::kBf || R.seen_by_all(A, j0, P::kVTok)) return;
       unsigned char* st = sm + P::kOffStage + (at % P::kStages) * P::kStage;
+      constexpr int kCh = P::kVCols / 8;
       bool odd = false;
-#pragma unroll 4
-      for (int id = lane; id < P::kVTok * (P::kVCols / 8); id += 32) {
-        const int tr = id / (P::kVCols / 8), ch = id % (P::kVCols / 8);
-        uint4* piece = reinterpret_cast<uint4*>(st + (ch >> 3) * (P::kVTok * 128) + tr * 128 + ((ch & 7) << 4));
-        if (!R.seen_by_any(j0 + tr)) {
-          *piece = make_uint4(0u, 0u, 0u, 0u);
-        } else if (!R.seen_by_all(A, j0 + tr)) {
-          const uint4 w = *piece, m = not_finite_in<FMT>(w);
-          if (any4(m)) *piece = without4(w, m), odd = true;
+      auto piece = [&](int id) {
+        const int tr = id / kCh, ch = id % kCh;
+        return reinterpret_cast<uint4*>(st + (ch >> 3) * (P::kVTok * 128) + tr * 128 + ((ch & 7) << 4));
+      };
+      // (context tokens t0 .. t1 - 1, as far as the stage has them)
+      auto zero = [&](int t0, int t1) {
+        for (int id = max(t0 - j0, 0) * kCh + lane; id < min(t1 - j0, P::kVTok) * kCh; id += 32) *piece(id) = make_uint4(0u, 0u, 0u, 0u);
+      };
+      auto sift = [&](int t0, int t1) {
+        const int end = min(t1 - j0, P::kVTok) * kCh;
+        for (int id0 = max(t0 - j0, 0) * kCh + lane; id0 < end; id0 += 256) {
+          bool any = false;
+#pragma unroll
+          for (int u = 0; u < 8; ++u) any |= id0 + 32 * u < end && any_not_finite<FMT>(*piece(id0 + 32 * u));
+          if (!any) continue;
+          for (int id = id0; id < end && id < id0 + 256; id += 32) *piece(id) = without4(*piece(id), not_finite_in<FMT>(*piece(id)));
+          odd = true;
         }
+      };
+      const int ahead = R.p0 + R.t0 + 1;  // from here on some row does not see a token yet
+      if (A.window) {
+        zero(R.sink, R.lo);
+        sift(max(R.sink, R.lo), min(R.hi - A.window, ahead));  // (some row's window has left these)
       }
+      sift(ahead, R.hi);
+      zero(R.hi, j0 + P::kVTok);
       if (odd) A.mend[0] = 1u;
       fence_async();
       __syncwarp();

@@ -172,3 +172,35 @@ def test_cost_of_a_value_that_is_not_finite(pkg, sampler, form, dim, lens, token
         assert (err <= 2.0 ** -7 * want[:-1].float().abs() + 2.0 ** -7 * c.vd.abs().nan_to_num(posinf=0.0).max().item()).all()
     slow = milliseconds(run)
     assert slow < most * plain, f"{plain * 1e3:.0f} -> {slow * 1e3:.0f} us"
+
+
+@pytest.mark.parametrize("dim,lens,group", [(64, [(6, 130), (3, 65)], 2), (128, [(9, 300)], 5), (256, [(7, 210)], 2),
+                                            (64, [(200, 260), (40, 65)], 4), (128, [(300, 500), (5, 5)], 1), (256, [(200, 300)], 3)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (60, 8)])
+@pytest.mark.parametrize("form", ["bf16", "e4m3"])
+def test_single_elements_that_only_some_rows_see(pkg, sampler, form, dim, lens, group, window, sinks):
+    """NaN elements in new tokens, at the windows' edge and in a sink that not every row has reached: they are in the
+    results of the rows that see them, column by column, and in no other."""
+    c = Case(sampler, pkg, lens, 2, group, dim, 16, form, seed=dim, window=window, sinks=sinks)
+    clean = c.reference()
+    bad = {}
+    for b, (nq, n) in enumerate(lens):
+        at = [n - 1, n - 1 - nq // 2] + ([max(sinks, n - nq + nq // 3 - window + 1)] if window else [])
+        if nq == n:
+            at.append(2)
+        for i, j in enumerate(at):
+            pg, off, col = int(c.table[b, j // 16]), j % 16, (7 * i + 3 * b) % dim
+            c.cache.v.view(torch.int16 if form == "bf16" else torch.uint8)[pg, :, off, col] = 0x7fc0 if form == "bf16" else 0x7f
+            bad.setdefault((b, j), set()).add(col)
+    out, lse = c.run()
+    hit = torch.zeros_like(out, dtype=torch.bool)
+    for b, (nq, n) in enumerate(lens):
+        for t in range(nq):
+            p = n - nq + t
+            for (b2, j), cols in bad.items():
+                if b2 == b and j <= p and (not window or j > p - window or j < sinks):
+                    hit[c.starts[b] + t, :, list(cols)] = True
+    assert hit.any() and out[hit].isnan().all()
+    # (the other columns are the untouched cache's, since only the elements named were changed)
+    got = torch.where(hit, clean[0].to(out.dtype), out)
+    R.check_attend(got, lse, clean)
