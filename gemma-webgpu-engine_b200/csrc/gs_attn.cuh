@@ -124,14 +124,15 @@ __device__ __forceinline__ void row_power(uint32_t top, float& down, float& up) 
 // Larger magnitudes of two bf16 pairs, and of a pair's halves (patterns without sign order as values do).
 __device__ __forceinline__ uint32_t pair_max(uint32_t a, uint32_t b) { return __vmaxu2(a & 0x7fff7fffu, b & 0x7fff7fffu); }
 
-// Rows [r0, r0 + cap) of sequence b, context tiles of kTile tokens.
+// Rows [r0, r0 + cap) of sequence b, context tiles of kTile tokens.  note: whether this thread reports what is wrong with the
+// sequence's entries.
 template <int kTile>
-__device__ __forceinline__ RowRange row_range(const AttnArgs& A, int b, int r0, int cap) {
+__device__ __forceinline__ RowRange row_range(const AttnArgs& A, int b, int r0, int cap, bool note) {
   RowRange R;
   R.q0 = A.q_start ? A.q_start[b] : b;
   int q1 = A.q_start ? A.q_start[b + 1] : b + 1;
   R.len = A.kv_len[b];
-  bool bad = R.len > A.max_kv || R.len < 0 || R.q0 < 0 || q1 > A.tokens || q1 - R.q0 > A.max_q;
+  const bool bad = R.len > A.max_kv || R.len < 0 || R.q0 < 0 || q1 > A.tokens || q1 < R.q0 || q1 - R.q0 > A.max_q;
   R.len = min(max(R.len, 0), A.max_kv);
   R.q0 = max(R.q0, 0);
   q1 = static_cast<int>(min(static_cast<int64_t>(q1), A.tokens));
@@ -144,10 +145,10 @@ __device__ __forceinline__ RowRange row_range(const AttnArgs& A, int b, int r0, 
   if (R.rows <= 0) {
     R.rows = 0;
     R.tiles = 0;
-    if (bad && r0 == 0 && threadIdx.x == 0) atomicOr(A.flag, GS_KV_ERR_LENGTH);
+    if (bad && r0 == 0 && note) atomicOr(A.flag, GS_KV_ERR_LENGTH);
     return R;
   }
-  if (bad && threadIdx.x == 0) atomicOr(A.flag, GS_KV_ERR_LENGTH);
+  if (bad && note) atomicOr(A.flag, GS_KV_ERR_LENGTH);
   const int pf = R.p0 + R.t0, pl = R.p0 + (r0 + R.rows - 1) / A.group;
   R.hi = max(pl + 1, 0);
   R.lo = A.window ? max(pf - A.window + 1, 0) : 0;

@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
   const int b = blockIdx.z;
   const int head = blockIdx.y % A.kv.kv_heads, rb = blockIdx.y / A.kv.kv_heads;
   const int r0 = rb * kRows;
-  const RowRange R = row_range<kRT>(A, b, r0, kRows);
+  const RowRange R = row_range<kRT>(A, b, r0, kRows, tid == 0);
   if (R.rows == 0) return;  // (the whole cluster)
   // this block's tiles: an even share of the context's
   const int share = (R.tiles + A.splits * A.cluster - 1) / (A.splits * A.cluster);

@@ -274,7 +274,7 @@ __device__ __forceinline__ bool next_piece(const AttnArgs& A, Cursor& c, Piece& 
   if constexpr (!BAL) {
     if (c.x >= c.x1) return false;
     c.x = c.x1;
-    p.R = row_range<kTT>(A, c.b, c.rb * ROWS, ROWS);
+    p.R = row_range<kTT>(A, c.b, c.rb * ROWS, ROWS, threadIdx.x == 0);
     int nsplit = (p.R.tiles + A.chunk_tiles - 1) / A.chunk_tiles;
     nsplit = nsplit < 1 ? 1 : nsplit > A.splits ? A.splits : nsplit;
     if (p.R.rows == 0 || c.off >= nsplit) return false;
@@ -286,7 +286,7 @@ __device__ __forceinline__ bool next_piece(const AttnArgs& A, Cursor& c, Piece& 
     return true;
   }
   while (c.x < c.x1 && c.head < A.kv.kv_heads) {
-    p.R = row_range<kTT>(A, c.b, c.rb * ROWS, ROWS);
+    p.R = row_range<kTT>(A, c.b, c.rb * ROWS, ROWS, false);  // (noted when the tiles were counted)
     const int w = p.R.rows == 0 ? 0 : max(p.R.tiles, 1);
     const int take = static_cast<int>(min(static_cast<int64_t>(w - c.off), c.x1 - c.x));
     const bool got = take > 0;
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     // every unit's (sequence, row block) tiles, their running sum, and where this group's stretch begins
     int* sums = reinterpret_cast<int*>(sm + P::kOffStage);  // [units + 1]
     for (int u = tid; u < A.units; u += P::kThreads) {
-      const RowRange R = row_range<kTT>(A, u / A.row_blocks, u % A.row_blocks * kGroupRows, kGroupRows);
+      const RowRange R = row_range<kTT>(A, u / A.row_blocks, u % A.row_blocks * kGroupRows, kGroupRows, blockIdx.x == 0);
       sums[u] = R.rows == 0 ? 0 : max(R.tiles, 1);
     }
     __syncthreads();
@@ -1223,7 +1223,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ 
   __shared__ float s_red[4], s_lse[4];
   const int b = blockIdx.z, head = blockIdx.y % A.kv.kv_heads, rb = blockIdx.y / A.kv.kv_heads;
   const int r = blockIdx.x, r0 = rb * rows_per_block, tid = threadIdx.x;
-  const RowRange R = row_range<kTT>(A, b, r0, rows_per_block);
+  const RowRange R = row_range<kTT>(A, b, r0, rows_per_block, false);
   if (r >= R.rows) return;
   int nsplit = (R.tiles + A.chunk_tiles - 1) / A.chunk_tiles;
   nsplit = nsplit < 1 ? 1 : nsplit > A.splits ? A.splits : nsplit;
@@ -1285,7 +1285,7 @@ __global__ void __launch_bounds__(128) attn_mend_kernel(const __grid_constant__ 
   const int span = (kMostRows + A.group - 2) / A.group + 1;  // tokens that a block's rows are of, at most
   for (int u = blockIdx.x; u < A.seqs * A.kv.kv_heads; u += gridDim.x) {
     const int b = u / A.kv.kv_heads, head = u % A.kv.kv_heads;
-    const RowRange R = row_range<kTT>(A, b, 0, 0x7fffffff);
+    const RowRange R = row_range<kTT>(A, b, 0, 0x7fffffff, false);
     const int32_t* table = A.table + b * A.table_stride;
     for (int64_t e = threadIdx.x + static_cast<int64_t>(blockIdx.y) * 128; e < static_cast<int64_t>(R.rows) * pieces; e += gridDim.y * 128) {
       const int r = static_cast<int>(e / pieces), d = static_cast<int>(e % pieces) * 4, t = r / A.group, g = r % A.group;

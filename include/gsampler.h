@@ -370,7 +370,7 @@ const char* gs_kv_cache_last_error(const gs_kv_cache* c);
 /* Errors that the kernels found in device data since the last check (synchronising):
  * a slot past the cache (skipped), a page-table entry outside [0, pages) or past the
  * table's columns (page 0 is read in its place), a sequence longer than max_q / max_kv (cut
- * off).  GS_EINVAL when any bit is set; GS_ETIMEOUT when a bounded wait ran out. */
+ * off) or whose q_start entries descend or leave the tokens (its rows outside them are not formed).  GS_EINVAL when any bit is set; GS_ETIMEOUT when a bounded wait ran out. */
 #define GS_KV_ERR_SLOT 1
 #define GS_KV_ERR_PAGE 2
 #define GS_KV_ERR_LENGTH 4
@@ -410,6 +410,7 @@ gs_status gs_kv_read(gs_kv_cache* c, const gs_kv_rows* rows, void* stream);
  * their product with the value's scale to float16.  (Beside an 8-bit cache q enters the first
  * product as float16 after an exact power of two per row: components below 2^-17 of the row's
  * largest lose bits.)  The same call gives the same bits every time.
+ * Rows of q that lie in no sequence are not read, and their out and lse not written.
  * The calls of one context use its workspace: order them on the GPU (one stream, or
  * events between streams), as for gs_sample. */
 typedef struct gs_attention_args {

@@ -204,3 +204,20 @@ def test_single_elements_that_only_some_rows_see(pkg, sampler, form, dim, lens, 
     # (the other columns are the untouched cache's, since only the elements named were changed)
     got = torch.where(hit, clean[0].to(out.dtype), out)
     R.check_attend(got, lse, clean)
+
+
+@pytest.mark.parametrize("lens", [[(2, 40), (3, 50), (1, 60)], [(40, 90), (50, 200), (30, 60)],
+                                  [(40, 90), (50, 2000), (30, 60)] * 20])
+def test_starts_that_descend_are_reported(pkg, sampler, lens):
+    c = Case(sampler, pkg, lens, 8, 2, 64, 16, "bf16")
+    good, _ = c.run()
+    n = c.starts[-2]
+    c.q_start[-1] = n - 1  # (the last sequence: less than no tokens)
+    out = torch.full_like(good, 7.0)
+    c.cache.attend(c.q, c.q_start, c.kv_len, c.table, max_q=c.max_q, max_kv=c.max_kv, scale=c.scale, out=out)
+    with pytest.raises(ValueError, match="outside"):
+        c.cache.check()
+    c.cache.check()
+    assert (out[n:] == 7).all()
+    tol = 2.0 ** -6 * c.vd.abs().max().item()  # (the shares of a divided call change with its tiles, and with them a bit here and there)
+    assert (out[:n].float() - good[:n].float()).abs().max().item() <= tol
