@@ -130,7 +130,11 @@ cudaError_t ctx_attn_workspace(gs_ctx* c, size_t bytes, size_t zeroed_tail, unsi
   if (!c->attn_ws) {
     e = cudaMalloc(&c->attn_ws, bytes);
     if (e != cudaSuccess) c->attn_ws = nullptr;
-    else e = cudaMemset(c->attn_ws + bytes - zeroed_tail, 0, zeroed_tail);
+    else e = clear_now(c->attn_ws + bytes - zeroed_tail, zeroed_tail);
+    if (e != cudaSuccess && c->attn_ws) {
+      cudaFree(c->attn_ws);
+      c->attn_ws = nullptr;
+    }
   }
   *out = c->attn_ws;
   return e;

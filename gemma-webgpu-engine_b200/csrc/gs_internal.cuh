@@ -146,6 +146,12 @@ inline void mark_device_done(std::atomic<uint64_t>& seen) {
   cudaGetDevice(&d);
   seen.fetch_or(1ull << (d & 63), std::memory_order_release);
 }
+// Device memory set to zero, over when it returns: a memset of the default stream alone may still be pending then, and
+// streams that do not block on that one (torch's side streams) are not ordered after it.
+inline cudaError_t clear_now(void* p, size_t bytes) {
+  const cudaError_t e = cudaMemset(p, 0, bytes);
+  return e == cudaSuccess ? cudaStreamSynchronize(cudaStreamLegacy) : e;
+}
 int ctx_device(const gs_ctx* c);                 // the device a context is bound to
 void ctx_set_error(gs_ctx* c, const char* msg);  // the message gs_last_error returns
 cudaError_t ctx_attn_workspace(gs_ctx* c, size_t bytes, size_t zeroed_tail, unsigned char** out);  // one size for every caller

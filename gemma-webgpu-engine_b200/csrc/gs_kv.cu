@@ -360,7 +360,7 @@ gs_status gs_kv_cache_create(gs_ctx* ctx, const gs_kv_cache_desc* d, gs_kv_cache
   c->page_shift = shift;
   DeviceScope scope(c->device);
   cudaError_t er = cudaMalloc(&c->flag, 4);
-  if (er == cudaSuccess) er = cudaMemset(c->flag, 0, 4);
+  if (er == cudaSuccess) er = clear_now(c->flag, 4);
   if (er == cudaSuccess) er = ctx_attn_workspace(ctx, kAttnWsBytes + kAttnTicketBytes + kAttnMendBytes, kAttnTicketBytes + kAttnMendBytes, &c->ws);
   if (er == cudaSuccess) er = cudaDeviceGetAttribute(&c->num_sms, cudaDevAttrMultiProcessorCount, c->device);
   if (er != cudaSuccess) {
@@ -396,10 +396,10 @@ gs_status gs_kv_cache_check(gs_kv_cache* c, int32_t* bits) {
   int32_t f = 0;
   cudaError_t e = cudaDeviceSynchronize();
   if (e == cudaSuccess) e = cudaMemcpy(&f, c->flag, 4, cudaMemcpyDeviceToHost);
-  if (e == cudaSuccess && f) e = cudaMemset(c->flag, 0, 4);
+  if (e == cudaSuccess && f) e = clear_now(c->flag, 4);
+  if (e == cudaSuccess && (f & GS_KV_ERR_TIMEOUT)) e = clear_now(c->ws + kAttnWsBytes, kAttnTicketBytes + kAttnMendBytes);  // (a piece may not have counted)
   if (e != cudaSuccess) return kfail(c, GS_ECUDA, cudaGetErrorString(e));
   *bits = f;
-  if (f & GS_KV_ERR_TIMEOUT) cudaMemset(c->ws + kAttnWsBytes, 0, kAttnTicketBytes + kAttnMendBytes);  // (a piece may not have counted)
   if (f & GS_KV_ERR_TIMEOUT) return kfail(c, GS_ETIMEOUT, "a bounded wait inside the attention kernel ran out");
   if (f & GS_KV_ERR_SLOT) return kfail(c, GS_EINVAL, "a slot lies past the cache");
   if (f & GS_KV_ERR_PAGE) return kfail(c, GS_EINVAL, "a page-table entry is outside the cache");
