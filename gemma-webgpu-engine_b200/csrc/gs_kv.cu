@@ -13,6 +13,7 @@
 #include <new>
 
 #include "gs_attn.cuh"
+#include "gs_overlap.h"
 
 namespace gs {
 namespace {
@@ -284,17 +285,20 @@ gs_status move_rows(gs_kv_cache* c, const gs_kv_rows* r, void* stream, bool writ
   if (r->tokens > (1ll << 30)) return kfail(c, GS_EUNSUPPORTED, "at most 2^30 tokens per call");
   const int64_t e = r->dtype == GS_DTYPE_F32 ? 4 : 2;
   const int64_t st[4] = {r->k_token_stride, r->k_head_stride, r->v_token_stride, r->v_head_stride};
+  for (int64_t s : st)
+    if (s < 0 || s >= (1ll << 32)) return kfail(c, GS_EUNSUPPORTED, "strides of k and v must be in [0, 2^32)");
   if (!write) {
     const int64_t D = c->d.head_dim;
     if ((c->d.kv_heads > 1 && (st[1] < D || st[3] < D)) || (r->tokens > 1 && (st[0] < D || st[2] < D)))
       return kfail(c, GS_EINVAL, "output strides must not make rows overlap");
+    const RowGrid k{reinterpret_cast<uintptr_t>(r->k), r->tokens, c->d.kv_heads, st[0] * e, st[1] * e, D * e};
+    const RowGrid v{reinterpret_cast<uintptr_t>(r->v), r->tokens, c->d.kv_heads, st[2] * e, st[3] * e, D * e};
+    if (rows_overlap(k) || rows_overlap(v) || rows_overlap(k, v)) return kfail(c, GS_EINVAL, "output rows must not overlap");
   }
   KvRowsArgs a{};
   a.kv = pool_of(c);
   a.k = static_cast<unsigned char*>(r->k);
   a.v = static_cast<unsigned char*>(r->v);
-  for (int64_t s : st)
-    if (s < 0 || s >= (1ll << 32)) return kfail(c, GS_EUNSUPPORTED, "strides of k and v must be in [0, 2^32)");
   a.k_token = static_cast<uint32_t>(st[0]), a.k_head = static_cast<uint32_t>(st[1]);
   a.v_token = static_cast<uint32_t>(st[2]), a.v_head = static_cast<uint32_t>(st[3]);
   a.slots = r->slots;
@@ -437,6 +441,10 @@ gs_status gs_attention(gs_kv_cache* c, const gs_attention_args* p, void* stream)
       return kfail(c, GS_EINVAL, "q and out strides must be >= head_dim, multiples of 8 and below 2^31");
   if (reinterpret_cast<uintptr_t>(p->q) % 16 || reinterpret_cast<uintptr_t>(p->out) % 16)
     return kfail(c, GS_EINVAL, "q and out must be 16-byte aligned");
+  const RowGrid q{reinterpret_cast<uintptr_t>(p->q), p->tokens, p->q_heads, st[0] * 2, st[1] * 2, c->d.head_dim * 2};
+  const RowGrid o{reinterpret_cast<uintptr_t>(p->out), p->tokens, p->q_heads, st[2] * 2, st[3] * 2, c->d.head_dim * 2};
+  if (rows_overlap(o)) return kfail(c, GS_EINVAL, "out rows must not overlap");
+  if (rows_overlap(q, o)) return kfail(c, GS_EINVAL, "out must not overlap q");
   const int64_t group = p->q_heads / c->d.kv_heads;
   const int64_t most_rows = static_cast<int64_t>(p->max_q) * group;
   // (the many-row grid's second dimension holds blocks of at least 128 rows for every head)

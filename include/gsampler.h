@@ -390,7 +390,8 @@ typedef struct gs_kv_rows {
   int32_t dtype;            /* GS_DTYPE_F32 / GS_DTYPE_BF16 */
 } gs_kv_rows;
 gs_status gs_kv_write(gs_kv_cache* c, const gs_kv_rows* rows, void* stream);
-/* The rows at slots[t] read back (code · scale, rounded once); zeros for a negative slot. */
+/* The rows at slots[t] read back (code · scale, rounded once); zeros for a negative slot.  Rows of
+ * the outputs must not overlap. */
 gs_status gs_kv_read(gs_kv_cache* c, const gs_kv_rows* rows, void* stream);
 
 /* Attention of new tokens over the cache.  Sequence b has the new tokens
@@ -415,7 +416,8 @@ gs_status gs_kv_read(gs_kv_cache* c, const gs_kv_rows* rows, void* stream);
  * events between streams), as for gs_sample. */
 typedef struct gs_attention_args {
   const void* q;            /* device bf16 [tokens][q_heads][head_dim] by the strides below */
-  void* out;                /* device bf16, same shape; must not overlap q */
+  void* out;                /* device bf16, same shape; rows must not overlap one another's or q's (two views of
+                             * one buffer are told apart when they have the same token stride) */
   float* lse;               /* device [tokens][q_heads], or NULL */
   const int32_t* q_start;   /* device [seqs + 1], or NULL (tokens == seqs, one each) */
   const int32_t* kv_len;    /* device [seqs] */

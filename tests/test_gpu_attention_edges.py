@@ -221,3 +221,24 @@ def test_starts_that_descend_are_reported(pkg, sampler, lens):
     assert (out[n:] == 7).all()
     tol = 2.0 ** -6 * c.vd.abs().max().item()  # (the shares of a divided call change with its tiles, and with them a bit here and there)
     assert (out[:n].float() - good[:n].float()).abs().max().item() <= tol
+
+
+@pytest.mark.parametrize("lens", [[(1, 30), (2, 40)], [(70, 140), (9, 9)]])
+def test_results_that_overlap_the_query_or_themselves_are_refused(pkg, sampler, lens):
+    c = Case(sampler, pkg, lens, 2, 2, 64, 16, "bf16")
+    want, _ = c.run()
+    n = c.q.shape[0]
+    buf = torch.zeros((n + 4, 12, 64), dtype=torch.bfloat16, device="cuda")
+    buf[:n, :4] = c.q
+    c.q = buf[:n, :4]
+    flat = buf.view(-1)
+    lone = torch.zeros(n * 768, dtype=torch.bfloat16, device="cuda")
+    for out in (buf[1:n + 1, :4], buf[:n, 2:6], buf[:n, 0:8:2], flat[:n * 256].view(n, 4, 64),  # q's
+                torch.as_strided(lone, (n, 4, 64), (64, 64, 1)), torch.as_strided(lone, (n, 4, 64), (128, 64, 1))):  # their own
+        with pytest.raises(ValueError, match="must not"):
+            c.run(out=out)
+    for out in (buf[:n, 4:8], buf[:n, 4:12:2]):  # beside the query in its own buffer
+        got, _ = c.run(out=out)
+        assert torch.equal(got, want)
+    by_head = torch.empty((4, n, 64), dtype=torch.bfloat16, device="cuda").transpose(0, 1)
+    assert torch.equal(c.run(out=by_head)[0], want)
