@@ -192,6 +192,13 @@ def current_stream(device) -> int:
     return _raw_stream(device.index)
 
 
+def on_stream(stream: int, device):
+    """torch's current stream set to the raw handle ``stream``: what is allocated here belongs to it, so that
+    memory which work pending on another stream still uses is not handed out, nor this one's to another too early."""
+    import torch
+    return torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device))
+
+
 def build(force: bool = False) -> str:
     """Compiles libgsampler.so for sm_100a (make, nvcc)."""
     if force or not os.path.exists(LIB_PATH):

@@ -4,6 +4,8 @@ The caller owns the pools: ``k`` and ``v`` [pages, kv_heads, page_size, head_dim
 with contiguous, 16-byte aligned rows) of bfloat16, float8_e4m3fn or int8; 8-bit pools have
 one float32 scale per page, head and token, [pages, kv_heads, page_size].  A slot is
 page · page_size + offset; a sequence's cached token j lies in page page_table[b, j // page_size].
+``stream`` of a call is a raw stream handle in place of torch's current stream; outputs that the call
+allocates belong to the stream it runs on.
 """
 from __future__ import annotations
 
@@ -120,13 +122,20 @@ class GpuKvCache:
         (int32 [tokens]; negative: skipped)."""
         self._move(self._L.gs_kv_write, k, v, slots, stream)
 
+    def _new(self, slots, dtype):
+        heads, dim = self.kv_heads, self.head_dim
+        t = self._torch.bfloat16 if dtype is None else dtype
+        k = self._torch.empty_strided((slots.shape[0], heads, dim), (heads * dim, dim, 1), dtype=t, device=self._device)
+        return k, self._torch.empty_like(k)
+
     def read(self, slots, out=None, dtype=None, stream=None):
         """(k, v) [tokens, kv_heads, head_dim] at ``slots`` as ``dtype`` (bfloat16, or float32)."""
         if out is None:
-            heads, dim = self.kv_heads, self.head_dim
-            t = self._torch.bfloat16 if dtype is None else dtype
-            k = self._torch.empty_strided((slots.shape[0], heads, dim), (heads * dim, dim, 1), dtype=t, device=self._device)
-            out = (k, self._torch.empty_like(k))
+            if stream is None:
+                out = self._new(slots, dtype)
+            else:
+                with _lib.on_stream(stream, self._device):
+                    out = self._new(slots, dtype)
         self._move(self._L.gs_kv_read, out[0], out[1], slots, stream)
         return out
 
@@ -157,6 +166,11 @@ class GpuKvCache:
             if q_start.shape[0] != seqs + 1:
                 raise ValueError("q_start must hold one entry more than kv_len")
             starts = q_start.data_ptr()
+        if stream is not None and (out is None or (lse and lse_out is None)):
+            with _lib.on_stream(stream, self._device):
+                out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+                if lse and lse_out is None:
+                    lse_out = torch.empty((tokens, heads), dtype=torch.float32, device=self._device)
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
             ot, oh = heads * dim, dim

@@ -69,9 +69,19 @@ class GpuRmsNorm:
             raise ValueError(f"{what} rows must be contiguous")
         return s0 if rows > 1 else self.hidden
 
+    def _new(self, x, rows, with_residual):
+        torch, dev = self._torch, self._device
+        return RmsNormResult(
+            torch.empty_like(x, dtype=self._out_type, memory_format=torch.contiguous_format),
+            torch.empty_strided((rows, self.groups), (self.groups, 1), dtype=torch.float32, device=dev)
+            if self.out == "e4m3" else None,
+            torch.empty_like(x, memory_format=torch.contiguous_format) if with_residual else None,
+            torch.empty(rows, dtype=torch.float32, device=dev) if self.out == "srq" else None)
+
     def __call__(self, x, residual=None, *, out: RmsNormResult | None = None, stream=None) -> RmsNormResult:
         """The norm of x (+ residual), both [rows, hidden] float32 or bfloat16.  ``out``: a result
-        to write into (its ``residual`` may be the residual itself)."""
+        to write into (its ``residual`` may be the residual itself).  ``stream``: a raw stream handle in place of
+        torch's current one; results allocated here then belong to that stream."""
         torch, hidden, xt = self._torch, self.hidden, x.dtype
         dtype = self._types.get(xt)
         if dtype is None:
@@ -82,13 +92,11 @@ class GpuRmsNorm:
         ld_x = self._stride(x, "x", rows, xt)
         ld_r = self._stride(residual, "residual", rows, xt) if residual is not None else 0
         if out is None:
-            dev = self._device
-            out = RmsNormResult(
-                torch.empty_like(x, dtype=self._out_type, memory_format=torch.contiguous_format),
-                torch.empty_strided((rows, self.groups), (self.groups, 1), dtype=torch.float32, device=dev)
-                if self.out == "e4m3" else None,
-                torch.empty_like(x, memory_format=torch.contiguous_format) if residual is not None else None,
-                torch.empty(rows, dtype=torch.float32, device=dev) if self.out == "srq" else None)
+            if stream is None:
+                out = self._new(x, rows, residual is not None)
+            else:
+                with _lib.on_stream(stream, self._device):
+                    out = self._new(x, rows, residual is not None)
             ld_out = ld_ro = hidden
         else:
             ld_out = self._stride(out.out, "out.out", rows, self._out_type)

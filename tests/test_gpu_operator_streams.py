@@ -43,3 +43,53 @@ def test_an_error_right_after_a_check_is_kept(pkg, sampler):
         with pytest.raises(ValueError, match="slot"):
             cache.check()
     cache.check()
+
+
+class Pending:
+    """Memory that was freed while the current stream has still to write to it."""
+
+    def __init__(self, *shapes_and_types):
+        torch.cuda.synchronize()
+        torch.cuda.empty_cache()
+        held = [torch.empty(s, dtype=t, device="cuda") for s, t in shapes_and_types]
+        torch.cuda._sleep(int(1e8))
+        for t in held:
+            t.view(torch.uint8).fill_(0x7f)
+
+
+def test_outputs_of_another_stream_are_its_own(pkg, sampler):
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    side = torch.cuda.Stream()
+    x = torch.randn((64, 1024), generator=gen, device="cuda").to(torch.bfloat16)
+    norm = pkg.GpuRmsNorm(sampler, hidden=1024, out="e4m3", group=128)
+    want = norm(x, x)
+    Pending(((64, 1024), torch.uint8), ((64, 8), torch.float32), ((64, 1024), torch.bfloat16))
+    got = norm(x, x, stream=side.cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(got.out.view(torch.uint8), want.out.view(torch.uint8))
+    assert torch.equal(got.scale, want.scale) and torch.equal(got.residual, want.residual)
+
+    cache = pkg.GpuKvCache.allocate(sampler, 32, 4, 16, 128, "bf16")
+    kv = torch.randn((500, 8, 128), generator=gen, device="cuda").to(torch.bfloat16)
+    slots = torch.arange(500, dtype=torch.int32, device="cuda")
+    cache.write(kv[:, :4], kv[:, 4:], slots)
+    Pending(((500, 4, 128), torch.bfloat16), ((500, 4, 128), torch.bfloat16))
+    k, v = cache.read(slots, stream=side.cuda_stream)
+    torch.cuda.synchronize()
+    assert torch.equal(k, kv[:, :4]) and torch.equal(v, kv[:, 4:])
+
+    q = torch.randn((40, 8, 128), generator=gen, device="cuda").to(torch.bfloat16)
+    starts, n = (torch.tensor(t, dtype=torch.int32, device="cuda") for t in ([0, 40], [500]))
+    table = torch.arange(32, dtype=torch.int32, device="cuda")[None]
+    call = dict(max_q=40, max_kv=512, scale=0.1, lse=True)
+    want = cache.attend(q, starts, n, table, **call)
+    Pending(((40, 8, 128), torch.bfloat16), ((40, 8), torch.float32))
+    got = cache.attend(q, starts, n, table, stream=side.cuda_stream, **call)
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    # given outputs are used as they are, and the default stream has a handle too
+    out = torch.empty_like(q)
+    assert cache.attend(q, starts, n, table, stream=0, out=out, **call)[0] is out
+    torch.cuda.synchronize()
+    assert torch.equal(out, want[0])
+    cache.check()
