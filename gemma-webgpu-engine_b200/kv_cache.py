@@ -62,6 +62,8 @@ class GpuKvCache:
         self._int32, self._bf16 = torch.int32, torch.bfloat16
         self._types = {torch.bfloat16: _lib.GS_DTYPE_BF16, torch.float32: _lib.GS_DTYPE_F32}
         self._h = ctypes.c_void_p()
+        if not sampler.handle:
+            raise ValueError("the sampler is closed")
         st = self._L.gs_kv_cache_create(sampler.handle, ctypes.byref(d), ctypes.byref(self._h))
         if st != _lib.GS_OK:
             msg = sampler.last_error()
@@ -95,6 +97,12 @@ class GpuKvCache:
         msg = (self._L.gs_kv_cache_last_error(self._h) or b"").decode()
         raise ValueError(msg) if st == _lib.GS_EINVAL else SamplerError(st, msg)
 
+    def _open(self):
+        # (the attention workspace is the context's: a closed sampler has given it back)
+        if not self._h or not self._sampler.handle:
+            raise ValueError("the cache or its sampler is closed")
+        return self._h
+
     def _index(self, t, what, dims):
         if t.dtype is not self._int32 or t.dim() != dims or t.get_device() != self._sampler.device:
             raise ValueError(f"{what} must be an int32 tensor of {dims} dimension(s) on the sampler's device")
@@ -112,7 +120,7 @@ class GpuKvCache:
         v0, v1, v2 = v.stride() if v.dim() == 3 else (0, 0, 0)
         if k.shape != shape or v.shape != shape or k2 != 1 or v2 != 1 or k.get_device() != dev or v.get_device() != dev:
             raise ValueError(f"k and v must be {list(shape)} with contiguous rows on the sampler's device")
-        st = call(self._h, _KV_ROWS.pack(k.data_ptr(), v.data_ptr(), k0, k1, v0, v1, slots.data_ptr(), n, dtype),
+        st = call(self._open(), _KV_ROWS.pack(k.data_ptr(), v.data_ptr(), k0, k1, v0, v1, slots.data_ptr(), n, dtype),
                   _lib.current_stream(self._device) if stream is None else stream)
         if st != _lib.GS_OK:
             self._fail(st)
@@ -186,7 +194,7 @@ class GpuKvCache:
         elif lse:
             lse_out = torch.empty_strided((tokens, heads), (heads, 1), dtype=torch.float32, device=self._device)
         st = self._L.gs_attention(
-            self._h, _ATTENTION_ARGS.pack(
+            self._open(), _ATTENTION_ARGS.pack(
                 q.data_ptr(), out.data_ptr(), lse_out.data_ptr() if lse_out is not None else 0, starts, kv_len.data_ptr(),
                 page_table.data_ptr(), tokens, qt, qh, ot, oh, page_table.stride(0) if seqs > 1 else cols, cols, seqs, heads,
                 max_q, max_kv, window, sinks, scale),
@@ -199,6 +207,6 @@ class GpuKvCache:
         """Raises when a kernel met a bad slot, page-table entry or length since the last check
         (synchronises)."""
         bits = ctypes.c_int32()
-        st = self._L.gs_kv_cache_check(self._h, ctypes.byref(bits))
+        st = self._L.gs_kv_cache_check(self._open(), ctypes.byref(bits))
         if st != _lib.GS_OK:
             self._fail(st)

@@ -105,6 +105,8 @@ class GpuRmsNorm:
                 if t is not None and (t.dtype != torch.float32 or t.shape != shape or not t.is_contiguous() or
                                       t.get_device() != self._sampler.device):
                     raise ValueError(f"out's scale and row_sum must be contiguous float32 {shape} on the sampler's device")
+        if not self._sampler.handle:
+            raise ValueError("the sampler is closed")
         a = _RMS_NORM_ARGS.pack(
             x.data_ptr(), residual.data_ptr() if residual is not None else 0, self._weight_ptr,
             out.residual.data_ptr() if out.residual is not None else 0, out.out.data_ptr(),

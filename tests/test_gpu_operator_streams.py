@@ -93,3 +93,31 @@ def test_outputs_of_another_stream_are_its_own(pkg, sampler):
     torch.cuda.synchronize()
     assert torch.equal(out, want[0])
     cache.check()
+
+
+def test_closed_handles_are_refused(pkg):
+    sampler = pkg.GpuSampler(0)
+    cache, other = (pkg.GpuKvCache.allocate(sampler, 4, 2, 16, 64, "bf16") for _ in range(2))
+    norm = pkg.GpuRmsNorm(sampler, hidden=64)
+    x = torch.zeros((1, 2, 64), dtype=torch.bfloat16, device="cuda")
+    slots, n = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+    table = torch.zeros((1, 1), dtype=torch.int32, device="cuda")
+
+    def calls(c):
+        return (lambda: c.write(x, x, slots), lambda: c.read(slots), c.check,
+                lambda: c.attend(x, None, n, table, max_kv=16, scale=0.1))
+    for f in calls(cache):
+        f()
+    other.close()
+    for f in calls(other):
+        with pytest.raises(ValueError, match="closed"):
+            f()
+    for f in calls(cache):
+        f()
+    torch.cuda.synchronize()
+    sampler.close()
+    for f in calls(cache) + (lambda: norm(x[0]), lambda: pkg.GpuKvCache.allocate(sampler, 4, 2, 16, 64, "bf16")):
+        with pytest.raises(ValueError, match="closed"):
+            f()
+    cache.close()
+    other.close()
