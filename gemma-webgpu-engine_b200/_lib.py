@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import subprocess
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -190,6 +191,14 @@ def current_stream(device) -> int:
         import torch
         _raw_stream = torch._C._cuda_getCurrentRawStream
     return _raw_stream(device.index)
+
+
+def pack_args(packer, *values) -> bytes:
+    """An argument structure's bytes; a number that its field does not hold is a ValueError like other bad arguments."""
+    try:
+        return packer.pack(*values)
+    except (struct.error, OverflowError) as e:
+        raise ValueError(f"an argument is out of range: {e}") from None
 
 
 def on_stream(stream: int, device):

@@ -120,7 +120,7 @@ class GpuKvCache:
         v0, v1, v2 = v.stride() if v.dim() == 3 else (0, 0, 0)
         if k.shape != shape or v.shape != shape or k2 != 1 or v2 != 1 or k.get_device() != dev or v.get_device() != dev:
             raise ValueError(f"k and v must be {list(shape)} with contiguous rows on the sampler's device")
-        st = call(self._open(), _KV_ROWS.pack(k.data_ptr(), v.data_ptr(), k0, k1, v0, v1, slots.data_ptr(), n, dtype),
+        st = call(self._open(), _lib.pack_args(_KV_ROWS, k.data_ptr(), v.data_ptr(), k0, k1, v0, v1, slots.data_ptr(), n, dtype),
                   _lib.current_stream(self._device) if stream is None else stream)
         if st != _lib.GS_OK:
             self._fail(st)
@@ -194,8 +194,8 @@ class GpuKvCache:
         elif lse:
             lse_out = torch.empty_strided((tokens, heads), (heads, 1), dtype=torch.float32, device=self._device)
         st = self._L.gs_attention(
-            self._open(), _ATTENTION_ARGS.pack(
-                q.data_ptr(), out.data_ptr(), lse_out.data_ptr() if lse_out is not None else 0, starts, kv_len.data_ptr(),
+            self._open(), _lib.pack_args(
+                _ATTENTION_ARGS, q.data_ptr(), out.data_ptr(), lse_out.data_ptr() if lse_out is not None else 0, starts, kv_len.data_ptr(),
                 page_table.data_ptr(), tokens, qt, qh, ot, oh, page_table.stride(0) if seqs > 1 else cols, cols, seqs, heads,
                 max_q, max_kv, window, sinks, scale),
             _lib.current_stream(self._device) if stream is None else stream)

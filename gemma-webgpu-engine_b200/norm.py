@@ -107,8 +107,8 @@ class GpuRmsNorm:
                     raise ValueError(f"out's scale and row_sum must be contiguous float32 {shape} on the sampler's device")
         if not self._sampler.handle:
             raise ValueError("the sampler is closed")
-        a = _RMS_NORM_ARGS.pack(
-            x.data_ptr(), residual.data_ptr() if residual is not None else 0, self._weight_ptr,
+        a = _lib.pack_args(
+            _RMS_NORM_ARGS, x.data_ptr(), residual.data_ptr() if residual is not None else 0, self._weight_ptr,
             out.residual.data_ptr() if out.residual is not None else 0, out.out.data_ptr(),
             out.scale.data_ptr() if out.scale is not None else 0, out.row_sum.data_ptr() if out.row_sum is not None else 0,
             rows, hidden, ld_x, ld_r, ld_ro, ld_out, dtype, *self._tail)

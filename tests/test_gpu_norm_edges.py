@@ -37,3 +37,10 @@ def test_a_nan_row_reaches_the_sampler(pkg, sampler):
     res = head.sample(r.out, r.row_sum, pkg.params_from_config(dict(pkg.DEFAULT_DECODING_CONFIG, temperature=0)))
     flags = res.flags.tolist()
     assert flags[1] & pkg._lib.FLAG_ERR_NONFINITE and not (flags[0] | flags[2]) & pkg._lib.FLAG_ERRORS
+
+
+def test_numbers_out_of_range_are_refused(pkg, sampler):
+    x = torch.ones((2, 64), device="cuda")
+    for bad in (dict(eps=1e300), dict(weight_offset=-1e300), dict(group=2 ** 40, out="e4m3")):
+        with pytest.raises(ValueError):
+            pkg.GpuRmsNorm(sampler, hidden=64, **bad)(x)
