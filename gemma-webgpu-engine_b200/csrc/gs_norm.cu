@@ -80,20 +80,6 @@ __device__ __forceinline__ void square_row(const float (&a)[V], float2& s) {
       s = __ffma2_rn(x, x, s);
     }
 }
-// 448 / a for a >= 2^-64 by the approximate reciprocal and one step that takes up its remainder (the
-// reciprocal is 0 from 2^126 on: there the quotient), and a / 448 by the same step.  Without the step each is an
-// ulp off now and then, and a twentieth more codes fall on the other side of a rounding boundary than with the quotients.
-__device__ __forceinline__ float norm_inv(float a) {
-  const float f = quant_floor(a);
-  if (!(f < 8.0e37f)) return __fdiv_rn(kE4m3Max, f);
-  const float r = __fdividef(1.0f, f), q = kE4m3Max * r;
-  return fmaf(fmaf(-q, f, kE4m3Max), r, q);
-}
-__device__ __forceinline__ float norm_scale(float a) {
-  const float f = quant_floor(a), q = f * (1.0f / kE4m3Max);
-  return f < INFINITY ? fmaf(fmaf(-q, kE4m3Max, f), 1.0f / kE4m3Max, q) : q;
-}
-
 // x within [lo, hi]; a NaN stays one (fminf and fmaxf alone would make it a code like any other).
 __device__ __forceinline__ float clamp_nan(float x, float lo, float hi) { return x != x ? x : fminf(fmaxf(x, lo), hi); }
 
@@ -250,7 +236,7 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(const __grid_constant__ Norm
         if (span > 8) gm[p] = max_nan(gm[p], __shfl_xor_sync(kFullMask, gm[p], 8));
         const int col = (t + p * tpr) * V;
         if (col < A.hidden && live && (lane & (span - 1)) == 0)
-          scales[col >> A.shift] = norm_scale(gm[p]);
+          scales[col >> A.shift] = quant_scale(gm[p], kE4m3Max);
       }
     } else {
       int* gr = gmax + threadIdx.y * A.groups;
@@ -276,7 +262,7 @@ __global__ void __launch_bounds__(MAXT) norm_kernel(const __grid_constant__ Norm
     for (int p = 0; p < PIECES; ++p) {
       const int col = (t + p * tpr) * V;
       if (in[p]) {
-        const float inv = norm_inv(gm[p]);
+        const float inv = quant_inv(gm[p], kE4m3Max);
         if constexpr (V == 8) {
           uint2 c;
           scale_row(h[p], inv);

@@ -44,3 +44,22 @@ def test_numbers_out_of_range_are_refused(pkg, sampler):
     for bad in (dict(eps=1e300), dict(weight_offset=-1e300), dict(group=2 ** 40, out="e4m3")):
         with pytest.raises(ValueError):
             pkg.GpuRmsNorm(sampler, hidden=64, **bad)(x)
+
+
+@pytest.mark.parametrize("rows,hidden", [(3, 64), (700, 1536), (5, 77), (400, 1111), (300, 8192)])
+@pytest.mark.parametrize("group", [0, 32, 128])
+def test_codes_and_scales_are_the_quotients(pkg, sampler, rows, hidden, group):
+    """scale = a / 448 and code = round(y · (448 / a)), each quotient rounded once, on the y that the same norm
+    gives as float32; a from 2^-64 up."""
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.randn((rows, hidden), generator=gen, device="cuda") * torch.exp2(torch.randint(-30, 30, (1, hidden), generator=gen, device="cuda").float())
+    w = torch.randn(hidden, generator=gen, device="cuda") * torch.exp2(torch.randint(-90, 60, (hidden,), generator=gen, device="cuda").float())
+    y = pkg.GpuRmsNorm(sampler, w, out="f32")(x).out
+    got = pkg.GpuRmsNorm(sampler, w, out="e4m3", group=group)(x)
+    g = group or hidden
+    for i in range(0, hidden, g):
+        part = y[:, i:i + g]
+        a = part.abs().amax(dim=1, keepdim=True).clamp(min=2.0 ** -64)
+        most = torch.full_like(a, 448.0)  # (a quotient of tensors: torch turns one by a number into a product)
+        assert torch.equal(got.scale[:, i // g:i // g + 1], a / most)
+        assert torch.equal(got.out[:, i:i + g].view(torch.uint8), (part * (most / a)).to(torch.float8_e4m3fn).view(torch.uint8))
