@@ -291,15 +291,23 @@ cudaError_t launch_norm_v(const NormArgs& a, cudaStream_t st) {
   const unsigned grid = static_cast<unsigned>((a.rows + rpb - 1) / rpb);
   const size_t smem = (OUT == kOutE4m3 && V == 1 && a.groups > 1) ? sizeof(int) * rpb * a.groups : 0;
   const bool wide = tpr > 256;
-  if (per <= 1 && !wide) norm_kernel<BF16, OUT, V, 1, 256><<<grid, block, smem, st>>>(a);
-  else if (per <= 1) norm_kernel<BF16, OUT, V, 1, 1024><<<grid, block, smem, st>>>(a);
-  else if (per <= 2 && !wide) norm_kernel<BF16, OUT, V, 2, 256><<<grid, block, smem, st>>>(a);
-  else if (per <= 2) norm_kernel<BF16, OUT, V, 2, 1024><<<grid, block, smem, st>>>(a);
-  else if (per <= 4 && !wide) norm_kernel<BF16, OUT, V, 4, 256><<<grid, block, smem, st>>>(a);
-  else if (per <= 4) norm_kernel<BF16, OUT, V, 4, 1024><<<grid, block, smem, st>>>(a);
-  else if (per <= 8) norm_kernel<BF16, OUT, V, V == 1 ? 8 : 4, 1024><<<grid, block, smem, st>>>(a);
-  else if (per <= 16) norm_kernel<BF16, OUT, V, V == 1 ? 16 : 4, 1024><<<grid, block, smem, st>>>(a);
-  else norm_kernel<BF16, OUT, V, V == 1 ? 32 : 4, 1024><<<grid, block, smem, st>>>(a);
+  // (V = 8: at most 4096 pieces, so at most 2 a thread but for rows of 1024 threads; V = 1: at most 32768)
+  auto run = [&](auto pieces_, auto threads_) {
+    norm_kernel<BF16, OUT, V, decltype(pieces_)::value, decltype(threads_)::value><<<grid, block, smem, st>>>(a);
+  };
+  using std::integral_constant;
+  constexpr integral_constant<int, 256> narrow{};
+  constexpr integral_constant<int, 1024> most{};
+  if (per <= 1 && !wide) run(integral_constant<int, 1>{}, narrow);
+  else if (per <= 1) run(integral_constant<int, 1>{}, most);
+  else if (per <= 2 && !wide) run(integral_constant<int, 2>{}, narrow);
+  else if (per <= 2) run(integral_constant<int, 2>{}, most);
+  else if constexpr (V == 8) run(integral_constant<int, 4>{}, most);
+  else if (per <= 4 && !wide) run(integral_constant<int, 4>{}, narrow);
+  else if (per <= 4) run(integral_constant<int, 4>{}, most);
+  else if (per <= 8) run(integral_constant<int, 8>{}, most);
+  else if (per <= 16) run(integral_constant<int, 16>{}, most);
+  else run(integral_constant<int, 32>{}, most);
   return cudaGetLastError();
 }
 
