@@ -48,6 +48,7 @@ constexpr int kRowsWarps = 4;
 constexpr int kRowsThreads = kRowsWarps * 32;
 constexpr int kRT = 16;  // tokens per warp tile
 constexpr float kPScale = 128.0f;
+constexpr float kLeastScale = 7.888609052210118e-31f;  // 2^-100: reference of V scales below it (its reciprocal is finite)
 constexpr float kSlack = 8.0f;  // log2 units a score may pass the reference by
 
 template <int D, int FMT>
@@ -527,12 +528,12 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
         // new references: every row's largest score so far, the largest V scale so far
         float vfac = 1.0f;
         if constexpr (!kBf) {
-          float vm = fmaxf(vref, fmaxf(fabsf(vsc[0]), fabsf(vsc[1])));
+          float vm = fmaxf(fmaxf(vref, kLeastScale), fmaxf(fabsf(vsc[0]), fabsf(vsc[1])));
 #pragma unroll
           for (int d = 4; d < 32; d <<= 1) vm = fmaxf(vm, __shfl_xor_sync(kFullMask, vm, d));
           vfac = vm > vref ? vref / vm : 1.0f;
           vref = vm;
-          vinv = vref > 0.0f ? kPScale / vref : 0.0f;
+          vinv = kPScale / vref;
         }
         float al[NB][2];
 #pragma unroll

@@ -410,7 +410,9 @@ gs_status gs_kv_read(gs_kv_cache* c, const gs_kv_rows* rows, void* stream);
  * e^(s_j - running max) are rounded to bf16 for the second product, beside an 8-bit cache
  * their product with the value's scale to float16.  (Beside an 8-bit cache q enters the first
  * product as float16 after an exact power of two per row: components below 2^-17 of the row's
- * largest lose bits.)  The same call gives the same bits every time.
+ * largest lose bits.  V scales have their full accuracy from 2^-60 to 2^60; weights beside smaller or
+ * larger ones lose bits.)  Weights reach 2^8 before they are divided by their sum: |v| times the tokens
+ * times 2^8 has to be a float32.  The same call gives the same bits every time.
  * Rows of q that lie in no sequence are not read, and their out and lse not written.
  * The calls of one context use its workspace: order them on the GPU (one stream, or
  * events between streams), as for gs_sample. */

@@ -242,3 +242,22 @@ def test_results_that_overlap_the_query_or_themselves_are_refused(pkg, sampler, 
         assert torch.equal(got, want)
     by_head = torch.empty((4, n, 64), dtype=torch.bfloat16, device="cuda").transpose(0, 1)
     assert torch.equal(c.run(out=by_head)[0], want)
+
+
+@pytest.mark.parametrize("lens", [FEW, MANY])
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("form", ["e4m3", "int8"])
+@pytest.mark.parametrize("factor", [0.0, 2.0 ** -30, 2.0 ** -126, 2.0 ** 55])
+def test_cache_scales_of_any_size(pkg, sampler, form, dim, lens, factor):
+    """Down to scales whose reciprocal is no float32: the result is finite, and small where the values are."""
+    c = Case(sampler, pkg, lens, 2, 3, dim, 16, form, seed=dim)
+    c.cache.v_scale.mul_(factor)
+    c.vd = R.pool_values(c.cache.v, c.cache.v_scale)
+    out, lse = c.run()
+    ref = c.reference()
+    assert out.isfinite().all()
+    if 2.0 ** -60 < c.cache.v_scale.max().item():
+        scaled = [ref[0] / factor, ref[1], ref[2] / factor, ref[3]]
+        R.check_attend((out.double() / factor), lse, scaled)
+    else:
+        assert (out.double() - ref[0]).abs().max().item() <= 2.0 ** -80
