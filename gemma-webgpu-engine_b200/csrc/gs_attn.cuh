@@ -101,6 +101,11 @@ struct RowRange {
     return t0 + t;
   }
   __device__ __forceinline__ bool seen_by_any(int j) const { return j < hi && (j >= lo || j < sink); }
+  // Tokens that some rows see and others do not: from ahead0 to hi (some row's position is before them), and from left0 to left1
+  // (some row's window has left them).
+  __device__ __forceinline__ int ahead0() const { return max(p0 + t0 + 1, 0); }
+  __device__ __forceinline__ int left0() const { return max(sink, lo); }
+  __device__ __forceinline__ int left1(const AttnArgs& A) const { return min(hi - A.window, p0 + t0 + 1); }
   // Whether every row sees the tokens j .. j + n - 1.
   __device__ __forceinline__ bool seen_by_all(const AttnArgs& A, int j, int n = 1) const {
     return j + n - 1 <= p0 + t0 && (!A.window || j > hi - 1 - A.window || j + n <= sink);
@@ -188,13 +193,28 @@ template <int FMT>
 __device__ __forceinline__ uint4 not_finite_in(uint4 w) {
   return make_uint4(not_finite_in<FMT>(w.x), not_finite_in<FMT>(w.y), not_finite_in<FMT>(w.z), not_finite_in<FMT>(w.w));
 }
-// Whether there are any among four words: the next larger exponent (e4m3: code) carries into the sign's place.
+// Whether there are any: four words' elements are added to a NaN or a number other than zero for the first that is one, else zero
+// (bf16: an infinity or a NaN times zero; e4m3: the next code after the largest carries into the sign's place).
+template <int FMT>
+__device__ __forceinline__ void look_for_not_finite(uint4 w, uint32_t& found) {
+  if constexpr (FMT == GS_DTYPE_BF16) {
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(found) : "r"(x[i]), "r"(0u));
+  } else if constexpr (FMT == GS_DTYPE_E4M3) {
+    constexpr uint32_t kCode = 0x7f7f7f7fu, kOne = 0x01010101u;
+    found |= ((w.x & kCode) + kOne) | ((w.y & kCode) + kOne) | ((w.z & kCode) + kOne) | ((w.w & kCode) + kOne);
+  }
+}
+template <int FMT>
+__device__ __forceinline__ bool found_not_finite(uint32_t found) {
+  return FMT == GS_DTYPE_BF16 ? (found & 0x7fff7fffu) != 0u : FMT == GS_DTYPE_E4M3 ? (found & 0x80808080u) != 0u : false;
+}
 template <int FMT>
 __device__ __forceinline__ bool any_not_finite(uint4 w) {
-  if constexpr (FMT == GS_DTYPE_INT8) return false;
-  constexpr uint32_t kField = FMT == GS_DTYPE_BF16 ? 0x7f807f80u : 0x7f7f7f7fu, kOne = FMT == GS_DTYPE_BF16 ? 0x00800080u : 0x01010101u;
-  const uint32_t m = ((w.x & kField) + kOne) | ((w.y & kField) + kOne) | ((w.z & kField) + kOne) | ((w.w & kField) + kOne);
-  return (m & (FMT == GS_DTYPE_BF16 ? 0x80008000u : 0x80808080u)) != 0u;
+  uint32_t found = 0u;
+  look_for_not_finite<FMT>(w, found);
+  return found_not_finite<FMT>(found);
 }
 __device__ __forceinline__ uint4 without4(uint4 w, uint4 m) { return make_uint4(w.x & ~m.x, w.y & ~m.y, w.z & ~m.z, w.w & ~m.w); }
 

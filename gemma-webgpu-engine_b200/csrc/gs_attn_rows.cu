@@ -18,7 +18,7 @@
 // A row's reference point m moves only when a score passes it by 2^8 (as V's reference scale does
 // when a larger one comes), so the usual tile needs one vote instead of reductions and rescaling.
 // Values of tokens hidden from every row of the block are set to zero before they are used, and so is what is not finite in
-// those hidden from some, which is added to the other rows' output as it stands.
+// those hidden from some, whose columns are then a NaN in the rows that see them.
 //
 // A context is shared evenly by the blocks of a cluster (up to 8), which join their (m, l, O) through
 // distributed shared memory; of several clusters per context the last to finish joins their partial
@@ -192,6 +192,45 @@ constexpr int rows_occupancy() {
   return by_smem < by_regs ? (by_smem < 1 ? 1 : by_smem) : by_regs;
 }
 
+// What is not finite in the V tile at vs (tokens j0 ..) and in tokens that some rows of the block see and others do not: set to
+// zero, and its columns marked in the rows that see it (odd: words of 32 columns; scale_odd: tokens whose scale is not finite, all of
+// their columns).  By a warp; whether this lane wrote to the tile.  (R lies in shared memory: the main loop has no registers for it.  What this
+// costs drafted tokens: 20 rows of 256 25.5 -> 26.0 us bf16, 24.7 -> 25.5 e4m3, 32 rows of 128 49.1 -> 50.7 bf16, most of it
+// by the registers of the main loop.)
+template <int D, int FMT>
+__device__ __forceinline__ bool leave_odd_out(const AttnArgs& A, const RowRange& R, uint32_t vs, int j0, unsigned scale_odd, uint32_t* odd, int* any) {
+  using P = RowsPlan<D, FMT>;
+  constexpr int kPc = P::kRow / 16;
+  const int lane = threadIdx.x & 31;
+  uint32_t all = 0u;
+#pragma unroll
+  for (int id = lane; id < kRT * kPc; id += 32) {
+    uint32_t found = 0u;
+    look_for_not_finite<FMT>(ld_shared4(vs + piece<P::kInner>(id / kPc, id % kPc)), found);
+    all |= found;
+  }
+  if (!__any_sync(kFullMask, found_not_finite<FMT>(all)) && scale_odd == 0u) return false;
+  bool wrote = false;
+  for (int t = 0; t < kRT; ++t) {
+    const int j = j0 + t;
+    if (!R.seen_by_any(j) || R.seen_by_all(A, j)) continue;
+    for (int at = lane * 4; at < P::kRow; at += 128) {  // a word of the token's row
+      const uint32_t w = vs + piece<P::kInner>(t, at / 16) + (at & 12), x = ld_shared1(w), m = scale_odd >> t & 1u ? ~0u : not_finite_in<FMT>(x);
+      if (m == 0u) continue;
+      asm volatile("st.shared.u32 [%0], %1;" ::"r"(w), "r"(x & ~m) : "memory");
+      wrote = true;
+      *any = 1;
+      for (int r = 0, g = R.g0, p = R.p0 + R.t0; r < R.rows; ++r, ++g) {
+        if (g == A.group) g = 0, ++p;
+        if (j > p || (A.window && j <= p - A.window && j >= A.sinks)) continue;
+        for (int b = 0; b < 4; b += P::kEl)
+          if (m >> (8 * b) & 1u) atomicOr(odd + (r * D + (at + b) / P::kEl) / 32, 1u << ((at + b) / P::kEl & 31));
+      }
+    }
+  }
+  return wrote;
+}
+
 template <int D, int FMT, int NB>
 __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
     attn_rows_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ RowsMaps maps) {
@@ -208,6 +247,9 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
   __shared__ float s_m[kRowsWarps][kRows], s_l[kRowsWarps][kRows], s_f[kRowsWarps];
   __shared__ float s_qf[kRows];
   __shared__ __align__(8) float s_ml[kRows][2];  // the block's joined maximum and sum
+  __shared__ uint32_t s_odd[kRows][D / 32];  // columns of rows that have a value which is not finite and was left out of the product
+  __shared__ int s_any;                      // whether there are any
+  __shared__ RowRange s_range;
   __shared__ __align__(8) uint64_t s_bar[kRowsWarps][P::kStages];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -222,6 +264,8 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
   const int i_begin = min(static_cast<int>(blockIdx.x) * share, R.tiles);
   const int i_end = min(i_begin + share, R.tiles);
   if (lane < P::kStages) mbar_init(&s_bar[warp][lane], 1);
+  for (int i = tid; i < kRows * (D / 32); i += kRowsThreads) s_odd[0][i] = 0u;
+  if (tid == 0) s_any = 0, s_range = R;
   __syncwarp();
 
   // ---- the warp's ring: stage i holds the warp's step i, tiles i_begin + (i · 4 + warp) · kSub .., or (halves)
@@ -445,65 +489,25 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
         if (!ok) break;
       }
       if (!whole) {
-        // tokens no row sees (past the context, before every window): their pages may hold anything; of tokens that some rows
-        // see, what is not finite (rows of one token all see the same ones)
+        // tokens no row sees (past the context, before every window): their pages may hold anything
         constexpr int kPc = P::kRow / 16;
         bool wrote = false;
-        unsigned odd = 0u;  // tokens with such values
         for (int id = lane; id < kRT * kPc; id += 32) {
           const int r = id / kPc, ch = id % kPc;
-          const uint32_t at = vs + piece<P::kInner>(r, ch);
           if (!R.seen_by_any(j0 + r)) {
-            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0u) : "memory");
-            wrote = true;
-          } else if (FMT != GS_DTYPE_INT8 && A.max_q > 1 && !R.seen_by_all(A, j0 + r)) {
-            if (any_not_finite<FMT>(ld_shared4(at))) odd |= 1u << r;
-          }
-        }
-        bool scale_odd[2] = {false, false};  // (8-bit) of this lane's two tokens
-        if constexpr (!kBf) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            scale_odd[h] = !(fabsf(vsc[h]) < INFINITY) && A.max_q > 1 && !R.seen_by_all(A, j0 + g + 8 * h);
-            if (scale_odd[h]) odd |= 1u << (g + 8 * h), vsc[h] = 0.0f;
-          }
-        }
-        odd = __reduce_or_sync(kFullMask, odd);
-        if (odd) {
-          for (unsigned rest = odd; rest; rest &= rest - 1) {
-            const int r = __ffs(rest) - 1, j = j0 + r;
-            bool seen[NB][2];
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) seen[nb][h] = j <= pos[nb][h] && (!A.window || j > pos[nb][h] - A.window || j < A.sinks);
-            const bool all = __shfl_sync(kFullMask, (r < 8 ? scale_odd[0] : scale_odd[1]) ? 1 : 0, (r & 7) * 4) != 0;
-#pragma unroll
-            for (int k = 0; k < KS; ++k)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int at = (kBf ? 16 * k + g + 8 * h : 16 * k + 2 * g + h) * P::kEl;  // (this lane's value of O's column)
-                const uint32_t w = ld_shared1(vs + piece<P::kInner>(r, at / 16) + (at & 12));
-                const uint32_t el = kBf ? (w >> (at & 2) * 8) << 16 : (w >> (at & 3) * 8) & 0xffu;
-                const float x = kBf ? __uint_as_float(el) : all || (FMT == GS_DTYPE_E4M3 && (el & 0x7fu) == 0x7fu) ? NAN : 0.0f;
-                if (!(fabsf(x) < INFINITY)) {
-#pragma unroll
-                  for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u)
-                      if (seen[nb][u]) o[nb][k][2 * h + u] += x;
-                }
-              }
-          }
-          __syncwarp();
-          for (int id = lane; id < kRT * kPc; id += 32) {
-            const int r = id / kPc, ch = id % kPc;
-            if (!(odd >> r & 1u)) continue;
-            const uint32_t at = vs + piece<P::kInner>(r, ch);
-            const uint4 w = ld_shared4(at), x = without4(w, not_finite_in<FMT>(w));
-            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(x.x), "r"(x.y), "r"(x.z), "r"(x.w) : "memory");
+            asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vs + piece<P::kInner>(r, ch)), "r"(0u) : "memory");
             wrote = true;
           }
+        }
+        if (A.max_q > 1) {  // (rows of one token all see the same ones)
+          unsigned scale_odd = 0u;
+          if constexpr (!kBf) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (!(fabsf(vsc[h]) < INFINITY) && !s_range.seen_by_all(A, j0 + g + 8 * h)) scale_odd |= 1u << (g + 8 * h), vsc[h] = 0.0f;
+            scale_odd = __reduce_or_sync(kFullMask, scale_odd);
+          }
+          if (FMT != GS_DTYPE_INT8 || scale_odd) wrote |= leave_odd_out<D, FMT>(A, s_range, vs, j0, scale_odd, &s_odd[0][0], &s_any);
         }
         if (wrote) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // (before the stage's next copy)
         __syncwarp();
@@ -643,6 +647,11 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
       }
   __syncthreads();
   float* oj = reinterpret_cast<float*>(smem);
+  if (s_any) {  // (into warp 0's part: whatever is added to it is a NaN)
+    for (int i = tid; i < R.rows * D; i += kRowsThreads)
+      if (s_odd[i / D][i % D / 32] >> (i % 32) & 1u) oj[i / D * (D + 4) + i % D] = NAN;
+    __syncthreads();
+  }
   const bool alone = A.cluster == 1;
   // the (m, l, O) of a row's four values as the result
   auto put = [&](int r, int d, float M, float L, float4 acc) {

@@ -372,6 +372,9 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
   uint64_t* raw_full = q_full + 1;                  // [kRawStages]
   uint64_t* raw_free = raw_full + P::kRawStages;    // [kRawStages]
   uint64_t* peer_full = raw_free + P::kRawStages;   // [kStages] (CG 2, first block): the other block's stage is there
+  uint64_t* looked = peer_full + (CG == 2 ? P::kStages : 0);  // [2] (fixed, bf16): V of the tokens that some rows' windows have left, or
+  int* odd_v = reinterpret_cast<int*>(looked + 2);            // that some rows do not reach, has been looked at; whether there is what is not finite
+  static_assert(8 * (2 * P::kStages + 2 * P::kRawStages + (CG == 2 ? P::kStages : 0) + 12) <= 512, "barriers");
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(m_done + 1);
   volatile int* stop = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -480,6 +483,9 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       mbar_init(raw_full + s, 1);
       mbar_init(raw_free + s, P::kWideners);
     }
+    mbar_init(looked, 2);
+    mbar_init(looked + 1, 2);
+    *odd_v = 0;
     *stop = 0;
   }
   if (warp == P::kMmaWarp) {
@@ -632,8 +638,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       const unsigned char* src = sm + P::kOffRaw + rs * P::kRawStage;
       unsigned char* dst = sm + P::kOffStage + at * P::kStage;
       // TOKS tokens in column blocks of INNER codes.  MIXED: a V stage with tokens that not every row sees: those that no row sees are
-      // zeros, and where there are codes that are not finite (looked for in all pieces at once: a branch in
-      // each costs 4% of a call of short windows) their pieces are taken again without them.
+      // zeros, and codes that are not finite are left out of the others.
       auto turn = [&](auto mixed_, auto toks_, auto inner_) {
         constexpr bool MIXED = decltype(mixed_)::value;
         constexpr int TOKS = decltype(toks_)::value, INNER = decltype(inner_)::value;
@@ -650,21 +655,20 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
           *reinterpret_cast<uint4*>(rowp + (((c0 + odd) ^ (tr & 7)) << 4)) = odd ? hi : lo;
           *reinterpret_cast<uint4*>(rowp + (((c0 + 1 - odd) ^ (tr & 7)) << 4)) = odd ? lo : hi;
         };
-        bool any = false;
+        if constexpr (!MIXED) {
 #pragma unroll
-        for (int u = 0; u < kPieces; ++u) {
-          const int id = lt + P::kWideners * u;
-          const uint4 x = *reinterpret_cast<const uint4*>(src + id * 16);
-          if constexpr (MIXED) any |= any_not_finite<FMT>(x);
-          put(id, x, MIXED && !R.seen_by_any(jt + id / (INNER / 16) % TOKS));
-        }
-        if (MIXED && any) {
+          for (int u = 0; u < kPieces; ++u) put(lt + P::kWideners * u, *reinterpret_cast<const uint4*>(src + (lt + P::kWideners * u) * 16), false);
+        } else {
+#pragma unroll 1
           for (int u = 0; u < kPieces; ++u) {
             const int id = lt + P::kWideners * u, tok = jt + id / (INNER / 16) % TOKS;
-            const uint4 x = *reinterpret_cast<const uint4*>(src + id * 16);
-            if (!any_not_finite<FMT>(x) || !R.seen_by_any(tok) || R.seen_by_all(A, tok)) continue;
-            put(id, without4(x, not_finite_in<FMT>(x)), false);
-            A.mend[0] = 1u;  // (attn_mend_kernel)
+            uint4 x = *reinterpret_cast<const uint4*>(src + id * 16);
+            const bool hide = !R.seen_by_any(tok);
+            if (any_not_finite<FMT>(x) && !hide && !R.seen_by_all(A, tok)) {
+              x = without4(x, not_finite_in<FMT>(x));
+              A.mend[0] = 1u;  // (attn_mend_kernel)
+            }
+            put(id, x, hide);
           }
         }
       };
@@ -1071,43 +1075,54 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     };
     // Zeros in the rows of a V stage that no query row of the block sees (their weights are 0, and what the pages hold there may
     // be a NaN), and in place of what is not finite in rows that only some see (attn_mend_kernel adds it to those).
-    // This runs while the softmax works on the same tile's scores.
+    int have_looked = 0;
     auto clean = [&](int at, int j, int h) {
       const RowRange& R = pc.R;
       const int j0 = R.tile(pc.t_begin + j) * kTT + h * P::kVTok;
-      if (!P::kBf || R.seen_by_all(A, j0, P::kVTok)) return;
+      if (!P::kBf || R.seen_by_all(A, j0, P::kVTok)) return true;
       unsigned char* st = sm + P::kOffStage + (at % P::kStages) * P::kStage;
       constexpr int kCh = P::kVCols / 8;
-      bool odd = false;
+      bool odd = false, wrote = false;
       auto piece = [&](int id) {
         const int tr = id / kCh, ch = id % kCh;
         return reinterpret_cast<uint4*>(st + (ch >> 3) * (P::kVTok * 128) + tr * 128 + ((ch & 7) << 4));
       };
       // (context tokens t0 .. t1 - 1, as far as the stage has them)
       auto zero = [&](int t0, int t1) {
-        for (int id = max(t0 - j0, 0) * kCh + lane; id < min(t1 - j0, P::kVTok) * kCh; id += 32) *piece(id) = make_uint4(0u, 0u, 0u, 0u);
+        for (int id = max(t0 - j0, 0) * kCh + lane; id < min(t1 - j0, P::kVTok) * kCh; id += 32) *piece(id) = make_uint4(0u, 0u, 0u, 0u), wrote = true;
       };
       auto sift = [&](int t0, int t1) {
         const int end = min(t1 - j0, P::kVTok) * kCh;
         for (int id0 = max(t0 - j0, 0) * kCh + lane; id0 < end; id0 += 256) {
-          bool any = false;
+          uint4 w[8];
+          uint32_t found = 0u;
 #pragma unroll
-          for (int u = 0; u < 8; ++u) any |= id0 + 32 * u < end && any_not_finite<FMT>(*piece(id0 + 32 * u));
-          if (!any) continue;
+          for (int u = 0; u < 8; ++u) w[u] = *piece(min(id0 + 32 * u, end - 1));
+#pragma unroll
+          for (int u = 0; u < 8; ++u) look_for_not_finite<FMT>(w[u], found);
+          if (!found_not_finite<FMT>(found)) continue;
           for (int id = id0; id < end && id < id0 + 256; id += 32) *piece(id) = without4(*piece(id), not_finite_in<FMT>(*piece(id)));
           odd = true;
         }
       };
-      const int ahead = R.p0 + R.t0 + 1;  // from here on some row does not see a token yet
-      if (A.window) {
-        zero(R.sink, R.lo);
-        sift(max(R.sink, R.lo), min(R.hi - A.window, ahead));  // (some row's window has left these)
-      }
-      sift(ahead, R.hi);
+      if (A.window) zero(R.sink, R.lo);
       zero(R.hi, j0 + P::kVTok);
+      auto range = [&](int k, int t0, int t1) {
+        if (t0 >= min(t1, j0 + P::kVTok) || t1 <= j0) return true;
+        if (!BAL) {
+          if (!(have_looked >> k & 1) && !__all_sync(kFullMask, mbar_wait(looked + k, 0, kWaitNs))) return false;
+          have_looked |= 1 << k;
+          if (!(*reinterpret_cast<volatile int*>(odd_v) >> k & 1)) return true;
+        }
+        sift(t0, t1);
+        return true;
+      };
+      if (A.window && !range(0, R.left0(), R.left1(A))) return false;
+      if (!range(1, R.ahead0(), R.hi)) return false;
       if (odd) A.mend[0] = 1u;
-      fence_async();
+      if (odd || wrote) fence_async();
       __syncwarp();
+      return true;
     };
     bool ok = true;
     const bool issues = CG == 1 || rank == 0;
@@ -1122,7 +1137,8 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         for (int h = 0; ok && h < P::kPer; ++h, ++cnt) {
           ok = stage_ready(cnt);
           if (!ok) break;
-          if (value) clean(cnt, j, h);
+          if (value) ok = clean(cnt, j, h);
+          if (!ok) break;
           if (lane == 0) arrive_first<CG>(peer_full + cnt % P::kStages);
           __syncwarp();
         }
@@ -1155,7 +1171,7 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
         if (s == 0)
           for (int h = 0; ok && h < P::kPer; ++h) {
             ok = stage_ready(v_at + h);
-            if (ok) clean(v_at + h, j, h);
+            ok = ok && clean(v_at + h, j, h);
             ok = ok && peer_ready(v_at + h);
           }
         ok = ok && __all_sync(kFullMask, wait_group<CG>(p_full + buf, static_cast<uint32_t>((((s == 0 ? g0 : g1) + j) / SB) & 1)));
@@ -1201,6 +1217,32 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     if (!__all_sync(kFullMask, mbar_wait(m_done, 0, kWaitNs))) give_up();
    } else if (warp == P::kLoadWarp) {
     load();
+   } else if (P::kBf && !BAL) {
+    // ---------------- the two warps left: a look at V ahead of the products ----------------
+    // (A call of short windows waits for V: 6 chunks of up to 1500 tokens, windows of 1024, heads of 256, without a look 192 us, with
+    // one in the stages 205, with this 200.  Blocks that walk several items have time for it in the stages: 2048 tokens over 16384,
+    // heads of 128, 516 us with and without.)
+    const RowRange& R = pc.R;
+    constexpr int kCh = P::kVCols / 8, kBatch = NQ == 1 ? 16 : 8;
+    auto look = [&](int k, int t0, int t1) {
+      uint32_t found = 0u;
+      const int n = (t1 - t0) * kCh;
+      for (int id0 = (warp & 1) * 32 + lane; id0 < n; id0 += 64 * kBatch) {
+        uint4 w[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int id = min(id0 + 64 * u, n - 1), tok = t0 + id / kCh;
+          w[u] = __ldg(reinterpret_cast<const uint4*>(A.kv.at(true, page_of(pc.b, tok), pc.head, tok & page_mask)) + rank * kCh + id % kCh);
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) look_for_not_finite<FMT>(w[u], found);
+      }
+      if (found_not_finite<FMT>(found)) atomicOr(odd_v, 1 << k);
+      __syncwarp();
+      if (lane == 0) arrive_on(looked + k);
+    };
+    if (A.window) look(0, R.left0(), R.left1(A));
+    look(1, R.ahead0(), R.hi);
    }
   } else if constexpr (!P::kBf) {
    set_regs<P::kRegs, P::kLoadRegs>();
