@@ -179,8 +179,9 @@ __device__ __forceinline__ float ex2(float x) { return ex2_approx(x); }
 // Values that are not finite.  The kernels' second product runs over whole tiles, where a token hidden from a row has the weight
 // 0 in it, and 0 times an infinity is a NaN.  Tokens that no row of a block sees are zeroed before the product.  Of tokens that
 // some rows see and others do not (at the causal edge and at the window's, as many as a block has new tokens) the elements
-// that are not finite are zeroed, and added to the rows that do see them apart from the product.  (Beside an 8-bit cache a scale that is not
-// finite counts for all of its row.)  Tokens that all rows see go through the product as they are.
+// that are not finite are zeroed, and the rows that see them get what is not finite apart from the product (few rows: a NaN; many: the
+// value).  Beside an 8-bit cache a scale that is not finite counts for all of its row.  Tokens that all rows see go through
+// the product as they are.
 //
 // The elements of a word of a cached row that are not finite, all bits of each.
 template <int FMT>
@@ -193,8 +194,8 @@ template <int FMT>
 __device__ __forceinline__ uint4 not_finite_in(uint4 w) {
   return make_uint4(not_finite_in<FMT>(w.x), not_finite_in<FMT>(w.y), not_finite_in<FMT>(w.z), not_finite_in<FMT>(w.w));
 }
-// Whether there are any: four words' elements are added to a NaN or a number other than zero for the first that is one, else zero
-// (bf16: an infinity or a NaN times zero; e4m3: the next code after the largest carries into the sign's place).
+// Looks for them in four words: `found`, zero at first, tells later whether there was one (bf16: an infinity or a NaN times zero
+// is a NaN, all else adds zero; e4m3: the code after the largest finite one carries into the sign's place).
 template <int FMT>
 __device__ __forceinline__ void look_for_not_finite(uint4 w, uint32_t& found) {
   if constexpr (FMT == GS_DTYPE_BF16) {

@@ -18,7 +18,7 @@
 // A row's reference point m moves only when a score passes it by 2^8 (as V's reference scale does
 // when a larger one comes), so the usual tile needs one vote instead of reductions and rescaling.
 // Values of tokens hidden from every row of the block are set to zero before they are used, and so is what is not finite in
-// those hidden from some, whose columns are then a NaN in the rows that see them.
+// tokens hidden from some rows, whose columns are then a NaN in the rows that see them.
 //
 // A context is shared evenly by the blocks of a cluster (up to 8), which join their (m, l, O) through
 // distributed shared memory; of several clusters per context the last to finish joins their partial
