@@ -231,7 +231,9 @@ __device__ __forceinline__ bool leave_odd_out(const AttnArgs& A, const RowRange&
   return wrote;
 }
 
-template <int D, int FMT, int NB>
+// TOKENS: a sequence may have more than one new token, so that the rows of a block need not see the same ones (the code for that costs the
+// main loop registers and time: 64 sequences of 8192 tokens, one token each, e4m3 188 -> 194 us with it, int8 211 -> 216).
+template <int D, int FMT, int NB, bool TOKENS>
 __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
     attn_rows_kernel(const __grid_constant__ AttnArgs A, const __grid_constant__ RowsMaps maps) {
   using P = RowsPlan<D, FMT>;
@@ -247,8 +249,9 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
   __shared__ float s_m[kRowsWarps][kRows], s_l[kRowsWarps][kRows], s_f[kRowsWarps];
   __shared__ float s_qf[kRows];
   __shared__ __align__(8) float s_ml[kRows][2];  // the block's joined maximum and sum
-  __shared__ uint32_t s_odd[kRows][D / 32];  // columns of rows that have a value which is not finite and was left out of the product
-  __shared__ int s_any;                      // whether there are any
+  // (TOKENS) columns of rows that have a value which is not finite and was left out of the product; whether there are any
+  __shared__ uint32_t s_odd[TOKENS ? kRows : 1][D / 32];
+  __shared__ int s_any;
   __shared__ RowRange s_range;
   __shared__ __align__(8) uint64_t s_bar[kRowsWarps][P::kStages];
 
@@ -264,8 +267,10 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
   const int i_begin = min(static_cast<int>(blockIdx.x) * share, R.tiles);
   const int i_end = min(i_begin + share, R.tiles);
   if (lane < P::kStages) mbar_init(&s_bar[warp][lane], 1);
-  for (int i = tid; i < kRows * (D / 32); i += kRowsThreads) s_odd[0][i] = 0u;
-  if (tid == 0) s_any = 0, s_range = R;
+  if constexpr (TOKENS) {
+    for (int i = tid; i < kRows * (D / 32); i += kRowsThreads) s_odd[0][i] = 0u;
+    if (tid == 0) s_any = 0, s_range = R;
+  }
   __syncwarp();
 
   // ---- the warp's ring: stage i holds the warp's step i, tiles i_begin + (i · 4 + warp) · kSub .., or (halves)
@@ -499,7 +504,7 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
             wrote = true;
           }
         }
-        if (A.max_q > 1) {  // (rows of one token all see the same ones)
+        if constexpr (TOKENS) {
           unsigned scale_odd = 0u;
           if constexpr (!kBf) {
 #pragma unroll
@@ -647,7 +652,7 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
       }
   __syncthreads();
   float* oj = reinterpret_cast<float*>(smem);
-  if (s_any) {  // (into warp 0's part: whatever is added to it is a NaN)
+  if (TOKENS && s_any) {  // (into warp 0's part: whatever is added to it is a NaN)
     for (int i = tid; i < R.rows * D; i += kRowsThreads)
       if (s_odd[i / D][i % D / 32] >> (i % 32) & 1u) oj[i / D * (D + 4) + i % D] = NAN;
     __syncthreads();
@@ -772,7 +777,7 @@ __global__ void __launch_bounds__(kRowsThreads, (rows_occupancy<D, FMT, NB>()))
   cluster_sync();  // (no block leaves while its shared memory is read)
 }
 
-template <int D, int FMT, int NB>
+template <int D, int FMT, int NB, bool TOKENS>
 cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
   constexpr int kRows = 8 * NB;
   using P = RowsPlan<D, FMT>;
@@ -782,7 +787,7 @@ cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   static std::atomic<int> held{0};  // clusters of 8 that the device holds at once (a GPU process runs on one kind of device)
   if (device_todo(done)) {
-    cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<D, FMT, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = cudaFuncSetAttribute(attn_rows_kernel<D, FMT, NB, TOKENS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t q{};
     cudaLaunchAttribute at{};
@@ -794,7 +799,7 @@ cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
     q.attrs = &at;
     q.numAttrs = 1;
     int n = 0;
-    e = cudaOccupancyMaxActiveClusters(&n, attn_rows_kernel<D, FMT, NB>, &q);
+    e = cudaOccupancyMaxActiveClusters(&n, attn_rows_kernel<D, FMT, NB, TOKENS>, &q);
     if (e != cudaSuccess) return e;
     held.store(n > 0 ? n : 1);
     mark_device_done(done);
@@ -837,23 +842,27 @@ cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, attn_rows_kernel<D, FMT, NB>, a, *reinterpret_cast<const RowsMaps*>(c->maps + 256));
+  return cudaLaunchKernelEx(&cfg, attn_rows_kernel<D, FMT, NB, TOKENS>, a, *reinterpret_cast<const RowsMaps*>(c->maps + 256));
 }
 
-template <int D, int FMT>
+template <int D, int FMT, bool TOKENS>
 cudaError_t go_nb(const gs_kv_cache* c, const AttnArgs& a, cudaStream_t st) {
   const int64_t rows = static_cast<int64_t>(a.max_q) * a.group;
-  if (rows <= 8) return go<D, FMT, 1>(c, a, st);
+  if (rows <= 8) return go<D, FMT, 1, TOKENS>(c, a, st);
   // (32 rows of head_dim 256 would need 256 registers a thread for O alone: two passes of 16)
-  if (rows <= 16 || D == 256) return go<D, FMT, 2>(c, a, st);
-  return go<D, FMT, D == 256 ? 2 : 4>(c, a, st);
+  if (rows <= 16 || D == 256) return go<D, FMT, 2, TOKENS>(c, a, st);
+  return go<D, FMT, D == 256 ? 2 : 4, TOKENS>(c, a, st);
+}
+template <int D, int FMT>
+cudaError_t go_tokens(const gs_kv_cache* c, const AttnArgs& a, cudaStream_t st) {
+  return a.max_q > 1 ? go_nb<D, FMT, true>(c, a, st) : go_nb<D, FMT, false>(c, a, st);
 }
 template <int D>
 cudaError_t go_fmt(const gs_kv_cache* c, const AttnArgs& a, cudaStream_t st) {
   switch (c->d.format) {
-    case GS_DTYPE_BF16: return go_nb<D, GS_DTYPE_BF16>(c, a, st);
-    case GS_DTYPE_E4M3: return go_nb<D, GS_DTYPE_E4M3>(c, a, st);
-    default: return go_nb<D, GS_DTYPE_INT8>(c, a, st);
+    case GS_DTYPE_BF16: return go_tokens<D, GS_DTYPE_BF16>(c, a, st);
+    case GS_DTYPE_E4M3: return go_tokens<D, GS_DTYPE_E4M3>(c, a, st);
+    default: return go_tokens<D, GS_DTYPE_INT8>(c, a, st);
   }
 }
 
