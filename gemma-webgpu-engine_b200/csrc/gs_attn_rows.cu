@@ -24,11 +24,11 @@
 // distributed shared memory; of several clusters per context the last to finish joins their partial
 // results.
 //
-// Measured (one token a sequence, 32 query heads on 8 of 128): 64 sequences of 8192 tokens bf16 304 us,
-// 7.1 TB/s, e4m3 179 us, 6.2 TB/s, ragged 184 and 119 us; two of 131072 tokens (4 heads) 89 us, 6.0 TB/s;
-// one of 777 tokens (2 heads of 256) 7.5 us: launch, table and query loads, one round of tiles, join.
+// Measured (calls in a row; one token a sequence, 32 query heads on 8 of 128): 64 sequences of 8192 tokens bf16 313 us,
+// 6.9 TB/s, e4m3 188 us, 5.9 TB/s, ragged 187 and 123 us; two of 131072 tokens (4 heads) 91 us, 5.9 TB/s;
+// one of 777 tokens (2 heads of 256) 7 us on the device: launch, table and query loads, one round of tiles, join.
 // Beside 8-bit codes the widening keeps the issue slots half busy and the ragged last round is the
-// other loss; 20 rows of 256 (16 windows of 1028 tokens, int8, 25 us) take two passes of 16 rows at 1.5 us
+// other loss; 20 rows of 256 (16 windows of 1028 tokens, int8, 27 us) take two passes of 16 rows at 1.5 us
 // a tile and warp: bound by the products' latency, not by bytes.
 //
 // 8-bit codes are widened to float16 (exact for e4m3 and int8) in registers, K's scale
@@ -61,8 +61,8 @@ struct RowsPlan {
   static constexpr int kTileBytes = kRT * kRow;              // K or V of one tile
   static constexpr int kSub = kTileBytes <= 1024 ? 2 : 1;    // tiles per stage
   // A stage holds K and V of its tiles, or, where those are 16 KB, one of them, in turn: three stages of 8 KB a warp
-  // then leave room for a second block on the SM (32 rows, 8 sequences of 4000 tokens, 8 heads of 256: 78 -> 48 us), at the
-  // price of two waits and two fetches a tile (narrower rows lose by it: heads of 64 161 -> 187 us).
+  // then leave room for a second block on the SM (32 rows, 8 sequences of 4000 tokens, 8 heads of 256: 38% less time), at the
+  // price of two waits and two fetches a tile (narrower rows lose by it: heads of 64 16%).
   static constexpr bool kHalves = kTileBytes >= 8192;
   static constexpr int kParts = kHalves ? 1 : 2;
   static constexpr int kStage = kSub * kParts * kTileBytes;
@@ -194,9 +194,8 @@ constexpr int rows_occupancy() {
 
 // What is not finite in the V tile at vs (tokens j0 ..) and in tokens that some rows of the block see and others do not: set to
 // zero, and its columns marked in the rows that see it (odd: words of 32 columns; scale_odd: tokens whose scale is not finite, all of
-// their columns).  By a warp; whether this lane wrote to the tile.  (R lies in shared memory: the main loop has no registers for it.  What this
-// costs drafted tokens: 20 rows of 256 25.5 -> 26.0 us bf16, 24.7 -> 25.5 e4m3, 32 rows of 128 49.1 -> 50.7 bf16, most of it
-// by the registers of the main loop.)
+// their columns).  By a warp; whether this lane wrote to the tile.  (R lies in shared memory: the main loop has no registers for it.  With
+// and without this: 20 rows of 256 25.4 and 25.3 us bf16, 25.4 and 25.1 e4m3, 32 rows of 256 59 and 57 e4m3, 64 rows of 128 50 and 49 bf16.)
 template <int D, int FMT>
 __device__ __forceinline__ bool leave_odd_out(const AttnArgs& A, const RowRange& R, uint32_t vs, int j0, unsigned scale_odd, uint32_t* odd, int* any) {
   using P = RowsPlan<D, FMT>;
@@ -806,7 +805,7 @@ cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
   }
   // Blocks per context: one round of what the device holds (in clusters of 8, which have to find their SMs
   // in one GPC: fewer than the SMs alone would), each block with at least a stage a warp.  (Two sequences of 131072 tokens, 4 heads
-  // of 128: bf16 86 us in one round, 102 in two.)  Up to 8 blocks are one cluster; more are
+  // of 128, bf16: two rounds take 19% longer.)  Up to 8 blocks are one cluster; more are
   // clusters of 8 whose partial results are joined.
   const int64_t tiles = most_tiles(a, kRT, kRows);
   int64_t want = 8ll * held.load() / items;
@@ -815,9 +814,8 @@ cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
   int cluster = 1;
   while (cluster < 8 && cluster * 2 <= want) cluster *= 2;
   // More contexts than blocks at once: two blocks each all the same where a warp still has 32 tiles, since shorter blocks
-  // leave a shorter last round (64 sequences of up to 8192 tokens, 8 heads, ragged: heads of 128 189 -> 185 us bf16, 122 ->
-  // 120 e4m3, of 256 366 -> 354, 222 -> 209; all alike 308 -> 306, 188 -> 180, but 596 -> 601, 326 -> 341; 128 of 2000 tokens
-  // 94 -> 100 us).
+  // leave a shorter last round (64 sequences of up to 8192 tokens, 8 heads, ragged: 2% less time at 128, 3% bf16 and 6% e4m3
+  // at 256; all alike 1% and 4% less at 128, 1% and 5% more at 256; 128 sequences of 2000 tokens 6% more).
   if (cluster < 2 && tiles >= 2 * kRowsWarps * 32) cluster = 2;
   int64_t splits = want / cluster;
   const int64_t by_ws = static_cast<int64_t>(kAttnWsBytes) / (items * kRows * (D / 4) * 24);

@@ -15,12 +15,12 @@
 // as long as the softmax and the output alone fills half of tensor memory: one query tile, two
 // score buffers.
 //
-// Measured (2048 new tokens over 16384): 32 / 8 heads of 128 bf16 438 us, 1177 TFLOP/s, both the tensor pipe and
-// the 2^x unit 55 % busy (back to back at the 1000 W cap and 1.7 GHz: 508 us, 1014 TFLOP/s; starting the
-// second product at three quarters of P gained nothing: 440 -> 446 us); of 64 378 us; 16 / 8 heads of 256
-// 402 us, 1281 TFLOP/s, bound by what L2 delivers of K and V (6.3 TB/s); e4m3 of 128 665 us, of 256 475 us: widening
-// and softmax share the issue slots and shared memory.  Six ragged chunks of up to 1500 tokens, windows of 1024,
-// heads of 256: e4m3 222 us, bf16 193 us; an item's 11 tiles take 25 of its 38 us, query loads from HBM 4, output 3.
+// Measured (2048 new tokens over 16384, calls in a row, the clock at 1.7 GHz under the 1000 W cap): 32 / 8 heads of 128 bf16
+// 516 us, 1.0 PFLOP/s, both the tensor pipe and the 2^x unit 55 % busy (starting the second product at three quarters of P
+// gained nothing: 1% more time); of 64 377 us; 16 / 8 heads of 256 510 us, 1.0 PFLOP/s, bound by what L2 delivers of K and V;
+// e4m3 of 64 518, of 128 661, of 256 500 us, int8 530, 704, 532 us: widening and softmax share the issue slots and shared
+// memory.  Six ragged chunks of up to 1500 tokens, windows of 1024, heads of 256: e4m3 223 us, bf16 200 us; an
+// item's 11 tiles take 25 of its 38 us, query loads from HBM 4, output 3.
 //
 // Tensor memory (512 columns): S0 at 0, S1 at 128, O0 at 256, O1 at 256 + D.
 // Warps: softmax warpgroup(s) first (warp % 4 = its tensor-memory lanes), then the MMA issuer and the
@@ -135,7 +135,7 @@ __device__ __forceinline__ void arrive_on(uint64_t* bar) {
 // Arrival on the first block's barrier (the one that issues the products).  It releases at block scope: what the products
 // read lies in the arriving block's own shared memory, handed to the async proxy by its writers before, or in tensor
 // memory, ordered by the tcgen05 fences.  At cluster scope each arrival waits for all of the thread's memory traffic, 1000
-// clocks a tile (2048 x 16384 tokens, heads of 256: 402 -> 480 us).
+// clocks a tile (2048 x 16384 tokens, heads of 256: 19% more time).
 template <int CG>
 __device__ __forceinline__ void arrive_first(uint64_t* bar) {
   if constexpr (CG == 1) {
@@ -457,8 +457,8 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
     }
   }
   const Piece& pc = BAL ? walk->piece : only;
-  // (A piece of at most 128 rows leaves the second query tile out: 8 sequences of 4000 tokens, 128 rows of 128: 66 -> 60 us
-  // bf16, 84 -> 69 int8; the counting costs chunks over 8-bit caches with heads of 64 3%.)
+  // (A piece of at most 128 rows leaves the second query tile out: 8 sequences of 4000 tokens, 128 rows of 128, 9% less time
+  // bf16, 18% int8; the counting costs chunks over 8-bit caches with heads of 64 3%.)
   auto query_tiles = [&]() { return NQ == 2 && pc.R.rows <= 128 ? 1 : NQ; };  // (with rows of the piece)
   auto another = [&]() {  // the next piece, once a warp is done with this one
     if constexpr (BAL) return *stop == 0 && next_piece<kGroupRows>(A, walk, lane);
@@ -800,8 +800,8 @@ __global__ void __launch_bounds__(TilePlan<D, FMT, CG>::kThreads, 1)
       const bool whole = j0 + kTT - 1 <= p && (j0 >= lo || j0 + kTT <= R.sink);
       if (!__all_sync(kFullMask, whole)) {
         // One bound where one is enough: a causal edge, a window's edge past the sinks (6 sequences of windows of
-        // 1024 at head_dim 256: 226 -> 222 us e4m3; not with two query tiles beside an 8-bit cache, whose
-        // softmax has no registers left for it: 735 -> 797 us at head_dim 128).
+        // 1024 at head_dim 256, e4m3: 2% less time; not with two query tiles beside an 8-bit cache, whose
+        // softmax has no registers left for it: 8% more at head_dim 128).
         constexpr bool kEdges = P::kBf || NQ == 1;
         const int hi_c = p + 1 - j0, lo_c = lo - j0, sk_c = R.sink - j0;
         if (kEdges && __all_sync(kFullMask, lo_c <= 0)) {
@@ -1436,10 +1436,9 @@ cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
   if constexpr (P::kBalance) {
     // Balanced: every block takes an equal stretch of all items' tiles.  Against the rounds of a fixed grid
     // this saves the last round's idle blocks and costs a block about one more beginning and end (about 5
-    // tiles' time) and the joining of what is cut (as much again): 2048 tokens over 16384 in 1.73 rounds, head_dim
-    // 128: 476 -> 446 us, head_dim 64: 419 -> 387 us; 1024-token windows (10 tiles): 70 -> 86 us, so not there.
-    // (8-bit at head_dim 64: e4m3 553 -> 512 us; at 128 the softmax spills for it, 665 -> 820 us; at head_dim 256 there
-    // are half as many groups and it gains nothing: 474 -> 498 us.)
+    // tiles' time) and the joining of what is cut (as much again): 2048 tokens over 16384 in 1.73 rounds take 6% less time
+    // at head_dim 128, 8% at 64, 1024-token windows (10 tiles) 23% more, so not there.  (8-bit caches: at head_dim 64 7% less; at 128
+    // the softmax spills for it, 23% more; at head_dim 256 there are half as many groups, 5% more.)
     const int64_t rounds = (items + groups - 1) / groups;
     const bool gains = rounds * groups * (tiles + 5) > items * tiles + (items + 2 * groups) * 5;
     if (2 * items > groups && gains && units <= kBalancedUnits && groups <= kMaxGroups) {
@@ -1474,8 +1473,8 @@ cudaError_t go(const gs_kv_cache* c, AttnArgs a, cudaStream_t st) {
 template <int D, int FMT>
 cudaError_t go_cg(const gs_kv_cache* c, const AttnArgs& a, cudaStream_t st) {
   // Two blocks a group at head_dim 256, where one block's 128 rows read K and V faster than L2 gives them
-  // (2048 x 16384 tokens, 16 / 8 heads: bf16 627 -> 402 us, e4m3 871 -> 484 us).  At head_dim 128 a block has
-  // 256 rows of its own, and two of them gain nothing (32 / 8 heads: e4m3 665 -> 673 us, int8 704 -> 682 us).
+  // (2048 x 16384 tokens, 16 / 8 heads: bf16 36% less time, e4m3 44%).  At head_dim 128 a block has
+  // 256 rows of its own, and two of them gain nothing (32 / 8 heads: e4m3 1% more, int8 3% less).
   if constexpr (D == 256) {
     if (static_cast<int64_t>(a.max_q) * a.group > TilePlan<D, FMT, 1>::kRows) return go<D, FMT, 2>(c, a, st);
   }

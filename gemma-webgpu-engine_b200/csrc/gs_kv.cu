@@ -7,8 +7,10 @@
 // covers keys and values.  Both directions move 3 bytes an element (bf16 beside codes) and
 // are bound by HBM for long chunks, by launch latency for one step.
 //
-// Measured: 16384 tokens of 8 heads of 128, bf16 -> e4m3: 21 us written, 20 us read back (4.9
-// TB/s, 0.75 of a copy's rate); 32768 tokens of 4 heads of 256 read: 35 us, 5.8 TB/s.
+// Measured (calls in a row, 16384 tokens of 8 heads of 128, bf16 outside): e4m3 or int8 22.5 us written, 20.5 us read back
+// (4.5 and 5.0 TB/s, 0.69 and 0.76 of a copy's rate), bf16 25.1 and 25.2 us (5.3 TB/s, 0.82); 32768 tokens of 4 heads of 256
+// read from e4m3: 35 us, 5.8 TB/s.  What holds the write back is the bytes in flight: two tokens a thread in 64 registers keep 42 % of
+// the warps active.
 #include <cmath>
 #include <new>
 
@@ -248,9 +250,9 @@ cudaError_t launch_rows(const KvRowsArgs& a, int fmt, bool write, bool bf16, boo
 }
 
 // Rows (new tokens × heads of a group) up to which the few-row kernel is taken (8 sequences of 4000 tokens, 8
-// heads, few rows against many: 64 rows of 128: 47 and 53 us bf16, 58 and 63 us int8, 128 rows: 83 and 60,
-// 102 and 69; 32 rows of 256: 64 and 83 us int8, 64 rows: 110 and 87; where contexts fill the device the lines cross
-// earlier: 26 sequences of 4000, 55 rows of 128, int8 101 and 90).
+// heads, few rows against many: 64 rows of 128 50 and 59 us bf16, 61 and 69 int8, 96 rows 81 and 62, 104 and 72;
+// 32 rows of 256 62 and 74 us bf16, 66 and 80 int8, 64 rows 100 and 78, 111 and 84.  Where contexts fill the device the lines cross
+// earlier: 26 sequences of 4000, 55 rows of 128, 158 and 120 us bf16, 198 and 178 int8).
 int64_t few_rows(int head_dim) { return head_dim == 256 ? 32 : 64; }
 
 gs_status kfail(gs_kv_cache* c, gs_status s, const char* m) {
