@@ -451,7 +451,7 @@ gs_status gs_attention(gs_kv_cache* c, const gs_attention_args* p, void* stream)
   const int64_t most_rows = static_cast<int64_t>(p->max_q) * group;
   // (the many-row grid's second dimension holds blocks of at least 128 rows for every head)
   if (most_rows > (1ll << 23) || (most_rows + 127) / 128 * c->d.kv_heads > 65535)
-    return kfail(c, GS_EUNSUPPORTED, "max_q * (q_heads / kv_heads) times kv_heads is at most 2^23 - 128");
+    return kfail(c, GS_EUNSUPPORTED, "max_q * q_heads has to stay below 2^23 - 2^17");
   if (p->seqs > 65535) return kfail(c, GS_EUNSUPPORTED, "at most 65535 sequences per call");
   AttnArgs a{};
   a.kv = pool_of(c);
